@@ -16,7 +16,9 @@ CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(HERE, "libcbq_hip.so")
 ARCH = "gfx950"
 SOURCES = ["cbq_fixed.hip", "cbq_huffman.hip", "cbq_prefill.hip", "cbq_prefill_f32.hip",
-           "cbq_decode.hip", "cbq_split.hip", "cbq_tiny.hip", "cbq_gemm.hip"]
+           "cbq_decode.hip", "cbq_split.hip", "cbq_tiny.hip", "cbq_gemm.hip",
+           "cbq_paged_append.hip", "cbq_prefix_attn.hip", "cbq_prefix_attn_f32.hip",
+           "cbq_prefix_attn_bf16.hip", "cbq_prefix_attn_f16.hip"]
 # host-only C++ (no device code): compiled by the host compiler
 HOST_SOURCES = ["cbq_huff_host.cpp", "cbq_io.cpp"]
 HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-pthread", "-D__HIP_PLATFORM_AMD__=1",
@@ -45,7 +47,7 @@ def host_sources():
 
 TIMELINE_SO = os.path.join(HERE, "libcbq_hip_timeline.so")
 TORCH_SO = os.path.join(HERE, "libcbq_torch.so")
-TORCH_SRC = os.path.join(CSRC, "cbq_torch_ops.cpp")
+TORCH_SRC = [os.path.join(CSRC, s) for s in ("cbq_torch_ops.cpp", "cbq_torch_serve.cpp")]
 
 
 def torch_ops_command(out: str = TORCH_SO):
@@ -57,7 +59,7 @@ def torch_ops_command(out: str = TORCH_SO):
     return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1",
              "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
              "-I/opt/rocm/include", f"-I{tdir}/include",
-             f"-I{tdir}/include/torch/csrc/api/include", TORCH_SRC, "-o", out,
+             f"-I{tdir}/include/torch/csrc/api/include", *TORCH_SRC, "-o", out,
              f"-L{tdir}/lib", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip",
              f"-L{HERE}", "-lcbq_hip", "-Wl,-rpath,$ORIGIN"])
 
@@ -69,7 +71,7 @@ def build_torch_ops(verbose: bool = False, out: str = TORCH_SO) -> str:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError("g++ failed on cbq_torch_ops.cpp:\n" + res.stderr[-4000:])
+        raise RuntimeError("g++ failed on the torch operators:\n" + res.stderr[-4000:])
     os.replace(out + ".tmp", out)
     return out
 

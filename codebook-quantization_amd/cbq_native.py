@@ -1,5 +1,5 @@
 """ctypes binding of libcbq_hip.so, the gfx950 C ABI (include/cbq_hip.h,
-include/cbq_decode.h).
+include/cbq_decode.h, include/cbq_serve.h).
 
 The library is loaded after torch so that it binds to the HIP runtime torch
 already loaded (same SONAME), which makes torch's device pointers and
@@ -53,6 +53,13 @@ class SplitMatrix(ctypes.Structure):
 class UploadPart(ctypes.Structure):
     """struct cbq_upload_part (include/cbq_hip.h)."""
     _fields_ = [("file_offset", _i64), ("nbytes", _i64), ("dst", _vp)]
+
+
+class PagedKV(ctypes.Structure):
+    """struct cbq_paged_kv (include/cbq_serve.h)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3),
+                ("n_pages", _i64), ("page", ctypes.c_int32), ("n_kv", ctypes.c_int32),
+                ("hd", ctypes.c_int32), ("dtype", ctypes.c_int32)]
 
 
 # name -> (restype, argtypes); every symbol declared in include/*.h
@@ -135,6 +142,19 @@ SIGNATURES = {
     "cbq_argmax_step": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "cbq_silu_mul_f32": (_i, [_vp, _vp, _vp, _i64, _vp]),
     "cbq_causal_softmax_f32": (_i, [_vp, _i64, _i, _i, _i, ctypes.c_float, _vp]),
+    # include/cbq_serve.h
+    "cbq_paged_append": (_i, [_vp] * 3 + [_i] + [_vp] * 5 + [_i64, _i] + [_vp] * 2 + [_i]
+                         + [_vp] * 2 + [ctypes.c_float, _vp, ctypes.POINTER(PagedKV), _i64, _i,
+                                        _vp]),
+    "cbq_prefix_attn_decode_workspace": (ctypes.c_size_t, [ctypes.POINTER(PagedKV), _i64, _i, _i,
+                                                           _i]),
+    "cbq_prefix_attn_decode": (_i, [_vp, _vp, ctypes.POINTER(PagedKV), _vp, _i64, _vp, _i64, _i,
+                                    _vp, _i, _i, ctypes.c_float, _vp, _vp, ctypes.c_size_t, _vp]),
+    "cbq_prefix_attn_prompt_workspace": (ctypes.c_size_t, [ctypes.POINTER(PagedKV), _i64, _i, _i,
+                                                           _i64, _i]),
+    "cbq_prefix_attn_prompt": (_i, [_vp, _vp, _vp, ctypes.POINTER(PagedKV), _vp, _i64, _vp, _i64,
+                                    _i, _vp, _i, _i64, _i, ctypes.c_float, _vp, _vp,
+                                    ctypes.c_size_t, _vp]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -1,0 +1,212 @@
+// Addresses of a paged key/value cache and the launch plans of the attention
+// over it: plain C++ that the kernels, the host entry points and the CPU test
+// of them (tests/native/cbq_paged_host.cpp) share.
+#pragma once
+
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#define CBQ_PAGED_FN __host__ __device__ __forceinline__
+#else
+#define CBQ_PAGED_FN static inline
+#endif
+
+// n / d for 0 <= n < 2^31 by one 64-bit product: with 2^(s-1) < d <= 2^s and
+// mul = ceil(2^(31+s) / d), mul * d - 2^(31+s) < d <= 2^s, so the product's
+// error n * (mul * d - 2^(31+s)) / (d * 2^(31+s)) is below 1 / d: too small to
+// reach the next integer.
+struct CbqDiv {
+    uint32_t d, mul, shift;
+};
+
+CBQ_PAGED_FN CbqDiv cbq_div_make(uint32_t d)
+{
+    uint32_t s = 0;
+    while ((1ull << s) < d) s++;
+    return CbqDiv{d, (uint32_t)(((1ull << (31 + s)) + d - 1) / d), 31 + s};
+}
+
+CBQ_PAGED_FN uint32_t cbq_div(uint32_t n, const CbqDiv &q)
+{
+    return (uint32_t)(((uint64_t)n * q.mul) >> q.shift);
+}
+
+// The keys that a block walks: `prefix` shared ones, then own ones up to `end`
+// (an index on the joint axis).
+struct CbqKeys {
+    const int32_t *shared, *own;
+    int32_t prefix, end;
+};
+
+// Table entry of key j, or null where there is none (j outside [0, end)).
+CBQ_PAGED_FN const int32_t *cbq_key_entry(const CbqKeys &a, const CbqDiv &page, int32_t j,
+                                          int32_t &row)
+{
+    const bool shared = j < a.prefix;
+    const uint32_t i = (uint32_t)(shared ? j : j - a.prefix);
+    if (j < 0 || j >= a.end) {
+        row = 0;
+        return nullptr;
+    }
+    const uint32_t e = cbq_div(i, page);
+    row = (int32_t)(i - e * page.d);
+    return (shared ? a.shared : a.own) + e;
+}
+
+CBQ_PAGED_FN int32_t cbq_clamp_length(int32_t n, int64_t capacity)
+{
+    return n < 0 ? 0 : n > capacity ? (int32_t)capacity : n;
+}
+
+// Run b of a prompt batch: its first token and its length, inside [0, N).
+CBQ_PAGED_FN void cbq_run(const int32_t *q_start, int b, int32_t N, int32_t &first, int32_t &count)
+{
+    const int32_t lo = cbq_clamp_length(q_start[b], N), hi = cbq_clamp_length(q_start[b + 1], N);
+    first = lo;
+    count = hi > lo ? hi - lo : 0;
+}
+
+CBQ_PAGED_FN int64_t cbq_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
+CBQ_PAGED_FN int64_t cbq_min(int64_t a, int64_t b) { return a < b ? a : b; }
+CBQ_PAGED_FN int64_t cbq_max(int64_t a, int64_t b) { return a > b ? a : b; }
+
+namespace cbq_attn {
+
+// ---- launch plans ---------------------------------------------------------------------------
+struct Plan {
+    int rt;                                 // 64 rt rows a block, or 0: 16
+    int32_t tiles;                          // row tiles: of the prefix rows; of a prompt, at most
+    int32_t pre_parts, pre_chunk;           // decode: parts of the prefix and their keys
+    int32_t own_parts, own_chunk, own_tiles;    // decode: parts of the own keys, 16-row tiles
+    int32_t parts;                          // decode: all of them; prompt: key parts of a tile
+    int64_t blocks, bytes;
+};
+
+constexpr int64_t kCus = 256;                // of an MI355X
+constexpr int kAttnWaves = 4;                // of a block
+
+
+// Keys of a block's tile (K and V, two buffers: 64 KiB at most) and of a
+// wave's own (K and V, one buffer: 16 KiB, 32 KiB for rows of 1024 bytes).
+constexpr int block_keys(int row_bytes) { return row_bytes <= 256 ? 64 : 16384 / row_bytes; }
+constexpr int wave_keys(int row_bytes) { return row_bytes <= 512 ? 8192 / row_bytes : 16; }
+
+// 128 rows a block where a wave's 32 fit its registers beside a tile under way
+constexpr int widest(int row_bytes) { return row_bytes <= 256 ? 2 : 1; }
+
+inline int64_t part_bytes(int64_t parts, int64_t N, int n_q, int hd)
+{
+    return parts > 1 ? parts * N * n_q * (hd + 2) * 4 : 0;
+}
+
+inline Plan plan_decode(int row_bytes, int hd, int n_kv, int rep, int64_t prefix, int64_t capacity,
+                        int64_t batch)
+{
+    Plan p = {};
+    const int64_t rows = batch * rep, bk = block_keys(row_bytes), wk = kAttnWaves * wave_keys(row_bytes);
+    p.rt = rows <= 16 ? 0 : rows <= 64 ? 1 : widest(row_bytes);
+    int64_t tiles = cbq_ceil(rows, p.rt ? 64 * p.rt : 16), pre_parts = 0, pre_chunk = 1;
+    if (prefix > 0) {
+        // one block a CU: more parts cost their fp32 sums, written and read once
+        const int64_t least = p.rt ? 2 * bk : wk, want = cbq_max(1, kCus / (tiles * n_kv));
+        const int64_t unit = p.rt ? bk : wk;
+        pre_chunk = cbq_max(least, cbq_ceil(cbq_ceil(prefix, want), unit) * unit);
+        pre_parts = cbq_ceil(prefix, pre_chunk);
+    } else {
+        tiles = 0;
+    }
+    const int64_t own_tiles = cbq_ceil(rep, 16);
+    // about eight blocks a CU of the full capacity, a tile a wave at least and
+    // eight at most
+    const int64_t share = cbq_ceil(capacity * batch * n_kv * own_tiles, 8 * kCus);
+    const int64_t own_chunk = cbq_min(cbq_max(cbq_ceil(share, wk), 1), 8) * wk;
+    const int64_t own_parts = cbq_max(cbq_ceil(capacity, own_chunk), pre_parts ? 0 : 1);
+    p.blocks = n_kv * (tiles * pre_parts + batch * own_tiles * own_parts);
+    p.bytes = part_bytes(pre_parts + own_parts, batch, n_kv * rep, hd);
+    p.tiles = (int32_t)tiles;
+    p.pre_parts = (int32_t)pre_parts;
+    p.pre_chunk = (int32_t)pre_chunk;
+    p.own_parts = (int32_t)own_parts;
+    p.own_chunk = (int32_t)own_chunk;
+    p.own_tiles = (int32_t)own_tiles;
+    p.parts = (int32_t)(pre_parts + own_parts);
+    return p;
+}
+
+inline Plan plan_prompt(int row_bytes, int hd, int n_kv, int rep, int64_t prefix, int64_t capacity,
+                        int64_t batch, int64_t N)
+{
+    Plan p = {};
+    const int64_t rows = N * rep, small = (cbq_ceil(rows, 16) + batch) * n_kv;
+    const int64_t keys = cbq_max(prefix + capacity, 1);
+    if (rows <= 16 * batch || (small <= 2 * kCus && keys <= 2048)) p.rt = 0;
+    else p.rt = rows <= 64 * batch ? 1 : widest(row_bytes);
+    // a run's last tile may be part full: one more a run than the rows need
+    const int64_t tiles = rows / (p.rt ? 64 * p.rt : 16) + cbq_min(batch, N);
+    const int64_t unit = p.rt ? block_keys(row_bytes) : kAttnWaves * wave_keys(row_bytes);
+    const int64_t blocks = tiles * n_kv;
+    const int64_t parts = blocks >= kCus
+        ? 1 : cbq_max(1, cbq_min(cbq_ceil(2 * kCus, blocks), keys / (4 * unit)));
+    p.blocks = blocks * parts;
+    p.bytes = part_bytes(parts, N, n_kv * rep, hd);
+    p.tiles = (int32_t)tiles;
+    p.parts = (int32_t)parts;
+    return p;
+}
+
+inline bool plan_fits(const Plan &p)
+{
+    return p.blocks > 0 && p.blocks < (1ll << 31) && p.parts < (1ll << 20);
+}
+
+// ---- what a block does ------------------------------------------------------------------------
+// Decode: blocks of the prefix's parts first (they compute), then own parts
+// (they read), so that both kinds share the CUs.
+struct DecodeWork {
+    bool skip;                              // nothing to do
+    int h, tile, part, seq;                 // seq -1: the prefix
+    int32_t first, end;                     // keys
+};
+
+CBQ_PAGED_FN DecodeWork decode_work(const Plan &p, uint32_t block, int n_kv, int batch,
+                                    int32_t prefix, const int32_t *lengths, int64_t capacity)
+{
+    DecodeWork w;
+    uint32_t i = block;
+    const uint32_t pre = (uint32_t)p.tiles * p.pre_parts * n_kv;
+    const bool shared = i < pre;
+    if (!shared) i -= pre;
+    w.h = (int)(i % n_kv);
+    i /= n_kv;
+    w.skip = false;
+    if (shared) {
+        w.tile = (int)(i % p.tiles);
+        w.part = (int)(i / p.tiles);
+        w.seq = -1;
+        w.first = w.part * p.pre_chunk;
+        w.end = (int32_t)cbq_min((int64_t)w.first + p.pre_chunk, prefix);
+        return w;
+    }
+    w.tile = (int)(i % p.own_tiles);
+    i /= p.own_tiles;
+    w.seq = (int)(i % batch);
+    const int chunk = (int)(i / batch);
+    const int32_t len = cbq_clamp_length(lengths[w.seq], capacity);
+    const int64_t first = (int64_t)chunk * p.own_chunk;
+    w.part = p.pre_parts + chunk;
+    w.first = (int32_t)cbq_min(first, len);
+    w.end = (int32_t)cbq_min(first + p.own_chunk, len);
+    w.skip = first >= len && (p.parts > 1 || chunk > 0);
+    return w;
+}
+
+// Prompt: the keys of part `part` of a tile whose rows see `sees` keys at most.
+CBQ_PAGED_FN void prompt_keys(int32_t sees, int parts, int part, int unit, int32_t &first,
+                              int32_t &end)
+{
+    const int64_t share = cbq_ceil(cbq_ceil(sees, parts), unit) * unit;
+    first = (int32_t)cbq_min(part * share, sees);
+    end = (int32_t)cbq_min(first + share, sees);
+}
+
+}  // namespace cbq_attn

@@ -1,0 +1,720 @@
+// Attention of a batch over a paged key/value cache with a shared prefix
+// (include/cbq_serve.h): the kernels, as templates on the cache's type and the
+// head size; cbq_prefix_attn_{f32,bf16,f16}.hip hold one type each.
+//
+// out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s), s_j = scale q.k_j,
+// in one pass over the keys: a running maximum m, sum l and weighted values o
+// of each query row, o and l scaled by exp(m_old - m_new) when m grows.
+//
+// Rows.  The n_q / n_kv query heads that read one kv head are rows beside the
+// tokens: row r of kv head h is token r / rep, head h * rep + r % rep, so the
+// heads of a group share each key read.  Of a shared prefix, the rows are the
+// whole batch's.
+//
+// Products.  Both are matrix-core products with the keys in the left operand:
+// S^T = K Q^T (16 keys x 16 rows a tile) leaves a lane with one row (lane % 16)
+// and four keys (4 * (lane / 16) + i), which is, for two tiles side by side, the
+// right operand of O^T = V^T P^T up to an order of the keys that V's loads
+// follow.  So weights never leave their lane, a row's maximum needs two
+// exchanges between lane groups, and m, l and the rescaling are one value a lane.
+// V^T comes out of row-major V by the LDS transpose read (16-bit types); fp32
+// uses the 16x16x4 fp32 products, whose operand is one element a lane.
+//
+// Tiles of keys go global -> registers -> LDS, the loads of a tile being under
+// way while the one before is computed; 16-byte slots of a row are stored at
+// slot ^ (row % 16), which spreads both operands' reads over the banks.
+#pragma once
+
+#include "cbq_device.h"
+#include "cbq_paged.h"
+#include "../../include/cbq_serve.h"
+
+namespace cbq_attn {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kWaves = kAttnWaves, kThreads = kWaves * CBQ_WAVE;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct AttnArgs {
+    const void *q;
+    int64_t q_st[2];
+    cbq_paged_kv kv;
+    const int32_t *prefix_table, *tables, *lengths, *q_start;
+    int64_t table_st, capacity;             // own keys that a table row can name
+    void *out;
+    float *part_o;                          // [part][token][n_q][hd]
+    float2 *part_ml;                        // [part][token][n_q]: running maximum, sum
+    CbqDiv page;
+    int32_t prefix, batch, N, n_q, rep;
+    float c, q_mul;                         // exp2(c * (q_mul q) . k); q_mul folds scale's sign
+    Plan plan;
+};
+
+// ---- the matrix products of one type ---------------------------------------------
+template <typename T> struct Mma;
+template <> struct Mma<__bf16> {
+    static __device__ __forceinline__ f32x4 qk(u32x4 a, u32x4 b, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 pv16(u32x2 a, u32x2 b, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a),
+                                                         __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mma<_Float16> {
+    static __device__ __forceinline__ f32x4 qk(u32x4 a, u32x4 b, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 pv16(u32x2 a, u32x2 b, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a),
+                                                     __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mma<float> {
+    static __device__ __forceinline__ f32x4 qk(u32x4 a, u32x4 b, f32x4 c)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]),
+                                                     c, 0, 0, 0);
+        return c;
+    }
+};
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, t2{(T)a, (T)b});
+}
+
+// max / sum over the four lanes that hold one row (lane, lane ^ 16, ^ 32, ^ 48)
+__device__ __forceinline__ float groups_max(float x)
+{
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float groups_sum(float x)
+{
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// ---- geometry of a type and head size ---------------------------------------------
+template <typename T, int HD> struct Geo {
+    static constexpr int kEl = 16 / (int)sizeof(T);         // elements of a 16-byte slot
+    static constexpr int kSlots = HD / kEl;                 // slots of a row
+    static constexpr int kSwz = (kSlots < 16 ? kSlots : 16) - 1;
+    static constexpr int kQ = kSlots / 4;                   // slots of a query row a lane holds
+    static constexpr int kD = HD / 16;                      // 16-value pieces of a row
+    // keys of a block's tile (K and V, two buffers: 64 KiB at most) and of a
+    // wave's own tile (K and V, one buffer: 16 KiB, 32 KiB for fp32 rows of 256)
+    static constexpr int kBlockKeys = block_keys(HD * (int)sizeof(T));
+    static constexpr int kWaveKeys = wave_keys(HD * (int)sizeof(T));
+};
+
+// ---- a tile of keys and values: global -> registers -> LDS --------------------------
+// NT threads (a block or a wave) move KEYS rows of K and of V; `id` holds the
+// page ids of the tile that load() takes next, so a table entry is under way
+// while the tile before it is.
+template <typename T, int HD, int KEYS, int NT> struct Stage {
+    using G = Geo<T, HD>;
+    static constexpr int kRows = NT / G::kSlots, kPer = KEYS / kRows;
+    static_assert(NT % G::kSlots == 0 && KEYS % kRows == 0, "whole passes");
+    u32x4 k[kPer], v[kPer];
+    int32_t id[kPer], row[kPer];
+    uint32_t ok;                                            // bit i: pass i's key is there
+
+    __device__ __forceinline__ void look(const AttnArgs &a, const CbqKeys &keys, int32_t key0,
+                                         int tid)
+    {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int32_t *e = cbq_key_entry(keys, a.page, key0 + i * kRows + tid / G::kSlots,
+                                             row[i]);
+            id[i] = e ? *e : -1;
+        }
+    }
+    __device__ __forceinline__ void load(const AttnArgs &a, int h, int tid)
+    {
+        const int64_t at = tid % G::kSlots * G::kEl;
+        const T *kp = (const T *)a.kv.k + h * a.kv.k_stride[1] + at;
+        const T *vp = (const T *)a.kv.v + h * a.kv.v_stride[1] + at;
+        ok = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            // an id outside the pool (or no key) reads page 0, row 0 and becomes zeros
+            const bool in = id[i] >= 0 && id[i] < a.kv.n_pages;
+            ok |= (uint32_t)in << i;
+            const int64_t p = in ? id[i] : 0, r = in ? row[i] : 0;
+            k[i] = *(const u32x4 *)(kp + p * a.kv.k_stride[0] + r * a.kv.k_stride[2]);
+            v[i] = *(const u32x4 *)(vp + p * a.kv.v_stride[0] + r * a.kv.v_stride[2]);
+        }
+    }
+    // bias[key]: 0, or -inf for a key that is not there
+    __device__ __forceinline__ void store(u32x4 *K, u32x4 *V, float *bias, int tid)
+    {
+        const int slot = tid % G::kSlots;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int r = i * kRows + tid / G::kSlots;
+            const bool in = ok >> i & 1;
+            const int at = r * G::kSlots + (slot ^ (r & G::kSwz));
+            const u32x4 z = {0, 0, 0, 0};
+            K[at] = in ? k[i] : z;
+            V[at] = in ? v[i] : z;
+            if (slot == 0) bias[r] = in ? 0.f : -INFINITY;
+        }
+    }
+};
+
+// ---- RT x 16 query rows of one wave --------------------------------------------------
+template <typename T, int HD, int RT> struct Rows {
+    using G = Geo<T, HD>;
+    u32x4 q[RT][G::kQ];
+    f32x4 o[RT][G::kD];
+    float m[RT], l[RT];                     // m in exp2's domain; l: this lane's keys only
+    int32_t sees[RT];                       // keys of the joint axis that the row sees
+
+    // Rows first .. first + 16 RT - 1 of n; token0 is the token of row 0.
+    __device__ __forceinline__ void load(const AttnArgs &a, int h, int64_t token0, int first, int n)
+    {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int r = first + t * 16 + (lane & 15);
+            const int token = r / a.rep;
+            const T *x = (const T *)a.q + (token0 + token) * a.q_st[0] +
+                         (int64_t)(h * a.rep + r - token * a.rep) * a.q_st[1];
+#pragma unroll
+            for (int c = 0; c < G::kQ; c++) {
+                u32x4 w = {0, 0, 0, 0};
+                if (r < n) w = *(const u32x4 *)(x + (c * 4 + g) * G::kEl);
+                if (a.q_mul != 1.0f) {
+                    union { u32x4 u; T e[G::kEl]; } y = {w};
+#pragma unroll
+                    for (int i = 0; i < G::kEl; i++) y.e[i] = (T)((float)y.e[i] * a.q_mul);
+                    w = y.u;
+                }
+                q[t][c] = w;
+            }
+#pragma unroll
+            for (int d = 0; d < G::kD; d++) o[t][d] = f32x4{0, 0, 0, 0};
+            m[t] = -INFINITY;
+            l[t] = 0.f;
+        }
+    }
+
+    // One tile of KEYS keys, the first of them key0; MASK: a row sees keys
+    // below sees[] only.
+    template <int KEYS, bool MASK>
+    __device__ __forceinline__ void tile(const u32x4 *K, const u32x4 *V, const float *bias,
+                                         int32_t key0, float c)
+    {
+        constexpr int NK = KEYS / 16;
+        const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+        f32x4 s[RT][NK];
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            const f32x4 b = *(const f32x4 *)(bias + k * 16 + 4 * g);
+#pragma unroll
+            for (int t = 0; t < RT; t++) s[t][k] = b;
+#pragma unroll
+            for (int d = 0; d < G::kQ; d++) {
+                const u32x4 w = K[(k * 16 + r) * G::kSlots + ((d * 4 + g) ^ (r & G::kSwz))];
+#pragma unroll
+                for (int t = 0; t < RT; t++) s[t][k] = Mma<T>::qk(w, q[t][d], s[t][k]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            if (MASK) {
+#pragma unroll
+                for (int k = 0; k < NK; k++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (key0 + k * 16 + 4 * g + i >= sees[t]) s[t][k][i] = -INFINITY;
+            }
+            float top = s[t][0][0];
+#pragma unroll
+            for (int k = 0; k < NK; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) top = fmaxf(top, s[t][k][i]);
+            top = fmaxf(m[t], groups_max(top) * c);
+            const float base = top == -INFINITY ? 0.f : top;    // a row that has seen no key
+            if (__any(top > m[t])) {
+                const float f = __builtin_amdgcn_exp2f(m[t] - base);
+                l[t] *= f;
+#pragma unroll
+                for (int d = 0; d < G::kD; d++) o[t][d] *= f;
+                m[t] = top;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < NK; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    s[t][k][i] = __builtin_amdgcn_exp2f(fmaf(s[t][k][i], c, -base));
+                    sum += s[t][k][i];
+                }
+            l[t] += sum;
+        }
+        values<NK>(V, s);
+    }
+
+    template <int NK> __device__ __forceinline__ void values(const u32x4 *V, f32x4 (&s)[RT][NK])
+    {
+        const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+        if constexpr (sizeof(T) == 4) {
+            const float *F = (const float *)V;
+#pragma unroll
+            for (int k = 0; k < NK; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int key = k * 16 + 4 * g + i;
+#pragma unroll
+                    for (int d = 0; d < G::kD; d++) {
+                        const float w = F[(key * G::kSlots + ((d * 4 + (r >> 2)) ^ (key & G::kSwz)))
+                                          * 4 + (r & 3)];
+#pragma unroll
+                        for (int t = 0; t < RT; t++)
+                            o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, s[t][k][i], o[t][d],
+                                                                           0, 0, 0);
+                    }
+                }
+        } else {
+            // lane (g, r) points the transpose read at key 4g + r / 4, values
+            // 4 (r % 4) .. + 3 and gets keys 4g .. 4g + 3 of value r
+            const int key = 4 * g + (r >> 2), half = r & 1, sub = (r & 3) >> 1;
+            auto piece = [&](int k, int d) {
+                const int row = k * 16 + key;
+                const u32x4 *p = V + row * G::kSlots + ((d * 2 + sub) ^ (row & G::kSwz));
+                return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_s16x4 *)((const u32x2 *)p + half)));
+            };
+            if constexpr (NK % 2 == 0) {
+#pragma unroll
+                for (int k = 0; k < NK; k += 2) {
+                    u32x4 p[RT];
+#pragma unroll
+                    for (int t = 0; t < RT; t++)
+                        p[t] = u32x4{pack2<T>(s[t][k][0], s[t][k][1]),
+                                     pack2<T>(s[t][k][2], s[t][k][3]),
+                                     pack2<T>(s[t][k + 1][0], s[t][k + 1][1]),
+                                     pack2<T>(s[t][k + 1][2], s[t][k + 1][3])};
+#pragma unroll
+                    for (int d = 0; d < G::kD; d++) {
+                        const u32x2 x = piece(k, d), y = piece(k + 1, d);
+                        const u32x4 w = {x[0], x[1], y[0], y[1]};
+#pragma unroll
+                        for (int t = 0; t < RT; t++) o[t][d] = Mma<T>::qk(w, p[t], o[t][d]);
+                    }
+                }
+            } else {
+                static_assert(NK == 1, "one 16-key piece");
+#pragma unroll
+                for (int d = 0; d < G::kD; d++) {
+                    const u32x2 w = piece(0, d);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+                        const u32x2 p = {pack2<T>(s[t][0][0], s[t][0][1]),
+                                         pack2<T>(s[t][0][2], s[t][0][3])};
+                        o[t][d] = Mma<T>::pv16(w, p, o[t][d]);
+                    }
+                }
+            }
+        }
+    }
+};
+
+// Four values of a row, at hd position d: into the output (part < 0, with the
+// row's sum) or a part's sums.
+template <typename T, int HD>
+__device__ __forceinline__ void put_values(const AttnArgs &a, int part, int64_t token, int head, int d,
+                                           f32x4 x, float sum)
+{
+    const int64_t row = token * a.n_q + head;
+    if (part >= 0) {
+        *(f32x4 *)(a.part_o + ((int64_t)part * a.N * a.n_q + row) * HD + d) = x;
+        return;
+    }
+    const float f = sum == 0.f ? 0.f : 1.0f / sum;
+    x *= f;
+    T *y = (T *)a.out + row * HD + d;
+    if constexpr (sizeof(T) == 4) *(f32x4 *)y = x;
+    else *(u32x2 *)y = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+}
+
+__device__ __forceinline__ void put_stats(const AttnArgs &a, int part, int64_t token, int head,
+                                          float m, float l)
+{
+    if (part >= 0) a.part_ml[((int64_t)part * a.N + token) * a.n_q + head] = make_float2(m, l);
+}
+
+// ---- 64 RT rows of a block against keys [first, end), tiles shared by the waves ----------
+template <typename T, int HD, int RT, bool CAUSAL>
+__device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, int64_t token0,
+                                           int row0, int n, const CbqKeys &keys, int32_t first,
+                                           int32_t past, int part)
+{
+    using G = Geo<T, HD>;
+    constexpr int KEYS = G::kBlockKeys, kTile = KEYS * G::kSlots;
+    u32x4 *K = (u32x4 *)lds, *V = K + 2 * kTile;
+    float *bias = (float *)(V + 2 * kTile);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int mine = row0 + wave * 16 * RT;
+    Rows<T, HD, RT> w;
+    Stage<T, HD, KEYS, kThreads> st;
+    st.look(a, keys, first, tid);
+    w.load(a, h, token0, mine, n);
+    int32_t all = INT32_MAX;                    // keys that every row of the block sees
+    if (CAUSAL) {
+        all = keys.prefix + (past + row0 / a.rep + 1 > 0 ? past + row0 / a.rep + 1 : 0);
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int32_t own = past + (mine + t * 16 + (lane & 15)) / a.rep + 1;
+            w.sees[t] = keys.prefix + (own > 0 ? own : 0);
+        }
+    }
+    const int tiles = keys.end > first ? (keys.end - first + KEYS - 1) / KEYS : 0;
+    if (tiles > 0) {
+        st.load(a, h, tid);
+        st.look(a, keys, first + KEYS, tid);
+        st.store(K, V, bias, tid);
+        st.load(a, h, tid);
+        st.look(a, keys, first + 2 * KEYS, tid);
+        __syncthreads();
+        for (int i = 0; i < tiles; i++) {
+            const int b = i & 1;
+            const int32_t key0 = first + i * KEYS;
+            if (CAUSAL && key0 + KEYS > all)
+                w.template tile<KEYS, true>(K + b * kTile, V + b * kTile, bias + b * KEYS, key0, a.c);
+            else
+                w.template tile<KEYS, false>(K + b * kTile, V + b * kTile, bias + b * KEYS, key0, a.c);
+            if (i + 1 < tiles) {
+                st.store(K + (b ^ 1) * kTile, V + (b ^ 1) * kTile, bias + (b ^ 1) * KEYS, tid);
+                st.load(a, h, tid);
+                st.look(a, keys, first + (i + 3) * KEYS, tid);
+            }
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int r = mine + t * 16 + (lane & 15);
+        const float l = groups_sum(w.l[t]);
+        if (r >= n) continue;
+        const int64_t token = token0 + r / a.rep;
+        const int head = h * a.rep + r % a.rep;
+#pragma unroll
+        for (int d = 0; d < G::kD; d++)
+            put_values<T, HD>(a, part, token, head, d * 16 + 4 * (lane >> 4), w.o[t][d], l);
+        if (lane < 16) put_stats(a, part, token, head, w.m[t], l);
+    }
+}
+
+// ---- 16 rows of a block, the keys [first, end) dealt to its waves ------------------------
+// For few rows: each wave walks tiles of its own through its own LDS without a
+// barrier, and the four running states are merged at the end.
+template <typename T, int HD, bool CAUSAL>
+__device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, int64_t token0,
+                                          int row0, int n, const CbqKeys &keys, int32_t first,
+                                          int32_t past, int part)
+{
+    using G = Geo<T, HD>;
+    constexpr int KEYS = G::kWaveKeys, kTile = KEYS * G::kSlots;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int g = lane >> 4, r = lane & 15;
+    u32x4 *K = (u32x4 *)lds + wave * 2 * kTile, *V = K + kTile;
+    float *bias = (float *)((u32x4 *)lds + kWaves * 2 * kTile) + wave * KEYS;
+    Rows<T, HD, 1> w;
+    Stage<T, HD, KEYS, CBQ_WAVE> st;
+    st.look(a, keys, first + wave * KEYS, lane);
+    w.load(a, h, token0, row0, n);
+    int32_t all = INT32_MAX;
+    if (CAUSAL) {
+        all = keys.prefix + (past + row0 / a.rep + 1 > 0 ? past + row0 / a.rep + 1 : 0);
+        const int32_t own = past + (row0 + r) / a.rep + 1;
+        w.sees[0] = keys.prefix + (own > 0 ? own : 0);
+    }
+    const int32_t begin = first + wave * KEYS, step = kWaves * KEYS;
+    if (begin < keys.end) {
+        st.load(a, h, lane);
+        st.look(a, keys, begin + step, lane);
+    }
+    for (int32_t key0 = begin; key0 < keys.end; key0 += step) {
+        st.store(K, V, bias, lane);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (key0 + step < keys.end) {
+            st.load(a, h, lane);
+            st.look(a, keys, key0 + 2 * step, lane);
+        }
+        if (CAUSAL && key0 + KEYS > all) w.template tile<KEYS, true>(K, V, bias, key0, a.c);
+        else w.template tile<KEYS, false>(K, V, bias, key0, a.c);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    // merge: statistics first, then the weighted values, each wave's scaled to
+    // the common maximum
+    __syncthreads();                            // every wave is past its tiles
+    float *O = (float *)lds, *ML = O + kWaves * 16 * HD;
+    const float l = groups_sum(w.l[0]);
+    if (lane < 16) {
+        ML[(wave * 16 + r) * 2] = w.m[0];
+        ML[(wave * 16 + r) * 2 + 1] = l;
+    }
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) top = fmaxf(top, ML[(i * 16 + r) * 2]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int i = 0; i < kWaves; i++)
+        sum += __builtin_amdgcn_exp2f(ML[(i * 16 + r) * 2] - base) * ML[(i * 16 + r) * 2 + 1];
+    const float f = __builtin_amdgcn_exp2f(w.m[0] - base);
+    // row r's pieces at (piece ^ r): 16 rows of one piece would share their banks
+#pragma unroll
+    for (int d = 0; d < G::kD; d++)
+        *(f32x4 *)(O + (wave * 16 + r) * HD + (((d * 4 + g) ^ r) & (HD / 4 - 1)) * 4) = w.o[0][d] * f;
+    if (wave == 0 && lane < 16) ML[kWaves * 32 + r] = sum;
+    __syncthreads();
+    const int rows = n - row0 < 16 ? n - row0 : 16;
+    for (int e = tid; e < rows * (HD / 4); e += kThreads) {
+        const int rr = e / (HD / 4), d = e % (HD / 4);
+        f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < kWaves; i++)
+            x += *(const f32x4 *)(O + (i * 16 + rr) * HD + ((d ^ rr) & (HD / 4 - 1)) * 4);
+        const int token = (row0 + rr) / a.rep;
+        put_values<T, HD>(a, part, token0 + token, h * a.rep + row0 + rr - token * a.rep, d * 4, x,
+                          ML[kWaves * 32 + rr]);
+    }
+    if (wave == 0 && lane < rows) {
+        const int token = (row0 + r) / a.rep;
+        put_stats(a, part, token0 + token, h * a.rep + row0 + r - token * a.rep, top, sum);
+    }
+}
+
+template <typename T, int HD> constexpr int wave_lds()
+{
+    using G = Geo<T, HD>;
+    constexpr int tiles = kWaves * (2 * G::kWaveKeys * G::kSlots * 16 + G::kWaveKeys * 4);
+    constexpr int merge = kWaves * 16 * HD * 4 + kWaves * 16 * 8 + 16 * 4;
+    return tiles > merge ? tiles : merge;
+}
+template <typename T, int HD> constexpr int block_lds()
+{
+    using G = Geo<T, HD>;
+    return 4 * G::kBlockKeys * G::kSlots * 16 + 2 * G::kBlockKeys * 4;
+}
+
+// ---- decode: parts of the prefix for all sequences, parts of each one's own keys ------------
+// PT: 64 PT prefix rows a block; 0: the prefix rows are 16 at most and go as the
+// own ones do.
+template <typename T, int HD, int PT>
+__global__ __launch_bounds__(kThreads, 1) void decode_kernel(AttnArgs a)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const DecodeWork w = decode_work(a.plan, blockIdx.x, a.kv.n_kv, a.batch, a.prefix, a.lengths,
+                                     a.capacity);
+    if (w.skip) return;                             // the merge counts own parts by the length
+    const int to = a.plan.parts > 1 ? w.part : -1;
+    if (w.seq < 0) {
+        const CbqKeys keys = {a.prefix_table, nullptr, a.prefix, w.end};
+        const int rows = a.batch * a.rep;
+        if constexpr (PT > 0)
+            block_rows<T, HD, PT, false>(a, lds, w.h, 0, w.tile * 64 * PT, rows, keys, w.first, 0, to);
+        else
+            wave_rows<T, HD, false>(a, lds, w.h, 0, w.tile * 16, rows, keys, w.first, 0, to);
+        return;
+    }
+    const CbqKeys keys = {nullptr, a.tables + w.seq * a.table_st, 0, w.end};
+    wave_rows<T, HD, false>(a, lds, w.h, w.seq, w.tile * 16, a.rep, keys, w.first, 0, to);
+}
+
+// ---- prompt: tiles of each run's rows against the keys they see -----------------------------
+// RT: 64 RT rows a block; 0: 16 rows.
+template <typename T, int HD, int RT>
+__global__ __launch_bounds__(kThreads, 1) void prompt_kernel(AttnArgs a)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int M = RT ? 64 * RT : 16;
+    const int lane = threadIdx.x & 63, n_kv = a.kv.n_kv;
+    uint32_t i = blockIdx.x;
+    const int h = i % n_kv;
+    i /= n_kv;
+    const int part = i % a.plan.parts;
+    // later tiles of a run see more keys: they start first
+    int32_t want = a.plan.tiles - 1 - (int32_t)(i / a.plan.parts);
+    if (blockIdx.x == 0) {                          // tokens of no run
+        const int64_t lo = cbq_clamp_length(a.q_start[0], a.N),
+                      hi = cbq_max(cbq_clamp_length(a.q_start[a.batch], a.N), lo);
+        T *out = (T *)a.out;
+        const int64_t w = (int64_t)a.n_q * HD;
+        for (int64_t e = threadIdx.x; e < (lo + a.N - hi) * w; e += kThreads)
+            out[e < lo * w ? e : e + (hi - lo) * w] = (T)0.f;
+    }
+    // the run that holds tile `want`: its count of tiles, summed over the runs
+    int32_t before = 0, run = -1, tile = 0, first_token = 0, count = 0;
+    for (int b0 = 0; b0 < a.batch && run < 0; b0 += CBQ_WAVE) {
+        int32_t f = 0, n = 0;
+        if (b0 + lane < a.batch) cbq_run(a.q_start, b0 + lane, a.N, f, n);
+        const int32_t mine = (int32_t)(((int64_t)n * a.rep + M - 1) / M);
+        int32_t upto = mine;
+        for (int o = 1; o < CBQ_WAVE; o <<= 1) {
+            const int32_t x = __shfl_up(upto, o);
+            if (lane >= o) upto += x;
+        }
+        const uint64_t over = __ballot(before + upto > want);
+        if (over) {
+            const int at = __builtin_ctzll(over);
+            run = b0 + at;
+            tile = want - before - __shfl(upto - mine, at);
+            first_token = __shfl(f, at);
+            count = __shfl(n, at);
+        } else {
+            before += __shfl(upto, CBQ_WAVE - 1);
+        }
+    }
+    run = __builtin_amdgcn_readfirstlane(run);
+    if (run < 0) return;                            // fewer tiles than the grid allows for
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    first_token = __builtin_amdgcn_readfirstlane(first_token);
+    count = __builtin_amdgcn_readfirstlane(count);
+    const int32_t len = cbq_clamp_length(a.lengths[run], a.capacity), past = len - count;
+    const int rows = count * a.rep, row0 = tile * M;
+    const int last = (row0 + M < rows ? row0 + M : rows) - 1;
+    const int32_t own = past + last / a.rep + 1;
+    const int32_t sees = a.prefix + (own > 0 ? own : 0);        // of the tile's last row
+    int32_t first = 0, end = sees;
+    if (a.plan.parts > 1)
+        prompt_keys(sees, a.plan.parts, part,
+                    RT ? Geo<T, HD>::kBlockKeys : Geo<T, HD>::kWaveKeys, first, end);
+    const CbqKeys keys = {a.prefix_table, a.tables + run * a.table_st, a.prefix, end};
+    if constexpr (RT > 0)
+        block_rows<T, HD, RT, true>(a, lds, h, first_token, row0, rows, keys, first, past,
+                                    a.plan.parts > 1 ? part : -1);
+    else
+        wave_rows<T, HD, true>(a, lds, h, first_token, row0, rows, keys, first, past,
+                               a.plan.parts > 1 ? part : -1);
+}
+
+// ---- merge of the parts: a wave a (token, head) ----------------------------------------------
+template <typename T, int HD> __global__ __launch_bounds__(kThreads) void merge_kernel(AttnArgs a)
+{
+    constexpr int V = HD / CBQ_WAVE;
+    const int64_t row = (int64_t)blockIdx.x * kWaves + threadIdx.x / CBQ_WAVE;
+    const int64_t rows = (int64_t)a.N * a.n_q;
+    const int lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    const int64_t token = row / a.n_q;
+    int parts = a.plan.parts;
+    if (a.plan.own_chunk > 0) {                          // decode: as many own parts as the length has
+        const int32_t len = cbq_clamp_length(a.lengths[token], a.capacity);
+        parts = a.plan.pre_parts + (int)cbq_ceil(len, a.plan.own_chunk);
+    } else {                                        // prompt: a token of no run keeps its zeros
+        if (token < a.q_start[0] || token >= a.q_start[a.batch]) return;
+    }
+    float top = -INFINITY, sum = 0.f, x[V] = {};
+    for (int p0 = 0; p0 < parts; p0 += CBQ_WAVE) {
+        const int n = parts - p0 < CBQ_WAVE ? parts - p0 : CBQ_WAVE;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < n) ml = a.part_ml[(p0 + lane) * rows + row];
+        float now = ml.x;
+        for (int o = 32; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor(now, o));
+        now = fmaxf(now, top);
+        const float base = now == -INFINITY ? 0.f : now;
+        const float f = __builtin_amdgcn_exp2f(top - base), w = __builtin_amdgcn_exp2f(ml.x - base);
+        float s = w * ml.y;                         // 0 of an empty part; a NaN stays
+        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+        sum = sum * f + s;
+        top = now;
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] *= f;
+        const float *o = a.part_o + (p0 * rows + row) * HD + lane * V;
+#pragma unroll 8
+        for (int p = 0; p < n; p++) {
+            const float wp = __shfl(w, p);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float y = o[p * rows * HD + i];       // unwritten where the part saw no key
+                x[i] = wp == 0.f ? x[i] : fmaf(wp, y, x[i]);
+            }
+        }
+    }
+    const float f = sum == 0.f ? 0.f : 1.0f / sum;
+    T *y = (T *)a.out + row * HD + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; i++) y[i] = (T)(x[i] * f);
+}
+
+// ---- launches of one type -------------------------------------------------------------------
+template <typename K> int run_kernel(K kernel, int64_t blocks, int lds, const AttnArgs &a,
+                                     hipStream_t stream, const char *what)
+{
+    if (lds > 65536 &&
+        hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) !=
+            hipSuccess)
+        return cbq_launch_status(what);
+    kernel<<<dim3((unsigned)blocks), dim3(kThreads), lds, stream>>>(a);
+    return cbq_launch_status(what);
+}
+
+template <typename T, int HD> int launch(const AttnArgs &a, const Plan &p, bool prompt,
+                                         hipStream_t stream)
+{
+    constexpr int wl = wave_lds<T, HD>(), bl = block_lds<T, HD>(), both = wl > bl ? wl : bl;
+    constexpr int wide = widest(HD * (int)sizeof(T));
+    int rc;
+    if (prompt) {
+        const char *what = "cbq_prefix_attn_prompt";
+        if (p.rt == 0) rc = run_kernel(prompt_kernel<T, HD, 0>, p.blocks, wl, a, stream, what);
+        else if (p.rt == 1) rc = run_kernel(prompt_kernel<T, HD, 1>, p.blocks, bl, a, stream, what);
+        else rc = run_kernel(prompt_kernel<T, HD, wide>, p.blocks, bl, a, stream, what);
+    } else {
+        const char *what = "cbq_prefix_attn_decode";
+        if (p.rt == 0 || !p.pre_parts)
+            rc = run_kernel(decode_kernel<T, HD, 0>, p.blocks, wl, a, stream, what);
+        else if (p.rt == 1) rc = run_kernel(decode_kernel<T, HD, 1>, p.blocks, both, a, stream, what);
+        else rc = run_kernel(decode_kernel<T, HD, wide>, p.blocks, both, a, stream, what);
+    }
+    if (rc != CK_SUCCESS || p.parts == 1) return rc;
+    return run_kernel(merge_kernel<T, HD>, cbq_ceil((int64_t)a.N * a.n_q, kWaves), 0, a, stream,
+                      "cbq_prefix_attn merge");
+}
+
+template <typename T> int launch_hd(const AttnArgs &a, const Plan &p, bool prompt,
+                                    hipStream_t stream)
+{
+    switch (a.kv.hd) {
+    case 64: return launch<T, 64>(a, p, prompt, stream);
+    case 128: return launch<T, 128>(a, p, prompt, stream);
+    default: return launch<T, 256>(a, p, prompt, stream);
+    }
+}
+
+int launch_f32(const AttnArgs &a, const Plan &p, bool prompt, hipStream_t stream);
+int launch_bf16(const AttnArgs &a, const Plan &p, bool prompt, hipStream_t stream);
+int launch_f16(const AttnArgs &a, const Plan &p, bool prompt, hipStream_t stream);
+
+}  // namespace cbq_attn

@@ -1,0 +1,11 @@
+// cbq_prefix_attn.h's kernels for f32 caches.
+#include "cbq_prefix_attn.h"
+
+namespace cbq_attn {
+
+int launch_f32(const AttnArgs &a, const Plan &p, bool prompt, hipStream_t stream)
+{
+    return launch_hd<float>(a, p, prompt, stream);
+}
+
+}  // namespace cbq_attn

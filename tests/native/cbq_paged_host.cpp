@@ -1,0 +1,183 @@
+// The paged cache's addresses and the attention's launch plans
+// (csrc/cbq_paged.h, the code that the kernels run) on the CPU, under address
+// and undefined-behaviour sanitizers: division, table entries of every key a
+// block walks (tables allocated to the entry), every (row, key) visited once,
+// parts inside the workspace, lengths, runs and page ids that are out of range.
+#include <stdio.h>
+#include <stdlib.h>
+
+#include <map>
+#include <random>
+#include <vector>
+
+#include "../../codebook-quantization_amd/csrc/cbq_paged.h"
+
+using namespace cbq_attn;
+
+static std::mt19937 rng(7);
+static int64_t pick(int64_t lo, int64_t hi) { return lo + (int64_t)(rng() % (uint64_t)(hi - lo + 1)); }
+
+#define CHECK(c) do { if (!(c)) { printf("line %d: %s\n", __LINE__, #c); exit(1); } } while (0)
+
+static void divisions()
+{
+    for (uint32_t d = 1; d <= 65536; d = d < 300 ? d + 1 : d + 1 + rng() % 257) {
+        const CbqDiv q = cbq_div_make(d);
+        const uint32_t near[] = {0, 1, d - 1, d, d + 1, 0x7fffffffu, 0x7fffffffu / d * d,
+                                 0x7fffffffu / d * d - 1, 0x7ffffffeu};
+        for (uint32_t n : near)
+            if (n < 0x80000000u) CHECK(cbq_div(n, q) == n / d);
+        for (int i = 0; i < 200; i++) {
+            const uint32_t n = rng() & 0x7fffffffu;
+            CHECK(cbq_div(n, q) == n / d);
+        }
+    }
+    for (uint32_t d : {65537u, 1000003u, 0x7fffffffu, 0x40000000u, 0x40000001u}) {
+        const CbqDiv q = cbq_div_make(d);
+        for (uint32_t n : {0u, 1u, d - 1, d, d + 1, 0x7fffffffu, 0x7ffffffeu})
+            if (n < 0x80000000u) CHECK(cbq_div(n, q) == n / d);
+    }
+}
+
+// The keys that a block's tiles and their look-ahead touch; those inside are counted.
+static void walk(const CbqKeys &keys, const CbqDiv &page, int32_t first, int step,
+                 const std::vector<int32_t> &prefix_table, const int32_t *own, int width,
+                 std::vector<int> &seen)
+{
+    for (int64_t j = first; j < (int64_t)keys.end + 3 * step; j++) {
+        int32_t row;
+        const int32_t *e = cbq_key_entry(keys, page, (int32_t)j, row);
+        CHECK((e != nullptr) == (j < keys.end));
+        if (!e) continue;
+        const int64_t i = j < keys.prefix ? j : j - keys.prefix;
+        const int32_t *base = j < keys.prefix ? prefix_table.data() : own;
+        CHECK(e == base + i / page.d && row == (int32_t)(i % page.d));
+        CHECK(j >= keys.prefix || e < prefix_table.data() + prefix_table.size());
+        CHECK(j < keys.prefix || e < own + width);
+        volatile int32_t id = *e;
+        (void)id;
+        seen[j]++;
+    }
+}
+
+static void decode()
+{
+    const int hds[] = {64, 128, 256}, pages[] = {1, 3, 16, 17, 64, 256};
+    const int hd = hds[pick(0, 2)], size = pick(0, 1) ? 2 : 4, page = pages[pick(0, 5)];
+    const int n_kv = pick(1, 3), rep = pick(1, 40), batch = pick(1, 40), width = pick(0, 3000 / page);
+    const int prefix = pick(0, 2) ? pick(1, 4000) : 0;
+    const int64_t capacity = (int64_t)width * page;
+    std::vector<int32_t> prefix_table(cbq_ceil(prefix, page)), tables((size_t)batch * width),
+        lengths(batch);
+    for (auto &x : lengths) x = pick(0, 5) ? pick(0, capacity) : pick(0, 1) ? -5 : 1 << 30;
+    const Plan p = plan_decode(hd * size, hd, n_kv, rep, prefix, capacity, batch);
+    CHECK(plan_fits(p));
+    CHECK(p.bytes == (p.parts > 1 ? (int64_t)p.parts * batch * n_kv * rep * (hd + 2) * 4 : 0));
+    const CbqDiv pg = cbq_div_make(page);
+    // [kv head][row tile of 16 or 64 rt rows][key] for the prefix and each sequence
+    std::map<std::vector<int>, std::vector<int>> seen;
+    std::map<std::vector<int>, int> parts;
+    const int m = p.rt ? 64 * p.rt : 16, step = p.rt ? block_keys(hd * size) : wave_keys(hd * size) * kAttnWaves;
+    for (int64_t i = 0; i < p.blocks; i++) {
+        const DecodeWork w = decode_work(p, (uint32_t)i, n_kv, batch, prefix, lengths.data(), capacity);
+        CHECK(w.h >= 0 && w.h < n_kv);
+        if (w.seq < 0) {
+            CHECK(w.tile >= 0 && w.tile * m < batch * rep && w.part >= 0 && w.part < p.pre_parts);
+            auto &s = seen[{w.h, -1, w.tile}];
+            s.resize(prefix);
+            walk({prefix_table.data(), nullptr, prefix, w.end}, pg, w.first, step, prefix_table, nullptr, 0, s);
+        } else {
+            CHECK(w.seq < batch && w.tile * 16 < rep);
+            if (w.skip) continue;
+            CHECK(w.part >= p.pre_parts && w.part < p.parts);
+            const int32_t *own = tables.data() + (size_t)w.seq * width;
+            auto &s = seen[{w.h, w.seq, w.tile}];
+            s.resize(capacity);
+            walk({nullptr, own, 0, w.end}, pg, w.first, step, prefix_table, own, width, s);
+            parts[{w.h, w.seq, w.tile}]++;
+        }
+    }
+    for (int h = 0; h < n_kv; h++) {
+        for (int t = 0; prefix && t * m < batch * rep; t++)
+            for (int x : seen[{h, -1, t}]) CHECK(x == 1);
+        for (int b = 0; b < batch; b++)
+            for (int t = 0; t * 16 < rep; t++) {
+                const int32_t len = cbq_clamp_length(lengths[b], capacity);
+                auto &s = seen[{h, b, t}];
+                for (int j = 0; j < (int)s.size(); j++) CHECK(s[j] == (j < len));
+                CHECK(len == 0 || (int)s.size() == capacity);
+                // what the merge counts (a lone part always writes the output)
+                const int want = p.parts == 1 ? (p.pre_parts ? 0 : 1) : (int)cbq_ceil(len, p.own_chunk);
+                CHECK((parts[{h, b, t}]) == want);
+            }
+    }
+}
+
+static void prompt()
+{
+    const int hds[] = {64, 128, 256};
+    const int hd = hds[pick(0, 2)], size = pick(0, 1) ? 2 : 4, n_kv = pick(1, 4), rep = pick(1, 40);
+    const int batch = pick(1, 70), width = pick(0, 300), page = 16;
+    const int prefix = pick(0, 1) ? pick(1, 4000) : 0;
+    std::vector<int32_t> q_start(batch + 1);
+    for (int b = 0; b < batch; b++) q_start[b + 1] = q_start[b] + (pick(0, 4) ? pick(0, 90) : 0);
+    const int N = q_start[batch] + 1;
+    const Plan p = plan_prompt(hd * size, hd, n_kv, rep, prefix, (int64_t)width * page, batch, N);
+    CHECK(plan_fits(p));
+    const int m = p.rt ? 64 * p.rt : 16;
+    int64_t tiles = 0;
+    for (int b = 0; b < batch; b++) {
+        int32_t f, n;
+        cbq_run(q_start.data(), b, N, f, n);
+        CHECK(f == q_start[b] && n == q_start[b + 1] - q_start[b]);
+        tiles += cbq_ceil((int64_t)n * rep, m);
+    }
+    CHECK(tiles <= p.tiles && p.blocks == (int64_t)p.tiles * n_kv * p.parts);
+    for (int sees : {0, 1, 63, 64, 65, 1000, prefix + width * page}) {
+        int32_t at = 0;
+        for (int i = 0; i < p.parts; i++) {
+            int32_t first, end;
+            prompt_keys(sees, p.parts, i, p.rt ? block_keys(hd * size) : wave_keys(hd * size), first, end);
+            CHECK(first == at && end >= first && end <= sees);
+            at = end;
+        }
+        CHECK(at == sees);
+    }
+    // starts in no order and out of range stay inside the tokens
+    for (auto &x : q_start) x = (int32_t)rng();
+    for (int b = 0; b < batch; b++) {
+        int32_t f, n;
+        cbq_run(q_start.data(), b, N, f, n);
+        CHECK(f >= 0 && n >= 0 && f + n <= N);
+    }
+}
+
+static void far()
+{
+    // the largest axis: indexes near 2^31, and a look-ahead past the end
+    const int64_t most = (1ll << 31) - 65536;
+    const CbqDiv page = cbq_div_make(65536);
+    std::vector<int32_t> t(cbq_ceil(most, 65536));
+    std::vector<int> none;
+    for (int64_t j : {most - 1, most, most + 4000}) {
+        int32_t row;
+        const int32_t *e = cbq_key_entry({nullptr, t.data(), 0, (int32_t)most}, page, (int32_t)j, row);
+        CHECK((e != nullptr) == (j < most));
+        if (e) CHECK(e == &t.back() && row == (int32_t)((most - 1) % 65536));
+    }
+    const Plan p = plan_decode(256, 128, 8, 4, most / 2, most / 2, 1);
+    CHECK(p.pre_parts > 0 && p.pre_chunk > 0 && (int64_t)p.pre_parts * p.pre_chunk >= most / 2);
+    int32_t first, end;
+    prompt_keys((int32_t)most, 1000, 999, 64, first, end);
+    CHECK(end == most && first < end);
+}
+
+int main()
+{
+    divisions();
+    far();
+    for (int i = 0; i < 150; i++) decode();
+    for (int i = 0; i < 400; i++) prompt();
+    printf("all cases passed\n");
+    return 0;
+}
