@@ -38,19 +38,36 @@ struct CbqKeys {
     int32_t prefix, end;
 };
 
-// Table entry of key j, or null where there is none (j outside [0, end)).
-CBQ_PAGED_FN const int32_t *cbq_key_entry(const CbqKeys &a, const CbqDiv &page, int32_t j,
-                                          int32_t &row)
+// Key j's entry in the table of its kind and its row in that page; 0, 0 for a
+// key outside [0, end).
+CBQ_PAGED_FN void cbq_key_place(const CbqKeys &a, const CbqDiv &page, int32_t j, int32_t &entry,
+                                int32_t &row)
 {
+    const bool in = j >= 0 && j < a.end;
+    const uint32_t i = in ? (uint32_t)(j < a.prefix ? j : j - a.prefix) : 0;
+    entry = (int32_t)cbq_div(i, page);
+    row = (int32_t)(i - (uint32_t)entry * page.d);
+}
+
+// From key j >= 0 to key j + step, step = step_entry * page + step_row; j, entry
+// and row stay where they are at the end or past it.
+CBQ_PAGED_FN void cbq_key_advance(const CbqKeys &a, const CbqDiv &page, int32_t step,
+                                  int32_t step_entry, int32_t step_row, int32_t &j, int32_t &entry,
+                                  int32_t &row)
+{
+    if (j >= a.end) return;
     const bool shared = j < a.prefix;
-    const uint32_t i = (uint32_t)(shared ? j : j - a.prefix);
-    if (j < 0 || j >= a.end) {
-        row = 0;
-        return nullptr;
+    j += step;
+    if (shared && j >= a.prefix) {              // from the prefix's table to the own one
+        cbq_key_place(a, page, j, entry, row);
+        return;
     }
-    const uint32_t e = cbq_div(i, page);
-    row = (int32_t)(i - e * page.d);
-    return (shared ? a.shared : a.own) + e;
+    entry += step_entry;
+    row += step_row;
+    if (row >= (int32_t)page.d) {
+        row -= (int32_t)page.d;
+        entry++;
+    }
 }
 
 CBQ_PAGED_FN int32_t cbq_clamp_length(int32_t n, int64_t capacity)

@@ -54,6 +54,7 @@ struct AttnArgs {
     float2 *part_ml;                        // [part][token][n_q]: running maximum, sum
     CbqDiv page;
     int32_t prefix, batch, N, n_q, rep;
+    int32_t one_stride;                     // keys and values lie alike
     float c, q_mul;                         // exp2(c * (q_mul q) . k); q_mul folds scale's sign
     Plan plan;
 };
@@ -131,57 +132,93 @@ template <typename T, int HD> struct Geo {
 };
 
 // ---- a tile of keys and values: global -> registers -> LDS --------------------------
-// NT threads (a block or a wave) move KEYS rows of K and of V; `id` holds the
-// page ids of the tile that load() takes next, so a table entry is under way
-// while the tile before it is.
+// NT threads (a block or a wave) move KEYS rows of K and of V.  A row's slots are
+// read by neighbouring lanes; its address is found once, by one lane of the wave
+// that reads it (a wave's keys of a tile are 64 at most), and comes to the others
+// by a shuffle: page arithmetic in every lane cost more than the products.  A key's
+// table entry and row in its page advance with the tiles by additions, and the entry
+// of the next tile is under way while a tile is.
 template <typename T, int HD, int KEYS, int NT> struct Stage {
     using G = Geo<T, HD>;
-    static constexpr int kRows = NT / G::kSlots, kPer = KEYS / kRows;
-    static_assert(NT % G::kSlots == 0 && KEYS % kRows == 0, "whole passes");
+    static constexpr int kRows = NT / G::kSlots, kPer = KEYS / kRows;   // rows a pass, passes
+    static constexpr int kWide = CBQ_WAVE / G::kSlots, kMine = kPer * kWide;    // of a wave
+    static_assert(kRows * kPer == KEYS && kWide * G::kSlots == CBQ_WAVE && kMine <= CBQ_WAVE,
+                  "whole passes, a key a lane");
     u32x4 k[kPer], v[kPer];
-    int32_t id[kPer], row[kPer];
-    uint32_t ok;                                            // bit i: pass i's key is there
+    uint64_t there;                         // the wave's keys of the loaded tile that are there
+    int32_t key, entry, row, id;            // this lane's key: of the next tile
+    int32_t step, step_entry, step_row;
+    int at;                                 // the key's place in a tile
 
-    __device__ __forceinline__ void look(const AttnArgs &a, const CbqKeys &keys, int32_t key0,
-                                         int tid)
+    // The walk starts at `first` and goes on in steps of `by` keys.
+    __device__ __forceinline__ void start(const AttnArgs &a, const CbqKeys &keys, int32_t first,
+                                          int32_t by)
     {
-#pragma unroll
-        for (int i = 0; i < kPer; i++) {
-            const int32_t *e = cbq_key_entry(keys, a.page, key0 + i * kRows + tid / G::kSlots,
-                                             row[i]);
-            id[i] = e ? *e : -1;
-        }
+        const int lane = threadIdx.x & 63, wave = NT == CBQ_WAVE ? 0 : threadIdx.x >> 6;
+        at = lane / kWide * kRows + wave * kWide + lane % kWide;
+        if (lane >= kMine) at = -1;
+        step = by;
+        step_entry = (int32_t)cbq_div((uint32_t)by, a.page);
+        step_row = by - step_entry * (int32_t)a.page.d;
+        key = at < 0 ? -1 : first + at;
+        cbq_key_place(keys, a.page, key, entry, row);
+        look(keys);
     }
-    __device__ __forceinline__ void load(const AttnArgs &a, int h, int tid)
+    __device__ __forceinline__ void look(const CbqKeys &keys)
     {
-        const int64_t at = tid % G::kSlots * G::kEl;
-        const T *kp = (const T *)a.kv.k + h * a.kv.k_stride[1] + at;
-        const T *vp = (const T *)a.kv.v + h * a.kv.v_stride[1] + at;
-        ok = 0;
+        id = -1;
+        if (key >= 0 && key < keys.end) id = (key < keys.prefix ? keys.shared : keys.own)[entry];
+    }
+    // Loads the tile and moves on to the next one's table entries.
+    __device__ __forceinline__ void load(const AttnArgs &a, const CbqKeys &keys, int h)
+    {
+        const int lane = threadIdx.x & 63, from = lane / G::kSlots;
+        const int64_t slot = lane % G::kSlots * G::kEl;
+        const T *kp = (const T *)a.kv.k + h * a.kv.k_stride[1] + slot;
+        const T *vp = (const T *)a.kv.v + h * a.kv.v_stride[1] + slot;
+        // an id outside the pool (or no key) reads page 0, row 0 and becomes zeros
+        const bool in = id >= 0 && id < a.kv.n_pages;
+        there = __ballot(in);
+        const int64_t p = in ? id : 0, r = in ? row : 0;
+        const int64_t ko = p * a.kv.k_stride[0] + r * a.kv.k_stride[2];
 #pragma unroll
-        for (int i = 0; i < kPer; i++) {
-            // an id outside the pool (or no key) reads page 0, row 0 and becomes zeros
-            const bool in = id[i] >= 0 && id[i] < a.kv.n_pages;
-            ok |= (uint32_t)in << i;
-            const int64_t p = in ? id[i] : 0, r = in ? row[i] : 0;
-            k[i] = *(const u32x4 *)(kp + p * a.kv.k_stride[0] + r * a.kv.k_stride[2]);
-            v[i] = *(const u32x4 *)(vp + p * a.kv.v_stride[0] + r * a.kv.v_stride[2]);
+        for (int i = 0; i < kPer; i++) k[i] = *(const u32x4 *)(kp + shuffle(ko, i * kWide + from));
+        if (a.one_stride) {
+#pragma unroll
+            for (int i = 0; i < kPer; i++)
+                v[i] = *(const u32x4 *)(vp + shuffle(ko, i * kWide + from));
+        } else {
+            const int64_t vo = p * a.kv.v_stride[0] + r * a.kv.v_stride[2];
+#pragma unroll
+            for (int i = 0; i < kPer; i++)
+                v[i] = *(const u32x4 *)(vp + shuffle(vo, i * kWide + from));
         }
+        if (at >= 0) cbq_key_advance(keys, a.page, step, step_entry, step_row, key, entry, row);
+        look(keys);
+    }
+    static __device__ __forceinline__ int64_t shuffle(int64_t x, int lane)
+    {
+        const uint32_t lo = __shfl((int)(uint32_t)x, lane), hi = __shfl((int)(x >> 32), lane);
+        return (int64_t)((uint64_t)hi << 32 | lo);
     }
     // bias[key]: 0, or -inf for a key that is not there
-    __device__ __forceinline__ void store(u32x4 *K, u32x4 *V, float *bias, int tid)
+    __device__ __forceinline__ void store(u32x4 *K, u32x4 *V, float *bias)
     {
-        const int slot = tid % G::kSlots;
+        const int lane = threadIdx.x & 63, wave = NT == CBQ_WAVE ? 0 : threadIdx.x >> 6;
+        const int slot = lane % G::kSlots, sub = lane / G::kSlots;
+        constexpr uint64_t every = kMine == 64 ? ~0ull : (1ull << (kMine & 63)) - 1;
+        if (there != every) {
+#pragma unroll
+            for (int i = 0; i < kPer; i++)
+                if (!(there >> (i * kWide + sub) & 1)) k[i] = v[i] = u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            const int r = i * kRows + tid / G::kSlots;
-            const bool in = ok >> i & 1;
-            const int at = r * G::kSlots + (slot ^ (r & G::kSwz));
-            const u32x4 z = {0, 0, 0, 0};
-            K[at] = in ? k[i] : z;
-            V[at] = in ? v[i] : z;
-            if (slot == 0) bias[r] = in ? 0.f : -INFINITY;
+            const int r = i * kRows + wave * kWide + sub;
+            K[r * G::kSlots + (slot ^ (r & G::kSwz))] = k[i];
+            V[r * G::kSlots + (slot ^ (r & G::kSwz))] = v[i];
         }
+        if (at >= 0) bias[at] = there >> lane & 1 ? 0.f : -INFINITY;
     }
 };
 
@@ -222,11 +259,11 @@ template <typename T, int HD, int RT> struct Rows {
         }
     }
 
-    // One tile of KEYS keys, the first of them key0; MASK: a row sees keys
+    // One tile of KEYS keys, the first of them key0; mask: a row sees keys
     // below sees[] only.
-    template <int KEYS, bool MASK>
+    template <int KEYS>
     __device__ __forceinline__ void tile(const u32x4 *K, const u32x4 *V, const float *bias,
-                                         int32_t key0, float c)
+                                         int32_t key0, float c, bool mask)
     {
         constexpr int NK = KEYS / 16;
         const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
@@ -245,7 +282,7 @@ template <typename T, int HD, int RT> struct Rows {
         }
 #pragma unroll
         for (int t = 0; t < RT; t++) {
-            if (MASK) {
+            if (mask) {
 #pragma unroll
                 for (int k = 0; k < NK; k++)
 #pragma unroll
@@ -382,7 +419,7 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
     const int mine = row0 + wave * 16 * RT;
     Rows<T, HD, RT> w;
     Stage<T, HD, KEYS, kThreads> st;
-    st.look(a, keys, first, tid);
+    st.start(a, keys, first, KEYS);
     w.load(a, h, token0, mine, n);
     int32_t all = INT32_MAX;                    // keys that every row of the block sees
     if (CAUSAL) {
@@ -395,23 +432,18 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
     }
     const int tiles = keys.end > first ? (keys.end - first + KEYS - 1) / KEYS : 0;
     if (tiles > 0) {
-        st.load(a, h, tid);
-        st.look(a, keys, first + KEYS, tid);
-        st.store(K, V, bias, tid);
-        st.load(a, h, tid);
-        st.look(a, keys, first + 2 * KEYS, tid);
+        st.load(a, keys, h);
+        st.store(K, V, bias);
+        st.load(a, keys, h);
         __syncthreads();
         for (int i = 0; i < tiles; i++) {
             const int b = i & 1;
             const int32_t key0 = first + i * KEYS;
-            if (CAUSAL && key0 + KEYS > all)
-                w.template tile<KEYS, true>(K + b * kTile, V + b * kTile, bias + b * KEYS, key0, a.c);
-            else
-                w.template tile<KEYS, false>(K + b * kTile, V + b * kTile, bias + b * KEYS, key0, a.c);
+            w.template tile<KEYS>(K + b * kTile, V + b * kTile, bias + b * KEYS, key0, a.c,
+                                  CAUSAL && key0 + KEYS > all);
             if (i + 1 < tiles) {
-                st.store(K + (b ^ 1) * kTile, V + (b ^ 1) * kTile, bias + (b ^ 1) * KEYS, tid);
-                st.load(a, h, tid);
-                st.look(a, keys, first + (i + 3) * KEYS, tid);
+                st.store(K + (b ^ 1) * kTile, V + (b ^ 1) * kTile, bias + (b ^ 1) * KEYS);
+                st.load(a, keys, h);
             }
             __syncthreads();
         }
@@ -446,7 +478,7 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
     float *bias = (float *)((u32x4 *)lds + kWaves * 2 * kTile) + wave * KEYS;
     Rows<T, HD, 1> w;
     Stage<T, HD, KEYS, CBQ_WAVE> st;
-    st.look(a, keys, first + wave * KEYS, lane);
+    st.start(a, keys, first + wave * KEYS, kWaves * KEYS);
     w.load(a, h, token0, row0, n);
     int32_t all = INT32_MAX;
     if (CAUSAL) {
@@ -455,21 +487,14 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
         w.sees[0] = keys.prefix + (own > 0 ? own : 0);
     }
     const int32_t begin = first + wave * KEYS, step = kWaves * KEYS;
-    if (begin < keys.end) {
-        st.load(a, h, lane);
-        st.look(a, keys, begin + step, lane);
-    }
+    if (begin < keys.end) st.load(a, keys, h);
     for (int32_t key0 = begin; key0 < keys.end; key0 += step) {
-        st.store(K, V, bias, lane);
+        st.store(K, V, bias);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        if (key0 + step < keys.end) {
-            st.load(a, h, lane);
-            st.look(a, keys, key0 + 2 * step, lane);
-        }
-        if (CAUSAL && key0 + KEYS > all) w.template tile<KEYS, true>(K, V, bias, key0, a.c);
-        else w.template tile<KEYS, false>(K, V, bias, key0, a.c);
+        if (key0 + step < keys.end) st.load(a, keys, h);
+        w.template tile<KEYS>(K, V, bias, key0, a.c, CAUSAL && key0 + KEYS > all);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -515,6 +540,10 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
     }
 }
 
+// blocks a CU, whose waves' loads, products and exponentials overlap; rows of
+// 1024 bytes need a wave's whole register file
+constexpr int min_blocks(int row_bytes) { return row_bytes <= 512 ? 2 : 1; }
+
 template <typename T, int HD> constexpr int wave_lds()
 {
     using G = Geo<T, HD>;
@@ -532,7 +561,7 @@ template <typename T, int HD> constexpr int block_lds()
 // PT: 64 PT prefix rows a block; 0: the prefix rows are 16 at most and go as the
 // own ones do.
 template <typename T, int HD, int PT>
-__global__ __launch_bounds__(kThreads, 1) void decode_kernel(AttnArgs a)
+__global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void decode_kernel(AttnArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const DecodeWork w = decode_work(a.plan, blockIdx.x, a.kv.n_kv, a.batch, a.prefix, a.lengths,
@@ -555,7 +584,7 @@ __global__ __launch_bounds__(kThreads, 1) void decode_kernel(AttnArgs a)
 // ---- prompt: tiles of each run's rows against the keys they see -----------------------------
 // RT: 64 RT rows a block; 0: 16 rows.
 template <typename T, int HD, int RT>
-__global__ __launch_bounds__(kThreads, 1) void prompt_kernel(AttnArgs a)
+__global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void prompt_kernel(AttnArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int M = RT ? 64 * RT : 16;

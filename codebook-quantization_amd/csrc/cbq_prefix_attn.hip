@@ -61,6 +61,8 @@ int attend(const void *q, const int64_t *q_stride, const int32_t *q_start,
     a.q_st[0] = q_stride[0];
     a.q_st[1] = q_stride[1];
     a.kv = *cache;
+    a.one_stride = cache->k_stride[0] == cache->v_stride[0] &&
+                   cache->k_stride[2] == cache->v_stride[2];
     a.prefix_table = prefix_table; a.tables = tables; a.lengths = lengths; a.q_start = q_start;
     a.table_st = table_stride;
     a.capacity = (int64_t)width * cache->page;

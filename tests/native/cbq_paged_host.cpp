@@ -39,24 +39,29 @@ static void divisions()
     }
 }
 
-// The keys that a block's tiles and their look-ahead touch; those inside are counted.
+// The keys that a block's walks touch, `step` of them side by side: those inside
+// are counted, and a walk that looks past the end names no entry.
 static void walk(const CbqKeys &keys, const CbqDiv &page, int32_t first, int step,
                  const std::vector<int32_t> &prefix_table, const int32_t *own, int width,
                  std::vector<int> &seen)
 {
-    for (int64_t j = first; j < (int64_t)keys.end + 3 * step; j++) {
-        int32_t row;
-        const int32_t *e = cbq_key_entry(keys, page, (int32_t)j, row);
-        CHECK((e != nullptr) == (j < keys.end));
-        if (!e) continue;
-        const int64_t i = j < keys.prefix ? j : j - keys.prefix;
-        const int32_t *base = j < keys.prefix ? prefix_table.data() : own;
-        CHECK(e == base + i / page.d && row == (int32_t)(i % page.d));
-        CHECK(j >= keys.prefix || e < prefix_table.data() + prefix_table.size());
-        CHECK(j < keys.prefix || e < own + width);
-        volatile int32_t id = *e;
-        (void)id;
-        seen[j]++;
+    const int32_t step_entry = (int32_t)cbq_div(step, page), step_row = step - step_entry * (int32_t)page.d;
+    for (int lane = 0; lane < step; lane++) {
+        int32_t key = first + lane, entry, row;
+        cbq_key_place(keys, page, key, entry, row);
+        for (int64_t j = key; j < (int64_t)keys.end + 3 * step; j += step) {
+            if (key >= 0 && key < keys.end) {
+                const int64_t i = j < keys.prefix ? j : j - keys.prefix;
+                CHECK(key == j && entry == i / page.d && row == i % page.d);
+                CHECK(entry < (j < keys.prefix ? (int64_t)prefix_table.size() : width));
+                volatile int32_t id = (j < keys.prefix ? keys.shared : keys.own)[entry];
+                (void)id;
+                seen[j]++;
+            } else {
+                CHECK(j >= keys.end);
+            }
+            cbq_key_advance(keys, page, step, step_entry, step_row, key, entry, row);
+        }
     }
 }
 
@@ -143,6 +148,18 @@ static void prompt()
         }
         CHECK(at == sees);
     }
+    // a run's keys: the prefix, then its own
+    std::vector<int32_t> prefix_table(cbq_ceil(prefix, page)), own(width);
+    const int32_t sees = prefix + (width ? (int32_t)pick(1, width * page) : 0);
+    std::vector<int> seen(sees);
+    const int unit = p.rt ? block_keys(hd * size) : wave_keys(hd * size) * kAttnWaves;
+    for (int i = 0; i < p.parts; i++) {
+        int32_t first, end;
+        prompt_keys(sees, p.parts, i, p.rt ? unit : wave_keys(hd * size), first, end);
+        walk({prefix_table.data(), own.data(), prefix, end}, cbq_div_make(page), first, unit, prefix_table,
+             own.data(), width, seen);
+    }
+    for (int x : seen) CHECK(x == 1);
     // starts in no order and out of range stay inside the tokens
     for (auto &x : q_start) x = (int32_t)rng();
     for (int b = 0; b < batch; b++) {
@@ -158,13 +175,14 @@ static void far()
     const int64_t most = (1ll << 31) - 65536;
     const CbqDiv page = cbq_div_make(65536);
     std::vector<int32_t> t(cbq_ceil(most, 65536));
-    std::vector<int> none;
-    for (int64_t j : {most - 1, most, most + 4000}) {
-        int32_t row;
-        const int32_t *e = cbq_key_entry({nullptr, t.data(), 0, (int32_t)most}, page, (int32_t)j, row);
-        CHECK((e != nullptr) == (j < most));
-        if (e) CHECK(e == &t.back() && row == (int32_t)((most - 1) % 65536));
+    const CbqKeys keys = {nullptr, t.data(), 0, (int32_t)most};
+    int32_t key = (int32_t)(most - 300), entry, row;
+    cbq_key_place(keys, page, key, entry, row);
+    for (int i = 0; i < 5; i++) {
+        if (key < keys.end) CHECK(entry == key / 65536 && row == key % 65536 && entry < (int)t.size());
+        cbq_key_advance(keys, page, 256, 0, 256, key, entry, row);
     }
+    CHECK(key == most - 300 + 512);
     const Plan p = plan_decode(256, 128, 8, 4, most / 2, most / 2, 1);
     CHECK(p.pre_parts > 0 && p.pre_chunk > 0 && (int64_t)p.pre_parts * p.pre_chunk >= most / 2);
     int32_t first, end;
