@@ -133,9 +133,9 @@ inline Plan plan_decode(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
         tiles = 0;
     }
     const int64_t own_tiles = cbq_ceil(rep, 16);
-    // about eight blocks a CU of the full capacity, a tile a wave at least and
+    // about two blocks a CU of the full capacity, a tile a wave at least and
     // eight at most
-    const int64_t share = cbq_ceil(capacity * batch * n_kv * own_tiles, 8 * kCus);
+    const int64_t share = cbq_ceil(capacity * batch * n_kv * own_tiles, 2 * kCus);
     const int64_t own_chunk = cbq_min(cbq_max(cbq_ceil(share, wk), 1), 8) * wk;
     const int64_t own_parts = cbq_max(cbq_ceil(capacity, own_chunk), pre_parts ? 0 : 1);
     p.blocks = n_kv * (tiles * pre_parts + batch * own_tiles * own_parts);

@@ -25,6 +25,8 @@
 // slot ^ (row % 16), which spreads both operands' reads over the banks.
 #pragma once
 
+#include <atomic>
+
 #include "cbq_device.h"
 #include "cbq_paged.h"
 #include "../../include/cbq_serve.h"
@@ -648,64 +650,85 @@ __global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void pro
                                a.plan.parts > 1 ? part : -1);
 }
 
-// ---- merge of the parts: a wave a (token, head) ----------------------------------------------
+// ---- merge of the parts: a block a (token, head) -----------------------------------------------
+// HD / 4 lanes take a part's values, so a block has 1024 / HD parts under way at
+// once; the first of them are requested before the common maximum is known.
 template <typename T, int HD> __global__ __launch_bounds__(kThreads) void merge_kernel(AttnArgs a)
 {
-    constexpr int V = HD / CBQ_WAVE;
-    const int64_t row = (int64_t)blockIdx.x * kWaves + threadIdx.x / CBQ_WAVE;
-    const int64_t rows = (int64_t)a.N * a.n_q;
-    const int lane = threadIdx.x & 63;
-    if (row >= rows) return;
-    const int64_t token = row / a.n_q;
+    constexpr int kLanes = HD / 4, kGroups = kThreads / kLanes, kAhead = 4;
+    __shared__ __attribute__((aligned(16))) float sums[kGroups][HD];
+    __shared__ float totals[kGroups];
+    const int64_t row = blockIdx.x, rows = (int64_t)a.N * a.n_q, token = row / a.n_q;
+    const int tid = threadIdx.x, lane = tid & 63, group = tid / kLanes, d = tid % kLanes * 4;
     int parts = a.plan.parts;
-    if (a.plan.own_chunk > 0) {                          // decode: as many own parts as the length has
+    if (a.plan.own_chunk > 0) {                     // decode: as many own parts as the length has
         const int32_t len = cbq_clamp_length(a.lengths[token], a.capacity);
         parts = a.plan.pre_parts + (int)cbq_ceil(len, a.plan.own_chunk);
     } else {                                        // prompt: a token of no run keeps its zeros
         if (token < a.q_start[0] || token >= a.q_start[a.batch]) return;
     }
-    float top = -INFINITY, sum = 0.f, x[V] = {};
-    for (int p0 = 0; p0 < parts; p0 += CBQ_WAVE) {
-        const int n = parts - p0 < CBQ_WAVE ? parts - p0 : CBQ_WAVE;
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < n) ml = a.part_ml[(p0 + lane) * rows + row];
-        float now = ml.x;
-        for (int o = 32; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor(now, o));
-        now = fmaxf(now, top);
-        const float base = now == -INFINITY ? 0.f : now;
-        const float f = __builtin_amdgcn_exp2f(top - base), w = __builtin_amdgcn_exp2f(ml.x - base);
-        float s = w * ml.y;                         // 0 of an empty part; a NaN stays
-        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-        sum = sum * f + s;
-        top = now;
-#pragma unroll
-        for (int i = 0; i < V; i++) x[i] *= f;
-        const float *o = a.part_o + (p0 * rows + row) * HD + lane * V;
-#pragma unroll 8
-        for (int p = 0; p < n; p++) {
-            const float wp = __shfl(w, p);
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                const float y = o[p * rows * HD + i];       // unwritten where the part saw no key
-                x[i] = wp == 0.f ? x[i] : fmaf(wp, y, x[i]);
-            }
+    f32x4 o[kAhead];
+    float2 ml[kAhead];
+    auto part = [&](int p, f32x4 &x, float2 &s) {
+        x = f32x4{0, 0, 0, 0};
+        s = make_float2(-INFINITY, 0.f);
+        if (p < parts) {
+            x = *(const f32x4 *)(a.part_o + (p * rows + row) * HD + d);
+            s = a.part_ml[p * rows + row];
         }
-    }
-    const float f = sum == 0.f ? 0.f : 1.0f / sum;
-    T *y = (T *)a.out + row * HD + lane * V;
+    };
 #pragma unroll
-    for (int i = 0; i < V; i++) y[i] = (T)(x[i] * f);
+    for (int i = 0; i < kAhead; i++) part(group + i * kGroups, o[i], ml[i]);
+    float top = -INFINITY;
+    for (int p = lane; p < parts; p += CBQ_WAVE) top = fmaxf(top, a.part_ml[p * rows + row].x);
+    for (int i = 32; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+    const float base = top == -INFINITY ? 0.f : top;
+    f32x4 x = {0, 0, 0, 0};
+    float sum = 0.f;
+    for (int p0 = group;; p0 += kAhead * kGroups) {
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const float w = __builtin_amdgcn_exp2f(ml[i].x - base);
+            sum += w * ml[i].y;                     // 0 of an empty part; a NaN stays
+            // the values of a part that saw no key are not written
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = w == 0.f ? x[e] : fmaf(w, o[i][e], x[e]);
+        }
+        if (p0 + kAhead * kGroups >= parts) break;
+#pragma unroll
+        for (int i = 0; i < kAhead; i++)
+            part(p0 + (kAhead + i) * kGroups, o[i], ml[i]);
+    }
+    *(f32x4 *)&sums[group][d] = x;
+    if (tid % kLanes == 0) totals[group] = sum;
+    __syncthreads();
+    if (tid >= kLanes) return;
+#pragma unroll
+    for (int i = 1; i < kGroups; i++) {
+        x += *(const f32x4 *)&sums[i][d];
+        sum += totals[i];
+    }
+    put_values<T, HD>(a, -1, token, (int)(row - token * a.n_q), d, x, sum);
 }
 
 // ---- launches of one type -------------------------------------------------------------------
-template <typename K> int run_kernel(K kernel, int64_t blocks, int lds, const AttnArgs &a,
-                                     hipStream_t stream, const char *what)
+// More than 64 KiB of LDS is asked for once a kernel and device.
+template <auto K> int run_kernel(int64_t blocks, int lds, const AttnArgs &a, hipStream_t stream,
+                                 const char *what)
 {
-    if (lds > 65536 &&
-        hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) !=
-            hipSuccess)
-        return cbq_launch_status(what);
-    kernel<<<dim3((unsigned)blocks), dim3(kThreads), lds, stream>>>(a);
+    static std::atomic<uint64_t> asked{0};
+    if (lds > 65536) {
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess) return cbq_launch_status(what);
+        const uint64_t bit = 1ull << (dev & 63);
+        if (dev > 63 || !(asked.load(std::memory_order_relaxed) & bit)) {
+            if (hipFuncSetAttribute((const void *)K, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                    lds) != hipSuccess)
+                return cbq_launch_status(what);
+            asked.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
+    K<<<dim3((unsigned)blocks), dim3(kThreads), lds, stream>>>(a);
     return cbq_launch_status(what);
 }
 
@@ -717,18 +740,18 @@ template <typename T, int HD> int launch(const AttnArgs &a, const Plan &p, bool 
     int rc;
     if (prompt) {
         const char *what = "cbq_prefix_attn_prompt";
-        if (p.rt == 0) rc = run_kernel(prompt_kernel<T, HD, 0>, p.blocks, wl, a, stream, what);
-        else if (p.rt == 1) rc = run_kernel(prompt_kernel<T, HD, 1>, p.blocks, bl, a, stream, what);
-        else rc = run_kernel(prompt_kernel<T, HD, wide>, p.blocks, bl, a, stream, what);
+        if (p.rt == 0) rc = run_kernel<prompt_kernel<T, HD, 0>>(p.blocks, wl, a, stream, what);
+        else if (p.rt == 1) rc = run_kernel<prompt_kernel<T, HD, 1>>(p.blocks, bl, a, stream, what);
+        else rc = run_kernel<prompt_kernel<T, HD, wide>>(p.blocks, bl, a, stream, what);
     } else {
         const char *what = "cbq_prefix_attn_decode";
         if (p.rt == 0 || !p.pre_parts)
-            rc = run_kernel(decode_kernel<T, HD, 0>, p.blocks, wl, a, stream, what);
-        else if (p.rt == 1) rc = run_kernel(decode_kernel<T, HD, 1>, p.blocks, both, a, stream, what);
-        else rc = run_kernel(decode_kernel<T, HD, wide>, p.blocks, both, a, stream, what);
+            rc = run_kernel<decode_kernel<T, HD, 0>>(p.blocks, wl, a, stream, what);
+        else if (p.rt == 1) rc = run_kernel<decode_kernel<T, HD, 1>>(p.blocks, both, a, stream, what);
+        else rc = run_kernel<decode_kernel<T, HD, wide>>(p.blocks, both, a, stream, what);
     }
     if (rc != CK_SUCCESS || p.parts == 1) return rc;
-    return run_kernel(merge_kernel<T, HD>, cbq_ceil((int64_t)a.N * a.n_q, kWaves), 0, a, stream,
+    return run_kernel<merge_kernel<T, HD>>((int64_t)a.N * a.n_q, 0, a, stream,
                       "cbq_prefix_attn merge");
 }
 
