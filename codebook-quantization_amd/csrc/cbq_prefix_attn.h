@@ -43,6 +43,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int kWaves = kAttnWaves, kThreads = kWaves * CBQ_WAVE;
+constexpr float kSlack = 8.0f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct AttnArgs {
@@ -203,13 +204,14 @@ template <typename T, int HD, int KEYS, int NT> struct Stage {
         const uint32_t lo = __shfl((int)(uint32_t)x, lane), hi = __shfl((int)(x >> 32), lane);
         return (int64_t)((uint64_t)hi << 32 | lo);
     }
+    static constexpr uint64_t kEvery = kMine == 64 ? ~0ull : (1ull << (kMine & 63)) - 1;
+    __device__ __forceinline__ bool missing() const { return there != kEvery; }
     // bias[key]: 0, or -inf for a key that is not there
     __device__ __forceinline__ void store(u32x4 *K, u32x4 *V, float *bias)
     {
         const int lane = threadIdx.x & 63, wave = NT == CBQ_WAVE ? 0 : threadIdx.x >> 6;
         const int slot = lane % G::kSlots, sub = lane / G::kSlots;
-        constexpr uint64_t every = kMine == 64 ? ~0ull : (1ull << (kMine & 63)) - 1;
-        if (there != every) {
+        if (missing()) {
 #pragma unroll
             for (int i = 0; i < kPer; i++)
                 if (!(there >> (i * kWide + sub) & 1)) k[i] = v[i] = u32x4{0, 0, 0, 0};
@@ -224,12 +226,133 @@ template <typename T, int HD, int KEYS, int NT> struct Stage {
     }
 };
 
+// The same for a block's tile, straight into LDS: no registers and no stores, and
+// K and V are asked for at different times, K a tile ahead.  A lane's 16 bytes
+// land at its place in the wave's 1 KiB, so the slot ^ row order of the tile is
+// made by the lane's choice of global slot; rows that are not there come from a
+// slot of zeros.
+static __device__ const u32x4 kZeroSlot = {0, 0, 0, 0};
+
+// Written as asm so that the compiler orders no LDS read behind it: stage_wait's
+// barriers do.  M0 holds the LDS address; a wait state is needed between its
+// write and the load.
+__device__ __forceinline__ void copy_slots(uint32_t lds, const void *from)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(from) : "m0");
+}
+
+// Every copy and load of this wave, and its LDS accesses, are done; then all waves'.
+__device__ __forceinline__ void stage_wait()
+{
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+template <typename T, int HD, int KEYS> struct Copies {
+    using G = Geo<T, HD>;
+    static constexpr int kRows = kThreads / G::kSlots, kPer = KEYS / kRows;
+    static constexpr int kWide = CBQ_WAVE / G::kSlots, kMine = kPer * kWide;
+    static_assert(kRows * kPer == KEYS && kMine <= CBQ_WAVE, "whole passes, a key a lane");
+    const char *v[kPer];                    // this lane's slots of the values of the tile whose
+                                            // keys were asked for last
+    int32_t key, entry, row, id;            // this lane's key: of the next tile
+    int32_t step_entry, step_row;
+    int at;
+
+    __device__ __forceinline__ void start(const AttnArgs &a, const CbqKeys &keys, int32_t first)
+    {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        at = lane < kMine ? lane / kWide * kRows + wave * kWide + lane % kWide : -1;
+        step_entry = (int32_t)cbq_div((uint32_t)KEYS, a.page);
+        step_row = KEYS - step_entry * (int32_t)a.page.d;
+        key = at < 0 ? -1 : first + at;
+        cbq_key_place(keys, a.page, key, entry, row);
+        look(keys);
+    }
+    __device__ __forceinline__ void look(const CbqKeys &keys)
+    {
+        id = -1;
+        if (key >= 0 && key < keys.end) id = (key < keys.prefix ? keys.shared : keys.own)[entry];
+    }
+    // Asks for the next tile's keys and writes its bias (0, or -inf for a key that
+    // is not there) and this wave's flag of one that is not.
+    __device__ __forceinline__ void keys_to(const AttnArgs &a, const CbqKeys &keys, int h, uint32_t lds,
+                                            float *bias, int32_t *flags)
+    {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / G::kSlots;
+        const bool in = id >= 0 && id < a.kv.n_pages;
+        const uint64_t there = __ballot(in);
+        constexpr uint64_t every = kMine == 64 ? ~0ull : (1ull << (kMine & 63)) - 1;
+        const int64_t p = in ? id : 0, r = in ? row : 0;
+        const int64_t ko = p * a.kv.k_stride[0] + r * a.kv.k_stride[2];
+        const int64_t vo = a.one_stride ? ko : p * a.kv.v_stride[0] + r * a.kv.v_stride[2];
+        const T *kp = (const T *)a.kv.k + h * a.kv.k_stride[1];
+        const T *vp = (const T *)a.kv.v + h * a.kv.v_stride[1];
+        const int swz = (lane % G::kSlots) ^ ((wave * kWide + sub) & G::kSwz);
+        const char *k[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int slot = (swz ^ (i * kRows & G::kSwz)) * G::kEl;
+            const int64_t o = shuffle(ko, i * kWide + sub);
+            k[i] = (const char *)(kp + o + slot);
+            v[i] = (const char *)(vp + o + slot);
+        }
+        if (!a.one_stride) {
+#pragma unroll
+            for (int i = 0; i < kPer; i++)
+                v[i] = (const char *)(vp + shuffle(vo, i * kWide + sub) +
+                                      (swz ^ (i * kRows & G::kSwz)) * G::kEl);
+        }
+        if (there != every) {
+#pragma unroll
+            for (int i = 0; i < kPer; i++)
+                if (!(there >> (i * kWide + sub) & 1)) k[i] = v[i] = (const char *)&kZeroSlot;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; i++) copy_slots(lds + place(i, wave), k[i]);
+        if (at >= 0) bias[at] = in ? 0.f : -INFINITY;
+        if (lane == 0) flags[wave] = there != every;
+        if (at >= 0)
+            cbq_key_advance(keys, a.page, KEYS, step_entry, step_row, key, entry, row);
+        look(keys);
+    }
+    // Asks for the values of the tile whose keys keys_to() asked for last.
+    __device__ __forceinline__ void values_to(uint32_t lds)
+    {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) copy_slots(lds + place(i, threadIdx.x >> 6), v[i]);
+    }
+    static __device__ __forceinline__ uint32_t place(int i, int wave)
+    {
+        return (uint32_t)((i * kRows + wave * kWide) * G::kSlots * 16);
+    }
+    static __device__ __forceinline__ int64_t shuffle(int64_t x, int lane)
+    {
+        const uint32_t lo = __shfl((int)(uint32_t)x, lane), hi = __shfl((int)(x >> 32), lane);
+        return (int64_t)((uint64_t)hi << 32 | lo);
+    }
+};
+
+// The order of a stretch of code, for the compiler's scheduler: the first AHEAD
+// LDS reads, then GROUPS times matrix instructions and one more read.
+template <int GROUPS, int AHEAD, int MFMA> __device__ __forceinline__ void read_ahead()
+{
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < GROUPS; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, MFMA, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // ---- RT x 16 query rows of one wave --------------------------------------------------
 template <typename T, int HD, int RT> struct Rows {
     using G = Geo<T, HD>;
     u32x4 q[RT][G::kQ];
     f32x4 o[RT][G::kD];
-    float m[RT], l[RT];                     // m in exp2's domain; l: this lane's keys only
+    // m, base (m, or 0 where no key was seen) in exp2's domain; l: this lane's keys only
+    float m[RT], base[RT], l[RT];
     int32_t sees[RT];                       // keys of the joint axis that the row sees
 
     // Rows first .. first + 16 RT - 1 of n; token0 is the token of row 0.
@@ -257,24 +380,20 @@ template <typename T, int HD, int RT> struct Rows {
 #pragma unroll
             for (int d = 0; d < G::kD; d++) o[t][d] = f32x4{0, 0, 0, 0};
             m[t] = -INFINITY;
-            l[t] = 0.f;
+            base[t] = l[t] = 0.f;
+            sees[t] = INT32_MAX;
         }
     }
 
-    // One tile of KEYS keys, the first of them key0; mask: a row sees keys
-    // below sees[] only.
-    template <int KEYS>
-    __device__ __forceinline__ void tile(const u32x4 *K, const u32x4 *V, const float *bias,
-                                         int32_t key0, float c, bool mask)
+    // S^T of NK * 16 keys
+    template <int NK>
+    __device__ __forceinline__ void scores(const u32x4 *K, f32x4 (&s)[RT][NK])
     {
-        constexpr int NK = KEYS / 16;
         const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-        f32x4 s[RT][NK];
 #pragma unroll
         for (int k = 0; k < NK; k++) {
-            const f32x4 b = *(const f32x4 *)(bias + k * 16 + 4 * g);
 #pragma unroll
-            for (int t = 0; t < RT; t++) s[t][k] = b;
+            for (int t = 0; t < RT; t++) s[t][k] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int d = 0; d < G::kQ; d++) {
                 const u32x4 w = K[(k * 16 + r) * G::kSlots + ((d * 4 + g) ^ (r & G::kSwz))];
@@ -282,49 +401,84 @@ template <typename T, int HD, int RT> struct Rows {
                 for (int t = 0; t < RT; t++) s[t][k] = Mma<T>::qk(w, q[t][d], s[t][k]);
             }
         }
-#pragma unroll
-        for (int t = 0; t < RT; t++) {
-            if (mask) {
-#pragma unroll
-                for (int k = 0; k < NK; k++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (key0 + k * 16 + 4 * g + i >= sees[t]) s[t][k][i] = -INFINITY;
-            }
-            float top = s[t][0][0];
-#pragma unroll
-            for (int k = 0; k < NK; k++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) top = fmaxf(top, s[t][k][i]);
-            top = fmaxf(m[t], groups_max(top) * c);
-            const float base = top == -INFINITY ? 0.f : top;    // a row that has seen no key
-            if (__any(top > m[t])) {
-                const float f = __builtin_amdgcn_exp2f(m[t] - base);
-                l[t] *= f;
-#pragma unroll
-                for (int d = 0; d < G::kD; d++) o[t][d] *= f;
-                m[t] = top;
-            }
-            float sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < NK; k++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    s[t][k][i] = __builtin_amdgcn_exp2f(fmaf(s[t][k][i], c, -base));
-                    sum += s[t][k][i];
-                }
-            l[t] += sum;
-        }
-        values<NK>(V, s);
     }
 
-    template <int NK> __device__ __forceinline__ void values(const u32x4 *V, f32x4 (&s)[RT][NK])
+    // Keys that are not there (bias -inf; their products are 0, or NaN where the
+    // query is no number) or that a row does not see: -inf
+    template <int NK>
+    __device__ __forceinline__ void hide(f32x4 (&s)[RT][NK], const float *bias, int32_t key0)
+    {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            const f32x4 b = *(const f32x4 *)(bias + k * 16 + 4 * g);
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                s[t][k] += b;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    s[t][k][i] = key0 + k * 16 + 4 * g + i < sees[t] ? s[t][k][i] : -INFINITY;
+            }
+        }
+    }
+
+    // Each row's largest score of the tile, in exp2's domain
+    template <int NK>
+    __device__ __forceinline__ void top(const f32x4 (&s)[RT][NK], float c, float (&x)[RT])
+    {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            x[t] = s[t][0][0];
+#pragma unroll
+            for (int k = 0; k < NK; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[t] = fmaxf(x[t], s[t][k][i]);
+            x[t] = groups_max(x[t]) * c;
+        }
+    }
+
+    // The running maximum follows the scores once they pass it by kSlack: until
+    // then weights are at most 2^kSlack and nothing is rescaled.
+    __device__ __forceinline__ void raise(const float (&x)[RT])
+    {
+        bool over = false;
+#pragma unroll
+        for (int t = 0; t < RT; t++) over = over || x[t] > m[t] + kSlack;
+        if (!__any(over)) return;
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const float now = fmaxf(m[t], x[t]);
+            base[t] = now == -INFINITY ? 0.f : now;         // a row that has seen no key
+            const float f = __builtin_amdgcn_exp2f(m[t] - base[t]);
+            l[t] *= f;
+#pragma unroll
+            for (int d = 0; d < G::kD; d++) o[t][d] *= f;
+            m[t] = now;
+        }
+    }
+
+    // Four scores to weights, added to the row's sum
+    __device__ __forceinline__ f32x4 weigh(int t, f32x4 s, float c)
+    {
+        f32x4 p;
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base[t]));
+        l[t] += (p[0] + p[1]) + (p[2] + p[3]);
+        return p;
+    }
+
+    // Weights of the tile, and the values under them
+    template <int NK>
+    __device__ __forceinline__ void values(const u32x4 *V, const f32x4 (&s)[RT][NK], float c)
     {
         const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
         if constexpr (sizeof(T) == 4) {
             const float *F = (const float *)V;
 #pragma unroll
-            for (int k = 0; k < NK; k++)
+            for (int k = 0; k < NK; k++) {
+                f32x4 p[RT];
+#pragma unroll
+                for (int t = 0; t < RT; t++) p[t] = weigh(t, s[t][k], c);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int key = k * 16 + 4 * g + i;
@@ -334,10 +488,11 @@ template <typename T, int HD, int RT> struct Rows {
                                           * 4 + (r & 3)];
 #pragma unroll
                         for (int t = 0; t < RT; t++)
-                            o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, s[t][k][i], o[t][d],
-                                                                           0, 0, 0);
+                            o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, p[t][i], o[t][d], 0, 0,
+                                                                           0);
                     }
                 }
+            }
         } else {
             // lane (g, r) points the transpose read at key 4g + r / 4, values
             // 4 (r % 4) .. + 3 and gets keys 4g .. 4g + 3 of value r
@@ -349,34 +504,67 @@ template <typename T, int HD, int RT> struct Rows {
                     (lds_s16x4 *)((const u32x2 *)p + half)));
             };
             if constexpr (NK % 2 == 0) {
+                // Two 16-key tiles side by side are one product's keys.  Four pieces
+                // of hd are read while the four before them are in the products, and
+                // the weights of the next two tiles are made beside them.
+                constexpr int kParts = G::kD / 4, kAll = NK / 2 * kParts, kUnits = 2 * RT / kParts;
+                u32x2 v[2][4][2];
+                u32x4 p[2][RT];
+                auto read = [&](int j) {
 #pragma unroll
-                for (int k = 0; k < NK; k += 2) {
-                    u32x4 p[RT];
+                    for (int d = 0; d < 4; d++) {
+                        v[j & 1][d][0] = piece(j / kParts * 2, j % kParts * 4 + d);
+                        v[j & 1][d][1] = piece(j / kParts * 2 + 1, j % kParts * 4 + d);
+                    }
+                };
+                auto weights = [&](int pair, int u) {       // unit u of the pair: 4 scores a lane
+                    const int t = u / 2, k = u % 2;
+                    const f32x4 x = weigh(t, s[t][pair * 2 + k], c);
+                    p[pair & 1][t][k * 2] = pack2<T>(x[0], x[1]);
+                    p[pair & 1][t][k * 2 + 1] = pack2<T>(x[2], x[3]);
+                };
+                read(0);
 #pragma unroll
-                    for (int t = 0; t < RT; t++)
-                        p[t] = u32x4{pack2<T>(s[t][k][0], s[t][k][1]),
-                                     pack2<T>(s[t][k][2], s[t][k][3]),
-                                     pack2<T>(s[t][k + 1][0], s[t][k + 1][1]),
-                                     pack2<T>(s[t][k + 1][2], s[t][k + 1][3])};
+                for (int u = 0; u < 2 * RT; u++) weights(0, u);
 #pragma unroll
-                    for (int d = 0; d < G::kD; d++) {
-                        const u32x2 x = piece(k, d), y = piece(k + 1, d);
+                for (int j = 0; j < kAll; j++) {
+                    const int pair = j / kParts;
+                    if (j + 1 < kAll) read(j + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        const u32x2 x = v[j & 1][d][0], y = v[j & 1][d][1];
                         const u32x4 w = {x[0], x[1], y[0], y[1]};
 #pragma unroll
-                        for (int t = 0; t < RT; t++) o[t][d] = Mma<T>::qk(w, p[t], o[t][d]);
+                        for (int t = 0; t < RT; t++)
+                            o[t][j % kParts * 4 + d] = Mma<T>::qk(w, p[pair & 1][t],
+                                                                  o[t][j % kParts * 4 + d]);
                     }
+                    if (pair + 1 < NK / 2) {
+#pragma unroll
+                        for (int u = 0; u < kUnits; u++) weights(pair + 1, j % kParts * kUnits + u);
+#pragma unroll
+                        for (int i = 0; i < 4 * RT; i++) {
+                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x002, (10 * kUnits + 4 * RT - 1) / (4 * RT), 0);
+                            __builtin_amdgcn_sched_group_barrier(0x400, (4 * kUnits + 4 * RT - 1) / (4 * RT), 0);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             } else {
                 static_assert(NK == 1, "one 16-key piece");
+                u32x2 p[RT];
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    const f32x4 x = weigh(t, s[t][0], c);
+                    p[t] = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+                }
 #pragma unroll
                 for (int d = 0; d < G::kD; d++) {
                     const u32x2 w = piece(0, d);
 #pragma unroll
-                    for (int t = 0; t < RT; t++) {
-                        const u32x2 p = {pack2<T>(s[t][0][0], s[t][0][1]),
-                                         pack2<T>(s[t][0][2], s[t][0][3])};
-                        o[t][d] = Mma<T>::pv16(w, p, o[t][d]);
-                    }
+                    for (int t = 0; t < RT; t++) o[t][d] = Mma<T>::pv16(w, p[t], o[t][d]);
                 }
             }
         }
@@ -414,14 +602,18 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
                                            int32_t past, int part)
 {
     using G = Geo<T, HD>;
-    constexpr int KEYS = G::kBlockKeys, kTile = KEYS * G::kSlots;
+    constexpr int KEYS = G::kBlockKeys, NK = KEYS / 16, kTile = KEYS * G::kSlots;
+    constexpr uint32_t kBytes = kTile * 16;
     u32x4 *K = (u32x4 *)lds, *V = K + 2 * kTile;
     float *bias = (float *)(V + 2 * kTile);
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    int32_t *flags = (int32_t *)(bias + 2 * KEYS);
+    const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds,
+                   lds_v = lds_k + 2 * kBytes;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int mine = row0 + wave * 16 * RT;
     Rows<T, HD, RT> w;
-    Stage<T, HD, KEYS, kThreads> st;
-    st.start(a, keys, first, KEYS);
+    Copies<T, HD, KEYS> st;
+    st.start(a, keys, first);
     w.load(a, h, token0, mine, n);
     int32_t all = INT32_MAX;                    // keys that every row of the block sees
     if (CAUSAL) {
@@ -433,21 +625,36 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
         }
     }
     const int tiles = keys.end > first ? (keys.end - first + KEYS - 1) / KEYS : 0;
+    constexpr int kF = sizeof(T) == 4 ? 4 : 1;          // matrix instructions a product
+    auto step = [&](int i, int b) {
+        if (i + 1 < tiles) {
+            st.keys_to(a, keys, h, lds_k + (b ^ 1) * kBytes, bias + (b ^ 1) * KEYS,
+                       flags + (b ^ 1) * kWaves);
+            st.values_to(lds_v + (b ^ 1) * kBytes);
+        }
+        const int32_t key0 = first + i * KEYS;
+        const int4 miss = *(const int4 *)(flags + b * kWaves);
+        f32x4 s[RT][NK];
+        __builtin_amdgcn_sched_barrier(0);
+        w.scores(K + b * kTile, s);
+        read_ahead<NK * G::kQ, 4, RT * kF>();
+        if (key0 + KEYS > all || __builtin_amdgcn_readfirstlane(miss.x | miss.y | miss.z | miss.w))
+            w.hide(s, bias + b * KEYS, key0);
+        float top[RT];
+        w.top(s, a.c, top);
+        w.raise(top);
+        w.values(V + b * kTile, s, a.c);
+        stage_wait();
+    };
     if (tiles > 0) {
-        st.load(a, keys, h);
-        st.store(K, V, bias);
-        st.load(a, keys, h);
-        __syncthreads();
-        for (int i = 0; i < tiles; i++) {
-            const int b = i & 1;
-            const int32_t key0 = first + i * KEYS;
-            w.template tile<KEYS>(K + b * kTile, V + b * kTile, bias + b * KEYS, key0, a.c,
-                                  CAUSAL && key0 + KEYS > all);
-            if (i + 1 < tiles) {
-                st.store(K + (b ^ 1) * kTile, V + (b ^ 1) * kTile, bias + (b ^ 1) * KEYS);
-                st.load(a, keys, h);
-            }
-            __syncthreads();
+        st.keys_to(a, keys, h, lds_k, bias, flags);
+        st.values_to(lds_v);
+        stage_wait();
+        for (int i = 0;; i += 2) {
+            step(i, 0);
+            if (i + 1 >= tiles) break;
+            step(i + 1, 1);
+            if (i + 2 >= tiles) break;
         }
     }
 #pragma unroll
@@ -491,12 +698,19 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
     const int32_t begin = first + wave * KEYS, step = kWaves * KEYS;
     if (begin < keys.end) st.load(a, keys, h);
     for (int32_t key0 = begin; key0 < keys.end; key0 += step) {
+        const bool missing = st.missing();
         st.store(K, V, bias);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         if (key0 + step < keys.end) st.load(a, keys, h);
-        w.template tile<KEYS>(K, V, bias, key0, a.c, CAUSAL && key0 + KEYS > all);
+        f32x4 s[1][KEYS / 16];
+        w.scores(K, s);
+        if (missing || key0 + KEYS > all) w.hide(s, bias, key0);
+        float top[1];
+        w.top(s, a.c, top);
+        w.raise(top);
+        w.values(V, s, a.c);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -556,7 +770,7 @@ template <typename T, int HD> constexpr int wave_lds()
 template <typename T, int HD> constexpr int block_lds()
 {
     using G = Geo<T, HD>;
-    return 4 * G::kBlockKeys * G::kSlots * 16 + 2 * G::kBlockKeys * 4;
+    return 4 * G::kBlockKeys * G::kSlots * 16 + 2 * G::kBlockKeys * 4 + 2 * kWaves * 4;
 }
 
 // ---- decode: parts of the prefix for all sequences, parts of each one's own keys ------------
