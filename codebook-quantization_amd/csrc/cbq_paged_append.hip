@@ -18,6 +18,8 @@
 
 namespace {
 
+constexpr int64_t kFourThreads = 4 * 256 * 4 * 64;    // four waves a SIMD of 256 CUs
+
 struct AppendArgs {
     const void *q, *k, *v;
     int64_t q_st[2], k_st[2], v_st[2];
@@ -26,7 +28,7 @@ struct AppendArgs {
     void *q_out;
     cbq_paged_kv cache;
     int64_t n_pos, n_slots;
-    CbqDiv heads, page;                 // n_q + 2 n_kv; rows of a page
+    CbqDiv heads, page;                 // thread groups a token; rows of a page
     uint32_t rows;                      // N (n_q + 2 n_kv)
     int n_q, n_kv, hd, rot, norm;
     float eps;
@@ -51,33 +53,24 @@ template <typename T, int V> __device__ __forceinline__ void store_vec(T *p, con
     *(Pack<T, V> *)p = a;
 }
 
-// V values a side; U pairs of sides a thread; L lanes a row.
-template <typename TX, typename TC, int V, int U, int L>
+// V values a side; U pairs of sides a thread; L lanes a row; R neighbouring heads
+// of one token a thread, all of them queries, keys or values, which share what
+// the thread reads of the tables and weights.
+template <typename TX, typename TC, int V, int U, int L, int R>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 {
-    const uint32_t row = blockIdx.x * (256u / L) + threadIdx.x / L;
+    const uint32_t unit = blockIdx.x * (256u / L) + threadIdx.x / L;
     const int lane = threadIdx.x % L;
-    if (row >= a.rows) return;                          // whole rows: no lane waits on a left one
-    const int64_t t = cbq_div(row, a.heads);
-    const int i = (int)(row - (uint32_t)t * a.heads.d);
+    if (unit >= a.rows / R) return;                     // whole rows: no lane waits on a left one
+    const int64_t t = cbq_div(unit, a.heads);           // heads: groups of R of a token
+    const int i = (int)(unit - (uint32_t)t * a.heads.d) * R;
     const bool is_q = i < a.n_q, is_k = !is_q && i < a.n_q + a.n_kv;
     const int j = is_q ? i : is_k ? i - a.n_q : i - a.n_q - a.n_kv;
     const int64_t *st = is_q ? a.q_st : is_k ? a.k_st : a.v_st;
     const TX *x = (const TX *)(is_q ? a.q : is_k ? a.k : a.v) + t * st[0] + j * st[1];
     const int64_t p = a.positions[t], slot = a.slots[t];
-    const bool placed = p >= 0 && p < a.n_pos;
-    TC *y;
-    if (is_q) {
-        y = (TC *)a.q_out + (t * a.n_q + j) * a.hd;
-    } else {
-        if (!placed || slot < 0 || slot >= a.n_slots) return;       // uniform over the row's lanes
-        const uint32_t id = cbq_div((uint32_t)slot, a.page);
-        const int64_t r = (int64_t)((uint32_t)slot - id * a.page.d);
-        const int64_t *ps = is_k ? a.cache.k_stride : a.cache.v_stride;
-        y = (TC *)(is_k ? a.cache.k : a.cache.v) + id * ps[0] + j * ps[1] + r * ps[2];
-    }
     const int half = a.rot / 2, units = a.hd / (2 * V), turned = half / V;
-    float lo[U][V], hi[U][V];
+    float lo[R][U][V], hi[R][U][V];
     int at_lo[U], at_hi[U];
 #pragma unroll
     for (int n = 0; n < U; n++) {
@@ -85,29 +78,55 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
         at_lo[n] = u < turned ? u * V : a.rot + 2 * w * V;
         at_hi[n] = u < turned ? u * V + half : at_lo[n] + V;
         if (u < units) {
-            load_vec<TX, V>(x + at_lo[n], lo[n]);
-            load_vec<TX, V>(x + at_hi[n], hi[n]);
+#pragma unroll
+            for (int h = 0; h < R; h++) {
+                load_vec<TX, V>(x + h * st[1] + at_lo[n], lo[h][n]);
+                load_vec<TX, V>(x + h * st[1] + at_hi[n], hi[h][n]);
+            }
         }
+    }
+    const bool placed = p >= 0 && p < a.n_pos;
+    TC *y;
+    int64_t y_step;                                     // to the next head
+    if (is_q) {
+        y = (TC *)a.q_out + (t * a.n_q + j) * a.hd;
+        y_step = a.hd;
+    } else {
+        if (!placed || slot < 0 || slot >= a.n_slots) return;       // uniform over the row's lanes
+        const uint32_t id = cbq_div((uint32_t)slot, a.page);
+        const int64_t r = (int64_t)((uint32_t)slot - id * a.page.d);
+        const int64_t *ps = is_k ? a.cache.k_stride : a.cache.v_stride;
+        y = (TC *)(is_k ? a.cache.k : a.cache.v) + id * ps[0] + j * ps[1] + r * ps[2];
+        y_step = ps[1];
     }
     if (is_q || is_k) {
         if (a.norm) {
-            float s = 0.f;
-#pragma unroll
-            for (int n = 0; n < U; n++)
-                if (lane + n * L < units)
-#pragma unroll
-                    for (int e = 0; e < V; e++) s += lo[n][e] * lo[n][e] + hi[n][e] * hi[n][e];
-#pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, L);
-            const float r = 1.0f / sqrtf(s / (float)a.hd + a.eps);
             const float *w = is_q ? a.q_w : a.k_w;
+            float r[R];
+#pragma unroll
+            for (int h = 0; h < R; h++) {
+                float s = 0.f;
+#pragma unroll
+                for (int n = 0; n < U; n++)
+                    if (lane + n * L < units)
+#pragma unroll
+                        for (int e = 0; e < V; e++)
+                            s += lo[h][n][e] * lo[h][n][e] + hi[h][n][e] * hi[h][n][e];
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, L);
+                r[h] = 1.0f / sqrtf(s / (float)a.hd + a.eps);
+            }
 #pragma unroll
             for (int n = 0; n < U; n++)
                 if (lane + n * L < units)
 #pragma unroll
                     for (int e = 0; e < V; e++) {
-                        lo[n][e] *= r * (w ? w[at_lo[n] + e] : 1.0f);
-                        hi[n][e] *= r * (w ? w[at_hi[n] + e] : 1.0f);
+                        const float wl = w ? w[at_lo[n] + e] : 1.0f, wh = w ? w[at_hi[n] + e] : 1.0f;
+#pragma unroll
+                        for (int h = 0; h < R; h++) {
+                            lo[h][n][e] *= r[h] * wl;
+                            hi[h][n][e] *= r[h] * wh;
+                        }
                     }
         }
         const int64_t angle = (placed ? p : 0) * a.rot;
@@ -118,33 +137,49 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
                 load_vec<float, V>(a.cos_t + angle + at_lo[n], c);
                 load_vec<float, V>(a.sin_t + angle + at_lo[n], s);
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float b = lo[n][e], d = hi[n][e];
-                    lo[n][e] = b * c[e] - d * s[e];
-                    hi[n][e] = d * c[e] + b * s[e];
-                }
+                for (int h = 0; h < R; h++)
+#pragma unroll
+                    for (int e = 0; e < V; e++) {
+                        const float b = lo[h][n][e], d = hi[h][n][e];
+                        lo[h][n][e] = b * c[e] - d * s[e];
+                        hi[h][n][e] = d * c[e] + b * s[e];
+                    }
             }
     }
 #pragma unroll
     for (int n = 0; n < U; n++)
         if (lane + n * L < units) {
-            store_vec<TC, V>(y + at_lo[n], lo[n]);
-            store_vec<TC, V>(y + at_hi[n], hi[n]);
+#pragma unroll
+            for (int h = 0; h < R; h++) {
+                store_vec<TC, V>(y + h * y_step + at_lo[n], lo[h][n]);
+                store_vec<TC, V>(y + h * y_step + at_hi[n], hi[h][n]);
+            }
         }
 }
 
-template <typename TX, typename TC> int launch(const AppendArgs &a, bool wide, hipStream_t stream)
+template <typename TX, typename TC, int V, int U, int L>
+void launch_rows(AppendArgs &a, hipStream_t stream)
 {
-    auto go = [&](auto kernel, int lanes) {
-        const int64_t blocks = cbq_ceil((int64_t)a.rows * lanes, 256);
-        kernel<<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a);
-    };
+    // Four heads a thread where four waves a SIMD are left: 8 KiB of tables and
+    // weights a token instead of 32 (12500 bf16 tokens, 48 heads of 128: 98 -> 65
+    // us, 4.7 TB/s, a copy's rate; 900 tokens: 7.0 us with one head, 8.0 with four).
+    const bool four = V > 1 && a.n_q % 4 == 0 && a.n_kv % 4 == 0 &&
+                      (int64_t)a.rows * L / 4 >= kFourThreads;
+    const int R = four ? 4 : 1;
+    a.heads = cbq_div_make((uint32_t)(a.n_q + 2 * a.n_kv) / R);
+    const dim3 blocks((unsigned)cbq_ceil(a.rows / R, 256 / L)), threads(256);
+    if (four) paged_append_kernel<TX, TC, V, U, L, V == 1 ? 1 : 4><<<blocks, threads, 0, stream>>>(a);
+    else paged_append_kernel<TX, TC, V, U, L, 1><<<blocks, threads, 0, stream>>>(a);
+}
+
+template <typename TX, typename TC> int launch(AppendArgs &a, bool wide, hipStream_t stream)
+{
     // 16-byte pieces where hd is one of the decoders' and every address allows
     // it; else one value at a time, a wave a row (128 pairs at most).
-    if (wide && a.hd == 64) go(paged_append_kernel<TX, TC, 8, 1, 4>, 4);
-    else if (wide && a.hd == 128) go(paged_append_kernel<TX, TC, 8, 1, 8>, 8);
-    else if (wide && a.hd == 256) go(paged_append_kernel<TX, TC, 8, 1, 16>, 16);
-    else go(paged_append_kernel<TX, TC, 1, 2, 64>, 64);
+    if (wide && a.hd == 64) launch_rows<TX, TC, 8, 1, 4>(a, stream);
+    else if (wide && a.hd == 128) launch_rows<TX, TC, 8, 1, 8>(a, stream);
+    else if (wide && a.hd == 256) launch_rows<TX, TC, 8, 1, 16>(a, stream);
+    else launch_rows<TX, TC, 1, 2, 64>(a, stream);
     return cbq_launch_status("cbq_paged_append");
 }
 
@@ -196,7 +231,6 @@ extern "C" int cbq_paged_append(const void *q, const void *k, const void *v, int
     a.cache = *cache;
     a.n_pos = n_pos;
     a.n_slots = cache->n_pages * cache->page;
-    a.heads = cbq_div_make((uint32_t)heads);
     a.page = cbq_div_make((uint32_t)cache->page);
     a.rows = (uint32_t)(N * heads);
     a.n_q = n_q; a.n_kv = n_kv; a.hd = hd; a.rot = rot; a.norm = norm;
