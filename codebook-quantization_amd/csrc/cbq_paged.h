@@ -159,11 +159,17 @@ inline Plan plan_prompt(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
     if (rows <= 16 * batch || (small <= 2 * kCus && keys <= 2048)) p.rt = 0;
     else p.rt = rows <= 64 * batch ? 1 : widest(row_bytes);
     // a run's last tile may be part full: one more a run than the rows need
-    const int64_t tiles = rows / (p.rt ? 64 * p.rt : 16) + cbq_min(batch, N);
+    const int64_t m = p.rt ? 64 * p.rt : 16;
+    const int64_t tiles = rows / m + cbq_min(batch, N);
     const int64_t unit = p.rt ? block_keys(row_bytes) : kAttnWaves * wave_keys(row_bytes);
     const int64_t blocks = tiles * n_kv;
-    const int64_t parts = blocks >= kCus
-        ? 1 : cbq_max(1, cbq_min(cbq_ceil(2 * kCus, blocks), keys / (4 * unit)));
+    // Few tiles: their keys in parts, as many as two blocks a CU have room for at
+    // once (a few more would run alone, in a second turn).  Of the runs' last
+    // tiles, half are taken to be there beside the rows' whole ones.
+    const int64_t likely = (batch == 1 ? cbq_ceil(rows, m) : rows / m + cbq_ceil(cbq_min(batch, N), 2))
+                           * n_kv;
+    const int64_t parts = likely >= kCus
+        ? 1 : cbq_max(1, cbq_min(2 * kCus / likely, keys / (4 * unit)));
     p.blocks = blocks * parts;
     p.bytes = part_bytes(parts, N, n_kv * rep, hd);
     p.tiles = (int32_t)tiles;

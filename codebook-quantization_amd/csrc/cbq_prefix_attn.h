@@ -22,7 +22,7 @@
 //
 // Tiles of keys go global -> registers -> LDS, the loads of a tile being under
 // way while the one before is computed; 16-byte slots of a row are stored at
-// slot ^ (row % 16), which spreads both operands' reads over the banks.
+// slot ^ mix(row), which spreads both operands' reads over the banks.
 #pragma once
 
 #include <atomic>
@@ -125,7 +125,16 @@ __device__ __forceinline__ float groups_sum(float x)
 template <typename T, int HD> struct Geo {
     static constexpr int kEl = 16 / (int)sizeof(T);         // elements of a 16-byte slot
     static constexpr int kSlots = HD / kEl;                 // slots of a row
-    static constexpr int kSwz = (kSlots < 16 ? kSlots : 16) - 1;
+    // Slot s of a row lies at s ^ mix(row): 16 rows' equal slots in 16 (of rows of
+    // 128 bytes: 8) places, for the reads of K; and of 16-bit types, 8 rows' equal
+    // pairs of slots in 8 places, for the transpose reads of V (a row's 32 bytes
+    // apiece).  Bits are only moved, so mix(a | b) = mix(a) ^ mix(b) for a & b = 0.
+    static __device__ __forceinline__ constexpr int mix(int row)
+    {
+        if (sizeof(T) == 4) return row & 15;
+        if (kSlots == 8) return (row >> 1 & 3) << 1 | (row >> 3 & 1);
+        return (row & 7) << 1 | (row >> 3 & 1);
+    }
     static constexpr int kQ = kSlots / 4;                   // slots of a query row a lane holds
     static constexpr int kD = HD / 16;                      // 16-value pieces of a row
     // keys of a block's tile (K and V, two buffers: 64 KiB at most) and of a
@@ -219,8 +228,8 @@ template <typename T, int HD, int KEYS, int NT> struct Stage {
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
             const int r = i * kRows + wave * kWide + sub;
-            K[r * G::kSlots + (slot ^ (r & G::kSwz))] = k[i];
-            V[r * G::kSlots + (slot ^ (r & G::kSwz))] = v[i];
+            K[r * G::kSlots + (slot ^ G::mix(r))] = k[i];
+            V[r * G::kSlots + (slot ^ G::mix(r))] = v[i];
         }
         if (at >= 0) bias[at] = there >> lane & 1 ? 0.f : -INFINITY;
     }
@@ -288,11 +297,11 @@ template <typename T, int HD, int KEYS> struct Copies {
         const int64_t vo = a.one_stride ? ko : p * a.kv.v_stride[0] + r * a.kv.v_stride[2];
         const T *kp = (const T *)a.kv.k + h * a.kv.k_stride[1];
         const T *vp = (const T *)a.kv.v + h * a.kv.v_stride[1];
-        const int swz = (lane % G::kSlots) ^ ((wave * kWide + sub) & G::kSwz);
+        const int swz = (lane % G::kSlots) ^ G::mix(wave * kWide + sub);
         const char *k[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            const int slot = (swz ^ (i * kRows & G::kSwz)) * G::kEl;
+            const int slot = (swz ^ G::mix(i * kRows)) * G::kEl;
             const int64_t o = shuffle(ko, i * kWide + sub);
             k[i] = (const char *)(kp + o + slot);
             v[i] = (const char *)(vp + o + slot);
@@ -301,7 +310,7 @@ template <typename T, int HD, int KEYS> struct Copies {
 #pragma unroll
             for (int i = 0; i < kPer; i++)
                 v[i] = (const char *)(vp + shuffle(vo, i * kWide + sub) +
-                                      (swz ^ (i * kRows & G::kSwz)) * G::kEl);
+                                      (swz ^ G::mix(i * kRows)) * G::kEl);
         }
         if (there != every) {
 #pragma unroll
@@ -396,7 +405,7 @@ template <typename T, int HD, int RT> struct Rows {
             for (int t = 0; t < RT; t++) s[t][k] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int d = 0; d < G::kQ; d++) {
-                const u32x4 w = K[(k * 16 + r) * G::kSlots + ((d * 4 + g) ^ (r & G::kSwz))];
+                const u32x4 w = K[(k * 16 + r) * G::kSlots + ((d * 4 + g) ^ G::mix(r))];
 #pragma unroll
                 for (int t = 0; t < RT; t++) s[t][k] = Mma<T>::qk(w, q[t][d], s[t][k]);
             }
@@ -484,7 +493,7 @@ template <typename T, int HD, int RT> struct Rows {
                     const int key = k * 16 + 4 * g + i;
 #pragma unroll
                     for (int d = 0; d < G::kD; d++) {
-                        const float w = F[(key * G::kSlots + ((d * 4 + (r >> 2)) ^ (key & G::kSwz)))
+                        const float w = F[(key * G::kSlots + ((d * 4 + (r >> 2)) ^ G::mix(key)))
                                           * 4 + (r & 3)];
 #pragma unroll
                         for (int t = 0; t < RT; t++)
@@ -499,7 +508,7 @@ template <typename T, int HD, int RT> struct Rows {
             const int key = 4 * g + (r >> 2), half = r & 1, sub = (r & 3) >> 1;
             auto piece = [&](int k, int d) {
                 const int row = k * 16 + key;
-                const u32x4 *p = V + row * G::kSlots + ((d * 2 + sub) ^ (row & G::kSwz));
+                const u32x4 *p = V + row * G::kSlots + ((d * 2 + sub) ^ G::mix(row));
                 return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                     (lds_s16x4 *)((const u32x2 *)p + half)));
             };
