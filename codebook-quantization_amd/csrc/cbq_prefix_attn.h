@@ -26,6 +26,7 @@
 #pragma once
 
 #include <atomic>
+#include <type_traits>
 
 #include "cbq_device.h"
 #include "cbq_paged.h"
@@ -57,6 +58,9 @@ struct AttnArgs {
     float2 *part_ml;                        // [part][token][n_q]: running maximum, sum
     CbqDiv page;
     int32_t prefix, batch, N, n_q, rep;
+    // Page and row strides in `unit` bytes, a power of two that divides them all:
+    // a row's offset in the pool is one 32-bit number (the host has checked).
+    uint32_t unit, k_page, k_row, v_page, v_row;
     int32_t one_stride;                     // keys and values lie alike
     float c, q_mul;                         // exp2(c * (q_mul q) . k); q_mul folds scale's sign
     Plan plan;
@@ -125,15 +129,16 @@ __device__ __forceinline__ float groups_sum(float x)
 template <typename T, int HD> struct Geo {
     static constexpr int kEl = 16 / (int)sizeof(T);         // elements of a 16-byte slot
     static constexpr int kSlots = HD / kEl;                 // slots of a row
-    // Slot s of a row lies at s ^ mix(row): 16 rows' equal slots in 16 (of rows of
-    // 128 bytes: 8) places, for the reads of K; and of 16-bit types, 8 rows' equal
-    // pairs of slots in 8 places, for the transpose reads of V (a row's 32 bytes
-    // apiece).  Bits are only moved, so mix(a | b) = mix(a) ^ mix(b) for a & b = 0.
+    // Slot s of a row lies at s ^ mix(row): 16 rows' equal slots in 16 places (of
+    // rows of 128 bytes: 8, two rows a bank cycle), for the reads of K; and of
+    // 16-bit types, four rows' equal quads of slots in four places, for the
+    // transpose reads of V.  Bits are only moved, so mix(a | b) = mix(a) ^ mix(b)
+    // for a & b = 0.
     static __device__ __forceinline__ constexpr int mix(int row)
     {
         if (sizeof(T) == 4) return row & 15;
-        if (kSlots == 8) return (row >> 1 & 3) << 1 | (row >> 3 & 1);
-        return (row & 7) << 1 | (row >> 3 & 1);
+        if (kSlots == 8) return (row >> 1 & 1) << 2 | (row >> 3 & 1) << 1 | (row >> 2 & 1);
+        return (row & 3) << 2 | (row >> 2 & 3);
     }
     static constexpr int kQ = kSlots / 4;                   // slots of a query row a lane holds
     static constexpr int kD = HD / 16;                      // 16-value pieces of a row
@@ -191,27 +196,23 @@ template <typename T, int HD, int KEYS, int NT> struct Stage {
         // an id outside the pool (or no key) reads page 0, row 0 and becomes zeros
         const bool in = id >= 0 && id < a.kv.n_pages;
         there = __ballot(in);
-        const int64_t p = in ? id : 0, r = in ? row : 0;
-        const int64_t ko = p * a.kv.k_stride[0] + r * a.kv.k_stride[2];
+        const uint32_t p = in ? id : 0, r = in ? row : 0, ko = p * a.k_page + r * a.k_row;
+        uint32_t o[kPer];
 #pragma unroll
-        for (int i = 0; i < kPer; i++) k[i] = *(const u32x4 *)(kp + shuffle(ko, i * kWide + from));
-        if (a.one_stride) {
-#pragma unroll
-            for (int i = 0; i < kPer; i++)
-                v[i] = *(const u32x4 *)(vp + shuffle(ko, i * kWide + from));
-        } else {
-            const int64_t vo = p * a.kv.v_stride[0] + r * a.kv.v_stride[2];
-#pragma unroll
-            for (int i = 0; i < kPer; i++)
-                v[i] = *(const u32x4 *)(vp + shuffle(vo, i * kWide + from));
+        for (int i = 0; i < kPer; i++) {
+            o[i] = __shfl(ko, i * kWide + from);
+            k[i] = *(const u32x4 *)((const char *)kp + (uint64_t)o[i] * a.unit);
         }
+        if (!a.one_stride) {
+            const uint32_t vo = p * a.v_page + r * a.v_row;
+#pragma unroll
+            for (int i = 0; i < kPer; i++) o[i] = __shfl(vo, i * kWide + from);
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+            v[i] = *(const u32x4 *)((const char *)vp + (uint64_t)o[i] * a.unit);
         if (at >= 0) cbq_key_advance(keys, a.page, step, step_entry, step_row, key, entry, row);
         look(keys);
-    }
-    static __device__ __forceinline__ int64_t shuffle(int64_t x, int lane)
-    {
-        const uint32_t lo = __shfl((int)(uint32_t)x, lane), hi = __shfl((int)(x >> 32), lane);
-        return (int64_t)((uint64_t)hi << 32 | lo);
     }
     static constexpr uint64_t kEvery = kMine == 64 ? ~0ull : (1ull << (kMine & 63)) - 1;
     __device__ __forceinline__ bool missing() const { return there != kEvery; }
@@ -292,26 +293,25 @@ template <typename T, int HD, int KEYS> struct Copies {
         const bool in = id >= 0 && id < a.kv.n_pages;
         const uint64_t there = __ballot(in);
         constexpr uint64_t every = kMine == 64 ? ~0ull : (1ull << (kMine & 63)) - 1;
-        const int64_t p = in ? id : 0, r = in ? row : 0;
-        const int64_t ko = p * a.kv.k_stride[0] + r * a.kv.k_stride[2];
-        const int64_t vo = a.one_stride ? ko : p * a.kv.v_stride[0] + r * a.kv.v_stride[2];
+        const uint32_t p = in ? id : 0, r = in ? row : 0, ko = p * a.k_page + r * a.k_row;
         const T *kp = (const T *)a.kv.k + h * a.kv.k_stride[1];
         const T *vp = (const T *)a.kv.v + h * a.kv.v_stride[1];
         const int swz = (lane % G::kSlots) ^ G::mix(wave * kWide + sub);
         const char *k[kPer];
+        uint32_t o[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            const int slot = (swz ^ G::mix(i * kRows)) * G::kEl;
-            const int64_t o = shuffle(ko, i * kWide + sub);
-            k[i] = (const char *)(kp + o + slot);
-            v[i] = (const char *)(vp + o + slot);
+            o[i] = __shfl(ko, i * kWide + sub);
+            k[i] = (const char *)(kp + (swz ^ G::mix(i * kRows)) * G::kEl) + (uint64_t)o[i] * a.unit;
         }
         if (!a.one_stride) {
+            const uint32_t vo = p * a.v_page + r * a.v_row;
 #pragma unroll
-            for (int i = 0; i < kPer; i++)
-                v[i] = (const char *)(vp + shuffle(vo, i * kWide + sub) +
-                                      (swz ^ G::mix(i * kRows)) * G::kEl);
+            for (int i = 0; i < kPer; i++) o[i] = __shfl(vo, i * kWide + sub);
         }
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+            v[i] = (const char *)(vp + (swz ^ G::mix(i * kRows)) * G::kEl) + (uint64_t)o[i] * a.unit;
         if (there != every) {
 #pragma unroll
             for (int i = 0; i < kPer; i++)
@@ -335,11 +335,6 @@ template <typename T, int HD, int KEYS> struct Copies {
     {
         return (uint32_t)((i * kRows + wave * kWide) * G::kSlots * 16);
     }
-    static __device__ __forceinline__ int64_t shuffle(int64_t x, int lane)
-    {
-        const uint32_t lo = __shfl((int)(uint32_t)x, lane), hi = __shfl((int)(x >> 32), lane);
-        return (int64_t)((uint64_t)hi << 32 | lo);
-    }
 };
 
 // The order of a stretch of code, for the compiler's scheduler: the first AHEAD
@@ -355,6 +350,50 @@ template <int GROUPS, int AHEAD, int MFMA> __device__ __forceinline__ void read_
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// Four values of a row, at hd position d: into the output (part < 0, with the
+// row's sum) or a part's sums.
+template <typename T, int HD>
+__device__ __forceinline__ void put_values(const AttnArgs &a, int part, int64_t token, int head, int d,
+                                           f32x4 x, float sum)
+{
+    const int64_t row = token * a.n_q + head;
+    if (part >= 0) {
+        *(f32x4 *)(a.part_o + ((int64_t)part * a.N * a.n_q + row) * HD + d) = x;
+        return;
+    }
+    const float f = sum == 0.f ? 0.f : 1.0f / sum;
+    x *= f;
+    T *y = (T *)a.out + row * HD + d;
+    if constexpr (sizeof(T) == 4) *(f32x4 *)y = x;
+    else *(u32x2 *)y = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+}
+
+__device__ __forceinline__ void put_stats(const AttnArgs &a, int part, int64_t token, int head,
+                                          float m, float l)
+{
+    if (part >= 0) a.part_ml[((int64_t)part * a.N + token) * a.n_q + head] = make_float2(m, l);
+}
+
+// Keys that the run's token i sees: the prefix, and its own ones up to the token's
+__device__ __forceinline__ int32_t row_sees(int32_t prefix, int32_t past, int32_t i)
+{
+    return prefix + (past + i + 1 > 0 ? past + i + 1 : 0);
+}
+
+// 16 bytes of a query (zeros where the row is none), times scale's sign
+template <typename T> __device__ __forceinline__ u32x4 query_slot(const AttnArgs &a, const T *x, bool in)
+{
+    u32x4 w = {0, 0, 0, 0};
+    if (in) w = *(const u32x4 *)x;
+    if (a.q_mul != 1.0f) {
+        union { u32x4 u; T e[16 / sizeof(T)]; } y = {w};
+#pragma unroll
+        for (int i = 0; i < (int)(16 / sizeof(T)); i++) y.e[i] = (T)((float)y.e[i] * a.q_mul);
+        w = y.u;
+    }
+    return w;
+}
+
 // ---- RT x 16 query rows of one wave --------------------------------------------------
 template <typename T, int HD, int RT> struct Rows {
     using G = Geo<T, HD>;
@@ -363,6 +402,7 @@ template <typename T, int HD, int RT> struct Rows {
     // m, base (m, or 0 where no key was seen) in exp2's domain; l: this lane's keys only
     float m[RT], base[RT], l[RT];
     int32_t sees[RT];                       // keys of the joint axis that the row sees
+    template <int KEYS> using Scores = f32x4[RT][KEYS / 16];
 
     // Rows first .. first + 16 RT - 1 of n; token0 is the token of row 0.
     __device__ __forceinline__ void load(const AttnArgs &a, int h, int64_t token0, int first, int n)
@@ -376,15 +416,7 @@ template <typename T, int HD, int RT> struct Rows {
                          (int64_t)(h * a.rep + r - token * a.rep) * a.q_st[1];
 #pragma unroll
             for (int c = 0; c < G::kQ; c++) {
-                u32x4 w = {0, 0, 0, 0};
-                if (r < n) w = *(const u32x4 *)(x + (c * 4 + g) * G::kEl);
-                if (a.q_mul != 1.0f) {
-                    union { u32x4 u; T e[G::kEl]; } y = {w};
-#pragma unroll
-                    for (int i = 0; i < G::kEl; i++) y.e[i] = (T)((float)y.e[i] * a.q_mul);
-                    w = y.u;
-                }
-                q[t][c] = w;
+                q[t][c] = query_slot(a, x + (c * 4 + g) * G::kEl, r < n);
             }
 #pragma unroll
             for (int d = 0; d < G::kD; d++) o[t][d] = f32x4{0, 0, 0, 0};
@@ -410,6 +442,7 @@ template <typename T, int HD, int RT> struct Rows {
                 for (int t = 0; t < RT; t++) s[t][k] = Mma<T>::qk(w, q[t][d], s[t][k]);
             }
         }
+        read_ahead<NK * G::kQ, 4, RT * (sizeof(T) == 4 ? 4 : 1)>();
     }
 
     // Keys that are not there (bias -inf; their products are 0, or NaN where the
@@ -431,10 +464,12 @@ template <typename T, int HD, int RT> struct Rows {
         }
     }
 
-    // Each row's largest score of the tile, in exp2's domain
-    template <int NK>
-    __device__ __forceinline__ void top(const f32x4 (&s)[RT][NK], float c, float (&x)[RT])
+    // The running maximum follows the scores once they pass it by kSlack (in exp2's
+    // domain): until then weights are at most 2^kSlack and nothing is rescaled.
+    template <int NK> __device__ __forceinline__ void raise(const f32x4 (&s)[RT][NK], float c)
     {
+        float x[RT];
+        bool over = false;
 #pragma unroll
         for (int t = 0; t < RT; t++) {
             x[t] = s[t][0][0];
@@ -443,16 +478,8 @@ template <typename T, int HD, int RT> struct Rows {
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[t] = fmaxf(x[t], s[t][k][i]);
             x[t] = groups_max(x[t]) * c;
+            over = over || x[t] > m[t] + kSlack;
         }
-    }
-
-    // The running maximum follows the scores once they pass it by kSlack: until
-    // then weights are at most 2^kSlack and nothing is rescaled.
-    __device__ __forceinline__ void raise(const float (&x)[RT])
-    {
-        bool over = false;
-#pragma unroll
-        for (int t = 0; t < RT; t++) over = over || x[t] > m[t] + kSlack;
         if (!__any(over)) return;
 #pragma unroll
         for (int t = 0; t < RT; t++) {
@@ -463,6 +490,32 @@ template <typename T, int HD, int RT> struct Rows {
 #pragma unroll
             for (int d = 0; d < G::kD; d++) o[t][d] *= f;
             m[t] = now;
+        }
+    }
+
+    // Row r sees the prefix and the own keys up to its token's
+    __device__ __forceinline__ void see(const AttnArgs &a, int32_t prefix, int32_t past, int first)
+    {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+            sees[t] = row_sees(prefix, past, (first + t * 16 + (int)(threadIdx.x & 15)) / a.rep);
+    }
+
+    __device__ __forceinline__ void put(const AttnArgs &a, int part, int h, int64_t token0, int first,
+                                        int n)
+    {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int r = first + t * 16 + (lane & 15);
+            const float total = groups_sum(l[t]);
+            if (r >= n) continue;
+            const int64_t token = token0 + r / a.rep;
+            const int head = h * a.rep + r % a.rep;
+#pragma unroll
+            for (int d = 0; d < G::kD; d++)
+                put_values<T, HD>(a, part, token, head, d * 16 + 4 * (lane >> 4), o[t][d], total);
+            if (lane < 16) put_stats(a, part, token, head, m[t], total);
         }
     }
 
@@ -580,29 +633,185 @@ template <typename T, int HD, int RT> struct Rows {
     }
 };
 
-// Four values of a row, at hd position d: into the output (part < 0, with the
-// row's sum) or a part's sums.
-template <typename T, int HD>
-__device__ __forceinline__ void put_values(const AttnArgs &a, int part, int64_t token, int head, int d,
-                                           f32x4 x, float sum)
+// ---- 32 query rows of one wave, 16-bit types --------------------------------------------
+// Rows for 32 rows on the 32x32x16 products: half the matrix instructions, one row
+// a lane (lane % 32), and the vector unit overlaps them better (with four additions
+// a 16 cycles of product, 18 % less time a product than 16x16x32).  A lane has keys
+// 8 (i / 4) + 4 (lane / 32) + i % 4 of a 32-key tile, i < 16; eight of them are the
+// right operand of a 16-key value product.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c, __bf16)
 {
-    const int64_t row = token * a.n_q + head;
-    if (part >= 0) {
-        *(f32x4 *)(a.part_o + ((int64_t)part * a.N * a.n_q + row) * HD + d) = x;
-        return;
-    }
-    const float f = sum == 0.f ? 0.f : 1.0f / sum;
-    x *= f;
-    T *y = (T *)a.out + row * HD + d;
-    if constexpr (sizeof(T) == 4) *(f32x4 *)y = x;
-    else *(u32x2 *)y = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c, _Float16)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ void put_stats(const AttnArgs &a, int part, int64_t token, int head,
-                                          float m, float l)
-{
-    if (part >= 0) a.part_ml[((int64_t)part * a.N + token) * a.n_q + head] = make_float2(m, l);
-}
+template <typename T, int HD> struct Rows32 {
+    using G = Geo<T, HD>;
+    static constexpr int kC = HD / 16, kO = HD / 32;
+    u32x4 q[kC];
+    f32x16 o[kO];
+    float m, base, l;                       // as Rows; l: this lane's keys only
+    int32_t sees;
+    template <int KEYS> using Scores = f32x16[KEYS / 32];
+
+    __device__ __forceinline__ void load(const AttnArgs &a, int h, int64_t token0, int first, int n)
+    {
+        const int lane = threadIdx.x & 63, r = first + (lane & 31), token = r / a.rep;
+        const T *x = (const T *)a.q + (token0 + token) * a.q_st[0] +
+                     (int64_t)(h * a.rep + r - token * a.rep) * a.q_st[1];
+#pragma unroll
+        for (int c = 0; c < kC; c++) q[c] = query_slot(a, x + (c * 2 + (lane >> 5)) * G::kEl, r < n);
+#pragma unroll
+        for (int d = 0; d < kO; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] = 0.f;
+        m = -INFINITY;
+        base = l = 0.f;
+        sees = INT32_MAX;
+    }
+
+    template <int NK> __device__ __forceinline__ void scores(const u32x4 *K, f32x16 (&s)[NK])
+    {
+        const int lane = threadIdx.x & 63, r = lane & 31;
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[k][i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < kC; c++)
+#pragma unroll
+            for (int k = 0; k < NK; k++)
+                s[k] = mma32(K[(k * 32 + r) * G::kSlots + ((c * 2 + (lane >> 5)) ^ G::mix(r))], q[c],
+                             s[k], T());
+        read_ahead<NK * kC, 4, 1>();
+    }
+
+    template <int NK>
+    __device__ __forceinline__ void hide(f32x16 (&s)[NK], const float *bias, int32_t key0)
+    {
+        const int g = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int key = k * 32 + 8 * j + 4 * g;
+                const f32x4 b = *(const f32x4 *)(bias + key);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float x = s[k][4 * j + i] + b[i];
+                    s[k][4 * j + i] = key0 + key + i < sees ? x : -INFINITY;
+                }
+            }
+    }
+
+    template <int NK> __device__ __forceinline__ void raise(const f32x16 (&s)[NK], float c)
+    {
+        float x = s[0][0];
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) x = fmaxf(x, s[k][i]);
+        auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])) * c;
+        if (!__any(x > m + kSlack)) return;
+        x = fmaxf(m, x);
+        base = x == -INFINITY ? 0.f : x;
+        const float f = __builtin_amdgcn_exp2f(m - base);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < kO; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] *= f;
+        m = x;
+    }
+
+    __device__ __forceinline__ void see(const AttnArgs &a, int32_t prefix, int32_t past, int first)
+    {
+        sees = row_sees(prefix, past, (first + (int)(threadIdx.x & 31)) / a.rep);
+    }
+
+    __device__ __forceinline__ void put(const AttnArgs &a, int part, int h, int64_t token0, int first,
+                                        int n)
+    {
+        const int lane = threadIdx.x & 63, r = first + (lane & 31);
+        auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        const float total = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+        if (r >= n) return;
+        const int64_t token = token0 + r / a.rep;
+        const int head = h * a.rep + r % a.rep;
+#pragma unroll
+        for (int d = 0; d < kO; d++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                put_values<T, HD>(a, part, token, head, d * 32 + 8 * j + 4 * (lane >> 5),
+                                  f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]},
+                                  total);
+        if (lane < 32) put_stats(a, part, token, head, m, total);
+    }
+
+    // Weights of the tile, and the values under them: 16 keys' values are read while
+    // the 16 before them are in the products, beside which the 16 keys' weights after
+    // them are made.
+    template <int NK>
+    __device__ __forceinline__ void values(const u32x4 *V, const f32x16 (&s)[NK], float c)
+    {
+        const int lane = threadIdx.x & 63, r = lane & 15;
+        const int key = 4 * (lane >> 5) + (r >> 2), sub = (lane >> 4 & 1) * 2 + ((r & 3) >> 1);
+        auto piece = [&](int row0, int d) {
+            const int row = row0 + key;
+            const u32x4 *p = V + row * G::kSlots + ((d * 4 + sub) ^ G::mix(row));
+            return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4 *)((const u32x2 *)p + (r & 1))));
+        };
+        u32x2 v[2][kO][2];
+        u32x4 p[2];
+        auto read = [&](int j) {
+#pragma unroll
+            for (int d = 0; d < kO; d++) {
+                v[j & 1][d][0] = piece(j * 16, d);
+                v[j & 1][d][1] = piece(j * 16 + 8, d);
+            }
+        };
+        auto weigh = [&](int j) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                x[i] = __builtin_amdgcn_exp2f(fmaf(s[j / 2][j % 2 * 8 + i], c, -base));
+            l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+            p[j & 1] = u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]),
+                             pack2<T>(x[6], x[7])};
+        };
+        read(0);
+        weigh(0);
+#pragma unroll
+        for (int j = 0; j < 2 * NK; j++) {
+            if (j + 1 < 2 * NK) read(j + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < kO; d++) {
+                const u32x2 x = v[j & 1][d][0], y = v[j & 1][d][1];
+                o[d] = mma32(u32x4{x[0], x[1], y[0], y[1]}, p[j & 1], o[d], T());
+            }
+            if (j + 1 < 2 * NK) {
+                weigh(j + 1);
+#pragma unroll
+                for (int i = 0; i < kO; i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 20 / kO, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x400, 8 / kO, 0);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
 
 // ---- 64 RT rows of a block against keys [first, end), tiles shared by the waves ----------
 template <typename T, int HD, int RT, bool CAUSAL>
@@ -611,30 +820,25 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
                                            int32_t past, int part)
 {
     using G = Geo<T, HD>;
-    constexpr int KEYS = G::kBlockKeys, NK = KEYS / 16, kTile = KEYS * G::kSlots;
+    constexpr int KEYS = G::kBlockKeys, kTile = KEYS * G::kSlots;
     constexpr uint32_t kBytes = kTile * 16;
     u32x4 *K = (u32x4 *)lds, *V = K + 2 * kTile;
     float *bias = (float *)(V + 2 * kTile);
     int32_t *flags = (int32_t *)(bias + 2 * KEYS);
     const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds,
                    lds_v = lds_k + 2 * kBytes;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int mine = row0 + wave * 16 * RT;
-    Rows<T, HD, RT> w;
+    std::conditional_t<RT == 2 && sizeof(T) == 2, Rows32<T, HD>, Rows<T, HD, RT>> w;
     Copies<T, HD, KEYS> st;
     st.start(a, keys, first);
     w.load(a, h, token0, mine, n);
     int32_t all = INT32_MAX;                    // keys that every row of the block sees
     if (CAUSAL) {
-        all = keys.prefix + (past + row0 / a.rep + 1 > 0 ? past + row0 / a.rep + 1 : 0);
-#pragma unroll
-        for (int t = 0; t < RT; t++) {
-            const int32_t own = past + (mine + t * 16 + (lane & 15)) / a.rep + 1;
-            w.sees[t] = keys.prefix + (own > 0 ? own : 0);
-        }
+        all = row_sees(keys.prefix, past, row0 / a.rep);
+        w.see(a, keys.prefix, past, mine);
     }
     const int tiles = keys.end > first ? (keys.end - first + KEYS - 1) / KEYS : 0;
-    constexpr int kF = sizeof(T) == 4 ? 4 : 1;          // matrix instructions a product
     auto step = [&](int i, int b) {
         if (i + 1 < tiles) {
             st.keys_to(a, keys, h, lds_k + (b ^ 1) * kBytes, bias + (b ^ 1) * KEYS,
@@ -643,15 +847,12 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
         }
         const int32_t key0 = first + i * KEYS;
         const int4 miss = *(const int4 *)(flags + b * kWaves);
-        f32x4 s[RT][NK];
+        typename decltype(w)::template Scores<KEYS> s;
         __builtin_amdgcn_sched_barrier(0);
         w.scores(K + b * kTile, s);
-        read_ahead<NK * G::kQ, 4, RT * kF>();
         if (key0 + KEYS > all || __builtin_amdgcn_readfirstlane(miss.x | miss.y | miss.z | miss.w))
             w.hide(s, bias + b * KEYS, key0);
-        float top[RT];
-        w.top(s, a.c, top);
-        w.raise(top);
+        w.raise(s, a.c);
         w.values(V + b * kTile, s, a.c);
         stage_wait();
     };
@@ -666,18 +867,7 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
             if (i + 2 >= tiles) break;
         }
     }
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int r = mine + t * 16 + (lane & 15);
-        const float l = groups_sum(w.l[t]);
-        if (r >= n) continue;
-        const int64_t token = token0 + r / a.rep;
-        const int head = h * a.rep + r % a.rep;
-#pragma unroll
-        for (int d = 0; d < G::kD; d++)
-            put_values<T, HD>(a, part, token, head, d * 16 + 4 * (lane >> 4), w.o[t][d], l);
-        if (lane < 16) put_stats(a, part, token, head, w.m[t], l);
-    }
+    w.put(a, part, h, token0, mine, n);
 }
 
 // ---- 16 rows of a block, the keys [first, end) dealt to its waves ------------------------
@@ -700,9 +890,8 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
     w.load(a, h, token0, row0, n);
     int32_t all = INT32_MAX;
     if (CAUSAL) {
-        all = keys.prefix + (past + row0 / a.rep + 1 > 0 ? past + row0 / a.rep + 1 : 0);
-        const int32_t own = past + (row0 + r) / a.rep + 1;
-        w.sees[0] = keys.prefix + (own > 0 ? own : 0);
+        all = row_sees(keys.prefix, past, row0 / a.rep);
+        w.see(a, keys.prefix, past, row0);
     }
     const int32_t begin = first + wave * KEYS, step = kWaves * KEYS;
     if (begin < keys.end) st.load(a, keys, h);
@@ -716,9 +905,7 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
         f32x4 s[1][KEYS / 16];
         w.scores(K, s);
         if (missing || key0 + KEYS > all) w.hide(s, bias, key0);
-        float top[1];
-        w.top(s, a.c, top);
-        w.raise(top);
+        w.raise(s, a.c);
         w.values(V, s, a.c);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -858,8 +1045,7 @@ __global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void pro
     const int32_t len = cbq_clamp_length(a.lengths[run], a.capacity), past = len - count;
     const int rows = count * a.rep, row0 = tile * M;
     const int last = (row0 + M < rows ? row0 + M : rows) - 1;
-    const int32_t own = past + last / a.rep + 1;
-    const int32_t sees = a.prefix + (own > 0 ? own : 0);        // of the tile's last row
+    const int32_t sees = row_sees(a.prefix, past, last / a.rep);        // of the tile's last row
     int32_t first = 0, end = sees;
     if (a.plan.parts > 1)
         prompt_keys(sees, a.plan.parts, part,

@@ -1,5 +1,7 @@
 // C entry points of the attention over a paged cache (include/cbq_serve.h):
 // argument checks, launch plans, dispatch by type.
+#include <initializer_list>
+
 #include "cbq_prefix_attn.h"
 
 using namespace cbq_attn;
@@ -51,6 +53,16 @@ int attend(const void *q, const int64_t *q_stride, const int32_t *q_start,
     for (int i = 0; i < 3; i++)
         aligned = aligned && cache->k_stride[i] * e % 16 == 0 && cache->v_stride[i] * e % 16 == 0;
     if (!aligned) return CK_ERR_ARG;
+    // rows as 32-bit offsets in the strides' common power of two: 512 GiB with
+    // strides of whole 128 bytes
+    uint64_t bits = 4096;
+    for (int i = 0; i < 3; i += 2) bits |= (uint64_t)(cache->k_stride[i] * e | cache->v_stride[i] * e);
+    const int64_t unit = (int64_t)(bits & (~bits + 1));
+    for (const int64_t *st : {cache->k_stride, cache->v_stride})
+        if (st[0] < 0 || st[2] < 0 || st[0] >= (1ll << 40) || st[2] >= (1ll << 40) ||
+            ((double)cache->n_pages * (double)st[0] + (double)cache->page * (double)st[2]) * (double)e >=
+                4294967295.0 * (double)unit)
+            return CK_ERR_ARG;
     Plan p;
     if (!make_plan(cache, prefix, width, batch, N, n_q, prompt, p)) return CK_ERR_ARG;
     if (p.bytes && (!workspace || workspace_bytes < (size_t)p.bytes ||
@@ -61,6 +73,11 @@ int attend(const void *q, const int64_t *q_stride, const int32_t *q_start,
     a.q_st[0] = q_stride[0];
     a.q_st[1] = q_stride[1];
     a.kv = *cache;
+    a.unit = (uint32_t)unit;
+    a.k_page = (uint32_t)(cache->k_stride[0] * e / unit);
+    a.k_row = (uint32_t)(cache->k_stride[2] * e / unit);
+    a.v_page = (uint32_t)(cache->v_stride[0] * e / unit);
+    a.v_row = (uint32_t)(cache->v_stride[2] * e / unit);
     a.one_stride = cache->k_stride[0] == cache->v_stride[0] &&
                    cache->k_stride[2] == cache->v_stride[2];
     a.prefix_table = prefix_table; a.tables = tables; a.lengths = lengths; a.q_start = q_start;
