@@ -337,6 +337,35 @@ template <typename T, int HD, int KEYS> struct Copies {
     }
 };
 
+// Whether a tile of values holds one that is not finite; uniform over the wave.
+template <typename T, int HD, int KEYS> __device__ __forceinline__ bool odd_tile(const u32x4 *V)
+{
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    const int lane = threadIdx.x & 63;
+    constexpr int kTimes = KEYS * Geo<T, HD>::kSlots / CBQ_WAVE;
+    if constexpr (sizeof(T) == 4) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < kTimes; i++) {
+            const u32x4 w = V[i * CBQ_WAVE + lane];
+#pragma unroll
+            for (int j = 0; j < 4; j++) top = max(top, w[j] & 0x7fffffffu);
+        }
+        return __any(top >= 0x7f800000u);
+    } else {
+        u16x2 top = {0, 0};
+#pragma unroll
+        for (int i = 0; i < kTimes; i++) {
+            const u32x4 w = V[i * CBQ_WAVE + lane];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[j] & 0x7fff7fffu));
+        }
+        constexpr uint16_t inf = std::is_same_v<T, __bf16> ? 0x7f80 : 0x7c00;
+        return __any(top[0] >= inf || top[1] >= inf);
+    }
+}
+
 // The order of a stretch of code, for the compiler's scheduler: the first AHEAD
 // LDS reads, then GROUPS times matrix instructions and one more read.
 template <int GROUPS, int AHEAD, int MFMA> __device__ __forceinline__ void read_ahead()
@@ -813,6 +842,70 @@ template <typename T, int HD> struct Rows32 {
     }
 };
 
+// ---- rows key by key --------------------------------------------------------------------
+// A weight of 0 times an infinite value is no number, so in a matrix product a key
+// that only some of the rows see would reach the others too.  Blocks whose causal
+// masks cut a tile with such a value leave their products and do their rows `row0`
+// .. `row0 + m - 1` here, a wave a row, a lane a key, where a hidden key's value is
+// never touched.
+template <typename T, int HD>
+__device__ __forceinline__ void plain_rows(const AttnArgs &a, int h, int64_t token0, int row0, int m,
+                                           int n, const CbqKeys &keys, int32_t first, int32_t past,
+                                           int part)
+{
+    using G = Geo<T, HD>;
+    constexpr int kLane = HD / CBQ_WAVE;
+    const int lane = threadIdx.x & 63;
+    const int stop = row0 + m < n ? row0 + m : n;
+    for (int r = row0 + (int)(threadIdx.x >> 6); r < stop; r += blockDim.x >> 6) {
+        const int token = r / a.rep, head = h * a.rep + r - token * a.rep;
+        const T *x = (const T *)a.q + (token0 + token) * a.q_st[0] + head * a.q_st[1];
+        const int32_t sees = row_sees(keys.prefix, past, token), end = sees < keys.end ? sees : keys.end;
+        float top = -INFINITY, l = 0.f, o[kLane] = {};
+        for (int32_t key0 = first; key0 < end; key0 += CBQ_WAVE) {
+            const int32_t key = key0 + lane;
+            int32_t entry, row, id = -1;
+            cbq_key_place(keys, a.page, key, entry, row);
+            if (key < end) id = (key < keys.prefix ? keys.shared : keys.own)[entry];
+            const bool in = id >= 0 && id < a.kv.n_pages;
+            const int64_t p = in ? id : 0, at = in ? row : 0;
+            const T *k = (const T *)a.kv.k + p * a.kv.k_stride[0] + h * a.kv.k_stride[1] +
+                         at * a.kv.k_stride[2];
+            const int64_t vo = p * a.kv.v_stride[0] + at * a.kv.v_stride[2];
+            float s = 0.f;
+            for (int c = 0; c < G::kSlots; c++) {
+                union { u32x4 u; T e[G::kEl]; } kw = {*(const u32x4 *)(k + c * G::kEl)},
+                                                qw = {query_slot(a, x + c * G::kEl, true)};
+                for (int i = 0; i < G::kEl; i++) s = fmaf((float)kw.e[i], (float)qw.e[i], s);
+            }
+            s = in ? s * a.c : -INFINITY;
+            float now = s;
+            for (int i = 32; i > 0; i >>= 1) now = fmaxf(now, __shfl_xor(now, i));
+            now = fmaxf(top, now);
+            const float base = now == -INFINITY ? 0.f : now, f = __builtin_amdgcn_exp2f(top - base);
+            const float w = in ? __builtin_amdgcn_exp2f(s - base) : 0.f;
+            top = now;
+            l = l * f + w;
+            for (int i = 0; i < kLane; i++) o[i] *= f;
+            for (uint64_t b = __ballot(in); b; b &= b - 1) {
+                const int at = __builtin_ctzll(b);
+                const float wk = __shfl(w, at);
+                const T *v = (const T *)a.kv.v + h * a.kv.v_stride[1] + lane * kLane +
+                             ((int64_t)__shfl((int)(vo >> 32), at) << 32 |
+                              (uint32_t)__shfl((int)(uint32_t)vo, at));
+                for (int i = 0; i < kLane; i++) o[i] = fmaf(wk, (float)v[i], o[i]);
+            }
+        }
+        for (int i = 32; i > 0; i >>= 1) l += __shfl_xor(l, i);
+        const int64_t at = (token0 + token) * a.n_q + head;
+        for (int i = 0; i < kLane; i++) {
+            if (part >= 0) a.part_o[((int64_t)part * a.N * a.n_q + at) * HD + lane * kLane + i] = o[i];
+            else ((T *)a.out)[at * HD + lane * kLane + i] = (T)(l == 0.f ? 0.f : o[i] / l);
+        }
+        if (lane == 0) put_stats(a, part, token0 + token, head, top, l);
+    }
+}
+
 // ---- 64 RT rows of a block against keys [first, end), tiles shared by the waves ----------
 template <typename T, int HD, int RT, bool CAUSAL>
 __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, int64_t token0,
@@ -839,13 +932,14 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
         w.see(a, keys.prefix, past, mine);
     }
     const int tiles = keys.end > first ? (keys.end - first + KEYS - 1) / KEYS : 0;
-    auto step = [&](int i, int b) {
+    auto step = [&](int i, int b) -> bool {                 // false: a value that is not finite
         if (i + 1 < tiles) {
             st.keys_to(a, keys, h, lds_k + (b ^ 1) * kBytes, bias + (b ^ 1) * KEYS,
                        flags + (b ^ 1) * kWaves);
             st.values_to(lds_v + (b ^ 1) * kBytes);
         }
         const int32_t key0 = first + i * KEYS;
+        if (CAUSAL && key0 + KEYS > all && odd_tile<T, HD, KEYS>(V + b * kTile)) return false;
         const int4 miss = *(const int4 *)(flags + b * kWaves);
         typename decltype(w)::template Scores<KEYS> s;
         __builtin_amdgcn_sched_barrier(0);
@@ -855,17 +949,24 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
         w.raise(s, a.c);
         w.values(V + b * kTile, s, a.c);
         stage_wait();
+        return true;
     };
+    bool fine = true;                           // every wave looks at all of a tile: uniform
     if (tiles > 0) {
         st.keys_to(a, keys, h, lds_k, bias, flags);
         st.values_to(lds_v);
         stage_wait();
         for (int i = 0;; i += 2) {
-            step(i, 0);
-            if (i + 1 >= tiles) break;
-            step(i + 1, 1);
-            if (i + 2 >= tiles) break;
+            fine = step(i, 0);
+            if (!fine || i + 1 >= tiles) break;
+            fine = step(i + 1, 1);
+            if (!fine || i + 2 >= tiles) break;
         }
+    }
+    if (CAUSAL && !fine) {
+        stage_wait();                           // no copy is under way when the block ends
+        plain_rows<T, HD>(a, h, token0, row0, 16 * RT * kWaves, n, keys, first, past, part);
+        return;
     }
     w.put(a, part, h, token0, mine, n);
 }
@@ -894,6 +995,7 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
         w.see(a, keys.prefix, past, row0);
     }
     const int32_t begin = first + wave * KEYS, step = kWaves * KEYS;
+    int odd = 0;                                // a value that is not finite
     if (begin < keys.end) st.load(a, keys, h);
     for (int32_t key0 = begin; key0 < keys.end; key0 += step) {
         const bool missing = st.missing();
@@ -902,6 +1004,10 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         if (key0 + step < keys.end) st.load(a, keys, h);
+        if (CAUSAL && key0 + KEYS > all && odd_tile<T, HD, KEYS>(V)) {
+            odd = 1;
+            break;
+        }
         f32x4 s[1][KEYS / 16];
         w.scores(K, s);
         if (missing || key0 + KEYS > all) w.hide(s, bias, key0);
@@ -913,7 +1019,14 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
     }
     // merge: statistics first, then the weighted values, each wave's scaled to
     // the common maximum
-    __syncthreads();                            // every wave is past its tiles
+    if (CAUSAL) {
+        if (__syncthreads_or(odd)) {
+            plain_rows<T, HD>(a, h, token0, row0, 16, n, keys, first, past, part);
+            return;
+        }
+    } else {
+        __syncthreads();                        // every wave is past its tiles
+    }
     float *O = (float *)lds, *ML = O + kWaves * 16 * HD;
     const float l = groups_sum(w.l[0]);
     if (lane < 16) {

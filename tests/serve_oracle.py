@@ -13,7 +13,8 @@ and S = scale * max_j sum |q_i k_ij|:
   - sums of n weights, 16 or 64 at a time and joined over waves and parts, are
     off by fewer than n / 16 + 64 half steps of A;
   - 16-bit weights are rounded to the type: half a step of A, and for fp16,
-    whose smallest step is 2^-24, 2^-25 a weight: n 2^-25 max|v| / sum p.
+    whose smallest step is 2^-24, 2^-25 a weight: n 2^-25 max|v| / sum p, the
+    maximum over the keys.
 """
 import random
 
@@ -117,7 +118,7 @@ def attend(batch, q, q_start, scale):
                 if batch.dtype != torch.float32:
                     tol[t, h] += half * mass
                 if batch.dtype == torch.float16:
-                    tol[t, h] += n * 2.0 ** -25 * float(vs.abs().max()) / total + 2.0 ** -25
+                    tol[t, h] += n * 2.0 ** -25 * vs.abs().amax(0) / total + 2.0 ** -25
     return out, tol
 
 

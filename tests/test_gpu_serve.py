@@ -265,6 +265,42 @@ def test_not_numbers_stay_in_their_rows(cuda, ops, dtype):
     so.near(out[~nan], want[~nan], tol[~nan], "beside NaN")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd,runs,past,n_kv,rep", [
+    (64, [60, 60], 10, 1, 2),                                   # 16 rows a block
+    (128, [60, 60], 10, 1, 2),
+    (256, [40, 33], 3, 2, 1),
+    (64, [12] * 30, 7, 8, 4),                                   # 64 rows a block
+    (128, [12] * 30, 7, 8, 4),
+    (256, [12] * 30, 7, 8, 4),
+    (64, [300, 129], 20, 8, 4),                                 # the widest
+    (128, [300, 129], 20, 8, 4),
+    (256, [300, 129], 20, 8, 4),
+    (64, [30, 40], 3000, 1, 4),                                 # keys in parts
+    (128, [3, 5], 2500, 1, 2),
+])
+def test_values_not_finite(cuda, ops, dtype, hd, runs, past, n_kv, rep):
+    """Infinite values and NaN among the own keys: tokens before them keep their
+    outputs, tokens from them on get inf or NaN in the same places."""
+    b = Batch([past + n for n in runs], 0, n_kv, rep, hd, 16, dtype, seed=hd)
+    inf, nan = float("inf"), float("nan")
+    for i, (d, x) in enumerate([(3, inf), (17, -inf), (40, nan), (40, inf), (63, inf), (63, -inf)]):
+        j = past + 4 + 3 * (i // 2) - i % 2                     # keys of the last run, two side by side
+        p, r = int(b.tables[-1, j // 16]), j % 16
+        b.v[p, :, r, d] = x
+    for h, j in ((0, past + runs[0] // 2), (n_kv - 1, past + runs[0] - 1)):
+        b.v[int(b.tables[0, j // 16]), h, j % 16, hd - 1] = nan if h else -inf
+    q, q_start = b.queries(sum(runs), 1.5), starts(runs)
+    print(f"values not finite {dtype} hd={hd} runs={runs[:3]}", flush=True)
+    got = prompt(ops, b, q, q_start, hd ** -0.5).double().cpu()
+    want, tol = so.attend(b, q, q_start, hd ** -0.5)
+    odd = ~want.isfinite()
+    assert odd.any() and not odd.all()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    so.near(got[~odd], want[~odd], tol[~odd], "beside them")
+
+
 @pytest.mark.parametrize("parts", [False, True])
 def test_all_scores_nan(cuda, ops, parts):
     b = Batch([3000 if parts else 20], 0, 1, 1, 64, 16, "f32", seed=13)
