@@ -186,13 +186,12 @@ inline bool plan_fits(const Plan &p)
 // Decode: blocks of the prefix's parts first (they compute), then own parts
 // (they read), so that both kinds share the CUs.
 struct DecodeWork {
-    bool skip;                              // nothing to do
     int h, tile, part, seq;                 // seq -1: the prefix
-    int32_t first, end;                     // keys
+    int32_t first, end;                     // keys (own ones: as the capacity has them)
 };
 
 CBQ_PAGED_FN DecodeWork decode_work(const Plan &p, uint32_t block, int n_kv, int batch,
-                                    int32_t prefix, const int32_t *lengths, int64_t capacity)
+                                    int32_t prefix, int64_t capacity)
 {
     DecodeWork w;
     uint32_t i = block;
@@ -201,7 +200,6 @@ CBQ_PAGED_FN DecodeWork decode_work(const Plan &p, uint32_t block, int n_kv, int
     if (!shared) i -= pre;
     w.h = (int)(i % n_kv);
     i /= n_kv;
-    w.skip = false;
     if (shared) {
         w.tile = (int)(i % p.tiles);
         w.part = (int)(i / p.tiles);
@@ -214,12 +212,9 @@ CBQ_PAGED_FN DecodeWork decode_work(const Plan &p, uint32_t block, int n_kv, int
     i /= p.own_tiles;
     w.seq = (int)(i % batch);
     const int chunk = (int)(i / batch);
-    const int32_t len = cbq_clamp_length(lengths[w.seq], capacity);
-    const int64_t first = (int64_t)chunk * p.own_chunk;
     w.part = p.pre_parts + chunk;
-    w.first = (int32_t)cbq_min(first, len);
-    w.end = (int32_t)cbq_min(first + p.own_chunk, len);
-    w.skip = first >= len && (p.parts > 1 || chunk > 0);
+    w.first = (int32_t)cbq_min((int64_t)chunk * p.own_chunk, capacity);
+    w.end = (int32_t)cbq_min((int64_t)w.first + p.own_chunk, capacity);
     return w;
 }
 

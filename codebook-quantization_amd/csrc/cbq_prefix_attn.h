@@ -181,6 +181,7 @@ template <typename T, int HD, int KEYS, int NT> struct Stage {
         cbq_key_place(keys, a.page, key, entry, row);
         look(keys);
     }
+    // keys.end may be larger than the length, until load(): a look waits for no length
     __device__ __forceinline__ void look(const CbqKeys &keys)
     {
         id = -1;
@@ -194,7 +195,7 @@ template <typename T, int HD, int KEYS, int NT> struct Stage {
         const T *kp = (const T *)a.kv.k + h * a.kv.k_stride[1] + slot;
         const T *vp = (const T *)a.kv.v + h * a.kv.v_stride[1] + slot;
         // an id outside the pool (or no key) reads page 0, row 0 and becomes zeros
-        const bool in = id >= 0 && id < a.kv.n_pages;
+        const bool in = id >= 0 && id < a.kv.n_pages && key < keys.end;
         there = __ballot(in);
         const uint32_t p = in ? id : 0, r = in ? row : 0, ko = p * a.k_page + r * a.k_row;
         uint32_t o[kPer];
@@ -976,8 +977,9 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
 // barrier, and the four running states are merged at the end.
 template <typename T, int HD, bool CAUSAL>
 __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, int64_t token0,
-                                          int row0, int n, const CbqKeys &keys, int32_t first,
-                                          int32_t past, int part)
+                                          int row0, int n, CbqKeys keys, int32_t first,
+                                          int32_t past, int part, const int32_t *length = nullptr,
+                                          bool always = false)
 {
     using G = Geo<T, HD>;
     constexpr int KEYS = G::kWaveKeys, kTile = KEYS * G::kSlots;
@@ -993,6 +995,11 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
     if (CAUSAL) {
         all = row_sees(keys.prefix, past, row0 / a.rep);
         w.see(a, keys.prefix, past, row0);
+    }
+    if (length) {                               // decode: the own keys end there
+        const int32_t len = cbq_clamp_length(*length, a.capacity);
+        if (first >= len && !always) return;    // the merge counts own parts by the length
+        if (len < keys.end) keys.end = len;
     }
     const int32_t begin = first + wave * KEYS, step = kWaves * KEYS;
     int odd = 0;                                // a value that is not finite
@@ -1089,9 +1096,7 @@ template <typename T, int HD, int PT>
 __global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void decode_kernel(AttnArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const DecodeWork w = decode_work(a.plan, blockIdx.x, a.kv.n_kv, a.batch, a.prefix, a.lengths,
-                                     a.capacity);
-    if (w.skip) return;                             // the merge counts own parts by the length
+    const DecodeWork w = decode_work(a.plan, blockIdx.x, a.kv.n_kv, a.batch, a.prefix, a.capacity);
     const int to = a.plan.parts > 1 ? w.part : -1;
     if (w.seq < 0) {
         const CbqKeys keys = {a.prefix_table, nullptr, a.prefix, w.end};
@@ -1103,7 +1108,8 @@ __global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void dec
         return;
     }
     const CbqKeys keys = {nullptr, a.tables + w.seq * a.table_st, 0, w.end};
-    wave_rows<T, HD, false>(a, lds, w.h, w.seq, w.tile * 16, a.rep, keys, w.first, 0, to);
+    wave_rows<T, HD, false>(a, lds, w.h, w.seq, w.tile * 16, a.rep, keys, w.first, 0, to,
+                            a.lengths + w.seq, a.plan.parts == 1);
 }
 
 // ---- prompt: tiles of each run's rows against the keys they see -----------------------------
@@ -1129,10 +1135,13 @@ __global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void pro
             out[e < lo * w ? e : e + (hi - lo) * w] = (T)0.f;
     }
     // the run that holds tile `want`: its count of tiles, summed over the runs
-    int32_t before = 0, run = -1, tile = 0, first_token = 0, count = 0;
+    int32_t before = 0, run = -1, tile = 0, first_token = 0, count = 0, length = 0;
     for (int b0 = 0; b0 < a.batch && run < 0; b0 += CBQ_WAVE) {
-        int32_t f = 0, n = 0;
-        if (b0 + lane < a.batch) cbq_run(a.q_start, b0 + lane, a.N, f, n);
+        int32_t f = 0, n = 0, len = 0;
+        if (b0 + lane < a.batch) {
+            cbq_run(a.q_start, b0 + lane, a.N, f, n);
+            len = a.lengths[b0 + lane];
+        }
         const int32_t mine = (int32_t)(((int64_t)n * a.rep + M - 1) / M);
         int32_t upto = mine;
         for (int o = 1; o < CBQ_WAVE; o <<= 1) {
@@ -1146,6 +1155,7 @@ __global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void pro
             tile = want - before - __shfl(upto - mine, at);
             first_token = __shfl(f, at);
             count = __shfl(n, at);
+            length = __shfl(len, at);
         } else {
             before += __shfl(upto, CBQ_WAVE - 1);
         }
@@ -1155,7 +1165,8 @@ __global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void pro
     tile = __builtin_amdgcn_readfirstlane(tile);
     first_token = __builtin_amdgcn_readfirstlane(first_token);
     count = __builtin_amdgcn_readfirstlane(count);
-    const int32_t len = cbq_clamp_length(a.lengths[run], a.capacity), past = len - count;
+    const int32_t len = cbq_clamp_length(__builtin_amdgcn_readfirstlane(length), a.capacity),
+                  past = len - count;
     const int rows = count * a.rep, row0 = tile * M;
     const int last = (row0 + M < rows ? row0 + M : rows) - 1;
     const int32_t sees = row_sees(a.prefix, past, last / a.rep);        // of the tile's last row
@@ -1182,27 +1193,32 @@ template <typename T, int HD> __global__ __launch_bounds__(kThreads) void merge_
     __shared__ float totals[kGroups];
     const int64_t row = blockIdx.x, rows = (int64_t)a.N * a.n_q, token = row / a.n_q;
     const int tid = threadIdx.x, lane = tid & 63, group = tid / kLanes, d = tid % kLanes * 4;
-    int parts = a.plan.parts;
-    if (a.plan.own_chunk > 0) {                     // decode: as many own parts as the length has
-        const int32_t len = cbq_clamp_length(a.lengths[token], a.capacity);
-        parts = a.plan.pre_parts + (int)cbq_ceil(len, a.plan.own_chunk);
-    } else {                                        // prompt: a token of no run keeps its zeros
-        if (token < a.q_start[0] || token >= a.q_start[a.batch]) return;
-    }
+    // The first parts' loads wait for no length: what a part that was not written
+    // holds is dropped.
+    const int most = a.plan.parts;
     f32x4 o[kAhead];
     float2 ml[kAhead];
     auto part = [&](int p, f32x4 &x, float2 &s) {
         x = f32x4{0, 0, 0, 0};
         s = make_float2(-INFINITY, 0.f);
-        if (p < parts) {
+        if (p < most) {
             x = *(const f32x4 *)(a.part_o + (p * rows + row) * HD + d);
             s = a.part_ml[p * rows + row];
         }
     };
 #pragma unroll
     for (int i = 0; i < kAhead; i++) part(group + i * kGroups, o[i], ml[i]);
-    float top = -INFINITY;
-    for (int p = lane; p < parts; p += CBQ_WAVE) top = fmaxf(top, a.part_ml[p * rows + row].x);
+    float m0 = lane < most ? a.part_ml[lane * rows + row].x : -INFINITY;
+    int parts = most;
+    if (a.plan.own_chunk > 0) {                     // decode: as many own parts as the length has
+        const int32_t len = cbq_clamp_length(a.lengths[token], a.capacity);
+        parts = a.plan.pre_parts + (int)cbq_ceil(len, a.plan.own_chunk);
+    } else {                                        // prompt: a token of no run keeps its zeros
+        if (token < a.q_start[0] || token >= a.q_start[a.batch]) return;
+    }
+    float top = lane < parts ? m0 : -INFINITY;
+    for (int p = lane + CBQ_WAVE; p < parts; p += CBQ_WAVE)
+        top = fmaxf(top, a.part_ml[p * rows + row].x);
     for (int i = 32; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
     const float base = top == -INFINITY ? 0.f : top;
     f32x4 x = {0, 0, 0, 0};
@@ -1210,8 +1226,9 @@ template <typename T, int HD> __global__ __launch_bounds__(kThreads) void merge_
     for (int p0 = group;; p0 += kAhead * kGroups) {
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            const float w = __builtin_amdgcn_exp2f(ml[i].x - base);
-            sum += w * ml[i].y;                     // 0 of an empty part; a NaN stays
+            const bool in = p0 + i * kGroups < parts;
+            const float w = in ? __builtin_amdgcn_exp2f(ml[i].x - base) : 0.f;
+            sum += in ? w * ml[i].y : 0.f;          // 0 of an empty part; a NaN stays
             // the values of a part that saw no key are not written
 #pragma unroll
             for (int e = 0; e < 4; e++) x[e] = w == 0.f ? x[e] : fmaf(w, o[i][e], x[e]);

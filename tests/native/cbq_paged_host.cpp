@@ -84,7 +84,7 @@ static void decode()
     std::map<std::vector<int>, int> parts;
     const int m = p.rt ? 64 * p.rt : 16, step = p.rt ? block_keys(hd * size) : wave_keys(hd * size) * kAttnWaves;
     for (int64_t i = 0; i < p.blocks; i++) {
-        const DecodeWork w = decode_work(p, (uint32_t)i, n_kv, batch, prefix, lengths.data(), capacity);
+        const DecodeWork w = decode_work(p, (uint32_t)i, n_kv, batch, prefix, capacity);
         CHECK(w.h >= 0 && w.h < n_kv);
         if (w.seq < 0) {
             CHECK(w.tile >= 0 && w.tile * m < batch * rep && w.part >= 0 && w.part < p.pre_parts);
@@ -93,12 +93,20 @@ static void decode()
             walk({prefix_table.data(), nullptr, prefix, w.end}, pg, w.first, step, prefix_table, nullptr, 0, s);
         } else {
             CHECK(w.seq < batch && w.tile * 16 < rep);
-            if (w.skip) continue;
+            // as the kernel: first table entries by the capacity, then the length
+            int32_t entry, row;
+            for (int lane = 0; lane < 64; lane++) {
+                const int32_t j = w.first + lane;
+                cbq_key_place({nullptr, tables.data() + (size_t)w.seq * width, 0, w.end}, pg, j, entry, row);
+                CHECK(j >= w.end || entry < width);
+            }
+            const int32_t len = cbq_clamp_length(lengths[w.seq], capacity);
+            if (w.first >= len && p.parts > 1) continue;
             CHECK(w.part >= p.pre_parts && w.part < p.parts);
             const int32_t *own = tables.data() + (size_t)w.seq * width;
             auto &s = seen[{w.h, w.seq, w.tile}];
             s.resize(capacity);
-            walk({nullptr, own, 0, w.end}, pg, w.first, step, prefix_table, own, width, s);
+            walk({nullptr, own, 0, (int32_t)cbq_min(w.end, len)}, pg, w.first, step, prefix_table, own, width, s);
             parts[{w.h, w.seq, w.tile}]++;
         }
     }
