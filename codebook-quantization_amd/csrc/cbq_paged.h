@@ -96,6 +96,7 @@ struct Plan {
     int32_t pre_parts, pre_chunk;           // decode: parts of the prefix and their keys
     int32_t own_parts, own_chunk, own_tiles;    // decode: parts of the own keys, 16-row tiles
     int32_t parts;                          // decode: all of them; prompt: key parts of a tile
+    int32_t joint;                          // decode: a sequence's one part walks the prefix too
     int64_t blocks, bytes;
 };
 
@@ -121,6 +122,17 @@ inline Plan plan_decode(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
 {
     Plan p = {};
     const int64_t rows = batch * rep, bk = block_keys(row_bytes), wk = kAttnWaves * wave_keys(row_bytes);
+    if (prefix + capacity <= 4 * wk) {
+        // Few keys: prefix and own ones by one block a sequence and kv head, four
+        // tiles a wave at most.  Parts would be shorter by less than their merge
+        // takes (4 us): two sequences of 3..18 keys, room for 300: 9.6 -> 6 us.
+        p.joint = 1;
+        p.own_parts = p.parts = 1;
+        p.own_chunk = (int32_t)cbq_max(prefix + capacity, 1);
+        p.own_tiles = (int32_t)cbq_ceil(rep, 16);
+        p.blocks = n_kv * batch * p.own_tiles;
+        return p;
+    }
     p.rt = rows <= 16 ? 0 : rows <= 64 ? 1 : widest(row_bytes);
     int64_t tiles = cbq_ceil(rows, p.rt ? 64 * p.rt : 16), pre_parts = 0, pre_chunk = 1;
     if (prefix > 0) {
@@ -161,15 +173,17 @@ inline Plan plan_prompt(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
     // a run's last tile may be part full: one more a run than the rows need
     const int64_t m = p.rt ? 64 * p.rt : 16;
     const int64_t tiles = rows / m + cbq_min(batch, N);
-    const int64_t unit = p.rt ? block_keys(row_bytes) : kAttnWaves * wave_keys(row_bytes);
     const int64_t blocks = tiles * n_kv;
-    // Few tiles: their keys in parts, as many as two blocks a CU have room for at
-    // once (a few more would run alone, in a second turn).  Of the runs' last
-    // tiles, half are taken to be there beside the rows' whole ones.
+    // Few tiles: their keys in parts, as many as the CUs have room for at once (a
+    // few more would run alone, in a second turn): two blocks a CU, one of rows of
+    // 1024 bytes.  Of the runs' last tiles, half are taken to be there beside the
+    // rows' whole ones.  A part has four tiles at least (of 16-row blocks eight a
+    // wave: below that the merge takes longer).
+    const int64_t least = p.rt ? 4 * block_keys(row_bytes) : 8 * kAttnWaves * wave_keys(row_bytes);
     const int64_t likely = (batch == 1 ? cbq_ceil(rows, m) : rows / m + cbq_ceil(cbq_min(batch, N), 2))
                            * n_kv;
-    const int64_t parts = likely >= kCus
-        ? 1 : cbq_max(1, cbq_min(2 * kCus / likely, keys / (4 * unit)));
+    const int64_t room = row_bytes <= 512 ? 2 * kCus : kCus;
+    const int64_t parts = cbq_max(1, cbq_min(room / cbq_max(likely, 1), keys / least));
     p.blocks = blocks * parts;
     p.bytes = part_bytes(parts, N, n_kv * rep, hd);
     p.tiles = (int32_t)tiles;
@@ -187,7 +201,8 @@ inline bool plan_fits(const Plan &p)
 // (they read), so that both kinds share the CUs.
 struct DecodeWork {
     int h, tile, part, seq;                 // seq -1: the prefix
-    int32_t first, end;                     // keys (own ones: as the capacity has them)
+    int32_t first, end;                     // keys (own ones: as the capacity has them;
+                                            // joint: of both)
 };
 
 CBQ_PAGED_FN DecodeWork decode_work(const Plan &p, uint32_t block, int n_kv, int batch,
@@ -212,9 +227,10 @@ CBQ_PAGED_FN DecodeWork decode_work(const Plan &p, uint32_t block, int n_kv, int
     i /= p.own_tiles;
     w.seq = (int)(i % batch);
     const int chunk = (int)(i / batch);
+    const int64_t most = (p.joint ? prefix : 0) + capacity;
     w.part = p.pre_parts + chunk;
-    w.first = (int32_t)cbq_min((int64_t)chunk * p.own_chunk, capacity);
-    w.end = (int32_t)cbq_min((int64_t)w.first + p.own_chunk, capacity);
+    w.first = (int32_t)cbq_min((int64_t)chunk * p.own_chunk, most);
+    w.end = (int32_t)cbq_min((int64_t)w.first + p.own_chunk, most);
     return w;
 }
 

@@ -997,9 +997,9 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
         w.see(a, keys.prefix, past, row0);
     }
     if (length) {                               // decode: the own keys end there
-        const int32_t len = cbq_clamp_length(*length, a.capacity);
-        if (first >= len && !always) return;    // the merge counts own parts by the length
-        if (len < keys.end) keys.end = len;
+        const int32_t end = keys.prefix + cbq_clamp_length(*length, a.capacity);
+        if (first >= end && !always) return;    // the merge counts own parts by the length
+        if (end < keys.end) keys.end = end;
     }
     const int32_t begin = first + wave * KEYS, step = kWaves * KEYS;
     int odd = 0;                                // a value that is not finite
@@ -1107,7 +1107,8 @@ __global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void dec
             wave_rows<T, HD, false>(a, lds, w.h, 0, w.tile * 16, rows, keys, w.first, 0, to);
         return;
     }
-    const CbqKeys keys = {nullptr, a.tables + w.seq * a.table_st, 0, w.end};
+    const CbqKeys keys = {a.prefix_table, a.tables + w.seq * a.table_st, a.plan.joint ? a.prefix : 0,
+                          w.end};
     wave_rows<T, HD, false>(a, lds, w.h, w.seq, w.tile * 16, a.rep, keys, w.first, 0, to,
                             a.lengths + w.seq, a.plan.parts == 1);
 }
@@ -1183,16 +1184,20 @@ __global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void pro
                                a.plan.parts > 1 ? part : -1);
 }
 
-// ---- merge of the parts: a block a (token, head) -----------------------------------------------
-// HD / 4 lanes take a part's values, so a block has 1024 / HD parts under way at
-// once; the first of them are requested before the common maximum is known.
-template <typename T, int HD> __global__ __launch_bounds__(kThreads) void merge_kernel(AttnArgs a)
+// ---- merge of the parts: W waves a (token, head) -----------------------------------------------
+// HD / 4 lanes take a part's values, so a row has 256 W / HD parts under way at
+// once; the first of them are requested before the common maximum is known.  A
+// whole block a row for few rows and many parts, a wave a row for many.
+template <typename T, int HD, int W> __global__ __launch_bounds__(kThreads) void merge_kernel(AttnArgs a)
 {
-    constexpr int kLanes = HD / 4, kGroups = kThreads / kLanes, kAhead = 4;
-    __shared__ __attribute__((aligned(16))) float sums[kGroups][HD];
-    __shared__ float totals[kGroups];
-    const int64_t row = blockIdx.x, rows = (int64_t)a.N * a.n_q, token = row / a.n_q;
-    const int tid = threadIdx.x, lane = tid & 63, group = tid / kLanes, d = tid % kLanes * 4;
+    constexpr int kLanes = HD / 4, kGroups = W * CBQ_WAVE / kLanes, kAhead = 4;
+    __shared__ __attribute__((aligned(16))) float sums[kThreads / kLanes][HD];
+    __shared__ float totals[kThreads / kLanes];
+    const int tid = threadIdx.x, lane = tid & 63, all = tid / kLanes, d = tid % kLanes * 4;
+    const int group = all % kGroups;
+    const int64_t rows = (int64_t)a.N * a.n_q, row = (int64_t)blockIdx.x * (kWaves / W) + all / kGroups,
+                  token = row / a.n_q;
+    if (row >= rows) return;                        // whole waves; the barrier counts the rest
     // The first parts' loads wait for no length: what a part that was not written
     // holds is dropped.
     const int most = a.plan.parts;
@@ -1238,17 +1243,28 @@ template <typename T, int HD> __global__ __launch_bounds__(kThreads) void merge_
         for (int i = 0; i < kAhead; i++)
             part(p0 + (kAhead + i) * kGroups, o[i], ml[i]);
     }
-    *(f32x4 *)&sums[group][d] = x;
-    if (tid % kLanes == 0) totals[group] = sum;
-    __syncthreads();
-    if (tid >= kLanes) return;
+    if constexpr (kGroups > 1) {
+        *(f32x4 *)&sums[all][d] = x;
+        if (tid % kLanes == 0) totals[all] = sum;
+        if constexpr (W > 1) {
+            __syncthreads();
+        } else {                                    // the wave's own
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        }
+        if (group > 0) return;
 #pragma unroll
-    for (int i = 1; i < kGroups; i++) {
-        x += *(const f32x4 *)&sums[i][d];
-        sum += totals[i];
+        for (int i = 1; i < kGroups; i++) {
+            x += *(const f32x4 *)&sums[all + i][d];
+            sum += totals[all + i];
+        }
     }
     put_values<T, HD>(a, -1, token, (int)(row - token * a.n_q), d, x, sum);
 }
+
+// Rows from which a wave each fills the CUs
+constexpr int64_t kMergeRows = 4096;
 
 // ---- launches of one type -------------------------------------------------------------------
 // More than 64 KiB of LDS is asked for once a kernel and device.
@@ -1290,8 +1306,11 @@ template <typename T, int HD> int launch(const AttnArgs &a, const Plan &p, bool 
         else rc = run_kernel<decode_kernel<T, HD, wide>>(p.blocks, both, a, stream, what);
     }
     if (rc != CK_SUCCESS || p.parts == 1) return rc;
-    return run_kernel<merge_kernel<T, HD>>((int64_t)a.N * a.n_q, 0, a, stream,
-                      "cbq_prefix_attn merge");
+    const char *what = "cbq_prefix_attn merge";
+    const int64_t rows = (int64_t)a.N * a.n_q;
+    if (rows >= kMergeRows && p.parts <= 16)
+        return run_kernel<merge_kernel<T, HD, 1>>(cbq_ceil(rows, kWaves), 0, a, stream, what);
+    return run_kernel<merge_kernel<T, HD, kWaves>>(rows, 0, a, stream, what);
 }
 
 template <typename T> int launch_hd(const AttnArgs &a, const Plan &p, bool prompt,

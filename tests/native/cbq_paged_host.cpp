@@ -79,6 +79,7 @@ static void decode()
     CHECK(plan_fits(p));
     CHECK(p.bytes == (p.parts > 1 ? (int64_t)p.parts * batch * n_kv * rep * (hd + 2) * 4 : 0));
     const CbqDiv pg = cbq_div_make(page);
+    const int pre = p.joint ? prefix : 0;           // walked by each sequence itself
     // [kv head][row tile of 16 or 64 rt rows][key] for the prefix and each sequence
     std::map<std::vector<int>, std::vector<int>> seen;
     std::map<std::vector<int>, int> parts;
@@ -97,28 +98,29 @@ static void decode()
             int32_t entry, row;
             for (int lane = 0; lane < 64; lane++) {
                 const int32_t j = w.first + lane;
-                cbq_key_place({nullptr, tables.data() + (size_t)w.seq * width, 0, w.end}, pg, j, entry, row);
-                CHECK(j >= w.end || entry < width);
+                cbq_key_place({prefix_table.data(), tables.data() + (size_t)w.seq * width, pre, w.end}, pg, j, entry, row);
+                CHECK(j >= w.end || entry < (j < pre ? (int)prefix_table.size() : width));
             }
             const int32_t len = cbq_clamp_length(lengths[w.seq], capacity);
-            if (w.first >= len && p.parts > 1) continue;
+            if (w.first >= pre + len && p.parts > 1) continue;
             CHECK(w.part >= p.pre_parts && w.part < p.parts);
             const int32_t *own = tables.data() + (size_t)w.seq * width;
             auto &s = seen[{w.h, w.seq, w.tile}];
-            s.resize(capacity);
-            walk({nullptr, own, 0, (int32_t)cbq_min(w.end, len)}, pg, w.first, step, prefix_table, own, width, s);
+            s.resize(pre + capacity);
+            walk({prefix_table.data(), own, pre, (int32_t)cbq_min(w.end, pre + len)}, pg, w.first, step, prefix_table,
+                 own, width, s);
             parts[{w.h, w.seq, w.tile}]++;
         }
     }
     for (int h = 0; h < n_kv; h++) {
-        for (int t = 0; prefix && t * m < batch * rep; t++)
+        for (int t = 0; prefix && !p.joint && t * m < batch * rep; t++)
             for (int x : seen[{h, -1, t}]) CHECK(x == 1);
         for (int b = 0; b < batch; b++)
             for (int t = 0; t * 16 < rep; t++) {
                 const int32_t len = cbq_clamp_length(lengths[b], capacity);
                 auto &s = seen[{h, b, t}];
-                for (int j = 0; j < (int)s.size(); j++) CHECK(s[j] == (j < len));
-                CHECK(len == 0 || (int)s.size() == capacity);
+                for (int j = 0; j < (int)s.size(); j++) CHECK(s[j] == (j < pre + len));
+                CHECK(pre + len == 0 || (int)s.size() == pre + capacity);
                 // what the merge counts (a lone part always writes the output)
                 const int want = p.parts == 1 ? (p.pre_parts ? 0 : 1) : (int)cbq_ceil(len, p.own_chunk);
                 CHECK((parts[{h, b, t}]) == want);
