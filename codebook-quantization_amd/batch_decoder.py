@@ -191,3 +191,44 @@ class BatchDecoder:
             tokens.append(torch.argmax(self.step(tokens[-1]), -1))
         self.release()
         return torch.stack(tokens, 1).tolist()
+
+
+def main() -> None:
+    """A synthetic model's batch: prompts of several lengths behind one prefix."""
+    import argparse
+    import random
+    import time
+
+    import decoder
+    import synthetic
+    ap = argparse.ArgumentParser(description=main.__doc__)
+    ap.add_argument("--config", default="qwen3-1.7b", choices=sorted(synthetic.CONFIGS))
+    ap.add_argument("--layers", type=int, default=4)
+    ap.add_argument("--batch", type=int, default=8)
+    ap.add_argument("--prefix", type=int, default=512)
+    ap.add_argument("--new", type=int, default=32)
+    ap.add_argument("--cache", default="float32", choices=["float32", "bfloat16", "float16"])
+    a = ap.parse_args()
+    syn = synthetic.SyntheticDecoder(a.config, layers=a.layers, log=lambda *x: None)
+    c = syn.cfg
+    cfg = decoder.DecoderConfig(layers=c["layers"], hidden=c["hidden"], inter=c["inter"], n_q=c["n_q"],
+                                n_kv=c["n_kv"], head_dim=c["head_dim"], vocab=c["vocab"])
+    tensors = syn.build_fixed(syn.all_linears() + [syn.embed])
+    model = decoder.from_synthetic(cfg, tensors, max_len=a.prefix + 256 + a.new)
+    rng = random.Random(0)
+    prompts = [[rng.randrange(cfg.vocab) for _ in range(rng.randint(1, 256))] for _ in range(a.batch)]
+    per = -(-(256 + a.new) // 64)
+    batch = BatchDecoder(model, a.batch * per + -(-a.prefix // 64), dtype=getattr(torch, a.cache))
+    batch.set_prefix([rng.randrange(cfg.vocab) for _ in range(a.prefix)])
+    batch.generate(prompts, 2)                          # loads the kernels
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    tokens = batch.generate(prompts, a.new)
+    s = time.perf_counter() - t0
+    print(f"{a.batch} prompts of {sum(map(len, prompts))} tokens behind {a.prefix}: "
+          f"{a.batch * a.new} tokens in {s:.3f} s ({a.batch * a.new / s:.0f} tokens/s, prompts included)")
+    print("first tokens:", [t[:4] for t in tokens])
+
+
+if __name__ == "__main__":
+    main()

@@ -1,6 +1,6 @@
 """torch.ops.cbq: the compressed entry points registered with torch's
-dispatcher (libcbq_torch.so, built from csrc/cbq_torch_ops.cpp over the C
-ABI of libcbq_hip.so).
+dispatcher (libcbq_torch.so, built from csrc/cbq_torch_ops.cpp and
+csrc/cbq_torch_serve.cpp over the C ABI of libcbq_hip.so).
 
     linear(x, packed, codebook, M, bits)              fixed-width GEMV / GEMM
     linear_kind(x, packed, codebook, M, bits, cb_kind)    linear for a codebook whose
@@ -12,6 +12,17 @@ ABI of libcbq_hip.so).
     huff_linear(x, words, chunk_off, sub_len, lut1, lut2, canon, canon_pay,
                 value_cb, C, stage_words, M)           Huffman (stream format)
     huff_embedding(ids, <stream tensors>, C, stage_words, vocab, H)
+
+and the operators of batched serving over a paged key/value cache
+(include/cbq_serve.h; batch_decoder.py uses them):
+
+    paged_append(q, k, v, cos, sin, positions, slots, k_pages, v_pages, norm,
+                 q_weight, k_weight, eps)              head norm, rotation, pages; the
+                                                      turned queries
+    prefix_attention_decode(q, k_pages, v_pages, prefix_table, prefix, tables,
+                            lengths, scale)            one token a sequence
+    prefix_attention_prompt(q, q_start, k_pages, v_pages, prefix_table, prefix,
+                            tables, lengths, scale)    ragged runs, causal
 
 The modules (compressed_modules via gpu_accelerated_functions and
 gpu_huffman_functions) call these ops; they run on torch's current HIP

@@ -125,7 +125,7 @@ inline Plan plan_decode(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
     if (prefix + capacity <= 4 * wk) {
         // Few keys: prefix and own ones by one block a sequence and kv head, four
         // tiles a wave at most.  Parts would be shorter by less than their merge
-        // takes (4 us): two sequences of 3..18 keys, room for 300: 9.6 -> 6 us.
+        // takes (4 us): two sequences of 3..18 keys, room for 300: 9.7 -> 7.2 us.
         p.joint = 1;
         p.own_parts = p.parts = 1;
         p.own_chunk = (int32_t)cbq_max(prefix + capacity, 1);
@@ -136,7 +136,9 @@ inline Plan plan_decode(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
     p.rt = rows <= 16 ? 0 : rows <= 64 ? 1 : widest(row_bytes);
     int64_t tiles = cbq_ceil(rows, p.rt ? 64 * p.rt : 16), pre_parts = 0, pre_chunk = 1;
     if (prefix > 0) {
-        // one block a CU: more parts cost their fp32 sums, written and read once
+        // One block a CU, beside one of own keys: more parts cost their fp32 sums,
+        // written and read once, fewer leave CUs without products (64 sequences of 32
+        // heads behind 30011 keys: 133, 92, 98 and 107 us with 128, 256, 384 and 512).
         const int64_t least = p.rt ? 2 * bk : wk, want = cbq_max(1, kCus / (tiles * n_kv));
         const int64_t unit = p.rt ? bk : wk;
         pre_chunk = cbq_max(least, cbq_ceil(cbq_ceil(prefix, want), unit) * unit);
@@ -145,8 +147,9 @@ inline Plan plan_decode(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
         tiles = 0;
     }
     const int64_t own_tiles = cbq_ceil(rep, 16);
-    // about two blocks a CU of the full capacity, a tile a wave at least and
-    // eight at most
+    // About two blocks a CU of the full capacity, a tile a wave at least and eight at
+    // most (33 sequences of 24 heads, up to 2900 keys: 17.6 us; with half and twice the
+    // blocks 20).
     const int64_t share = cbq_ceil(capacity * batch * n_kv * own_tiles, 2 * kCus);
     const int64_t own_chunk = cbq_min(cbq_max(cbq_ceil(share, wk), 1), 8) * wk;
     const int64_t own_parts = cbq_max(cbq_ceil(capacity, own_chunk), pre_parts ? 0 : 1);
@@ -168,6 +171,7 @@ inline Plan plan_prompt(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
     Plan p = {};
     const int64_t rows = N * rep, small = (cbq_ceil(rows, 16) + batch) * n_kv;
     const int64_t keys = cbq_max(prefix + capacity, 1);
+    // 16 rows a block for runs that fill no more, and where a few rows meet few keys
     if (rows <= 16 * batch || (small <= 2 * kCus && keys <= 2048)) p.rt = 0;
     else p.rt = rows <= 64 * batch ? 1 : widest(row_bytes);
     // a run's last tile may be part full: one more a run than the rows need

@@ -20,9 +20,18 @@
 // V^T comes out of row-major V by the LDS transpose read (16-bit types); fp32
 // uses the 16x16x4 fp32 products, whose operand is one element a lane.
 //
-// Tiles of keys go global -> registers -> LDS, the loads of a tile being under
-// way while the one before is computed; 16-byte slots of a row are stored at
-// slot ^ mix(row), which spreads both operands' reads over the banks.
+// Tiles of keys go to LDS, straight (a block's) or through registers (a wave's
+// own), the loads of a tile being under way while the one before is computed;
+// 16-byte slots of a row are stored at slot ^ mix(row), which spreads both
+// operands' reads over the banks.
+//
+// What bounds it (MI355X; heads 32 on 8 of 128 unless said): long bf16 prompts the
+// card's power: 8192 tokens 565 us, 970 TFLOP/s, the matrix units busy 44 % of the
+// cycles at a clock that falls to 2.1 GHz as fewer cycles are needed (the
+// framework's large product runs at 1.2 PFLOP/s); one-token steps HBM: 64
+// sequences of 200..1500 own keys 58 us without a prefix (3.8 TB/s, launches and
+// merge included) and 87 behind 30011 shared keys; few keys two launches of 4 to 5
+// us and a chain of three dependent loads (length, page id, key).
 #pragma once
 
 #include <atomic>
@@ -45,7 +54,6 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int kWaves = kAttnWaves, kThreads = kWaves * CBQ_WAVE;
 constexpr float kSlack = 8.0f;
-constexpr float kLog2e = 1.44269504088896340736f;
 
 struct AttnArgs {
     const void *q;
@@ -63,6 +71,7 @@ struct AttnArgs {
     uint32_t unit, k_page, k_row, v_page, v_row;
     int32_t one_stride;                     // keys and values lie alike
     float c, q_mul;                         // exp2(c * (q_mul q) . k); q_mul folds scale's sign
+    float c_low;                            // what c's rounding left, for fp32's weights
     Plan plan;
 };
 
@@ -149,35 +158,30 @@ template <typename T, int HD> struct Geo {
 };
 
 // ---- a tile of keys and values: global -> registers -> LDS --------------------------
-// NT threads (a block or a wave) move KEYS rows of K and of V.  A row's slots are
-// read by neighbouring lanes; its address is found once, by one lane of the wave
-// that reads it (a wave's keys of a tile are 64 at most), and comes to the others
-// by a shuffle: page arithmetic in every lane cost more than the products.  A key's
+// A wave moves KEYS rows of K and of V (64 at most).  A row's slots are read by
+// neighbouring lanes; its address is found once, by one lane, and comes to the others
+// by a shuffle: page arithmetic in every lane cost more than the products (a prompt
+// of 8192 tokens 771 us with it, 700 without).  A key's
 // table entry and row in its page advance with the tiles by additions, and the entry
 // of the next tile is under way while a tile is.
-template <typename T, int HD, int KEYS, int NT> struct Stage {
+template <typename T, int HD, int KEYS> struct Stage {
     using G = Geo<T, HD>;
-    static constexpr int kRows = NT / G::kSlots, kPer = KEYS / kRows;   // rows a pass, passes
-    static constexpr int kWide = CBQ_WAVE / G::kSlots, kMine = kPer * kWide;    // of a wave
-    static_assert(kRows * kPer == KEYS && kWide * G::kSlots == CBQ_WAVE && kMine <= CBQ_WAVE,
-                  "whole passes, a key a lane");
+    static constexpr int kWide = CBQ_WAVE / G::kSlots, kPer = KEYS / kWide;     // rows a pass, passes
+    static_assert(kWide * kPer == KEYS && KEYS <= CBQ_WAVE, "whole passes, a key a lane");
     u32x4 k[kPer], v[kPer];
-    uint64_t there;                         // the wave's keys of the loaded tile that are there
+    uint64_t there;                         // the loaded tile's keys that are there
     int32_t key, entry, row, id;            // this lane's key: of the next tile
     int32_t step, step_entry, step_row;
-    int at;                                 // the key's place in a tile
 
     // The walk starts at `first` and goes on in steps of `by` keys.
     __device__ __forceinline__ void start(const AttnArgs &a, const CbqKeys &keys, int32_t first,
                                           int32_t by)
     {
-        const int lane = threadIdx.x & 63, wave = NT == CBQ_WAVE ? 0 : threadIdx.x >> 6;
-        at = lane / kWide * kRows + wave * kWide + lane % kWide;
-        if (lane >= kMine) at = -1;
+        const int lane = threadIdx.x & 63;
         step = by;
         step_entry = (int32_t)cbq_div((uint32_t)by, a.page);
         step_row = by - step_entry * (int32_t)a.page.d;
-        key = at < 0 ? -1 : first + at;
+        key = lane < KEYS ? first + lane : -1;
         cbq_key_place(keys, a.page, key, entry, row);
         look(keys);
     }
@@ -212,16 +216,15 @@ template <typename T, int HD, int KEYS, int NT> struct Stage {
 #pragma unroll
         for (int i = 0; i < kPer; i++)
             v[i] = *(const u32x4 *)((const char *)vp + (uint64_t)o[i] * a.unit);
-        if (at >= 0) cbq_key_advance(keys, a.page, step, step_entry, step_row, key, entry, row);
+        if (key >= 0) cbq_key_advance(keys, a.page, step, step_entry, step_row, key, entry, row);
         look(keys);
     }
-    static constexpr uint64_t kEvery = kMine == 64 ? ~0ull : (1ull << (kMine & 63)) - 1;
+    static constexpr uint64_t kEvery = KEYS == 64 ? ~0ull : (1ull << (KEYS & 63)) - 1;
     __device__ __forceinline__ bool missing() const { return there != kEvery; }
     // bias[key]: 0, or -inf for a key that is not there
     __device__ __forceinline__ void store(u32x4 *K, u32x4 *V, float *bias)
     {
-        const int lane = threadIdx.x & 63, wave = NT == CBQ_WAVE ? 0 : threadIdx.x >> 6;
-        const int slot = lane % G::kSlots, sub = lane / G::kSlots;
+        const int lane = threadIdx.x & 63, slot = lane % G::kSlots, sub = lane / G::kSlots;
         if (missing()) {
 #pragma unroll
             for (int i = 0; i < kPer; i++)
@@ -229,19 +232,19 @@ template <typename T, int HD, int KEYS, int NT> struct Stage {
         }
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            const int r = i * kRows + wave * kWide + sub;
+            const int r = i * kWide + sub;
             K[r * G::kSlots + (slot ^ G::mix(r))] = k[i];
             V[r * G::kSlots + (slot ^ G::mix(r))] = v[i];
         }
-        if (at >= 0) bias[at] = there >> lane & 1 ? 0.f : -INFINITY;
+        if (lane < KEYS) bias[lane] = there >> lane & 1 ? 0.f : -INFINITY;
     }
 };
 
-// The same for a block's tile, straight into LDS: no registers and no stores, and
-// K and V are asked for at different times, K a tile ahead.  A lane's 16 bytes
-// land at its place in the wave's 1 KiB, so the slot ^ row order of the tile is
-// made by the lane's choice of global slot; rows that are not there come from a
-// slot of zeros.
+// The same for a block's tile, straight into LDS: no registers (with them 700 us,
+// without and with the values read ahead of their products 573) and no stores.  A
+// lane's 16 bytes land at its place in the wave's 1 KiB, so the slot ^ mix(row)
+// order of the tile is made by the lane's choice of global slot; rows that are not
+// there come from a slot of zeros.
 static __device__ const u32x4 kZeroSlot = {0, 0, 0, 0};
 
 // Written as asm so that the compiler orders no LDS read behind it: stage_wait's
@@ -550,18 +553,20 @@ template <typename T, int HD, int RT> struct Rows {
     }
 
     // Four scores to weights, added to the row's sum
-    __device__ __forceinline__ f32x4 weigh(int t, f32x4 s, float c)
+    __device__ __forceinline__ f32x4 weigh(int t, f32x4 s, float c, float c_low)
     {
         f32x4 p;
 #pragma unroll
-        for (int i = 0; i < 4; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base[t]));
+        for (int i = 0; i < 4; i++)
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, sizeof(T) == 4 ? fmaf(s[i], c_low, -base[t])
+                                                                       : -base[t]));
         l[t] += (p[0] + p[1]) + (p[2] + p[3]);
         return p;
     }
 
     // Weights of the tile, and the values under them
     template <int NK>
-    __device__ __forceinline__ void values(const u32x4 *V, const f32x4 (&s)[RT][NK], float c)
+    __device__ __forceinline__ void values(const u32x4 *V, const f32x4 (&s)[RT][NK], float c, float c_low)
     {
         const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
         if constexpr (sizeof(T) == 4) {
@@ -570,7 +575,7 @@ template <typename T, int HD, int RT> struct Rows {
             for (int k = 0; k < NK; k++) {
                 f32x4 p[RT];
 #pragma unroll
-                for (int t = 0; t < RT; t++) p[t] = weigh(t, s[t][k], c);
+                for (int t = 0; t < RT; t++) p[t] = weigh(t, s[t][k], c, c_low);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int key = k * 16 + 4 * g + i;
@@ -611,7 +616,7 @@ template <typename T, int HD, int RT> struct Rows {
                 };
                 auto weights = [&](int pair, int u) {       // unit u of the pair: 4 scores a lane
                     const int t = u / 2, k = u % 2;
-                    const f32x4 x = weigh(t, s[t][pair * 2 + k], c);
+                    const f32x4 x = weigh(t, s[t][pair * 2 + k], c, c_low);
                     p[pair & 1][t][k * 2] = pack2<T>(x[0], x[1]);
                     p[pair & 1][t][k * 2 + 1] = pack2<T>(x[2], x[3]);
                 };
@@ -649,7 +654,7 @@ template <typename T, int HD, int RT> struct Rows {
                 u32x2 p[RT];
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
-                    const f32x4 x = weigh(t, s[t][0], c);
+                    const f32x4 x = weigh(t, s[t][0], c, c_low);
                     p[t] = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
                 }
 #pragma unroll
@@ -790,7 +795,7 @@ template <typename T, int HD> struct Rows32 {
     // the 16 before them are in the products, beside which the 16 keys' weights after
     // them are made.
     template <int NK>
-    __device__ __forceinline__ void values(const u32x4 *V, const f32x16 (&s)[NK], float c)
+    __device__ __forceinline__ void values(const u32x4 *V, const f32x16 (&s)[NK], float c, float)
     {
         const int lane = threadIdx.x & 63, r = lane & 15;
         const int key = 4 * (lane >> 5) + (r >> 2), sub = (lane >> 4 & 1) * 2 + ((r & 3) >> 1);
@@ -908,6 +913,12 @@ __device__ __forceinline__ void plain_rows(const AttnArgs &a, int h, int64_t tok
 }
 
 // ---- 64 RT rows of a block against keys [first, end), tiles shared by the waves ----------
+// 64 keys of K and V (rows of 256 bytes) in two buffers of 32 KiB, so that two blocks
+// share a CU.  32 rows a wave: 16 take 772 us instead of 560 for 8192 tokens (LDS
+// reads double).  Blocks of eight waves take 529 there, but 297 instead of 286 for
+// 16 ragged prompts and 366 instead of 327 at hd 64; deeper rings of tiles gain
+// nothing, and 32 rows of 512 bytes, which leave one wave a SIMD, lose (67 us
+// instead of 48 for two chunks against 20000 keys).
 template <typename T, int HD, int RT, bool CAUSAL>
 __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, int64_t token0,
                                            int row0, int n, const CbqKeys &keys, int32_t first,
@@ -948,7 +959,7 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
         if (key0 + KEYS > all || __builtin_amdgcn_readfirstlane(miss.x | miss.y | miss.z | miss.w))
             w.hide(s, bias + b * KEYS, key0);
         w.raise(s, a.c);
-        w.values(V + b * kTile, s, a.c);
+        w.values(V + b * kTile, s, a.c, a.c_low);
         stage_wait();
         return true;
     };
@@ -973,8 +984,11 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
 }
 
 // ---- 16 rows of a block, the keys [first, end) dealt to its waves ------------------------
-// For few rows: each wave walks tiles of its own through its own LDS without a
-// barrier, and the four running states are merged at the end.
+// For few rows: each wave walks tiles of its own (8 KiB of K and of V) through its
+// own LDS without a barrier, and the four running states are merged at the end.  A
+// decoder's rows of one sequence fill a quarter of a 16-row product or less; the
+// bytes bound them, and two blocks a CU keep 128 KiB under way.  200 fp32 prompt
+// tokens take 14 us this way, 23 with 64 rows a block.
 template <typename T, int HD, bool CAUSAL>
 __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, int64_t token0,
                                           int row0, int n, CbqKeys keys, int32_t first,
@@ -988,7 +1002,7 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
     u32x4 *K = (u32x4 *)lds + wave * 2 * kTile, *V = K + kTile;
     float *bias = (float *)((u32x4 *)lds + kWaves * 2 * kTile) + wave * KEYS;
     Rows<T, HD, 1> w;
-    Stage<T, HD, KEYS, CBQ_WAVE> st;
+    Stage<T, HD, KEYS> st;
     st.start(a, keys, first + wave * KEYS, kWaves * KEYS);
     w.load(a, h, token0, row0, n);
     int32_t all = INT32_MAX;
@@ -1019,7 +1033,7 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
         w.scores(K, s);
         if (missing || key0 + KEYS > all) w.hide(s, bias, key0);
         w.raise(s, a.c);
-        w.values(V, s, a.c);
+        w.values(V, s, a.c, a.c_low);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -1072,9 +1086,10 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
     }
 }
 
-// blocks a CU, whose waves' loads, products and exponentials overlap; rows of
-// 1024 bytes need a wave's whole register file
-constexpr int min_blocks(int row_bytes) { return row_bytes <= 512 ? 2 : 1; }
+// Waves a SIMD, and so blocks a CU, whose loads, products and exponentials overlap
+// (one: 1627 us instead of 771 for 8192 tokens); rows of 1024 bytes need a wave's
+// whole register file.
+constexpr int simd_waves(int row_bytes) { return row_bytes <= 512 ? 2 : 1; }
 
 template <typename T, int HD> constexpr int wave_lds()
 {
@@ -1093,7 +1108,7 @@ template <typename T, int HD> constexpr int block_lds()
 // PT: 64 PT prefix rows a block; 0: the prefix rows are 16 at most and go as the
 // own ones do.
 template <typename T, int HD, int PT>
-__global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void decode_kernel(AttnArgs a)
+__global__ __launch_bounds__(kThreads, simd_waves(HD * (int)sizeof(T))) void decode_kernel(AttnArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const DecodeWork w = decode_work(a.plan, blockIdx.x, a.kv.n_kv, a.batch, a.prefix, a.capacity);
@@ -1116,7 +1131,7 @@ __global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void dec
 // ---- prompt: tiles of each run's rows against the keys they see -----------------------------
 // RT: 64 RT rows a block; 0: 16 rows.
 template <typename T, int HD, int RT>
-__global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void prompt_kernel(AttnArgs a)
+__global__ __launch_bounds__(kThreads, simd_waves(HD * (int)sizeof(T))) void prompt_kernel(AttnArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int M = RT ? 64 * RT : 16;
@@ -1187,7 +1202,9 @@ __global__ __launch_bounds__(kThreads, min_blocks(HD * (int)sizeof(T))) void pro
 // ---- merge of the parts: W waves a (token, head) -----------------------------------------------
 // HD / 4 lanes take a part's values, so a row has 256 W / HD parts under way at
 // once; the first of them are requested before the common maximum is known.  A
-// whole block a row for few rows and many parts, a wave a row for many.
+// whole block a row for few rows and many parts (a wave a row that walks 40 parts
+// took 14 us, a block 5), a wave a row for many (9888 rows of 6 parts: 41 us with
+// the prompt, 30).
 template <typename T, int HD, int W> __global__ __launch_bounds__(kThreads) void merge_kernel(AttnArgs a)
 {
     constexpr int kLanes = HD / 4, kGroups = W * CBQ_WAVE / kLanes, kAhead = 4;

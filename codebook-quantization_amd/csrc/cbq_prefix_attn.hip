@@ -1,5 +1,6 @@
 // C entry points of the attention over a paged cache (include/cbq_serve.h):
 // argument checks, launch plans, dispatch by type.
+#include <cmath>
 #include <initializer_list>
 
 #include "cbq_prefix_attn.h"
@@ -94,7 +95,12 @@ int attend(const void *q, const int64_t *q_stride, const int32_t *q_start,
     // makes every score 0.
     const float mag = scale < 0.f ? -scale : scale;
     const bool zero = mag < 1.0e-30f;
-    a.c = zero ? 1.0f : mag * kLog2e;
+    // c below the exact factor and c_low above 0, so that a hidden key's -inf stays
+    // -inf times either.
+    const double exact = (double)mag * 1.4426950408889634074;
+    a.c = zero ? 1.0f : (float)exact;
+    if (!zero && (double)a.c >= exact) a.c = std::nextafter(a.c, 0.0f);
+    a.c_low = zero ? 1.0e-9f : (float)(exact - (double)a.c);
     a.q_mul = zero ? 0.0f : scale < 0.f ? -1.0f : 1.0f;
     a.plan = p;
     if (cache->dtype == CBQ_F32) return launch_f32(a, p, prompt, stream);

@@ -38,7 +38,10 @@ extern "C" {
  * is base[p * stride[0] + h * stride[1] + r * stride[2] + d]; strides are in
  * elements and d is contiguous, so both [pages, heads, rows, hd] and [pages,
  * rows, heads, hd] layouts, and keys and values in one tensor, are described.
- * 1 <= page <= 65536; n_pages * page < 2^31. */
+ * 1 <= page <= 65536; n_pages * page < 2^31.  The attention also needs page and
+ * row strides of 0 or more whose largest offset is below 2^32 times the largest
+ * power of two (4096 at most) that divides all of them in bytes: any pool up to
+ * 512 GiB if they are whole 128 bytes. */
 typedef struct cbq_paged_kv {
     void *k, *v;
     int64_t k_stride[3], v_stride[3];
