@@ -43,11 +43,11 @@ def test_attention_refusals(lib):
     p = (ctypes.addressof(buf) + 15) // 16 * 16
     st = (ctypes.c_int64 * 2)(256, 64)
 
-    def call(c, q=p, strides=st, pt=p, prefix=10, t=p, width=3, lens=p, batch=2, n_q=4, scale=0.1,
+    def call(c, q=p, strides=st, pt=p, prefix=10, t=p, width=300, lens=p, batch=2, n_q=4, scale=0.1,
              out=p, ws=p, nws=1 << 40):
-        return lib.cbq_prefix_attn_decode(q, strides, ctypes.byref(c), pt, prefix, t, 3, width, lens,
+        return lib.cbq_prefix_attn_decode(q, strides, ctypes.byref(c), pt, prefix, t, 300, width, lens,
                                           batch, n_q, scale, out, ws, nws, None)
-    need = lib.cbq_prefix_attn_decode_workspace(ctypes.byref(_cache(p)), 10, 3, 2, 4)
+    need = lib.cbq_prefix_attn_decode_workspace(ctypes.byref(_cache(p)), 10, 300, 2, 4)
     assert need > 0
     bad = [dict(q=None), dict(strides=None), dict(pt=None), dict(t=None), dict(lens=None),
            dict(out=None), dict(ws=None), dict(nws=need - 1), dict(ws=p + 4), dict(q=p + 2),
@@ -62,6 +62,11 @@ def test_attention_refusals(lib):
         assert call(_cache(p, **kw)) == 2, kw
     c = _cache(p)
     c.v_stride[2] = 65
+    assert call(c) == 2
+    c = _cache(p, n_pages=1 << 26)
+    c.k_stride[0] = (1 << 20) + 8                               # 2^50 bytes in units of 16
+    assert call(c) == 2
+    c.k_stride[0], c.k_stride[2] = 1024, -64
     assert call(c) == 2
     assert call(_cache(p), batch=0) == 0                        # nothing to do
     prompt = lib.cbq_prefix_attn_prompt
