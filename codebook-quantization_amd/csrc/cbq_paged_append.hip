@@ -34,7 +34,7 @@ struct AppendArgs {
     float eps;
 };
 
-template <typename T, int V> struct alignas(sizeof(T) * V) Pack {
+template <typename T, int V> struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
     T e[V];
 };
 

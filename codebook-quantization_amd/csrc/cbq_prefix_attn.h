@@ -46,6 +46,7 @@ namespace cbq_attn {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -221,8 +222,8 @@ template <typename T, int HD, int KEYS> struct Stage {
     }
     static constexpr uint64_t kEvery = KEYS == 64 ? ~0ull : (1ull << (KEYS & 63)) - 1;
     __device__ __forceinline__ bool missing() const { return there != kEvery; }
-    // bias[key]: 0, or -inf for a key that is not there
-    __device__ __forceinline__ void store(u32x4 *K, u32x4 *V, float *bias)
+    // place[key]: its place on the joint axis, INT32_MAX for a key that is not there
+    __device__ __forceinline__ void store(u32x4 *K, u32x4 *V, int32_t *place, int32_t key0)
     {
         const int lane = threadIdx.x & 63, slot = lane % G::kSlots, sub = lane / G::kSlots;
         if (missing()) {
@@ -236,7 +237,7 @@ template <typename T, int HD, int KEYS> struct Stage {
             K[r * G::kSlots + (slot ^ G::mix(r))] = k[i];
             V[r * G::kSlots + (slot ^ G::mix(r))] = v[i];
         }
-        if (lane < KEYS) bias[lane] = there >> lane & 1 ? 0.f : -INFINITY;
+        if (lane < KEYS) place[lane] = there >> lane & 1 ? key0 + lane : INT32_MAX;
     }
 };
 
@@ -288,10 +289,10 @@ template <typename T, int HD, int KEYS> struct Copies {
         id = -1;
         if (key >= 0 && key < keys.end) id = (key < keys.prefix ? keys.shared : keys.own)[entry];
     }
-    // Asks for the next tile's keys and writes its bias (0, or -inf for a key that
-    // is not there) and this wave's flag of one that is not.
+    // Asks for the next tile's keys and writes their places (as Stage) and this wave's
+    // flag of one that is not there.
     __device__ __forceinline__ void keys_to(const AttnArgs &a, const CbqKeys &keys, int h, uint32_t lds,
-                                            float *bias, int32_t *flags)
+                                            int32_t *place, int32_t *flags)
     {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / G::kSlots;
         const bool in = id >= 0 && id < a.kv.n_pages;
@@ -322,8 +323,8 @@ template <typename T, int HD, int KEYS> struct Copies {
                 if (!(there >> (i * kWide + sub) & 1)) k[i] = v[i] = (const char *)&kZeroSlot;
         }
 #pragma unroll
-        for (int i = 0; i < kPer; i++) copy_slots(lds + place(i, wave), k[i]);
-        if (at >= 0) bias[at] = in ? 0.f : -INFINITY;
+        for (int i = 0; i < kPer; i++) copy_slots(lds + offset(i, wave), k[i]);
+        if (at >= 0) place[at] = in ? key : INT32_MAX;
         if (lane == 0) flags[wave] = there != every;
         if (at >= 0)
             cbq_key_advance(keys, a.page, KEYS, step_entry, step_row, key, entry, row);
@@ -333,9 +334,9 @@ template <typename T, int HD, int KEYS> struct Copies {
     __device__ __forceinline__ void values_to(uint32_t lds)
     {
 #pragma unroll
-        for (int i = 0; i < kPer; i++) copy_slots(lds + place(i, threadIdx.x >> 6), v[i]);
+        for (int i = 0; i < kPer; i++) copy_slots(lds + offset(i, threadIdx.x >> 6), v[i]);
     }
-    static __device__ __forceinline__ uint32_t place(int i, int wave)
+    static __device__ __forceinline__ uint32_t offset(int i, int wave)
     {
         return (uint32_t)((i * kRows + wave * kWide) * G::kSlots * 16);
     }
@@ -478,22 +479,18 @@ template <typename T, int HD, int RT> struct Rows {
         read_ahead<NK * G::kQ, 4, RT * (sizeof(T) == 4 ? 4 : 1)>();
     }
 
-    // Keys that are not there (bias -inf; their products are 0, or NaN where the
-    // query is no number) or that a row does not see: -inf
+    // Keys that are not there or that a row does not see: -inf
     template <int NK>
-    __device__ __forceinline__ void hide(f32x4 (&s)[RT][NK], const float *bias, int32_t key0)
+    __device__ __forceinline__ void hide(f32x4 (&s)[RT][NK], const int32_t *place)
     {
         const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
         for (int k = 0; k < NK; k++) {
-            const f32x4 b = *(const f32x4 *)(bias + k * 16 + 4 * g);
+            const i32x4 at = *(const i32x4 *)(place + k * 16 + 4 * g);
 #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                s[t][k] += b;
+            for (int t = 0; t < RT; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    s[t][k][i] = key0 + k * 16 + 4 * g + i < sees[t] ? s[t][k][i] : -INFINITY;
-            }
+                for (int i = 0; i < 4; i++) s[t][k][i] = at[i] < sees[t] ? s[t][k][i] : -INFINITY;
         }
     }
 
@@ -728,21 +725,17 @@ template <typename T, int HD> struct Rows32 {
         read_ahead<NK * kC, 4, 1>();
     }
 
-    template <int NK>
-    __device__ __forceinline__ void hide(f32x16 (&s)[NK], const float *bias, int32_t key0)
+    template <int NK> __device__ __forceinline__ void hide(f32x16 (&s)[NK], const int32_t *place)
     {
         const int g = (threadIdx.x & 63) >> 5;
 #pragma unroll
         for (int k = 0; k < NK; k++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int key = k * 32 + 8 * j + 4 * g;
-                const f32x4 b = *(const f32x4 *)(bias + key);
+                const i32x4 at = *(const i32x4 *)(place + k * 32 + 8 * j + 4 * g);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float x = s[k][4 * j + i] + b[i];
-                    s[k][4 * j + i] = key0 + key + i < sees ? x : -INFINITY;
-                }
+                for (int i = 0; i < 4; i++)
+                    s[k][4 * j + i] = at[i] < sees ? s[k][4 * j + i] : -INFINITY;
             }
     }
 
@@ -928,8 +921,7 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
     constexpr int KEYS = G::kBlockKeys, kTile = KEYS * G::kSlots;
     constexpr uint32_t kBytes = kTile * 16;
     u32x4 *K = (u32x4 *)lds, *V = K + 2 * kTile;
-    float *bias = (float *)(V + 2 * kTile);
-    int32_t *flags = (int32_t *)(bias + 2 * KEYS);
+    int32_t *place = (int32_t *)(V + 2 * kTile), *flags = place + 2 * KEYS;
     const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds,
                    lds_v = lds_k + 2 * kBytes;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -946,7 +938,7 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
     const int tiles = keys.end > first ? (keys.end - first + KEYS - 1) / KEYS : 0;
     auto step = [&](int i, int b) -> bool {                 // false: a value that is not finite
         if (i + 1 < tiles) {
-            st.keys_to(a, keys, h, lds_k + (b ^ 1) * kBytes, bias + (b ^ 1) * KEYS,
+            st.keys_to(a, keys, h, lds_k + (b ^ 1) * kBytes, place + (b ^ 1) * KEYS,
                        flags + (b ^ 1) * kWaves);
             st.values_to(lds_v + (b ^ 1) * kBytes);
         }
@@ -957,7 +949,7 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
         __builtin_amdgcn_sched_barrier(0);
         w.scores(K + b * kTile, s);
         if (key0 + KEYS > all || __builtin_amdgcn_readfirstlane(miss.x | miss.y | miss.z | miss.w))
-            w.hide(s, bias + b * KEYS, key0);
+            w.hide(s, place + b * KEYS);
         w.raise(s, a.c);
         w.values(V + b * kTile, s, a.c, a.c_low);
         stage_wait();
@@ -965,7 +957,7 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
     };
     bool fine = true;                           // every wave looks at all of a tile: uniform
     if (tiles > 0) {
-        st.keys_to(a, keys, h, lds_k, bias, flags);
+        st.keys_to(a, keys, h, lds_k, place, flags);
         st.values_to(lds_v);
         stage_wait();
         for (int i = 0;; i += 2) {
@@ -1000,7 +992,7 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, r = lane & 15;
     u32x4 *K = (u32x4 *)lds + wave * 2 * kTile, *V = K + kTile;
-    float *bias = (float *)((u32x4 *)lds + kWaves * 2 * kTile) + wave * KEYS;
+    int32_t *place = (int32_t *)((u32x4 *)lds + kWaves * 2 * kTile) + wave * KEYS;
     Rows<T, HD, 1> w;
     Stage<T, HD, KEYS> st;
     st.start(a, keys, first + wave * KEYS, kWaves * KEYS);
@@ -1020,7 +1012,7 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
     if (begin < keys.end) st.load(a, keys, h);
     for (int32_t key0 = begin; key0 < keys.end; key0 += step) {
         const bool missing = st.missing();
-        st.store(K, V, bias);
+        st.store(K, V, place, key0);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -1031,7 +1023,7 @@ __device__ __forceinline__ void wave_rows(const AttnArgs &a, char *lds, int h, i
         }
         f32x4 s[1][KEYS / 16];
         w.scores(K, s);
-        if (missing || key0 + KEYS > all) w.hide(s, bias, key0);
+        if (missing || key0 + KEYS > all) w.hide(s, place);
         w.raise(s, a.c);
         w.values(V, s, a.c, a.c_low);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");

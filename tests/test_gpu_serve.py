@@ -163,6 +163,44 @@ def test_prompt(cuda, ops, dtype, hd, runs, past, prefix, n_kv, rep, page):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("page", [1, 300, 4096])
+def test_pages_of_any_size(cuda, ops, dtype, page):
+    b = Batch([70, 1, 333], 401, 1, 4, 64, page, dtype, seed=page)
+    check_decode(ops, b, f"page {page}")
+    check_prompt(ops, b, [30, 1, 90], f"page {page}")
+
+
+@pytest.mark.parametrize("n_kv,rep", [(1, 1), (8, 4)])
+def test_many_sequences(cuda, ops, n_kv, rep):
+    """More runs than a wave has lanes, empty ones among them."""
+    rng = torch.Generator().manual_seed(2)
+    runs = [int(x) for x in torch.randint(0, 7, (150,), generator=rng)]
+    b = Batch([n + 3 for n in runs], 20, n_kv, rep, 64, 16, "bf16", seed=21)
+    check_prompt(ops, b, runs, "150 runs")
+    check_decode(ops, b, "150 sequences")
+
+
+def test_nothing_of_one_kind(cuda, ops):
+    """Tables without pages, no tokens, no sequences."""
+    b = Batch([0, 0], 33, 1, 2, 64, 16, "bf16", seed=22, room=0)
+    assert b.tables.shape == (2, 0)
+    check_decode(ops, b, "the prefix alone")
+    b2 = Batch([0, 0], 900, 2, 20, 64, 16, "bf16", seed=22, room=0)
+    check_decode(ops, b2, "a long prefix alone")
+    k, v, prefix_table, tables, lengths = b.cuda()
+    q = b.queries(5).cuda()
+    none = torch.zeros(0, dtype=torch.int32, device=cuda)
+    out = ops.prefix_attention_prompt(q, none.new_zeros(1), k, v, prefix_table, 33, tables[:0], none, 0.1)
+    assert out.shape == q.shape and not out.any()
+    for x in (ops.prefix_attention_decode(q[:0], k, v, prefix_table, 33, tables[:0], none, 0.1),
+              ops.prefix_attention_prompt(q[:0], none.new_zeros(3), k, v, prefix_table, 33, tables,
+                                          lengths, 0.1)):
+        assert x.shape == (0, 2, 64)
+    out = decode(ops, Batch([0], 0, 1, 2, 64, 16, "f32", room=0), torch.ones(1, 2, 64), 0.1)
+    assert not out.any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("rep", [4, 7])
 def test_prompt_many_rows(cuda, ops, dtype, rep):
     """Enough rows for the widest tiles: whole and part-full ones, masks that
@@ -299,6 +337,20 @@ def test_values_not_finite(cuda, ops, dtype, hd, runs, past, n_kv, rep):
     assert torch.equal(got.isnan(), want.isnan())
     assert torch.equal(got[want.isinf()], want[want.isinf()])
     so.near(got[~odd], want[~odd], tol[~odd], "beside them")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_nan_queries_without_keys(cuda, ops, dtype):
+    """A query of NaN that sees no key gets zeros as any other: hidden pages, no
+    keys, tokens before the first own key."""
+    b = Batch([40, 0, 40], 0, 2, 2, 64, 16, dtype, seed=20)
+    b.tables[0] = -1
+    q = torch.full((3, 4, 64), float("nan"), dtype=b.dtype)
+    out = decode(ops, b, q, 0.125)
+    assert not out[:2].any() and out[2].isnan().all()
+    b.lengths[2] = 5
+    out = prompt(ops, b, q.repeat(10, 1, 1), starts([10, 10, 10]), 0.125)
+    assert not out[:25].any() and out[25:].isnan().all()
 
 
 @pytest.mark.parametrize("parts", [False, True])
