@@ -165,33 +165,86 @@ inline Plan plan_decode(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
     return p;
 }
 
+// A prompt's block of 16, 64 or 128 rows (rt 0, 1, 2) takes this many us for 1000
+// keys, alone on its CU and beside another block (rows of 1024 bytes: there is
+// none), measured over 2000 to 4000 keys.
+inline void walk_us(int row_bytes, int hd, int rt, double &alone, double &paired)
+{
+    static const float us[2][3][3][2] = {
+        {{{5.4f, 8.2f}, {15, 17}, {17.5f, 20}},             // 16-bit types: hd 64, 128, 256
+         {{10.4f, 14.8f}, {20, 25}, {24, 32}},
+         {{22.5f, 31}, {38, 46}, {0, 0}}},
+        {{{17, 27}, {46, 68}, {75, 116}},                   // fp32
+         {{33, 50}, {84, 126}, {0, 0}},
+         {{96, 96}, {182, 182}, {0, 0}}}};
+    const float *u = us[row_bytes == 4 * hd][hd == 64 ? 0 : hd == 128 ? 1 : 2][rt];
+    alone = u[0];
+    paired = u[1];
+}
+
 inline Plan plan_prompt(int row_bytes, int hd, int n_kv, int rep, int64_t prefix, int64_t capacity,
                         int64_t batch, int64_t N)
 {
+    // Rows a block, and parts of the keys, by the least time: few rows a block
+    // spread over the CUs, many read the keys fewer times; parts shorten the walk
+    // and cost their fp32 sums, written and read, and a launch (4 us).  Tried are
+    // one part, and as many as fill each CU with one block or with two.  bf16, 32
+    // heads on 8 of 128: 256 tokens 9.3 us (16 rows, one part) against 17 (128 rows,
+    // two parts), 512 16 (64 rows) against 28 (128, three), 2048 60 (128) against 70
+    // (64); 48 behind 1500 shared keys 18 (64 rows, seven parts) against 21 (16, one).
+    // The lengths are device data: a sequence's own keys are taken halfway between
+    // the new tokens and the table's room, and no more than 1024 short of that.
+    const int64_t rows = N * rep, runs = cbq_max(cbq_min(batch, N), 1);
+    const int64_t own = cbq_max((capacity + N / runs) / 2, capacity - 1024);
+    const int64_t keys = cbq_max(prefix + own, 1);
+    const int64_t slots = row_bytes <= 512 ? 2 * kCus : kCus;
+    // bytes a us of the parts' sums, written and read; rows of 1 KiB go through faster
+    // (fp32 blocks of hd 256 start so slowly that parts pay later)
+    const double rate = row_bytes == 512 && hd == 256 ? 5e6 : 2.5e6;
+    double best = -1;
+    int best_rt = 0;
+    int64_t best_parts = 1;
+    for (int rt = 0; rt <= widest(row_bytes); rt++) {
+        const int64_t m = rt ? 64 * rt : 16;
+        // two tiles of keys a part: from four the few rows over 500 to 3000 keys took
+        // 1.1 to 1.3 times as long
+        const int64_t least = 2 * (rt ? block_keys(row_bytes) : kAttnWaves * wave_keys(row_bytes));
+        // of the runs' last tiles, half are taken to be there beside the whole ones
+        const int64_t likely = n_kv * cbq_max(runs == 1 ? cbq_ceil(rows, m) : rows / m + cbq_ceil(runs, 2),
+                                              runs);
+        double alone, paired;
+        walk_us(row_bytes, hd, rt, alone, paired);
+        for (int fill = 0; fill < 3; fill++) {
+            const int64_t parts = fill == 0 ? 1 : cbq_min((fill == 1 ? kCus : slots) / cbq_max(likely, 1),
+                                                          keys / least);
+            if (parts < 1 || (fill > 0 && parts == 1)) continue;
+            const double most = 0.001 * keys / parts;               // thousands of keys, the last tile's
+            const double mean = cbq_max(keys - N / runs / 2, 1) * 0.001 / parts;
+            const double blocks = (double)likely * parts;
+            // the block of the most keys shares its CU with one of few
+            const double beside = blocks > kCus ? cbq_max(2 * mean - most, 0.0) : 0;
+            double us = alone * most + (paired - alone) * beside;
+            if (blocks > slots) {
+                // more turns than one; each block begins with 3 us of dependent loads
+                const double turns = blocks / slots, all = turns * mean * paired + 3 * (turns - 1);
+                us = us > all ? us : all;
+            }
+            if (parts > 1) us += 4 + (double)parts * N * n_kv * rep * hd * 8 / rate;
+            if (best < 0 || us < best) {
+                best = us;
+                best_rt = rt;
+                best_parts = parts;
+            }
+        }
+    }
     Plan p = {};
-    const int64_t rows = N * rep, small = (cbq_ceil(rows, 16) + batch) * n_kv;
-    const int64_t keys = cbq_max(prefix + capacity, 1);
-    // 16 rows a block for runs that fill no more, and where a few rows meet few keys
-    if (rows <= 16 * batch || (small <= 2 * kCus && keys <= 2048)) p.rt = 0;
-    else p.rt = rows <= 64 * batch ? 1 : widest(row_bytes);
+    p.rt = best_rt;
     // a run's last tile may be part full: one more a run than the rows need
-    const int64_t m = p.rt ? 64 * p.rt : 16;
-    const int64_t tiles = rows / m + cbq_min(batch, N);
-    const int64_t blocks = tiles * n_kv;
-    // Few tiles: their keys in parts, as many as the CUs have room for at once (a
-    // few more would run alone, in a second turn): two blocks a CU, one of rows of
-    // 1024 bytes.  Of the runs' last tiles, half are taken to be there beside the
-    // rows' whole ones.  A part has four tiles at least (of 16-row blocks eight a
-    // wave: below that the merge takes longer).
-    const int64_t least = p.rt ? 4 * block_keys(row_bytes) : 8 * kAttnWaves * wave_keys(row_bytes);
-    const int64_t likely = (batch == 1 ? cbq_ceil(rows, m) : rows / m + cbq_ceil(cbq_min(batch, N), 2))
-                           * n_kv;
-    const int64_t room = row_bytes <= 512 ? 2 * kCus : kCus;
-    const int64_t parts = cbq_max(1, cbq_min(room / cbq_max(likely, 1), keys / least));
-    p.blocks = blocks * parts;
-    p.bytes = part_bytes(parts, N, n_kv * rep, hd);
+    const int64_t tiles = rows / (p.rt ? 64 * p.rt : 16) + runs;
+    p.blocks = tiles * n_kv * best_parts;
+    p.bytes = part_bytes(best_parts, N, n_kv * rep, hd);
     p.tiles = (int32_t)tiles;
-    p.parts = (int32_t)parts;
+    p.parts = (int32_t)best_parts;
     return p;
 }
 

@@ -139,6 +139,10 @@ static void prompt()
     const int N = q_start[batch] + 1;
     const Plan p = plan_prompt(hd * size, hd, n_kv, rep, prefix, (int64_t)width * page, batch, N);
     CHECK(plan_fits(p));
+    // parts only where CUs are left, and none shorter than two tiles
+    CHECK(p.parts == 1 || (int64_t)p.parts * n_kv * std::min(batch, N) <= 2 * kCus);
+    CHECK(p.parts == 1 || (int64_t)p.parts * 2 * (p.rt ? block_keys(hd * size) : kAttnWaves * wave_keys(hd * size)) <=
+                              prefix + std::max<int64_t>((int64_t)width * page, N));
     const int m = p.rt ? 64 * p.rt : 16;
     int64_t tiles = 0;
     for (int b = 0; b < batch; b++) {
