@@ -96,6 +96,7 @@ struct Plan {
     int32_t pre_parts, pre_chunk;           // decode: parts of the prefix and their keys
     int32_t own_parts, own_chunk, own_tiles;    // decode: parts of the own keys, 16-row tiles
     int32_t parts;                          // decode: all of them; prompt: key parts of a tile
+    int32_t streams;                        // prompt: halves of a block's keys, walked side by side
     int32_t joint;                          // decode: a sequence's one part walks the prefix too
     int64_t blocks, bytes;
 };
@@ -185,13 +186,15 @@ inline void walk_us(int row_bytes, int hd, int rt, double &alone, double &paired
 inline Plan plan_prompt(int row_bytes, int hd, int n_kv, int rep, int64_t prefix, int64_t capacity,
                         int64_t batch, int64_t N)
 {
-    // Rows a block, and parts of the keys, by the least time: few rows a block
-    // spread over the CUs, many read the keys fewer times; parts shorten the walk
-    // and cost their fp32 sums, written and read, and a launch (4 us).  Tried are
-    // one part, and as many as fill each CU with one block or with two.  bf16, 32
-    // heads on 8 of 128: 256 tokens 9.3 us (16 rows, one part) against 17 (128 rows,
-    // two parts), 512 16 (64 rows) against 28 (128, three), 2048 60 (128) against 70
-    // (64); 48 behind 1500 shared keys 18 (64 rows, seven parts) against 21 (16, one).
+    // Rows a block, parts of the keys, and streams a block, by the least time: few
+    // rows a block spread over the CUs, many read the keys fewer times; parts shorten
+    // the walk and cost their fp32 sums, written and read, and a launch (4 us); two
+    // streams halve it for a whole CU and a join in LDS.  bf16, 32 heads on 8 of 128:
+    // 256 tokens 9.2 us (16 rows, one part) against 17 (128 rows, two parts), 512 15
+    // (64 rows, two streams) against 28 (128, three parts) and 16 (64, one stream), 1024
+    // 29 against 43 (128, two parts), 2048 57 (128, two streams) against 70 (64); behind
+    // 1500 shared keys 48 18 (64 rows, seven parts) against 21 (16, one part), 1024 56
+    // (128, two streams) against 65 (64, one).
     // The lengths are device data: a sequence's own keys are taken halfway between
     // the new tokens and the table's room, and no more than 1024 short of that.
     const int64_t rows = N * rep, runs = cbq_max(cbq_min(batch, N), 1);
@@ -203,7 +206,7 @@ inline Plan plan_prompt(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
     const double rate = row_bytes == 512 && hd == 256 ? 5e6 : 2.5e6;
     double best = -1;
     int best_rt = 0;
-    int64_t best_parts = 1;
+    int64_t best_parts = 1, best_streams = 1;
     for (int rt = 0; rt <= widest(row_bytes); rt++) {
         const int64_t m = rt ? 64 * rt : 16;
         // two tiles of keys a part: from four the few rows over 500 to 3000 keys took
@@ -214,19 +217,33 @@ inline Plan plan_prompt(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
                                               runs);
         double alone, paired;
         walk_us(row_bytes, hd, rt, alone, paired);
-        for (int fill = 0; fill < 3; fill++) {
-            const int64_t parts = fill == 0 ? 1 : cbq_min((fill == 1 ? kCus : slots) / cbq_max(likely, 1),
-                                                          keys / least);
-            if (parts < 1 || (fill > 0 && parts == 1)) continue;
+        for (int way = 0; way < 5; way++) {
+            // one stream of keys a block: one part, parts to a block a CU, to two; two
+            // streams, which are two blocks' waves as one: one part, parts to a block a CU
+            const int streams = way < 3 ? 1 : 2;
+            if (streams == 2 && (rt == 0 || slots == kCus)) break;
+            const int64_t room = streams == 2 ? kCus : slots;
+            // two streams fill a CU: one block too many is a turn more
+            const int64_t blocks0 = streams == 2 ? n_kv * (runs == 1 ? cbq_ceil(rows, m) : rows / m + runs)
+                                                 : likely;
+            const int64_t parts = way % 3 == 0 ? 1 : cbq_min((way == 2 ? slots : kCus) / blocks0,
+                                                             keys / (streams * least));
+            if (parts < 1 || (way % 3 && parts == 1)) continue;
             const double most = 0.001 * keys / parts;               // thousands of keys, the last tile's
             const double mean = cbq_max(keys - N / runs / 2, 1) * 0.001 / parts;
-            const double blocks = (double)likely * parts;
-            // the block of the most keys shares its CU with one of few
-            const double beside = blocks > kCus ? cbq_max(2 * mean - most, 0.0) : 0;
-            double us = alone * most + (paired - alone) * beside;
-            if (blocks > slots) {
-                // more turns than one; each block begins with 3 us of dependent loads
-                const double turns = blocks / slots, all = turns * mean * paired + 3 * (turns - 1);
+            const double fewest = 2 * mean > most ? 2 * mean - most : 0;
+            const double blocks = (double)blocks0 * parts, both = streams == 2 ? 0.55 * paired : paired;
+            double us;
+            if (streams == 2)
+                us = both * most + 3;                               // and the join
+            else                // the block of the most keys shares its CU with one of few
+                us = alone * most + (blocks > kCus ? (paired - alone) * fewest : 0);
+            if (blocks > room) {
+                // more turns than one, the last as long as its blocks where all are alike;
+                // each block begins with 3 us of dependent loads
+                const int64_t whole = cbq_ceil(blocks0 * parts, room);
+                const double turns = blocks / room,
+                             all = both * (turns * mean + (whole - turns) * fewest) + 3 * (turns - 1);
                 us = us > all ? us : all;
             }
             if (parts > 1) us += 4 + (double)parts * N * n_kv * rep * hd * 8 / rate;
@@ -234,11 +251,13 @@ inline Plan plan_prompt(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
                 best = us;
                 best_rt = rt;
                 best_parts = parts;
+                best_streams = streams;
             }
         }
     }
     Plan p = {};
     p.rt = best_rt;
+    p.streams = (int32_t)best_streams;
     // a run's last tile may be part full: one more a run than the rows need
     const int64_t tiles = rows / (p.rt ? 64 * p.rt : 16) + runs;
     p.blocks = tiles * n_kv * best_parts;
@@ -298,6 +317,17 @@ CBQ_PAGED_FN void prompt_keys(int32_t sees, int parts, int part, int unit, int32
     const int64_t share = cbq_ceil(cbq_ceil(sees, parts), unit) * unit;
     first = (int32_t)cbq_min(part * share, sees);
     end = (int32_t)cbq_min(first + share, sees);
+}
+
+// The keys [first, end) of one of a block's streams: whole tiles to the streams in
+// turn, the first ones' share the larger.
+CBQ_PAGED_FN void stream_keys(int32_t from, int32_t upto, int unit, int streams, int stream,
+                              int32_t &first, int32_t &end)
+{
+    const int64_t keys = upto > from ? upto - from : 0;
+    const int64_t share = cbq_ceil(cbq_ceil(keys, unit), streams) * unit;
+    first = (int32_t)(from + cbq_min(stream * share, keys));
+    end = (int32_t)(from + cbq_min((stream + 1) * share, keys));
 }
 
 }  // namespace cbq_attn

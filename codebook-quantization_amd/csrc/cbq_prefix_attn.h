@@ -263,6 +263,23 @@ __device__ __forceinline__ void stage_wait()
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// This wave's number in its stream of four
+__device__ __forceinline__ int stream_wave() { return threadIdx.x >> 6 & (kWaves - 1); }
+
+// The same among one stream's four waves: each counts itself in, and waits until four
+// times `passed` have.  Its waves pass equally often, so every wait ends.
+__device__ __forceinline__ void stream_wait(uint32_t *count, uint32_t &passed)
+{
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    if ((threadIdx.x & 63) == 0)
+        __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    passed += kWaves;
+    while ((uint32_t)__builtin_amdgcn_readfirstlane(__hip_atomic_load(
+               count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)) < passed)
+        __builtin_amdgcn_s_sleep(1);
+    asm volatile("" ::: "memory");
+}
+
 template <typename T, int HD, int KEYS> struct Copies {
     using G = Geo<T, HD>;
     static constexpr int kRows = kThreads / G::kSlots, kPer = KEYS / kRows;
@@ -276,7 +293,7 @@ template <typename T, int HD, int KEYS> struct Copies {
 
     __device__ __forceinline__ void start(const AttnArgs &a, const CbqKeys &keys, int32_t first)
     {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int lane = threadIdx.x & 63, wave = stream_wave();
         at = lane < kMine ? lane / kWide * kRows + wave * kWide + lane % kWide : -1;
         step_entry = (int32_t)cbq_div((uint32_t)KEYS, a.page);
         step_row = KEYS - step_entry * (int32_t)a.page.d;
@@ -294,7 +311,7 @@ template <typename T, int HD, int KEYS> struct Copies {
     __device__ __forceinline__ void keys_to(const AttnArgs &a, const CbqKeys &keys, int h, uint32_t lds,
                                             int32_t *place, int32_t *flags)
     {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / G::kSlots;
+        const int lane = threadIdx.x & 63, wave = stream_wave(), sub = lane / G::kSlots;
         const bool in = id >= 0 && id < a.kv.n_pages;
         const uint64_t there = __ballot(in);
         constexpr uint64_t every = kMine == 64 ? ~0ull : (1ull << (kMine & 63)) - 1;
@@ -334,7 +351,7 @@ template <typename T, int HD, int KEYS> struct Copies {
     __device__ __forceinline__ void values_to(uint32_t lds)
     {
 #pragma unroll
-        for (int i = 0; i < kPer; i++) copy_slots(lds + offset(i, threadIdx.x >> 6), v[i]);
+        for (int i = 0; i < kPer; i++) copy_slots(lds + offset(i, stream_wave()), v[i]);
     }
     static __device__ __forceinline__ uint32_t offset(int i, int wave)
     {
@@ -412,6 +429,16 @@ __device__ __forceinline__ void put_stats(const AttnArgs &a, int part, int64_t t
 __device__ __forceinline__ int32_t row_sees(int32_t prefix, int32_t past, int32_t i)
 {
     return prefix + (past + i + 1 > 0 ? past + i + 1 : 0);
+}
+
+// Two states of a row to one: m, l and the factors of their values
+__device__ __forceinline__ void join(float &m, float &l, float2 other, float &f, float &g)
+{
+    const float top = fmaxf(m, other.x), base = top == -INFINITY ? 0.f : top;
+    f = __builtin_amdgcn_exp2f(m - base);
+    g = __builtin_amdgcn_exp2f(other.x - base);
+    l = l * f + other.y * g;
+    m = top;
 }
 
 // 16 bytes of a query (zeros where the row is none), times scale's sign
@@ -546,6 +573,29 @@ template <typename T, int HD, int RT> struct Rows {
             for (int d = 0; d < G::kD; d++)
                 put_values<T, HD>(a, part, token, head, d * 16 + 4 * (lane >> 4), o[t][d], total);
             if (lane < 16) put_stats(a, part, token, head, m[t], total);
+        }
+    }
+
+    // The state to LDS, and another wave's of the same rows, given there by the same
+    // lane, into this one
+    static constexpr int kGiven = RT * G::kD;
+    __device__ __forceinline__ void give(f32x4 *x, float2 *ml) const
+    {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            ml[t * kThreads] = make_float2(m[t], l[t]);
+#pragma unroll
+            for (int d = 0; d < G::kD; d++) x[(t * G::kD + d) * kThreads] = o[t][d];
+        }
+    }
+    __device__ __forceinline__ void take(const f32x4 *x, const float2 *ml)
+    {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            float f, g;
+            join(m[t], l[t], ml[t * kThreads], f, g);
+#pragma unroll
+            for (int d = 0; d < G::kD; d++) o[t][d] = o[t][d] * f + x[(t * G::kD + d) * kThreads] * g;
         }
     }
 
@@ -784,6 +834,31 @@ template <typename T, int HD> struct Rows32 {
         if (lane < 32) put_stats(a, part, token, head, m, total);
     }
 
+    static constexpr int kGiven = HD / 8;
+    __device__ __forceinline__ void give(f32x4 *x, float2 *ml) const
+    {
+        *ml = make_float2(m, l);
+#pragma unroll
+        for (int d = 0; d < kO; d++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                x[(d * 4 + j) * kThreads] = f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2],
+                                                  o[d][4 * j + 3]};
+    }
+    __device__ __forceinline__ void take(const f32x4 *x, const float2 *ml)
+    {
+        float f, g;
+        join(m, l, *ml, f, g);
+#pragma unroll
+        for (int d = 0; d < kO; d++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const f32x4 y = x[(d * 4 + j) * kThreads];
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[d][4 * j + i] = o[d][4 * j + i] * f + y[i] * g;
+            }
+    }
+
     // Weights of the tile, and the values under them: 16 keys' values are read while
     // the 16 before them are in the products, beside which the 16 keys' weights after
     // them are made.
@@ -905,6 +980,12 @@ __device__ __forceinline__ void plain_rows(const AttnArgs &a, int h, int64_t tok
     }
 }
 
+template <typename T, int HD> constexpr int block_lds()
+{
+    using G = Geo<T, HD>;
+    return 4 * G::kBlockKeys * G::kSlots * 16 + 2 * G::kBlockKeys * 4 + 2 * kWaves * 4;
+}
+
 // ---- 64 RT rows of a block against keys [first, end), tiles shared by the waves ----------
 // 64 keys of K and V (rows of 256 bytes) in two buffers of 32 KiB, so that two blocks
 // share a CU.  32 rows a wave: 16 take 772 us instead of 560 for 8192 tokens (LDS
@@ -912,19 +993,32 @@ __device__ __forceinline__ void plain_rows(const AttnArgs &a, int h, int64_t tok
 // 16 ragged prompts and 366 instead of 327 at hd 64; deeper rings of tiles gain
 // nothing, and 32 rows of 512 bytes, which leave one wave a SIMD, lose (67 us
 // instead of 48 for two chunks against 20000 keys).
-template <typename T, int HD, int RT, bool CAUSAL>
+//
+// With STREAMS 2 eight waves are two such groups, each with a half of the keys,
+// tiles and buffers of its own, in no step with the other (waits of all eight: 53 us
+// instead of 48 for two chunks against 20000 keys); their states are joined in LDS
+// at the end.  For grids of a block a CU, where four waves leave a SIMD one: bf16, 32
+// heads on 8 of 128, 512 tokens behind 1500 shared keys 37 us instead of 45, 1024 56
+// instead of 65; with more blocks two of four waves do as well (8192 tokens).
+template <typename T, int HD, int RT, bool CAUSAL, int STREAMS = 1>
 __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, int64_t token0,
-                                           int row0, int n, const CbqKeys &keys, int32_t first,
+                                           int row0, int n, const CbqKeys &whole, int32_t from,
                                            int32_t past, int part)
 {
     using G = Geo<T, HD>;
     constexpr int KEYS = G::kBlockKeys, kTile = KEYS * G::kSlots;
     constexpr uint32_t kBytes = kTile * 16;
-    u32x4 *K = (u32x4 *)lds, *V = K + 2 * kTile;
+    const int all_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = STREAMS > 1 ? all_wave & (kWaves - 1) : all_wave;
+    const int stream = STREAMS > 1 ? all_wave / kWaves : 0;
+    CbqKeys keys = whole;
+    int32_t first = from;
+    if (STREAMS > 1) stream_keys(from, whole.end, KEYS, STREAMS, stream, first, keys.end);
+    char *mem = lds + stream * block_lds<T, HD>();
+    u32x4 *K = (u32x4 *)mem, *V = K + 2 * kTile;
     int32_t *place = (int32_t *)(V + 2 * kTile), *flags = place + 2 * KEYS;
-    const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds,
+    const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)mem,
                    lds_v = lds_k + 2 * kBytes;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int mine = row0 + wave * 16 * RT;
     std::conditional_t<RT == 2 && sizeof(T) == 2, Rows32<T, HD>, Rows<T, HD, RT>> w;
     Copies<T, HD, KEYS> st;
@@ -936,6 +1030,15 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
         w.see(a, keys.prefix, past, mine);
     }
     const int tiles = keys.end > first ? (keys.end - first + KEYS - 1) / KEYS : 0;
+    uint32_t *counts = (uint32_t *)(lds + STREAMS * block_lds<T, HD>()), passed = 0;
+    if (STREAMS > 1) {
+        if (threadIdx.x < STREAMS) counts[threadIdx.x] = 0;
+        __syncthreads();
+    }
+    auto wait = [&]() {
+        if (STREAMS > 1) stream_wait(counts + stream, passed);
+        else stage_wait();
+    };
     auto step = [&](int i, int b) -> bool {                 // false: a value that is not finite
         if (i + 1 < tiles) {
             st.keys_to(a, keys, h, lds_k + (b ^ 1) * kBytes, place + (b ^ 1) * KEYS,
@@ -952,14 +1055,14 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
             w.hide(s, place + b * KEYS);
         w.raise(s, a.c);
         w.values(V + b * kTile, s, a.c, a.c_low);
-        stage_wait();
+        wait();
         return true;
     };
     bool fine = true;                           // every wave looks at all of a tile: uniform
     if (tiles > 0) {
         st.keys_to(a, keys, h, lds_k, place, flags);
         st.values_to(lds_v);
-        stage_wait();
+        wait();
         for (int i = 0;; i += 2) {
             fine = step(i, 0);
             if (!fine || i + 1 >= tiles) break;
@@ -967,10 +1070,23 @@ __device__ __forceinline__ void block_rows(const AttnArgs &a, char *lds, int h, 
             if (!fine || i + 2 >= tiles) break;
         }
     }
-    if (CAUSAL && !fine) {
-        stage_wait();                           // no copy is under way when the block ends
-        plain_rows<T, HD>(a, h, token0, row0, 16 * RT * kWaves, n, keys, first, past, part);
+    if (CAUSAL && !fine) wait();                // no copy is under way when the block ends
+    bool odd = CAUSAL && !fine;
+    if (STREAMS > 1) odd = __syncthreads_or(odd);
+    if (CAUSAL && odd) {
+        plain_rows<T, HD>(a, h, token0, row0, 16 * RT * kWaves, n, whole, from, past, part);
         return;
+    }
+    if constexpr (STREAMS > 1) {
+        static_assert(kThreads * (decltype(w)::kGiven * 16 + RT * 8) <= STREAMS * block_lds<T, HD>(),
+                      "a stream's state");
+        f32x4 *x = (f32x4 *)lds + (threadIdx.x & (kThreads - 1));
+        float2 *ml = (float2 *)((f32x4 *)lds + decltype(w)::kGiven * kThreads) +
+                     (threadIdx.x & (kThreads - 1));
+        if (stream) w.give(x, ml);
+        __syncthreads();
+        if (stream) return;
+        w.take(x, ml);
     }
     w.put(a, part, h, token0, mine, n);
 }
@@ -1090,11 +1206,6 @@ template <typename T, int HD> constexpr int wave_lds()
     constexpr int merge = kWaves * 16 * HD * 4 + kWaves * 16 * 8 + 16 * 4;
     return tiles > merge ? tiles : merge;
 }
-template <typename T, int HD> constexpr int block_lds()
-{
-    using G = Geo<T, HD>;
-    return 4 * G::kBlockKeys * G::kSlots * 16 + 2 * G::kBlockKeys * 4 + 2 * kWaves * 4;
-}
 
 // ---- decode: parts of the prefix for all sequences, parts of each one's own keys ------------
 // PT: 64 PT prefix rows a block; 0: the prefix rows are 16 at most and go as the
@@ -1122,8 +1233,8 @@ __global__ __launch_bounds__(kThreads, simd_waves(HD * (int)sizeof(T))) void dec
 
 // ---- prompt: tiles of each run's rows against the keys they see -----------------------------
 // RT: 64 RT rows a block; 0: 16 rows.
-template <typename T, int HD, int RT>
-__global__ __launch_bounds__(kThreads, simd_waves(HD * (int)sizeof(T))) void prompt_kernel(AttnArgs a)
+template <typename T, int HD, int RT, int STREAMS = 1>
+__global__ __launch_bounds__(STREAMS * kThreads, simd_waves(HD * (int)sizeof(T))) void prompt_kernel(AttnArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int M = RT ? 64 * RT : 16;
@@ -1139,7 +1250,7 @@ __global__ __launch_bounds__(kThreads, simd_waves(HD * (int)sizeof(T))) void pro
                       hi = cbq_max(cbq_clamp_length(a.q_start[a.batch], a.N), lo);
         T *out = (T *)a.out;
         const int64_t w = (int64_t)a.n_q * HD;
-        for (int64_t e = threadIdx.x; e < (lo + a.N - hi) * w; e += kThreads)
+        for (int64_t e = threadIdx.x; e < (lo + a.N - hi) * w; e += STREAMS * kThreads)
             out[e < lo * w ? e : e + (hi - lo) * w] = (T)0.f;
     }
     // the run that holds tile `want`: its count of tiles, summed over the runs
@@ -1184,8 +1295,8 @@ __global__ __launch_bounds__(kThreads, simd_waves(HD * (int)sizeof(T))) void pro
                     RT ? Geo<T, HD>::kBlockKeys : Geo<T, HD>::kWaveKeys, first, end);
     const CbqKeys keys = {a.prefix_table, a.tables + run * a.table_st, a.prefix, end};
     if constexpr (RT > 0)
-        block_rows<T, HD, RT, true>(a, lds, h, first_token, row0, rows, keys, first, past,
-                                    a.plan.parts > 1 ? part : -1);
+        block_rows<T, HD, RT, true, STREAMS>(a, lds, h, first_token, row0, rows, keys, first, past,
+                                             a.plan.parts > 1 ? part : -1);
     else
         wave_rows<T, HD, true>(a, lds, h, first_token, row0, rows, keys, first, past,
                                a.plan.parts > 1 ? part : -1);
@@ -1277,7 +1388,7 @@ constexpr int64_t kMergeRows = 4096;
 
 // ---- launches of one type -------------------------------------------------------------------
 // More than 64 KiB of LDS is asked for once a kernel and device.
-template <auto K> int run_kernel(int64_t blocks, int lds, const AttnArgs &a, hipStream_t stream,
+template <auto K, int STREAMS = 1> int run_kernel(int64_t blocks, int lds, const AttnArgs &a, hipStream_t stream,
                                  const char *what)
 {
     static std::atomic<uint64_t> asked{0};
@@ -1292,7 +1403,7 @@ template <auto K> int run_kernel(int64_t blocks, int lds, const AttnArgs &a, hip
             asked.fetch_or(bit, std::memory_order_relaxed);
         }
     }
-    K<<<dim3((unsigned)blocks), dim3(kThreads), lds, stream>>>(a);
+    K<<<dim3((unsigned)blocks), dim3(STREAMS * kThreads), lds, stream>>>(a);
     return cbq_launch_status(what);
 }
 
@@ -1304,9 +1415,17 @@ template <typename T, int HD> int launch(const AttnArgs &a, const Plan &p, bool 
     int rc;
     if (prompt) {
         const char *what = "cbq_prefix_attn_prompt";
+        // two streams where a wave leaves room for another on its SIMD
+        constexpr int two = simd_waves(HD * (int)sizeof(T));
         if (p.rt == 0) rc = run_kernel<prompt_kernel<T, HD, 0>>(p.blocks, wl, a, stream, what);
-        else if (p.rt == 1) rc = run_kernel<prompt_kernel<T, HD, 1>>(p.blocks, bl, a, stream, what);
-        else rc = run_kernel<prompt_kernel<T, HD, wide>>(p.blocks, bl, a, stream, what);
+        else if (p.rt == 1 && p.streams == 1)
+            rc = run_kernel<prompt_kernel<T, HD, 1>>(p.blocks, bl, a, stream, what);
+        else if (p.rt == 1)
+            rc = run_kernel<prompt_kernel<T, HD, 1, two>, two>(p.blocks, two * (bl + 8), a, stream, what);
+        else if (p.streams == 1)
+            rc = run_kernel<prompt_kernel<T, HD, wide>>(p.blocks, bl, a, stream, what);
+        else
+            rc = run_kernel<prompt_kernel<T, HD, wide, two>, two>(p.blocks, two * (bl + 8), a, stream, what);
     } else {
         const char *what = "cbq_prefix_attn_decode";
         if (p.rt == 0 || !p.pre_parts)

@@ -158,6 +158,18 @@ static void prompt()
             int32_t first, end;
             prompt_keys(sees, p.parts, i, p.rt ? block_keys(hd * size) : wave_keys(hd * size), first, end);
             CHECK(first == at && end >= first && end <= sees);
+            // a block's streams: whole tiles, one after the other, the first's the more
+            int32_t then = first, more = 0;
+            for (int j = 0; j < p.streams; j++) {
+                int32_t f, e;
+                stream_keys(first, end, block_keys(hd * size), p.streams, j, f, e);
+                CHECK(f == then && e >= f && (e == end || (e - first) % block_keys(hd * size) == 0));
+                CHECK(j == 0 || e - f <= more);
+                then = e;
+                more = e - f;
+            }
+            CHECK(then == end);
+            CHECK(p.streams == 1 || (p.rt > 0 && hd * size <= 512));
             at = end;
         }
         CHECK(at == sees);
@@ -204,12 +216,28 @@ static void far()
     CHECK(end == most && first < end);
 }
 
+// The shapes whose two streams of keys a block the GPU tests count on
+static void streams()
+{
+    for (int hd : {64, 128, 256})
+        for (int size : {2, 4}) {
+            const bool room = hd * size <= 512;
+            const Plan p = plan_prompt(hd * size, hd, 8, 8, 500, 384, 1, 191);
+            CHECK(!room || (p.rt == 1 && p.streams == 2));
+            const Plan r = plan_prompt(hd * size, hd, 8, 16, 1900, 119, 3, 151);
+            CHECK(hd * size > 256 || size == 4 || (r.rt == 2 && r.streams == 2));
+        }
+    const Plan few = plan_prompt(256, 128, 8, 4, 0, 64, 1, 40);
+    CHECK(few.streams == 1);
+}
+
 int main()
 {
     divisions();
     far();
     for (int i = 0; i < 150; i++) decode();
     for (int i = 0; i < 400; i++) prompt();
+    streams();
     printf("all cases passed\n");
     return 0;
 }

@@ -122,6 +122,35 @@ def attend(batch, q, q_start, scale):
     return out, tol
 
 
+def attend_prompt(batch, q, q_start, scale):
+    """attend() by matrix products, for larger prompts whose values are finite."""
+    out, tol = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    half = half_step(batch.dtype)
+    for b in range(len(batch.lens)):
+        k, v, there = batch.dense(b)
+        lo, hi = int(q_start[b]), int(q_start[b + 1])
+        if lo == hi:
+            continue
+        ends = batch.prefix + (int(batch.lengths[b]) - hi + 1 + torch.arange(lo, hi)).clamp(min=0)
+        see = there[None] & (torch.arange(len(k))[None] < ends[:, None])
+        assert see.any(-1).all(), "a row without keys"
+        for h in range(batch.n_q):
+            ks, vs, x = k[:, h // batch.rep], v[:, h // batch.rep], q[lo:hi, h].double()
+            s = (x @ ks.T * scale).masked_fill(~see, float("-inf"))
+            p = torch.exp(s - s.amax(-1, keepdim=True))
+            total = p.sum(-1, keepdim=True)
+            big = abs(scale) * (x.abs() @ ks.abs().T).masked_fill(~see, 0).amax(-1, keepdim=True)
+            n = see.sum(-1, keepdim=True)
+            out[lo:hi, h], mass = p / total @ vs, p / total @ vs.abs()
+            tol[lo:hi, h] = half * out[lo:hi, h].abs() + (2 * (batch.hd + 4) * big + n / 16 + 64) * HALF * mass
+            if batch.dtype != torch.float32:
+                tol[lo:hi, h] += half * mass
+            if batch.dtype == torch.float16:
+                top = (vs.abs() * there[:, None]).cummax(0).values[ends - 1]
+                tol[lo:hi, h] += n * 2.0 ** -25 * top / total + 2.0 ** -25
+    return out, tol
+
+
 def append_rows(x, weight, cos, sin, positions, norm, eps):
     """Normed and rotated heads [N, heads, hd] in 64 bits and the magnitude of
     each value's pair."""

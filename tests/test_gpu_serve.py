@@ -210,6 +210,47 @@ def test_prompt_many_rows(cuda, ops, dtype, rep):
     check_prompt(ops, b, runs, f"many rows {dtype} rep={rep}")
 
 
+# Prompts of a block or less a CU: two streams of keys a block (the plan of each is
+# checked by tests/native/cbq_paged_host.cpp).
+STREAMS = [
+    ([191], 100, 500, 8, 8, 64, 64),
+    ([191], 100, 500, 8, 8, 128, 64),
+    ([191], 100, 500, 8, 8, 256, 64),
+    ([84, 67, 0], 10, 1900, 8, 16, 64, 17),
+    ([84, 67, 0], 10, 1900, 8, 16, 128, 17),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("runs,past,prefix,n_kv,rep,hd,page", STREAMS)
+def test_prompt_streams(cuda, ops, dtype, runs, past, prefix, n_kv, rep, hd, page):
+    """With a page of the prefix and one of the first run's own that are not there."""
+    b = Batch([past + n for n in runs], prefix, n_kv, rep, hd, page, dtype, seed=hd)
+    b.prefix_table[3] = -1
+    b.tables[0, 1] = 1 << 30
+    q, q_start = b.queries(sum(runs), 2.0), starts(runs)
+    want, tol = so.attend_prompt(b, q, q_start, hd ** -0.5)
+    first = prompt(ops, b, q, q_start, hd ** -0.5)
+    so.near(first, want, tol, f"streams {dtype} hd={hd} {runs}")
+    assert torch.equal(first, prompt(ops, b, q, q_start, hd ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("at", [101, 200, 290])
+def test_prompt_streams_values_not_finite(cuda, ops, dtype, at):
+    """An infinite value of an own key reaches the tokens from it on, none before."""
+    runs, past, prefix, n_kv, rep, hd, page = STREAMS[1]
+    b = Batch([past + n for n in runs], prefix, n_kv, rep, hd, page, dtype, seed=at)
+    q, q_start = b.queries(sum(runs)), starts(runs)
+    want, tol = so.attend_prompt(b, q, q_start, hd ** -0.5)
+    b.v[int(b.tables[0, at // page]), 2, at % page, 7] = float("inf")
+    got = prompt(ops, b, q, q_start, hd ** -0.5).cpu()
+    hit = torch.zeros(got.shape, dtype=torch.bool)
+    hit[at - past:, 2 * rep:3 * rep, 7] = True
+    assert (got[hit] == float("inf")).all() and got[~hit].isfinite().all()
+    so.near(got[~hit], want[~hit], tol[~hit], f"beside an infinite value {dtype}")
+
+
 @pytest.mark.parametrize("prefix", [0, 20])
 def test_prompt_rows_without_keys(cuda, ops, prefix):
     """Fewer own keys than tokens: the first tokens see the prefix alone, or nothing."""
