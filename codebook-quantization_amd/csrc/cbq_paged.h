@@ -87,6 +87,22 @@ CBQ_PAGED_FN int64_t cbq_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 CBQ_PAGED_FN int64_t cbq_min(int64_t a, int64_t b) { return a < b ? a : b; }
 CBQ_PAGED_FN int64_t cbq_max(int64_t a, int64_t b) { return a > b ? a : b; }
 
+// A launch holds fewer than 2^32 threads in a dimension (more are dropped without an
+// error): of more than 2^22 blocks, of up to 512 threads, block b is (b % 2^22, b / 2^22).
+// A grid of two dimensions is filled up with blocks past the last, which do nothing.
+constexpr int kCbqGridBits = 22;
+struct CbqGrid {
+    uint32_t x, y;
+};
+
+static inline CbqGrid cbq_grid(int64_t blocks)
+{
+    const int64_t x = cbq_min(blocks, 1ll << kCbqGridBits);
+    return CbqGrid{(uint32_t)x, (uint32_t)cbq_ceil(blocks, x)};
+}
+
+CBQ_PAGED_FN uint32_t cbq_block(uint32_t x, uint32_t y) { return y << kCbqGridBits | x; }
+
 namespace cbq_attn {
 
 // ---- launch plans ---------------------------------------------------------------------------
@@ -103,7 +119,7 @@ struct Plan {
 
 constexpr int64_t kCus = 256;                // of an MI355X
 constexpr int kAttnWaves = 4;                // of a block
-
+constexpr int64_t kMaxBlocks = (1ll << 31) - 1, kMaxParts = 1 << 20;    // of a plan
 
 // Keys of a block's tile (K and V, two buffers: 64 KiB at most) and of a
 // wave's own (K and V, one buffer: 16 KiB, 32 KiB for rows of 1024 bytes).
@@ -152,7 +168,10 @@ inline Plan plan_decode(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
     // most (33 sequences of 24 heads, up to 2900 keys: 17.6 us; with half and twice the
     // blocks 20).
     const int64_t share = cbq_ceil(capacity * batch * n_kv * own_tiles, 2 * kCus);
-    const int64_t own_chunk = cbq_min(cbq_max(cbq_ceil(share, wk), 1), 8) * wk;
+    int64_t own_chunk = cbq_min(cbq_max(cbq_ceil(share, wk), 1), 8) * wk;
+    // more of a wider table than its parts and blocks are counted for
+    const int64_t most = cbq_min(kMaxParts / 2, (kMaxBlocks - n_kv * tiles * pre_parts) / (n_kv * batch * own_tiles));
+    if (most > 0) own_chunk = cbq_max(own_chunk, cbq_ceil(cbq_ceil(capacity, most), wk) * wk);
     const int64_t own_parts = cbq_max(cbq_ceil(capacity, own_chunk), pre_parts ? 0 : 1);
     p.blocks = n_kv * (tiles * pre_parts + batch * own_tiles * own_parts);
     p.bytes = part_bytes(pre_parts + own_parts, batch, n_kv * rep, hd);
@@ -269,7 +288,7 @@ inline Plan plan_prompt(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
 
 inline bool plan_fits(const Plan &p)
 {
-    return p.blocks > 0 && p.blocks < (1ll << 31) && p.parts < (1ll << 20);
+    return p.blocks > 0 && p.blocks <= kMaxBlocks && p.parts <= kMaxParts;
 }
 
 // ---- what a block does ------------------------------------------------------------------------

@@ -59,7 +59,7 @@ template <typename T, int V> __device__ __forceinline__ void store_vec(T *p, con
 template <typename TX, typename TC, int V, int U, int L, int R>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 {
-    const uint32_t unit = blockIdx.x * (256u / L) + threadIdx.x / L;
+    const uint32_t unit = cbq_block(blockIdx.x, blockIdx.y) * (256u / L) + threadIdx.x / L;
     const int lane = threadIdx.x % L;
     if (unit >= a.rows / R) return;                     // whole rows: no lane waits on a left one
     const int64_t t = cbq_div(unit, a.heads);           // heads: groups of R of a token
@@ -167,7 +167,8 @@ void launch_rows(AppendArgs &a, hipStream_t stream)
                       (int64_t)a.rows * L / 4 >= kFourThreads;
     const int R = four ? 4 : 1;
     a.heads = cbq_div_make((uint32_t)(a.n_q + 2 * a.n_kv) / R);
-    const dim3 blocks((unsigned)cbq_ceil(a.rows / R, 256 / L)), threads(256);
+    const CbqGrid grid = cbq_grid(cbq_ceil(a.rows / R, 256 / L));
+    const dim3 blocks(grid.x, grid.y), threads(256);
     if (four) paged_append_kernel<TX, TC, V, U, L, V == 1 ? 1 : 4><<<blocks, threads, 0, stream>>>(a);
     else paged_append_kernel<TX, TC, V, U, L, 1><<<blocks, threads, 0, stream>>>(a);
 }

@@ -1214,7 +1214,9 @@ template <typename T, int HD, int PT>
 __global__ __launch_bounds__(kThreads, simd_waves(HD * (int)sizeof(T))) void decode_kernel(AttnArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const DecodeWork w = decode_work(a.plan, blockIdx.x, a.kv.n_kv, a.batch, a.prefix, a.capacity);
+    const uint32_t block = cbq_block(blockIdx.x, blockIdx.y);
+    if (block >= (uint32_t)a.plan.blocks) return;
+    const DecodeWork w = decode_work(a.plan, block, a.kv.n_kv, a.batch, a.prefix, a.capacity);
     const int to = a.plan.parts > 1 ? w.part : -1;
     if (w.seq < 0) {
         const CbqKeys keys = {a.prefix_table, nullptr, a.prefix, w.end};
@@ -1239,13 +1241,15 @@ __global__ __launch_bounds__(STREAMS * kThreads, simd_waves(HD * (int)sizeof(T))
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int M = RT ? 64 * RT : 16;
     const int lane = threadIdx.x & 63, n_kv = a.kv.n_kv;
-    uint32_t i = blockIdx.x;
+    const uint32_t block = cbq_block(blockIdx.x, blockIdx.y);
+    if (block >= (uint32_t)a.plan.blocks) return;
+    uint32_t i = block;
     const int h = i % n_kv;
     i /= n_kv;
     const int part = i % a.plan.parts;
     // later tiles of a run see more keys: they start first
     int32_t want = a.plan.tiles - 1 - (int32_t)(i / a.plan.parts);
-    if (blockIdx.x == 0) {                          // tokens of no run
+    if (block == 0) {                               // tokens of no run
         const int64_t lo = cbq_clamp_length(a.q_start[0], a.N),
                       hi = cbq_max(cbq_clamp_length(a.q_start[a.batch], a.N), lo);
         T *out = (T *)a.out;
@@ -1315,8 +1319,8 @@ template <typename T, int HD, int W> __global__ __launch_bounds__(kThreads) void
     __shared__ float totals[kThreads / kLanes];
     const int tid = threadIdx.x, lane = tid & 63, all = tid / kLanes, d = tid % kLanes * 4;
     const int group = all % kGroups;
-    const int64_t rows = (int64_t)a.N * a.n_q, row = (int64_t)blockIdx.x * (kWaves / W) + all / kGroups,
-                  token = row / a.n_q;
+    const int64_t rows = (int64_t)a.N * a.n_q, block = cbq_block(blockIdx.x, blockIdx.y),
+                  row = block * (kWaves / W) + all / kGroups, token = row / a.n_q;
     if (row >= rows) return;                        // whole waves; the barrier counts the rest
     // The first parts' loads wait for no length: what a part that was not written
     // holds is dropped.
@@ -1403,7 +1407,8 @@ template <auto K, int STREAMS = 1> int run_kernel(int64_t blocks, int lds, const
             asked.fetch_or(bit, std::memory_order_relaxed);
         }
     }
-    K<<<dim3((unsigned)blocks), dim3(STREAMS * kThreads), lds, stream>>>(a);
+    const CbqGrid grid = cbq_grid(blocks);
+    K<<<dim3(grid.x, grid.y), dim3(STREAMS * kThreads), lds, stream>>>(a);
     return cbq_launch_status(what);
 }
 

@@ -65,7 +65,7 @@ typedef struct cbq_paged_kv {
  * q, k, v: element [t, h, d] at t * stride[0] + h * stride[1] + d.
  * A token whose position is outside [0, n_pos) stores nothing, and its query
  * is turned by row 0; two tokens with one slot leave either's row there.
- * hd even, 2..256; rot even, 2..hd. */
+ * hd even, 2..256; rot even, 2..hd; N * (n_q + 2 n_kv) < 2^31. */
 int cbq_paged_append(const void *q, const void *k, const void *v, int x_dtype,
                      const int64_t *q_stride, const int64_t *k_stride, const int64_t *v_stride,
                      const float *cos_table, const float *sin_table, int64_t n_pos, int rot,
@@ -82,7 +82,8 @@ int cbq_paged_append(const void *q, const void *k, const void *v, int x_dtype,
  * byte aligned as the pages are; out contiguous, of q's type, which is the
  * cache's.  Scores, maxima, sums and the weighted values are fp32; for 16-bit
  * types the weights exp(s - max) are rounded to that type for the matrix
- * cores.  hd in {64, 128, 256}; n_q % n_kv == 0; prefix + width * page < 2^31.
+ * cores.  hd in {64, 128, 256}; n_q % n_kv == 0; n_q < 2^20;
+ * batch < 2^30 and batch * n_q < 2^31; prefix + width * page <= 2^31 - 65536.
  * workspace: cbq_prefix_attn_decode_workspace bytes (which may be 0), 16-byte
  * aligned, overwritten by every call. */
 size_t cbq_prefix_attn_decode_workspace(const cbq_paged_kv *cache, int64_t prefix, int width,
@@ -98,7 +99,8 @@ int cbq_prefix_attn_decode(const void *q, const int64_t *q_stride, const cbq_pag
  * to N; tokens before the first run and after the last get zeros).  Its own
  * keys, lengths[b] of them, end with the run's: the token that is i-th from
  * the run's end sees the prefix and the own keys up to the i-th from the end.
- * Otherwise as cbq_prefix_attn_decode. */
+ * Otherwise as cbq_prefix_attn_decode; N * n_q < 2^31 and N / 16 * n_q +
+ * min(batch, N) * n_kv < 2^31. */
 size_t cbq_prefix_attn_prompt_workspace(const cbq_paged_kv *cache, int64_t prefix, int width,
                                         int batch, int64_t N, int n_q);
 int cbq_prefix_attn_prompt(const void *q, const int64_t *q_stride, const int32_t *q_start,

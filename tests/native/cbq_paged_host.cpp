@@ -231,10 +231,47 @@ static void streams()
     CHECK(few.streams == 1);
 }
 
+// Grids of any number of blocks: threads of a dimension below 2^32, every block there
+static void grids()
+{
+    for (int64_t n : {1ll, 2ll, 4194303ll, 4194304ll, 4194305ll, 16777216ll, 33554432ll, 33554433ll, 2147483647ll}) {
+        const CbqGrid g = cbq_grid(n);
+        CHECK(g.x > 0 && (int64_t)g.x * 512 < 1ll << 32 && g.y > 0 && g.y < 65536);
+        CHECK((int64_t)g.x * g.y >= n && (int64_t)g.x * (g.y - 1) < n);
+        CHECK(g.y == 1 || g.x == 1u << kCbqGridBits);           // so that indexes follow on
+        CHECK(cbq_block(0, 0) == 0 && cbq_block(g.x - 1, g.y - 1) == (int64_t)g.x * g.y - 1);
+        if (g.y > 1) CHECK(cbq_block(g.x - 1, 0) + 1 == cbq_block(0, 1));
+    }
+}
+
+// Tables of any width: own parts and blocks within their bounds cover the capacity
+static void wide()
+{
+    const int64_t most = (1ll << 31) - 65536;
+    for (int hd : {64, 128, 256})
+        for (int size : {2, 4})
+            for (int n_kv : {1, 8, 32})
+                for (int rep : {1, 17})
+                    for (int64_t batch : {1, 512, 4096})
+                        for (int64_t capacity : {(int64_t)1 << 20, (int64_t)1 << 30, most - 100})
+                            for (int64_t prefix : {0, 100}) {
+                                const Plan p = plan_decode(hd * size, hd, n_kv, rep, prefix, capacity, batch);
+                                CHECK(plan_fits(p) && !p.joint);
+                                CHECK((int64_t)p.own_parts * p.own_chunk >= capacity);
+                                CHECK((int64_t)(p.own_parts - 1) * p.own_chunk < capacity);
+                                const DecodeWork w = decode_work(p, (uint32_t)(p.blocks - 1), n_kv, (int)batch,
+                                                                 (int32_t)prefix, capacity);
+                                CHECK(w.seq == batch - 1 && w.part == p.parts - 1 && w.end == capacity);
+                                CHECK(p.bytes == (int64_t)p.parts * batch * n_kv * rep * (hd + 2) * 4);
+                            }
+}
+
 int main()
 {
     divisions();
     far();
+    grids();
+    wide();
     for (int i = 0; i < 150; i++) decode();
     for (int i = 0; i < 400; i++) prompt();
     streams();

@@ -1,0 +1,80 @@
+"""Batched serving at the ends of its ranges: launches of more threads than one
+grid dimension holds.  Tolerances: serve_oracle.py."""
+import pytest
+import torch
+
+import serve_oracle as so
+from serve_oracle import Batch
+from test_gpu_serve import ops, starts  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- launches of 2^24 blocks and more ---------------------------------------------
+
+def test_append_many_rows(cuda, ops):
+    """2^26 + 40 head rows, a wave each."""
+    N, n_q, n_kv, page = 2 ** 23 + 5, 6, 1, 4096
+    g = torch.Generator(device=cuda).manual_seed(1)
+    y = torch.randn(N, n_q + 2, 2, generator=g, device=cuda, dtype=torch.float16)
+    pages = torch.zeros(-(-N // page), 2, n_kv, page, 2, device=cuda, dtype=torch.float16)
+    angles = torch.rand(50, 1, generator=g, device=cuda, dtype=torch.float64) * 100
+    cos, sin = (torch.cat([t, t], 1).float() for t in (angles.cos(), angles.sin()))
+    positions = torch.randint(0, 50, (N,), generator=g, device=cuda)
+    slots = torch.randperm(N, generator=g, device=cuda)
+    print("append of 2^26 + 40 rows", flush=True)
+    out = ops.paged_append(y[:, :n_q], y[:, n_q:n_q + 1], y[:, n_q + 1:], cos, sin, positions, slots,
+                           pages[:, 0], pages[:, 1], False, None, None, 0.0)
+    rows = pages.permute(0, 3, 1, 2, 4).reshape(-1, 2, 2)[slots]        # [N, key and value, 2]
+    assert torch.equal(rows[:, 1], y[:, n_q + 1])
+    for lo in range(0, N, 1 << 20):
+        at = slice(lo, lo + (1 << 20))
+        want, mag = so.append_rows(y[at, :n_q + 1], None, cos, sin, positions[at], False, 0.0)
+        tol = 2.0 ** -11 * want.abs() + 32 * so.HALF * mag + 2.0 ** -25
+        got = torch.cat([out[at], rows[at, :1]], 1).double()
+        assert ((got - want).abs() <= tol).all(), lo
+
+
+def test_decode_many_blocks(cuda, ops):
+    """17 sequences of 2^20 - 1 heads, two parts of the own keys: 2^25 blocks and
+    more, and as many rows to merge as 2^24."""
+    heads, page, width = 2 ** 20 - 1, 2, 1100
+    g = torch.Generator(device=cuda).manual_seed(2)
+    pool = torch.randn(5, 2, heads, page, 64, generator=g, device=cuda, dtype=torch.bfloat16)
+    lens = [2100, 0, 1, 3] + [2] * 13
+    tables = torch.randint(0, 5, (17, width), dtype=torch.int32, generator=torch.Generator().manual_seed(3))
+    q = torch.randn(17, heads, 64, generator=g, device=cuda, dtype=torch.bfloat16)
+    print("decode of 2^25 blocks", flush=True)
+    out = ops.prefix_attention_decode(q, pool[:, 0], pool[:, 1], tables.new_zeros(0).cuda(), 0,
+                                      tables.cuda(), torch.tensor(lens, dtype=torch.int32, device=cuda),
+                                      0.125)
+    # some heads as a batch of their own: the first, the last, around 2^22 and 2^24 rows
+    some = [0, 1, 2 ** 18 - 1, 2 ** 18, heads // 2, 987654, heads - 2, heads - 1]
+    b = Batch([], 0, len(some), 1, 64, page, "bf16", room=0)
+    b.k, b.v = pool[:, 0, some].cpu(), pool[:, 1, some].cpu()
+    b.lens, b.tables, b.lengths = lens, tables, torch.tensor(lens)
+    so.near(out[:, some], *so.attend(b, q[:, some].cpu(), starts([1] * 17), 0.125), "some heads")
+    # one key a sequence: its value, whatever the query
+    one = pool[int(tables[2, 0]), 1, :, 0]
+    assert torch.equal(out[2], one) and not out[1].any()
+
+
+def test_prompt_many_blocks(cuda, ops):
+    """Five one-token runs of 2^20 - 1 heads: more than 2^22 blocks."""
+    heads = 2 ** 20 - 1
+    g = torch.Generator(device=cuda).manual_seed(4)
+    pool = torch.randn(3, 2, heads, 1, 64, generator=g, device=cuda, dtype=torch.bfloat16)
+    q = torch.randn(5, heads, 64, generator=g, device=cuda, dtype=torch.bfloat16)
+    tables = torch.tensor([[0, -1], [1, -1], [2, 0], [0, 1], [-1, -1]], dtype=torch.int32)
+    lens = [1, 1, 2, 2, 0]
+    print("prompt of 5 * 2^20 blocks", flush=True)
+    out = ops.prefix_attention_prompt(q, starts([1] * 5).cuda(), pool[:, 0], pool[:, 1],
+                                      tables.new_zeros(0).cuda(), 0, tables.cuda(),
+                                      torch.tensor(lens, dtype=torch.int32, device=cuda), 0.125)
+    assert torch.equal(out[0], pool[0, 1, :, 0]) and torch.equal(out[1], pool[1, 1, :, 0])
+    assert not out[4].any()
+    some = [0, 1, 2 ** 18, heads // 2, 987654, heads - 1]
+    b = Batch([], 0, len(some), 1, 64, 1, "bf16", room=0)
+    b.k, b.v = pool[:, 0, some].cpu(), pool[:, 1, some].cpu()
+    b.lens, b.tables, b.lengths = lens, tables, torch.tensor(lens)
+    so.near(out[:, some], *so.attend(b, q[:, some].cpu(), starts([1] * 5), 0.125), "some heads")
