@@ -54,7 +54,17 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int kWaves = kAttnWaves, kThreads = kWaves * CBQ_WAVE;
+
+// The running maximum follows the scores once they pass it by kSlack (in exp2's
+// domain).  So that no weight passes 1 all the same, and sums of values near the end
+// of their range stay inside it, a bf16 row's m stands kSlack above the largest score
+// of its last move (the shift costs a weight 2^-21, far below bf16's step), and fp32
+// weights are multiplied by 2^-kSlack, exactly.  fp16 weights keep the bits: 2^kSlack
+// times its largest value, 65504, leaves 2^104 of fp32's range.
 constexpr float kSlack = 8.0f;
+template <typename T> constexpr float kAbove = std::is_same_v<T, __bf16> ? kSlack : 0.0f;
+template <typename T> constexpr float kOver = kSlack - kAbove<T>;
+template <typename T> constexpr float kDown = sizeof(T) == 4 ? 1.0f / 256 : 1.0f;
 
 struct AttnArgs {
     const void *q;
@@ -521,8 +531,7 @@ template <typename T, int HD, int RT> struct Rows {
         }
     }
 
-    // The running maximum follows the scores once they pass it by kSlack (in exp2's
-    // domain): until then weights are at most 2^kSlack and nothing is rescaled.
+    // Until the scores pass the running maximum by kSlack nothing is rescaled.
     template <int NK> __device__ __forceinline__ void raise(const f32x4 (&s)[RT][NK], float c)
     {
         float x[RT];
@@ -535,12 +544,12 @@ template <typename T, int HD, int RT> struct Rows {
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[t] = fmaxf(x[t], s[t][k][i]);
             x[t] = groups_max(x[t]) * c;
-            over = over || x[t] > m[t] + kSlack;
+            over = over || x[t] > m[t] + kOver<T>;
         }
         if (!__any(over)) return;
 #pragma unroll
         for (int t = 0; t < RT; t++) {
-            const float now = fmaxf(m[t], x[t]);
+            const float now = fmaxf(m[t], x[t] + kAbove<T>);
             base[t] = now == -INFINITY ? 0.f : now;         // a row that has seen no key
             const float f = __builtin_amdgcn_exp2f(m[t] - base[t]);
             l[t] *= f;
@@ -606,7 +615,7 @@ template <typename T, int HD, int RT> struct Rows {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, sizeof(T) == 4 ? fmaf(s[i], c_low, -base[t])
-                                                                       : -base[t]));
+                                                                       : -base[t])) * kDown<T>;
         l[t] += (p[0] + p[1]) + (p[2] + p[3]);
         return p;
     }
@@ -798,8 +807,8 @@ template <typename T, int HD> struct Rows32 {
             for (int i = 0; i < 16; i++) x = fmaxf(x, s[k][i]);
         auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
         x = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])) * c;
-        if (!__any(x > m + kSlack)) return;
-        x = fmaxf(m, x);
+        if (!__any(x > m + kOver<T>)) return;
+        x = fmaxf(m, x + kAbove<T>);
         base = x == -INFINITY ? 0.f : x;
         const float f = __builtin_amdgcn_exp2f(m - base);
         l *= f;
@@ -955,9 +964,9 @@ __device__ __forceinline__ void plain_rows(const AttnArgs &a, int h, int64_t tok
             s = in ? s * a.c : -INFINITY;
             float now = s;
             for (int i = 32; i > 0; i >>= 1) now = fmaxf(now, __shfl_xor(now, i));
-            now = fmaxf(top, now);
+            now = fmaxf(top, now + kAbove<T>);
             const float base = now == -INFINITY ? 0.f : now, f = __builtin_amdgcn_exp2f(top - base);
-            const float w = in ? __builtin_amdgcn_exp2f(s - base) : 0.f;
+            const float w = in ? __builtin_amdgcn_exp2f(s - base) * kDown<T> : 0.f;
             top = now;
             l = l * f + w;
             for (int i = 0; i < kLane; i++) o[i] *= f;

@@ -1,11 +1,12 @@
 """Batched serving at the ends of its ranges: launches of more threads than one
-grid dimension holds.  Tolerances: serve_oracle.py."""
+grid dimension holds, values at the ends of their types.  Tolerances:
+serve_oracle.py."""
 import pytest
 import torch
 
 import serve_oracle as so
 from serve_oracle import Batch
-from test_gpu_serve import ops, starts  # noqa: F401
+from test_gpu_serve import check_decode, ops, prompt, starts  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +79,53 @@ def test_prompt_many_blocks(cuda, ops):
     b.k, b.v = pool[:, 0, some].cpu(), pool[:, 1, some].cpu()
     b.lens, b.tables, b.lengths = lens, tables, torch.tensor(lens)
     so.near(out[:, some], *so.attend(b, q[:, some].cpu(), starts([1] * 5), 0.125), "some heads")
+
+
+# ---- large values -------------------------------------------------------------------
+
+def _late_key(dtype, prefix, lens, at, value, n_kv=1, rep=2, hd=64):
+    """Scores 0 but for own key `at` of every sequence, which is 5.5 more (244 times
+    the others' weight), and values of one large magnitude."""
+    b = Batch(lens, prefix, n_kv, rep, hd, 16, dtype, seed=30)
+    b.k.zero_()
+    sign = torch.where(torch.rand(hd, generator=b.g) < 0.5, -1.0, 1.0)
+    b.v.copy_(value * sign * (1 - 0.5 * torch.rand(b.v.shape, generator=b.g)))
+    for row in b.tables:
+        b.k[int(row[at // 16]), :, at % 16, 0] = 5.5
+    q = torch.zeros(len(lens), b.n_q, hd, dtype=b.dtype)
+    q[:, :, 0] = 1.0
+    return b, q
+
+
+# fp16's largest values; of the other types, values whose sums stay below 2^128
+# while 2^8 times a value does not.
+LARGE = {"f32": 2.0 ** 122, "bf16": 2.0 ** 122, "f16": 60000.0}
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("prefix,n,hd", [(0, 400, 64), (0, 300, 128), (1200, 400, 64), (0, 3000, 128),
+                                         (600, 200, 256)])
+def test_large_values_decode(cuda, ops, dtype, prefix, n, hd):
+    """A later key's score above those before it by less than the slack that the
+    running maximum has."""
+    b, q = _late_key(dtype, prefix, [n, n], n - 7, LARGE[dtype], hd=hd)
+    out = check_decode(ops, b, f"large values {dtype} prefix={prefix} n={n} hd={hd}", 1.0, q)
+    assert out.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("prefix", [300, 1100])
+@pytest.mark.parametrize("n_kv,rep", [(1, 1), (8, 4), (8, 16)])
+def test_large_values_prompt(cuda, ops, dtype, prefix, n_kv, rep):
+    """The same in a prompt: blocks of 16, 64 and 128 rows, and row by row beside an
+    infinite value that the last token alone sees."""
+    n = 130
+    b, q1 = _late_key(dtype, prefix, [n], 0, LARGE[dtype], n_kv, rep)
+    q, q_start = q1.expand(n, -1, -1).contiguous(), starts([n])
+    want, tol = so.attend_prompt(b, q, q_start, 1.0)
+    print(f"large values {dtype} prefix={prefix} heads={n_kv}x{rep}", flush=True)
+    so.near(prompt(ops, b, q, q_start, 1.0), want, tol, "large values")
+    b.v[int(b.tables[0, (n - 1) // 16]), :, (n - 1) % 16, 3] = float("inf")
+    got = prompt(ops, b, q, q_start, 1.0)
+    assert (got[-1, :, 3] == float("inf")).all()
+    so.near(got[:-1], want[:-1], tol[:-1], "before an infinite value")
