@@ -90,17 +90,18 @@ int attend(const void *q, const int64_t *q_stride, const int32_t *q_start,
     a.page = cbq_div_make((uint32_t)cache->page);
     a.prefix = (int32_t)prefix; a.batch = (int32_t)batch; a.N = (int32_t)N;
     a.n_q = (int32_t)n_q; a.rep = (int32_t)(n_q / cache->n_kv);
-    // The running maximum needs a factor above 0: the queries take scale's
-    // sign, exactly, and a scale of 0 (or one that exp2 cannot tell from it)
-    // makes every score 0.
+    // The running maximum needs a factor above 0: the queries take scale's sign,
+    // exactly, and a scale of 0 makes every score 0, as does one below fp32's smallest
+    // step, 2^-149, whose scores of finite products are below 2^-20.
+    // c below the exact factor and c_low above 0 (denormal numbers count: kernels are
+    // built with them), so that a hidden key's -inf stays -inf times either.
     const float mag = scale < 0.f ? -scale : scale;
-    const bool zero = mag < 1.0e-30f;
-    // c below the exact factor and c_low above 0, so that a hidden key's -inf stays
-    // -inf times either.
     const double exact = (double)mag * 1.4426950408889634074;
-    a.c = zero ? 1.0f : (float)exact;
-    if (!zero && (double)a.c >= exact) a.c = std::nextafter(a.c, 0.0f);
-    a.c_low = zero ? 1.0e-9f : (float)(exact - (double)a.c);
+    a.c = (float)exact;
+    if ((double)a.c >= exact) a.c = std::nextafter(a.c, 0.0f);
+    a.c_low = std::fmax((float)(exact - (double)a.c), 0x1p-149f);
+    const bool zero = !(a.c > 0.f);
+    if (zero) a.c = 1.0f, a.c_low = 1.0e-9f;
     a.q_mul = zero ? 0.0f : scale < 0.f ? -1.0f : 1.0f;
     a.plan = p;
     if (cache->dtype == CBQ_F32) return launch_f32(a, p, prompt, stream);

@@ -1,5 +1,5 @@
 """Batched serving at the ends of its ranges: launches of more threads than one
-grid dimension holds, values at the ends of their types.  Tolerances:
+grid dimension holds, values and scales at the ends of their types.  Tolerances:
 serve_oracle.py."""
 import pytest
 import torch
@@ -129,3 +129,17 @@ def test_large_values_prompt(cuda, ops, dtype, prefix, n_kv, rep):
     got = prompt(ops, b, q, q_start, 1.0)
     assert (got[-1, :, 3] == float("inf")).all()
     so.near(got[:-1], want[:-1], tol[:-1], "before an infinite value")
+
+
+# ---- small scales -------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [1e-31, -1e-31, 2.0 ** -126, 2.0 ** -130])
+def test_small_scale_of_large_products(cuda, ops, dtype, scale):
+    """Queries and keys whose products are as large as the scale is small."""
+    large = min(abs(scale) ** -0.5, 2.0 ** 63)                  # products within fp32's range
+    b = Batch([300, 40], 100, 1, 2, 64, 16, dtype, seed=31, scale_k=large / 32)
+    q = b.queries(2, large)
+    check_decode(ops, b, f"scale {scale} {dtype}", scale, q)
+    want, tol = so.attend_prompt(b, q, torch.tensor([0, 1, 2], dtype=torch.int32), scale)
+    so.near(prompt(ops, b, q, starts([1, 1]), scale), want, tol, f"prompt, scale {scale} {dtype}")
