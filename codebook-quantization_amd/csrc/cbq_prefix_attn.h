@@ -1223,9 +1223,9 @@ template <typename T, int HD, int PT>
 __global__ __launch_bounds__(kThreads, simd_waves(HD * (int)sizeof(T))) void decode_kernel(AttnArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const uint32_t block = cbq_block(blockIdx.x, blockIdx.y);
-    if (block >= (uint32_t)a.plan.blocks) return;
-    const DecodeWork w = decode_work(a.plan, block, a.kv.n_kv, a.batch, a.prefix, a.capacity);
+    const DecodeWork w = decode_work(a.plan, cbq_block(blockIdx.x, blockIdx.y), a.kv.n_kv, a.batch, a.prefix,
+                                     a.capacity);
+    if (w.part >= a.plan.parts) return;             // past the plan's last block
     const int to = a.plan.parts > 1 ? w.part : -1;
     if (w.seq < 0) {
         const CbqKeys keys = {a.prefix_table, nullptr, a.prefix, w.end};
@@ -1251,7 +1251,6 @@ __global__ __launch_bounds__(STREAMS * kThreads, simd_waves(HD * (int)sizeof(T))
     constexpr int M = RT ? 64 * RT : 16;
     const int lane = threadIdx.x & 63, n_kv = a.kv.n_kv;
     const uint32_t block = cbq_block(blockIdx.x, blockIdx.y);
-    if (block >= (uint32_t)a.plan.blocks) return;
     uint32_t i = block;
     const int h = i % n_kv;
     i /= n_kv;
@@ -1266,9 +1265,10 @@ __global__ __launch_bounds__(STREAMS * kThreads, simd_waves(HD * (int)sizeof(T))
         for (int64_t e = threadIdx.x; e < (lo + a.N - hi) * w; e += STREAMS * kThreads)
             out[e < lo * w ? e : e + (hi - lo) * w] = (T)0.f;
     }
-    // the run that holds tile `want`: its count of tiles, summed over the runs
+    // the run that holds tile `want`: its count of tiles, summed over the runs (none
+    // past the plan's last block)
     int32_t before = 0, run = -1, tile = 0, first_token = 0, count = 0, length = 0;
-    for (int b0 = 0; b0 < a.batch && run < 0; b0 += CBQ_WAVE) {
+    for (int b0 = want < 0 ? a.batch : 0; b0 < a.batch && run < 0; b0 += CBQ_WAVE) {
         int32_t f = 0, n = 0, len = 0;
         if (b0 + lane < a.batch) {
             cbq_run(a.q_start, b0 + lane, a.N, f, n);

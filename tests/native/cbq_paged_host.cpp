@@ -262,6 +262,10 @@ static void wide()
                                 const DecodeWork w = decode_work(p, (uint32_t)(p.blocks - 1), n_kv, (int)batch,
                                                                  (int32_t)prefix, capacity);
                                 CHECK(w.seq == batch - 1 && w.part == p.parts - 1 && w.end == capacity);
+                                const CbqGrid g = cbq_grid(p.blocks);       // those that fill the grid up
+                                for (int64_t i : {p.blocks, (int64_t)g.x * g.y - 1})
+                                    CHECK(i < p.blocks || decode_work(p, (uint32_t)i, n_kv, (int)batch, (int32_t)prefix,
+                                                                      capacity).part >= p.parts);
                                 CHECK(p.bytes == (int64_t)p.parts * batch * n_kv * rep * (hd + 2) * 4);
                             }
 }
