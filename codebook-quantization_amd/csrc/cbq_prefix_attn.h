@@ -465,6 +465,12 @@ template <typename T> __device__ __forceinline__ u32x4 query_slot(const AttnArgs
     return w;
 }
 
+// A score's weight
+template <typename T> __device__ __forceinline__ float weight(float s, float c, float c_low, float base)
+{
+    return __builtin_amdgcn_exp2f(fmaf(s, c, sizeof(T) == 4 ? fmaf(s, c_low, -base) : -base)) * kDown<T>;
+}
+
 // ---- RT x 16 query rows of one wave --------------------------------------------------
 template <typename T, int HD, int RT> struct Rows {
     using G = Geo<T, HD>;
@@ -614,8 +620,7 @@ template <typename T, int HD, int RT> struct Rows {
         f32x4 p;
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, sizeof(T) == 4 ? fmaf(s[i], c_low, -base[t])
-                                                                       : -base[t])) * kDown<T>;
+            p[i] = weight<T>(s[i], c, c_low, base[t]);
         l[t] += (p[0] + p[1]) + (p[2] + p[3]);
         return p;
     }
@@ -895,7 +900,7 @@ template <typename T, int HD> struct Rows32 {
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                x[i] = __builtin_amdgcn_exp2f(fmaf(s[j / 2][j % 2 * 8 + i], c, -base));
+                x[i] = weight<T>(s[j / 2][j % 2 * 8 + i], c, 0.f, base);
             l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
             p[j & 1] = u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]),
                              pack2<T>(x[6], x[7])};
@@ -961,12 +966,11 @@ __device__ __forceinline__ void plain_rows(const AttnArgs &a, int h, int64_t tok
                                                 qw = {query_slot(a, x + c * G::kEl, true)};
                 for (int i = 0; i < G::kEl; i++) s = fmaf((float)kw.e[i], (float)qw.e[i], s);
             }
-            s = in ? s * a.c : -INFINITY;
-            float now = s;
+            float now = in ? s : -INFINITY;
             for (int i = 32; i > 0; i >>= 1) now = fmaxf(now, __shfl_xor(now, i));
-            now = fmaxf(top, now + kAbove<T>);
+            now = fmaxf(top, now * a.c + kAbove<T>);
             const float base = now == -INFINITY ? 0.f : now, f = __builtin_amdgcn_exp2f(top - base);
-            const float w = in ? __builtin_amdgcn_exp2f(s - base) * kDown<T> : 0.f;
+            const float w = in ? weight<T>(s, a.c, a.c_low, base) : 0.f;
             top = now;
             l = l * f + w;
             for (int i = 0; i < kLane; i++) o[i] *= f;

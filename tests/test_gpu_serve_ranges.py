@@ -1,6 +1,8 @@
 """Batched serving at the ends of its ranges: launches of more threads than one
 grid dimension holds, values and scales at the ends of their types.  Tolerances:
 serve_oracle.py."""
+import math
+
 import pytest
 import torch
 
@@ -143,3 +145,36 @@ def test_small_scale_of_large_products(cuda, ops, dtype, scale):
     check_decode(ops, b, f"scale {scale} {dtype}", scale, q)
     want, tol = so.attend_prompt(b, q, torch.tensor([0, 1, 2], dtype=torch.int32), scale)
     so.near(prompt(ops, b, q, starts([1, 1]), scale), want, tol, f"prompt, scale {scale} {dtype}")
+
+
+# ---- rows done key by key beside products ----------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_equal_scores_across_parts(cuda, ops, dtype):
+    """Every score the same, from exact products, in parts of which the last, with an
+    infinite value, is done key by key: the mean of the values.  No score's rounding
+    enters (one score, one weight), so the tolerance is the sums'."""
+    for scale in (1.0, 0.7, 1.1, 0.9, 0.3, 0.77):
+        b = Batch([3040], 0, 1, 4, 64, 16, dtype, seed=32)
+        b.k.zero_()
+        b.k[..., 0] = 60.0
+        q = torch.zeros(40, 4, 64, dtype=b.dtype)
+        q[..., 0] = 60.0
+        q_start = starts([40])
+        b.v.fill_(-1.0)
+        for j in range(2700, 3040):                             # inside the last part
+            b.v[int(b.tables[0, j // 16]), :, j % 16] = 1.0
+        b.v[int(b.tables[0, 3039 // 16]), 0, 3039 % 16, 5] = float("inf")
+        got = prompt(ops, b, q, q_start, scale).double().cpu()
+        v = b.dense(0)[1][:, 0]
+        for t in range(39):
+            n = 3000 + t + 1
+            want, mass = v[:n].mean(0), v[:n].abs().mean(0)
+            half = so.half_step(b.dtype)
+            tol = half * want.abs() + (n / 16 + 64) * so.HALF * mass
+            if dtype != "f32":
+                tol = tol + half * mass
+            if dtype == "f16":
+                tol = tol + 2.0 ** -25 * v[:n].abs().amax(0) + 2.0 ** -25
+            so.near(got[t], want.expand(4, 64), tol.expand(4, 64), f"scale {scale}, token {t}")
+        assert (got[39, :, 5] == math.inf).all()
