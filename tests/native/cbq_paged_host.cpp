@@ -8,6 +8,7 @@
 
 #include <map>
 #include <random>
+#include <string>
 #include <vector>
 
 #include "../../codebook-quantization_amd/csrc/cbq_paged.h"
@@ -270,8 +271,28 @@ static void wide()
                             }
 }
 
-int main()
+// "decode ROW_BYTES HD N_KV REP PREFIX CAPACITY BATCH" or "prompt ... N": the plan
+static int show(int argc, char **argv)
 {
+    const std::string kind = argv[1];
+    int64_t a[8] = {};
+    for (int i = 2; i < argc && i < 10; i++) a[i - 2] = atoll(argv[i]);
+    if (kind == "decode" && argc == 9) {
+        const Plan p = plan_decode(a[0], a[1], a[2], a[3], a[4], a[5], a[6]);
+        printf("joint %d rt %d pre_parts %d own_parts %d\n", p.joint, p.rt, p.pre_parts, p.own_parts);
+        return 0;
+    }
+    if (kind == "prompt" && argc == 10) {
+        const Plan p = plan_prompt(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7]);
+        printf("rt %d streams %d parts %d\n", p.rt, p.streams, p.parts);
+        return 0;
+    }
+    return 2;
+}
+
+int main(int argc, char **argv)
+{
+    if (argc > 1) return show(argc, argv);
     divisions();
     far();
     grids();
