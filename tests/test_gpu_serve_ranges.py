@@ -178,3 +178,31 @@ def test_equal_scores_across_parts(cuda, ops, dtype):
                 tol = tol + 2.0 ** -25 * v[:n].abs().amax(0) + 2.0 ** -25
             so.near(got[t], want.expand(4, 64), tol.expand(4, 64), f"scale {scale}, token {t}")
         assert (got[39, :, 5] == math.inf).all()
+
+
+# ---- inputs that ask for gradients --------------------------------------------------
+
+def test_no_gradients(cuda, ops):
+    """These operators serve: the same outputs, no graph in the pages, and a backward
+    pass through them says that there is none."""
+    b = Batch([30, 77], 20, 2, 2, 64, 16, "f32", seed=33, fill=0.0)
+    k, v, prefix_table, tables, lengths = b.cuda()
+    x = torch.randn(2, 8, 64, device=cuda)
+    at, table = torch.tensor([3, 4], device=cuda), torch.rand(8, 64, device=cuda)
+    slots = torch.tensor([int(b.tables[s, n // 16]) * 16 + n % 16 for s, n in enumerate((29, 76))],
+                         device=cuda)
+
+    def step(y):
+        q = ops.paged_append(y[:, :4], y[:, 4:6], y[:, 6:], table, table, at, slots, k, v, True, None,
+                             None, 1e-6)
+        return q, ops.prefix_attention_decode(q, k, v, prefix_table, 20, tables, lengths, 0.125), \
+            ops.prefix_attention_prompt(q, starts([1, 1]).cuda(), k, v, prefix_table, 20, tables, lengths,
+                                        0.125)
+    want = step(x)
+    y = x.clone().requires_grad_()
+    for a, c in zip(want, step(y)):
+        assert torch.equal(a, c)
+        with pytest.warns(UserWarning, match="autograd kernel was not registered"):
+            c.sum().backward(retain_graph=True)
+    assert y.grad is None or not y.grad.any()
+    assert not k.requires_grad and not v.requires_grad
