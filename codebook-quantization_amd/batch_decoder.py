@@ -186,6 +186,8 @@ class BatchDecoder:
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], n_new: int) -> List[List[int]]:
         """Greedy: n_new tokens of each prompt behind the prefix (EOS ignored)."""
+        if n_new < 1:
+            return [[] for _ in prompts]
         tokens = [torch.argmax(self.start(prompts, n_new), -1)]
         for _ in range(n_new - 1):
             tokens.append(torch.argmax(self.step(tokens[-1]), -1))

@@ -1,0 +1,44 @@
+"""BatchDecoder's bookkeeping on the CPU: tokens, pages and refusals, with layers that
+pass each token's id on and a head that picks the next one."""
+import pytest
+import torch
+
+import decoder
+from batch_decoder import BatchDecoder
+
+CFG = decoder.DecoderConfig(layers=1, hidden=8, inter=8, n_q=2, n_kv=1, head_dim=4, vocab=50)
+
+
+class Model:
+    cfg, device, max_len = CFG, torch.device("cpu"), 40
+    linears = {"lm_head": lambda x: torch.nn.functional.one_hot((x[:, 0].long() + 1) % CFG.vocab,
+                                                                CFG.vocab).float()}
+
+
+class Batch(BatchDecoder):
+    fail = False
+
+    def _layers(self, ids, positions, slots, attend):
+        if self.fail:
+            raise RuntimeError("no layers")
+        assert positions.shape == slots.shape == ids.shape
+        assert int(positions.max()) < self.model.max_len
+        assert 0 <= int(slots.min()) and int(slots.max()) < self.pool.pages.shape[1] * self.pool.page
+        self.written = slots.tolist()
+        return ids[:, None].float()
+
+
+@pytest.fixture
+def batch():
+    return Batch(Model(), n_pages=6, page=4)
+
+
+def free(batch):
+    return len(batch.pool._free)
+
+
+def test_no_new_tokens(batch):
+    """As the one-sequence decoder: none asked for, none given."""
+    assert batch.generate([[1, 2], [3]], 0) == [[], []]
+    assert batch.generate([[1, 2], [3]], 1) == [[3], [4]]
+    assert batch.generate([[1, 2], [3]], 3) == [[3, 4, 5], [4, 5, 6]] and free(batch) == 6
