@@ -188,7 +188,7 @@ class BatchDecoder:
         """Greedy: n_new tokens of each prompt behind the prefix (EOS ignored)."""
         if n_new < 1:
             return [[] for _ in prompts]
-        tokens = [torch.argmax(self.start(prompts, n_new), -1)]
+        tokens = [torch.argmax(self.start(prompts, n_new - 1), -1)]      # the last one is not run
         for _ in range(n_new - 1):
             tokens.append(torch.argmax(self.step(tokens[-1]), -1))
         self.release()

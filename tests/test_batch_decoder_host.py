@@ -42,3 +42,18 @@ def test_no_new_tokens(batch):
     assert batch.generate([[1, 2], [3]], 0) == [[], []]
     assert batch.generate([[1, 2], [3]], 1) == [[3], [4]]
     assert batch.generate([[1, 2], [3]], 3) == [[3, 4, 5], [4, 5, 6]] and free(batch) == 6
+
+
+def test_last_position(batch):
+    """The last new token is not run: a prompt and its tokens may pass max_len and the
+    pages by it, as one by one."""
+    batch.set_prefix(list(range(20)))                           # 5 of 6 pages
+    assert batch.generate([[7, 8]], 3) == [[9, 10, 11]]         # 2 + 2 rows: the last page
+    assert max(batch.written) < 24
+    with pytest.raises(RuntimeError, match="pages"):
+        batch.generate([[7, 8]], 4)
+    batch.set_prefix([])
+    long = Batch(Model(), n_pages=10, page=4)
+    assert long.generate([[1] * 30], 11) == [list(range(2, 13))]
+    with pytest.raises(ValueError, match="max_len"):
+        long.generate([[1] * 30], 12)
