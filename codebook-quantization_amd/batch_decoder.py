@@ -137,8 +137,12 @@ class BatchDecoder:
         if not len(ids):
             return
         pages = self.pool.take(len(ids))
-        table = self._ints(pages)
-        self._prompts([ids], table[None], [pages], 0, self._ints([]))
+        try:
+            table = self._ints(pages)
+            self._prompts([ids], table[None], [pages], 0, self._ints([]))
+        except BaseException:
+            self.pool.give(pages)
+            raise
         self._prefix_pages, self.prefix, self._prefix_table = pages, len(ids), table
 
     @torch.no_grad()
@@ -151,15 +155,15 @@ class BatchDecoder:
         if longest > self.model.max_len:
             raise ValueError(f"sequences of {longest} exceed max_len {self.model.max_len}")
         self.release()
-        for p in prompts:
-            try:
+        try:
+            for p in prompts:
                 self._own.append(self.pool.take(len(p) + room))
-            except RuntimeError:
-                self.release()
-                raise
-        width = max(len(r) for r in self._own)
-        self._tables = self._ints([r + [-1] * (width - len(r)) for r in self._own])
-        x = self._prompts(prompts, self._tables, self._own, self.prefix, self._prefix_table)
+            width = max(len(r) for r in self._own)
+            self._tables = self._ints([r + [-1] * (width - len(r)) for r in self._own])
+            x = self._prompts(prompts, self._tables, self._own, self.prefix, self._prefix_table)
+        except BaseException:
+            self.release()
+            raise
         self._lens = [len(p) for p in prompts]
         return self.model.linears["lm_head"](x)
 
@@ -174,13 +178,14 @@ class BatchDecoder:
         positions = self._ints([self.prefix + n for n in self._lens], torch.int64)
         slots = self._ints([row[n // page] * page + n % page for n, row in zip(self._lens, self._own)],
                            torch.int64)
-        self._lens = [n + 1 for n in self._lens]
-        lengths = self._ints(self._lens)
+        lens = [n + 1 for n in self._lens]
+        lengths = self._ints(lens)
 
         def attend(q, kp, vp):
             return self.ops.prefix_attention_decode(q, kp, vp, self._prefix_table, self.prefix,
                                                     self._tables, lengths, scale)
         x = self._layers(tokens, positions, slots, attend)
+        self._lens = lens
         return self.model.linears["lm_head"](x)
 
     @torch.no_grad()

@@ -57,3 +57,33 @@ def test_last_position(batch):
     assert long.generate([[1] * 30], 11) == [list(range(2, 13))]
     with pytest.raises(ValueError, match="max_len"):
         long.generate([[1] * 30], 12)
+
+
+def test_failures_lose_no_pages(batch):
+    batch.set_prefix([1, 2, 3, 4, 5])
+    batch.fail = True
+    with pytest.raises(RuntimeError, match="no layers"):
+        batch.start([[1, 2, 3]], 4)
+    assert free(batch) == 4                                     # the prefix stays
+    with pytest.raises(RuntimeError, match="no layers"):
+        batch.generate([[1, 2, 3]], 4)
+    assert free(batch) == 4
+    with pytest.raises(RuntimeError, match="no layers"):
+        batch.set_prefix([1, 2, 3])
+    assert free(batch) == 6 and batch.prefix == 0               # as without a prefix
+    batch.fail = False
+    with pytest.raises(RuntimeError, match="pages"):
+        batch.set_prefix(list(range(30)))
+    assert free(batch) == 6 and batch.generate([[1]], 2) == [[2, 3]]
+    batch.set_prefix([1, 2, 3])
+    batch.start([[1, 2, 3]], 4)
+    batch.fail = True
+    with pytest.raises(RuntimeError, match="no layers"):        # a step that failed is none
+        batch.step(torch.tensor([7]))
+    batch.fail = False
+    batch.step(torch.tensor([7]))
+    row = batch._own[0]
+    assert batch.written == [row[0] * 4 + 3]
+    batch.release()
+    batch.set_prefix([])
+    assert sorted(batch.pool._free) == list(range(6))
