@@ -31,6 +31,8 @@ class PagePool:
     values), and which of them are free."""
 
     def __init__(self, cfg, n_pages: int, page: int, dtype: torch.dtype, device):
+        if page < 1:
+            raise ValueError(f"pages of {page} rows")
         self.page = page
         self.pages = torch.zeros(cfg.layers, n_pages, 2, cfg.n_kv, page, cfg.head_dim, dtype=dtype,
                                  device=device)
@@ -151,6 +153,8 @@ class BatchDecoder:
         tokens each: logits [batch, vocab] of their last tokens."""
         if not prompts or not all(len(p) for p in prompts):
             raise ValueError("every prompt needs a token")
+        if room < 0:
+            raise ValueError(f"room for {room} more tokens")
         longest = self.prefix + max(len(p) for p in prompts) + room
         if longest > self.model.max_len:
             raise ValueError(f"sequences of {longest} exceed max_len {self.model.max_len}")
@@ -171,6 +175,10 @@ class BatchDecoder:
     def step(self, tokens: torch.Tensor) -> torch.Tensor:
         """One token of each sequence (device int64 [batch]): logits [batch, vocab]."""
         page, scale = self.pool.page, self.cfg.head_dim ** -0.5
+        if not self._lens:
+            raise ValueError("no sequences: start() first")
+        if tokens.numel() != len(self._lens):
+            raise ValueError(f"{tokens.numel()} tokens for {len(self._lens)} sequences")
         if any(n >= len(row) * page for n, row in zip(self._lens, self._own)):
             raise RuntimeError("no room for another token: start() with more")
         if self.prefix + max(self._lens) >= self.model.max_len:

@@ -87,3 +87,26 @@ def test_failures_lose_no_pages(batch):
     batch.release()
     batch.set_prefix([])
     assert sorted(batch.pool._free) == list(range(6))
+
+
+def test_refusals(batch):
+    for call in (lambda: batch.step(torch.tensor([1])),         # nothing was started
+                 lambda: batch.start([[1, 2]], -1), lambda: batch.start([], 1)):
+        with pytest.raises(ValueError):
+            call()
+    batch.start([[1, 2], [3]], 2)
+    with pytest.raises(ValueError, match="2 sequences"):
+        batch.step(torch.tensor([1]))
+    with pytest.raises(ValueError, match="2 sequences"):
+        batch.step(torch.tensor([1, 2, 3]))
+    assert batch._lens == [2, 1]
+    batch.step(torch.tensor([1, 2]))
+    batch.step(torch.tensor([1, 2]))
+    assert batch._lens == [4, 3]
+    with pytest.raises(RuntimeError, match="room"):
+        batch.step(torch.tensor([1, 2]))
+    batch.release()
+    with pytest.raises(ValueError, match="start"):
+        batch.step(torch.tensor([1, 2]))
+    with pytest.raises(ValueError, match="page"):
+        Batch(Model(), n_pages=4, page=0)
