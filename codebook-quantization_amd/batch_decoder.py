@@ -13,8 +13,9 @@ the few-token GEMM, more on the prompt GEMM).
     batch.set_prefix(system_ids)
     tokens = batch.generate([question_ids, other_ids, ...], n_new=64)
 
-Activations are fp32; the cache is fp32 or one of the 16-bit types, which
-rounds queries, keys and values once.  Tokens stay on the device between
+Activations are fp32; the cache is fp32 or one of the 16-bit types, to which
+queries, keys and values are rounded, and in the attention the softmax weights
+(whose sum is not) and the outputs.  Tokens stay on the device between
 steps; the host only counts positions and hands out pages.
 """
 from __future__ import annotations
