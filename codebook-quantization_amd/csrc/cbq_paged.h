@@ -5,6 +5,8 @@
 
 #include <stdint.h>
 
+#include <algorithm>
+
 #ifdef __HIPCC__
 #define CBQ_PAGED_FN __host__ __device__ __forceinline__
 #else
@@ -134,22 +136,28 @@ inline int64_t part_bytes(int64_t parts, int64_t N, int n_q, int hd)
     return parts > 1 ? parts * N * n_q * (hd + 2) * 4 : 0;
 }
 
+// A prompt's block of 16, 64 or 128 rows (rt 0, 1, 2) takes this many us for 1000
+// keys, alone on its CU and beside another block (rows of 1024 bytes: there is
+// none), measured over 2000 to 4000 keys.
+inline void walk_us(int row_bytes, int hd, int rt, double &alone, double &paired)
+{
+    static const float us[2][3][3][2] = {
+        {{{5.4f, 8.2f}, {15, 17}, {17.5f, 20}},             // 16-bit types: hd 64, 128, 256
+         {{10.4f, 14.8f}, {20, 25}, {24, 32}},
+         {{22.5f, 31}, {38, 46}, {0, 0}}},
+        {{{17, 27}, {46, 68}, {75, 116}},                   // fp32
+         {{33, 50}, {84, 126}, {0, 0}},
+         {{96, 96}, {182, 182}, {0, 0}}}};
+    const float *u = us[row_bytes == 4 * hd][hd == 64 ? 0 : hd == 128 ? 1 : 2][rt];
+    alone = u[0];
+    paired = u[1];
+}
+
 inline Plan plan_decode(int row_bytes, int hd, int n_kv, int rep, int64_t prefix, int64_t capacity,
                         int64_t batch)
 {
     Plan p = {};
     const int64_t rows = batch * rep, bk = block_keys(row_bytes), wk = kAttnWaves * wave_keys(row_bytes);
-    if (prefix + capacity <= 4 * wk) {
-        // Few keys: prefix and own ones by one block a sequence and kv head, four
-        // tiles a wave at most.  Parts would be shorter by less than their merge
-        // takes (4 us): two sequences of 3..18 keys, room for 300: 9.7 -> 7.2 us.
-        p.joint = 1;
-        p.own_parts = p.parts = 1;
-        p.own_chunk = (int32_t)cbq_max(prefix + capacity, 1);
-        p.own_tiles = (int32_t)cbq_ceil(rep, 16);
-        p.blocks = n_kv * batch * p.own_tiles;
-        return p;
-    }
     p.rt = rows <= 16 ? 0 : rows <= 64 ? 1 : widest(row_bytes);
     int64_t tiles = cbq_ceil(rows, p.rt ? 64 * p.rt : 16), pre_parts = 0, pre_chunk = 1;
     if (prefix > 0) {
@@ -182,24 +190,31 @@ inline Plan plan_decode(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
     p.own_chunk = (int32_t)own_chunk;
     p.own_tiles = (int32_t)own_tiles;
     p.parts = (int32_t)(pre_parts + own_parts);
+    if (prefix + capacity > 4 * wk) return p;
+    // Few keys, four tiles a wave at most: one block a sequence and kv head can walk
+    // prefix and own ones without a merge (3.5 us and its sums), where that is less
+    // than the tiles it adds to the blocks' turns beside the prefix's walk.  bf16, 8 kv
+    // heads of 128 of 4 queries, in one block and in parts: 2 sequences of 3..18 keys,
+    // room for 300, 7.2 and 9.7 us; 128 sequences behind 460 keys 22.5 and 19.9, 1024
+    // of them 140 and 97; one query a kv head of 64, 1024 behind 921 143 and 75.  Over
+    // 2616 sizes of 1 to 512 sequences 0.8 % above the shorter of both (one block
+    // everywhere 4.6 %, parts 24 %).
+    const double one = (double)(n_kv * batch * own_tiles) / (row_bytes <= 512 ? 2 * kCus : kCus);
+    const double tile = row_bytes > 512 ? 5.5 : row_bytes == 4 * hd ? 1.4 : 1.0;   // us of a wave's
+    double alone, paired, split = 0;
+    walk_us(row_bytes, hd, p.rt, alone, paired);
+    if (capacity > 0) split = tile * std::max(1.0, one * cbq_ceil(capacity, wk));
+    split += (double)tiles * n_kv * prefix * 0.001 * alone / kCus;
+    if (p.parts > 1) split += 3.5 + (double)p.parts * batch * n_kv * rep * hd * 8 / 5e6;
+    const bool alike = !pre_parts && p.parts == 1;          // one part of own keys either way
+    if (!alike && tile * std::max(1.0, one) * cbq_ceil(prefix + capacity, wk) > split) return p;
+    p = Plan{};
+    p.joint = 1;
+    p.own_parts = p.parts = 1;
+    p.own_chunk = (int32_t)cbq_max(prefix + capacity, 1);
+    p.own_tiles = (int32_t)own_tiles;
+    p.blocks = n_kv * batch * own_tiles;
     return p;
-}
-
-// A prompt's block of 16, 64 or 128 rows (rt 0, 1, 2) takes this many us for 1000
-// keys, alone on its CU and beside another block (rows of 1024 bytes: there is
-// none), measured over 2000 to 4000 keys.
-inline void walk_us(int row_bytes, int hd, int rt, double &alone, double &paired)
-{
-    static const float us[2][3][3][2] = {
-        {{{5.4f, 8.2f}, {15, 17}, {17.5f, 20}},             // 16-bit types: hd 64, 128, 256
-         {{10.4f, 14.8f}, {20, 25}, {24, 32}},
-         {{22.5f, 31}, {38, 46}, {0, 0}}},
-        {{{17, 27}, {46, 68}, {75, 116}},                   // fp32
-         {{33, 50}, {84, 126}, {0, 0}},
-         {{96, 96}, {182, 182}, {0, 0}}}};
-    const float *u = us[row_bytes == 4 * hd][hd == 64 ? 0 : hd == 128 ? 1 : 2][rt];
-    alone = u[0];
-    paired = u[1];
 }
 
 inline Plan plan_prompt(int row_bytes, int hd, int n_kv, int rep, int64_t prefix, int64_t capacity,

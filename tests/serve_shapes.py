@@ -84,3 +84,18 @@ DECODES = [
 def decode_plan_args(hd, size, lens, prefix, rep, room):
     capacity = (-(-max(lens) // PAGE) + room) * PAGE
     return hd * size, hd, 2, rep, prefix, capacity, len(lens)
+
+
+# The same for few keys: one block a sequence and kv head takes prefix and own ones
+# together (by head size), or parts do because the batch is large.
+JOINTS = [
+    (2, [3, 0, 18], 12, 3, 1, (1, 1, 1)),
+    (4, [3, 0, 18], 12, 3, 1, (1, 1, 1)),
+    (2, [200, 0, 31], 12, 20, 1, (1, 1, 1)),
+    (2, [90, 0, 31], 0, 3, 1, (1, 1, 1)),
+    (4, [60, 0, 31], 30, 3, 1, (1, 1, 0)),
+    (2, [3, 16, 0, 9] * 256, 210, 1, 0, (1, 1, 0)),
+    (4, [3, 16, 0, 9] * 128, 210, 1, 0, (1, 0, 0)),
+    (4, [3, 16, 0, 9] * 128, 470, 1, 0, (0, 0, 0)),
+    (2, [3, 16, 0, 9] * 256, 930, 1, 0, (0, 0, 0)),
+]

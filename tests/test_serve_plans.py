@@ -42,3 +42,11 @@ def test_decodes(plan, i, hd):
         assert not p["joint"] and p["rt"] == rt[i], (shape, p)
         assert prefix_parts is None or (p["pre_parts"] > 1) == prefix_parts, (shape, p)
         assert (p["own_parts"] > 1) == own_parts, (shape, p)
+
+
+@pytest.mark.parametrize("i,hd", list(enumerate((64, 128, 256))))
+def test_joints(plan, i, hd):
+    """Large batches of few keys behind a prefix read it once for all of them."""
+    for *shape, joint in sh.JOINTS:
+        p = plan("decode", *sh.decode_plan_args(hd, *shape))
+        assert p["joint"] == joint[i], (shape, p)
