@@ -86,6 +86,10 @@ def decode_plan_args(hd, size, lens, prefix, rep, room):
     return hd * size, hd, 2, rep, prefix, capacity, len(lens)
 
 
+# Thousands of rows of more than 16 parts: (bytes a value, own lengths, shared keys, query
+# heads of each of two kv heads, unused pages).
+MERGES = [(2, [777, 0, 5, 33] * 16, 1100, 32, 2000), (4, [777, 0, 5, 33] * 16, 1100, 32, 2000)]
+
 # The same for few keys: one block a sequence and kv head takes prefix and own ones
 # together (by head size), or parts do because the batch is large.
 JOINTS = [

@@ -60,13 +60,14 @@ def test_decodes(cuda, ops, dtype, hd, lens, prefix, rep, room):
 
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("dtype,lens,prefix,rep,room", [
-    (t, *shape[1:5]) for shape in sh.JOINTS for t in TYPES[shape[0]]])
-def test_joints(cuda, ops, dtype, hd, lens, prefix, rep, room):
-    """Few keys, in one walk and in parts; of a large batch some sequences."""
+    (t, *shape[1:5]) for shape in sh.JOINTS + sh.MERGES for t in TYPES[shape[0]]])
+def test_large_batches(cuda, ops, dtype, hd, lens, prefix, rep, room):
+    """Few keys, in one walk and in parts, and many rows of many parts; of a large
+    batch some sequences."""
     b = Batch(lens, prefix, 2, rep, hd, sh.PAGE, dtype, seed=hd + len(lens), room=room)
     b.tables[-1] = -1
     q, what = b.queries(len(lens), 1.5), f"{dtype} hd={hd} {len(lens)} sequences prefix={prefix}"
-    print("few keys " + what, flush=True)
+    print("large batch " + what, flush=True)
     out = decode(ops, b, q, hd ** -0.5)
     some = sorted({*range(min(9, len(lens))), len(lens) // 2, *range(max(len(lens) - 9, 0), len(lens))})
     b.lens, b.tables, b.lengths = [lens[i] for i in some], b.tables[some], b.lengths[some]

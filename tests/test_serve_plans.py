@@ -44,6 +44,13 @@ def test_decodes(plan, i, hd):
         assert (p["own_parts"] > 1) == own_parts, (shape, p)
 
 
+@pytest.mark.parametrize("hd", (64, 128, 256))
+def test_merges(plan, hd):
+    for shape in sh.MERGES:
+        p = plan("decode", *sh.decode_plan_args(hd, *shape))
+        assert p["pre_parts"] + p["own_parts"] > 16 and len(shape[1]) * 2 * shape[3] >= 4096, (shape, p)
+
+
 @pytest.mark.parametrize("i,hd", list(enumerate((64, 128, 256))))
 def test_joints(plan, i, hd):
     """Large batches of few keys behind a prefix read it once for all of them."""
