@@ -25,13 +25,14 @@
 // 16-byte slots of a row are stored at slot ^ mix(row), which spreads both
 // operands' reads over the banks.
 //
-// What bounds it (MI355X; heads 32 on 8 of 128 unless said): long bf16 prompts the
-// card's power: 8192 tokens 565 us, 970 TFLOP/s, the matrix units busy 44 % of the
-// cycles at a clock that falls to 2.1 GHz as fewer cycles are needed (the
-// framework's large product runs at 1.2 PFLOP/s); one-token steps HBM: 64
-// sequences of 200..1500 own keys 58 us without a prefix (3.8 TB/s, launches and
-// merge included) and 87 behind 30011 shared keys; few keys two launches of 4 to 5
-// us and a chain of three dependent loads (length, page id, key).
+// What bounds it (MI355X; heads 32 on 8 of 128 unless said): of long bf16 prompts
+// nothing alone: 8192 tokens 565 to 603 us by card (925 to 970 TFLOP/s; the
+// framework's large product runs at 1.2 PFLOP/s), the matrix units busy 44 % of the
+// cycles, the clock at 2.1 GHz and lower the fewer cycles are needed, and LDS copies
+// and reads in the way (eight waves a block 529); one-token steps HBM: 64 sequences of
+// 200..1500 own keys 58 us without a prefix and 85 behind 30011 shared keys (3.8 and
+// 4.2 TB/s, launches and merge included); few keys two launches of 4 to 5 us and a
+// chain of three dependent loads (length, page id, key).
 #pragma once
 
 #include <atomic>

@@ -64,7 +64,7 @@ typedef struct cbq_paged_kv {
  * contiguous, of the cache's type, and may not alias q, k or v.
  * q, k, v: element [t, h, d] at t * stride[0] + h * stride[1] + d.
  * A token whose position is outside [0, n_pos) stores nothing, and its query
- * is turned by row 0; two tokens with one slot leave either's row there.
+ * is turned by row 0; two tokens with one slot leave pieces of either's row.
  * hd even, 2..256; rot even, 2..hd; N * (n_q + 2 n_kv) < 2^31. */
 int cbq_paged_append(const void *q, const void *k, const void *v, int x_dtype,
                      const int64_t *q_stride, const int64_t *k_stride, const int64_t *v_stride,
@@ -78,12 +78,14 @@ int cbq_paged_append(const void *q, const void *k, const void *v, int x_dtype,
  * lengths[b] keys (pages tables[b * table_stride + i], i < width), and
  *   out[b, i] = softmax(q[b, i] . k_j * scale) . v_j     over the keys it sees,
  * query head i reading kv head i / (n_q / n_kv); a sequence that sees no key
- * gets zeros.  q [batch, n_q, hd] with strides {token, head} in elements, 16-
- * byte aligned as the pages are; out contiguous, of q's type, which is the
- * cache's.  Scores, maxima, sums and the weighted values are fp32; for 16-bit
- * types the weights exp(s - max) are rounded to that type for the matrix
- * cores.  hd in {64, 128, 256}; n_q % n_kv == 0; n_q < 2^20;
- * batch < 2^30 and batch * n_q < 2^31; prefix + width * page <= 2^31 - 65536.
+ * gets zeros.  The prefix is read once for all sequences, or by each where
+ * keys are so few that this takes less time.  q [batch, n_q, hd] with strides
+ * {token, head} in elements, 16-byte aligned as the pages are; out contiguous,
+ * of q's type, which is the cache's.  Scores, maxima, sums and the weighted
+ * values are fp32; for 16-bit types the weights exp(s - max) are rounded to
+ * that type for the matrix cores.  hd in {64, 128, 256}; n_q % n_kv == 0;
+ * n_q < 2^20, batch < 2^30, batch * n_q < 2^31; prefix + width * page <=
+ * 2^31 - 65536.
  * workspace: cbq_prefix_attn_decode_workspace bytes (which may be 0), 16-byte
  * aligned, overwritten by every call. */
 size_t cbq_prefix_attn_decode_workspace(const cbq_paged_kv *cache, int64_t prefix, int width,
