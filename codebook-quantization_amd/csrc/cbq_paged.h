@@ -192,22 +192,26 @@ inline Plan plan_decode(int row_bytes, int hd, int n_kv, int rep, int64_t prefix
     p.parts = (int32_t)(pre_parts + own_parts);
     if (prefix + capacity > 4 * wk) return p;
     // Few keys, four tiles a wave at most: one block a sequence and kv head can walk
-    // prefix and own ones without a merge (3.5 us and its sums), where that is less
-    // than the tiles it adds to the blocks' turns beside the prefix's walk.  bf16, 8 kv
-    // heads of 128 of 4 queries, in one block and in parts: 2 sequences of 3..18 keys,
-    // room for 300, 7.2 and 9.7 us; 128 sequences behind 460 keys 22.5 and 19.9, 1024
-    // of them 140 and 97; one query a kv head of 64, 1024 behind 921 143 and 75.  Over
-    // 2616 sizes of 1 to 512 sequences 0.8 % above the shorter of both (one block
-    // everywhere 4.6 %, parts 24 %).
+    // prefix and own ones without a merge (3 us and its sums), where that is less than
+    // the tiles it adds to the blocks' turns.  bf16, 8 kv heads of 128 of 4 queries, in
+    // one block and in parts: 2 sequences of 3..18 keys, room for 300, 7.2 and 9.7 us;
+    // 128 sequences behind 460 keys 22.5 and 19.9, 1024 of them 140 and 97; one query a
+    // kv head of 64, 1024 behind 921 143 and 75.  The lengths are device data: 0.4 of
+    // the room is taken for them.  Over sizes of 1 to 512 sequences the estimate's
+    // choice takes 0.5 % more than the shorter of both where lengths fill up to the
+    // room (2616 of them; one block everywhere 4.6 %, parts 24 %), 1.1 % where 256 keys
+    // of room are left (3360; 2.3 and 35 %).
+    const int64_t own = (2 * capacity + 4) / 5;
     const double one = (double)(n_kv * batch * own_tiles) / (row_bytes <= 512 ? 2 * kCus : kCus);
-    const double tile = row_bytes > 512 ? 5.5 : row_bytes == 4 * hd ? 1.4 : 1.0;   // us of a wave's
+    const double tile = row_bytes > 512 ? 5 : row_bytes == 4 * hd ? 1.8 : 1.2;      // us of a wave's
     double alone, paired, split = 0;
     walk_us(row_bytes, hd, p.rt, alone, paired);
-    if (capacity > 0) split = tile * std::max(1.0, one * cbq_ceil(capacity, wk));
+    if (own > 0) split = tile * std::max(1.0, one * cbq_ceil(own, wk));
     split += (double)tiles * n_kv * prefix * 0.001 * alone / kCus;
-    if (p.parts > 1) split += 3.5 + (double)p.parts * batch * n_kv * rep * hd * 8 / 5e6;
+    split = std::max(split, (double)cbq_min(pre_chunk, prefix) * 0.001 * alone);            // a prefix block
+    if (p.parts > 1) split += 3 + (double)p.parts * batch * n_kv * rep * hd * 8 / 5e6;
     const bool alike = !pre_parts && p.parts == 1;          // one part of own keys either way
-    if (!alike && tile * std::max(1.0, one) * cbq_ceil(prefix + capacity, wk) > split) return p;
+    if (!alike && tile * std::max(1.0, one) * cbq_ceil(prefix + own, wk) > split) return p;
     p = Plan{};
     p.joint = 1;
     p.own_parts = p.parts = 1;

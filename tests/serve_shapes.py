@@ -97,8 +97,8 @@ JOINTS = [
     (4, [3, 0, 18], 12, 3, 1, (1, 1, 1)),
     (2, [200, 0, 31], 12, 20, 1, (1, 1, 1)),
     (2, [90, 0, 31], 0, 3, 1, (1, 1, 1)),
-    (4, [60, 0, 31], 30, 3, 1, (1, 1, 0)),
-    (2, [3, 16, 0, 9] * 256, 210, 1, 0, (1, 1, 0)),
+    (4, [60, 0, 31], 30, 3, 1, (1, 1, 1)),
+    (2, [3, 16, 0, 9] * 256, 210, 1, 0, (1, 0, 0)),
     (4, [3, 16, 0, 9] * 128, 210, 1, 0, (1, 0, 0)),
     (4, [3, 16, 0, 9] * 128, 470, 1, 0, (0, 0, 0)),
     (2, [3, 16, 0, 9] * 256, 930, 1, 0, (0, 0, 0)),
