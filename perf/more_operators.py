@@ -15,7 +15,8 @@ elementary torch operations:
 
 Pages are [n_pages, n_kv, page, hd / 2] bytes and [n_pages, n_kv, page, hd / 64,
 2] bf16 numbers (scale s, mid m): 64 neighbouring values of a row are m + s (c -
-7.5), code c of the even ones in a byte's low half.  Head layouts and the
+7.5).  A row's codes lie four of each of its groups side by side (values 0..3, 64..67,
+.. 4..7, 68..71, ..), the first of two in a byte's low half.  Head layouts and the
 vocabulary are those of the two decoder configurations of
 codebook-quantization_amd/synthetic.py (32 and 16 query heads on 8 kv heads of
 128, 151936 tokens) and generic ones of the other head sizes.
@@ -311,13 +312,14 @@ def _quantised(x):
     scale = (torch.maximum(top - m, m - low) / 7.5).float().bfloat16()
     s = scale.double()[..., None]
     c = torch.where(s > 0, torch.floor((x - m[..., None]) / s) + 8, 8.0).clamp(0, 15).to(torch.uint8)
-    c = c.flatten(-2)
+    c = c.unflatten(-1, (-1, 4)).transpose(-3, -2).flatten(-3)      # four of each group in turn
     return c[..., 0::2] | c[..., 1::2] << 4, torch.stack([scale, mid], -1)
 
 
 def _values(codes, scales):
     """[..., hd / 2] and [..., hd / 64, 2] -> [..., hd] in 32 bits."""
-    c = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).unflatten(-1, (-1, GROUP)).float()
+    c = torch.stack([codes & 15, codes >> 4], -1).flatten(-2)
+    c = c.unflatten(-1, (GROUP // 4, -1, 4)).transpose(-3, -2).flatten(-2).float()
     return (scales[..., 1:].float() + scales[..., :1].float() * (c - 7.5)).flatten(-2)
 
 
@@ -463,8 +465,11 @@ def _exact_rows(codes, scales, places):
     page = codes.shape[1]
     byte = codes.reshape(-1, codes.shape[2])[places].long()
     pair = scales.reshape(codes.shape[0] * page, -1, 2)[places].double()
-    code = torch.empty(byte.shape[0], 2 * byte.shape[1], dtype=torch.float64, device="cuda")
-    code[:, 0::2], code[:, 1::2] = (byte % 16).double(), torch.div(byte, 16, rounding_mode="floor").double()
+    hd = 2 * byte.shape[1]
+    d = torch.arange(hd, device="cuda")
+    g, e = d // GROUP, d % GROUP
+    half = byte[:, e // 4 * (hd // 32) + 2 * g + e % 4 // 2]
+    code = torch.where(e % 2 == 0, half % 16, torch.div(half, 16, rounding_mode="floor")).double()
     each = pair.repeat_interleave(GROUP, 1)
     return (2 * code - 15) / 2 * each[..., 0] + each[..., 1]
 
