@@ -18,7 +18,9 @@ ARCH = "gfx950"
 SOURCES = ["cbq_fixed.hip", "cbq_huffman.hip", "cbq_prefill.hip", "cbq_prefill_f32.hip",
            "cbq_decode.hip", "cbq_split.hip", "cbq_tiny.hip", "cbq_gemm.hip",
            "cbq_paged_append.hip", "cbq_prefix_attn.hip", "cbq_prefix_attn_f32.hip",
-           "cbq_prefix_attn_bf16.hip", "cbq_prefix_attn_f16.hip"]
+           "cbq_prefix_attn_bf16.hip", "cbq_prefix_attn_f16.hip", "cbq_q4_append.hip",
+           "cbq_q4_attn.hip", "cbq_q4_attn_f32.hip", "cbq_q4_attn_bf16.hip", "cbq_q4_attn_f16.hip",
+           "cbq_verify.hip"]
 # host-only C++ (no device code): compiled by the host compiler
 HOST_SOURCES = ["cbq_huff_host.cpp", "cbq_io.cpp"]
 HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-pthread", "-D__HIP_PLATFORM_AMD__=1",
@@ -47,7 +49,8 @@ def host_sources():
 
 TIMELINE_SO = os.path.join(HERE, "libcbq_hip_timeline.so")
 TORCH_SO = os.path.join(HERE, "libcbq_torch.so")
-TORCH_SRC = [os.path.join(CSRC, s) for s in ("cbq_torch_ops.cpp", "cbq_torch_serve.cpp")]
+TORCH_SRC = [os.path.join(CSRC, s) for s in ("cbq_torch_ops.cpp", "cbq_torch_serve.cpp",
+                                               "cbq_torch_q4.cpp")]
 
 
 def torch_ops_command(out: str = TORCH_SO):

@@ -1,5 +1,5 @@
 """ctypes binding of libcbq_hip.so, the gfx950 C ABI (include/cbq_hip.h,
-include/cbq_decode.h, include/cbq_serve.h).
+include/cbq_decode.h, include/cbq_serve.h, include/cbq_serve_q4.h).
 
 The library is loaded after torch so that it binds to the HIP runtime torch
 already loaded (same SONAME), which makes torch's device pointers and
@@ -60,6 +60,13 @@ class PagedKV(ctypes.Structure):
     _fields_ = [("k", _vp), ("v", _vp), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3),
                 ("n_pages", _i64), ("page", ctypes.c_int32), ("n_kv", ctypes.c_int32),
                 ("hd", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class PagedQ4(ctypes.Structure):
+    """struct cbq_paged_q4 (include/cbq_serve_q4.h)."""
+    _fields_ = [("k_codes", _vp), ("v_codes", _vp), ("k_scales", _vp), ("v_scales", _vp),
+                ("code_stride", _i64 * 3), ("scale_stride", _i64 * 3), ("n_pages", _i64),
+                ("page", ctypes.c_int32), ("n_kv", ctypes.c_int32), ("hd", ctypes.c_int32)]
 
 
 # name -> (restype, argtypes); every symbol declared in include/*.h
@@ -155,6 +162,19 @@ SIGNATURES = {
     "cbq_prefix_attn_prompt": (_i, [_vp, _vp, _vp, ctypes.POINTER(PagedKV), _vp, _i64, _vp, _i64,
                                     _i, _vp, _i, _i64, _i, ctypes.c_float, _vp, _vp,
                                     ctypes.c_size_t, _vp]),
+    "cbq_verify_drafts_workspace": (ctypes.c_size_t, [_i, _i64]),
+    "cbq_verify_drafts": (_i, [_vp] * 5 + [_i] + [_vp] * 2 + [_i] * 2 + [_i64] + [_vp] * 3
+                          + [ctypes.c_size_t, _vp]),
+    # include/cbq_serve_q4.h
+    "cbq_paged_append_q4": (_i, [_vp] * 3 + [_i] + [_vp] * 5 + [_i64, _i] + [_vp] * 2 + [_i]
+                            + [_vp] * 2 + [ctypes.c_float, _vp, ctypes.POINTER(PagedQ4), _i64, _i,
+                                           _vp]),
+    "cbq_paged_read_q4": (_i, [ctypes.POINTER(PagedQ4), _vp, _i64, _i] + [_vp] * 3),
+    "cbq_prefix_attn_decode_q4_workspace": (ctypes.c_size_t, [ctypes.POINTER(PagedQ4), _i64]
+                                            + [_i] * 4),
+    "cbq_prefix_attn_decode_q4": (_i, [_vp, _vp, _i, ctypes.POINTER(PagedQ4), _vp, _i64, _vp, _i64,
+                                       _i, _vp, _i, _i, _i, ctypes.c_float, _vp, _vp,
+                                       ctypes.c_size_t, _vp]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

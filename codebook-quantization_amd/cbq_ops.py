@@ -1,6 +1,6 @@
 """torch.ops.cbq: the compressed entry points registered with torch's
-dispatcher (libcbq_torch.so, built from csrc/cbq_torch_ops.cpp and
-csrc/cbq_torch_serve.cpp over the C ABI of libcbq_hip.so).
+dispatcher (libcbq_torch.so, built from csrc/cbq_torch_ops.cpp, csrc/cbq_torch_serve.cpp
+and csrc/cbq_torch_q4.cpp over the C ABI of libcbq_hip.so).
 
     linear(x, packed, codebook, M, bits)              fixed-width GEMV / GEMM
     linear_kind(x, packed, codebook, M, bits, cb_kind)    linear for a codebook whose
@@ -23,6 +23,21 @@ and the operators of batched serving over a paged key/value cache
                             lengths, scale)            one token a sequence
     prefix_attention_prompt(q, q_start, k_pages, v_pages, prefix_table, prefix,
                             tables, lengths, scale)    ragged runs, causal
+    verify_drafts(probs, drafts, draft_probs, n_drafts, uniforms)
+                                                      drafted tokens against the target's
+                                                      probabilities: (tokens, counts)
+
+the same over a cache of 4 bits (include/cbq_serve_q4.h; codes uint8 [n_pages, n_kv,
+page, hd / 2], scales bfloat16 [n_pages, n_kv, page, hd / 64, 2]):
+
+    paged_append_q4(q, k, v, cos, sin, positions, slots, k_codes, k_scales, v_codes,
+                    v_scales, norm, q_weight, k_weight, eps)   as paged_append
+    paged_read_q4(k_codes, k_scales, v_codes, v_scales, slots, dtype)
+                                                      rows of the cache as values: (k, v)
+    prefix_attention_decode_q4(q, k_codes, k_scales, v_codes, v_scales, prefix_table,
+                               prefix, tables, lengths, scale)
+                                                      the newest tokens, as many of each
+                                                      sequence as q has rows for
 
 The modules (compressed_modules via gpu_accelerated_functions and
 gpu_huffman_functions) call these ops; they run on torch's current HIP

@@ -1,0 +1,119 @@
+// Launch plans of the attention over the 4-bit paged cache and what a block of them
+// does: plain C++ that the kernels, the host entry points and the CPU test of them
+// (tests/native/cbq_q4_host.cpp) share.
+#pragma once
+
+#include "cbq_paged.h"
+
+namespace cbq_q4 {
+
+constexpr int kTile = 32;                   // keys of a wave's tile
+constexpr int kAttnWaves = 4;               // waves a block, whose tiles take turns
+constexpr int64_t kMaxBlocks = (1ll << 31) - 1, kMaxParts = 1 << 20, kAttnCus = 256;
+
+struct Plan {
+    int32_t rt;                             // 16 rt rows a block of the prefix
+    int32_t tiles;                          // row tiles of the prefix, of all sequences
+    int32_t pre_parts, pre_chunk;           // parts of the prefix and their key tiles
+    int32_t own_parts, own_chunk, own_tiles;    // parts of the own keys; 16-row tiles of a sequence
+    int32_t parts;                          // all of them
+    int32_t joint;                          // one part: a sequence's own blocks walk the prefix too
+    int64_t blocks, bytes;
+};
+
+inline int64_t part_bytes(int64_t parts, int64_t rows, int hd)
+{
+    return parts > 1 ? parts * rows * (hd + 2) * 4 : 0;
+}
+
+// rows: query rows of a sequence and kv head (tokens times query heads a kv head)
+inline Plan plan(int hd, int n_kv, int64_t rows, int64_t prefix, int64_t capacity, int64_t batch)
+{
+    Plan p = {};
+    const int64_t pre_tiles = cbq_ceil(prefix, kTile), cap_tiles = cbq_ceil(capacity, kTile);
+    const int64_t own_tiles = cbq_ceil(rows, 16);
+    p.rt = 1;
+    p.own_tiles = (int32_t)own_tiles;
+    if (pre_tiles + cap_tiles <= 4 * kAttnWaves) {
+        p.joint = 1;
+        p.own_parts = p.parts = 1;
+        p.own_chunk = (int32_t)cbq_max(pre_tiles + cap_tiles, 1);
+        p.blocks = n_kv * batch * own_tiles;
+        return p;
+    }
+    int64_t tiles = cbq_ceil(batch * rows, 16 * p.rt), pre_parts = 0, pre_chunk = 1;
+    if (pre_tiles) {
+        const int64_t want = cbq_max(1, 2 * kAttnCus / (tiles * n_kv));
+        pre_chunk = cbq_max(2 * kAttnWaves, cbq_ceil(cbq_ceil(pre_tiles, want), kAttnWaves) * kAttnWaves);
+        pre_parts = cbq_ceil(pre_tiles, pre_chunk);
+    } else {
+        tiles = 0;
+    }
+    const int64_t share = cbq_ceil(cap_tiles * batch * n_kv * own_tiles, 4 * kAttnCus);
+    int64_t own_chunk = cbq_min(cbq_max(cbq_ceil(share, kAttnWaves), 1), 16) * kAttnWaves;
+    // more of a wider table than its parts and blocks are counted for
+    const int64_t most = cbq_min(kMaxParts / 2, (kMaxBlocks - n_kv * tiles * pre_parts) / (n_kv * batch * own_tiles));
+    if (most > 0) own_chunk = cbq_max(own_chunk, cbq_ceil(cbq_ceil(cap_tiles, most), kAttnWaves) * kAttnWaves);
+    const int64_t own_parts = cbq_max(cbq_ceil(cap_tiles, own_chunk), pre_parts ? 0 : 1);
+    p.tiles = (int32_t)tiles;
+    p.pre_parts = (int32_t)pre_parts;
+    p.pre_chunk = (int32_t)pre_chunk;
+    p.own_parts = (int32_t)own_parts;
+    p.own_chunk = (int32_t)own_chunk;
+    p.parts = (int32_t)(pre_parts + own_parts);
+    p.blocks = n_kv * (tiles * pre_parts + batch * own_tiles * own_parts);
+    p.bytes = part_bytes(pre_parts + own_parts, batch * rows * n_kv, hd);
+    return p;
+}
+
+inline bool plan_fits(const Plan &p)
+{
+    return p.blocks > 0 && p.blocks <= kMaxBlocks && p.parts <= kMaxParts;
+}
+
+// A block's rows and its key tiles [first, end): of the prefix from 0 on, then (own
+// parts, or all where joint) of the own keys from pre_tiles on.
+struct Work {
+    int h, tile, part, seq;                 // seq -1: prefix rows, of the whole batch
+    int32_t first, end;                     // as the capacity has them
+};
+
+CBQ_PAGED_FN Work work_of(const Plan &p, uint32_t block, int n_kv, int batch, int32_t pre_tiles,
+                          int32_t cap_tiles)
+{
+    Work w;
+    uint32_t i = block;
+    const uint32_t pre = (uint32_t)p.tiles * p.pre_parts * n_kv;
+    const bool shared = i < pre;
+    if (!shared) i -= pre;
+    w.h = (int)(i % n_kv);
+    i /= n_kv;
+    if (shared) {
+        w.tile = (int)(i % p.tiles);
+        w.part = (int)(i / p.tiles);
+        w.seq = -1;
+        w.first = w.part * p.pre_chunk;
+        w.end = (int32_t)cbq_min((int64_t)w.first + p.pre_chunk, pre_tiles);
+        return w;
+    }
+    w.tile = (int)(i % p.own_tiles);
+    i /= p.own_tiles;
+    w.seq = (int)(i % batch);
+    const int chunk = (int)(i / batch);
+    const int64_t from = p.joint ? 0 : pre_tiles, upto = (int64_t)pre_tiles + cap_tiles;
+    w.part = p.pre_parts + chunk;
+    w.first = (int32_t)cbq_min(from + (int64_t)chunk * p.own_chunk, upto);
+    w.end = (int32_t)cbq_min((int64_t)w.first + p.own_chunk, upto);
+    return w;
+}
+
+// Key `lane` of key tile `tile`: its place in its table's order and the keys of that
+// table, `prefix` shared or `length` own ones; place -1 past their end.
+CBQ_PAGED_FN int32_t tile_key(int32_t tile, int32_t pre_tiles, int32_t prefix, int32_t length, int lane)
+{
+    const bool shared = tile < pre_tiles;
+    const int32_t j = (shared ? tile : tile - pre_tiles) * kTile + lane;
+    return j < (shared ? prefix : length) ? j : -1;
+}
+
+}  // namespace cbq_q4

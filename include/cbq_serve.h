@@ -1,6 +1,7 @@
 /*
  * cbq_serve.h -- batched serving over a paged key/value cache
- * (libcbq_hip.so, csrc/cbq_paged_append.hip and csrc/cbq_prefix_attn*.hip).
+ * (libcbq_hip.so, csrc/cbq_paged_append.hip and csrc/cbq_prefix_attn*.hip), and
+ * the verification of drafted tokens (csrc/cbq_verify.hip).
  *
  * These entry points have no counterpart in the reference's C/HIP libraries:
  * its models run HF's attention over one dense cache per sequence.  They let
@@ -111,6 +112,34 @@ int cbq_prefix_attn_prompt(const void *q, const int64_t *q_stride, const int32_t
                            const int32_t *lengths, int batch, int64_t N, int n_q, float scale,
                            void *out, void *workspace, size_t workspace_bytes,
                            hipStream_t stream);
+
+/* Drafted tokens against the target's probabilities.  Sequence b has n = n_drafts[b]
+ * drafts (as a length, inside 0..drafts; all of them when n_drafts is NULL) d_i, drawn
+ * from q_i = draft_probs[b, i], the target's p_i = probs[b, i] (i <= n; p_n is the
+ * row behind them all) and random numbers u_i = uniforms[b, i] of [0, 1).  Drafts are
+ * kept while
+ *   u_i q_i(d_i) < p_i(d_i),
+ * and behind the a that are kept one token is drawn by u = uniforms[b, drafts] from
+ *   w = max(p_a - q_a, 0) if a < n, or from w = p_n:
+ * the first token whose sum w(0) + .. + w(token) exceeds u times the sum of all (the
+ * last one of w > 0 where rounding leaves none).  So the tokens are distributed as the
+ * target's.  Without draft_probs (NULL) a draft is taken as certain: q_i is 1 at d_i
+ * and 0 elsewhere.  Products, differences and sums are in 64 bits.
+ *   tokens[b] = d_0 .. d_(a-1), the drawn one, then -1;  counts[b] = a + 1.
+ * What is NaN or below 0 in w counts as 0; where all of w is 0, p_a is taken in its
+ * place, and where that is too, the token is -1.  A draft outside [0, vocab) has the
+ * probability 0; its q is 1 without draft_probs, else 0.
+ * probs, draft_probs: dtype CBQ_F32, CBQ_BF16 or CBQ_F16, element [b, i, v] at b *
+ * stride[0] + i * stride[1] + v.  drafts [batch, drafts], uniforms [batch, drafts + 1],
+ * tokens [batch, drafts + 1] and counts [batch] are contiguous.  1 <= vocab < 2^31,
+ * 0 <= drafts = n_max < 2^20, 0 <= batch < 2^24, batch * drafts < 2^30.
+ * workspace: cbq_verify_drafts_workspace bytes, 16-byte aligned, overwritten. */
+size_t cbq_verify_drafts_workspace(int batch, int64_t vocab);
+int cbq_verify_drafts(const void *probs, const int64_t *p_stride, const int64_t *drafts,
+                      const void *draft_probs, const int64_t *q_stride, int dtype,
+                      const int32_t *n_drafts, const float *uniforms, int batch, int n_max,
+                      int64_t vocab, int64_t *tokens, int32_t *counts, void *workspace,
+                      size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }
