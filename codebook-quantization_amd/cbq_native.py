@@ -171,7 +171,7 @@ SIGNATURES = {
                                            _vp]),
     "cbq_paged_read_q4": (_i, [ctypes.POINTER(PagedQ4), _vp, _i64, _i] + [_vp] * 3),
     "cbq_prefix_attn_decode_q4_workspace": (ctypes.c_size_t, [ctypes.POINTER(PagedQ4), _i64]
-                                            + [_i] * 4),
+                                            + [_i] * 5),
     "cbq_prefix_attn_decode_q4": (_i, [_vp, _vp, _i, ctypes.POINTER(PagedQ4), _vp, _i64, _vp, _i64,
                                        _i, _vp, _i, _i, _i, ctypes.c_float, _vp, _vp,
                                        ctypes.c_size_t, _vp]),

@@ -10,8 +10,12 @@
 // remainder.  Queries go in fp32.
 //
 // Sixteen lanes hold a row, four neighbouring values of each group a lane, which are
-// neighbours in the row's codes too; a group's range takes four exchanges.  The values
-// that a rotation pairs with a lane's are read as well (cache hits).
+// neighbours in the row's codes too; a row's sum and a group's range take four
+// exchanges among neighbours, by row rotations.  Where half the rotated part is whole
+// groups, or half a group, the values that turn together are the lane's own, or those of
+// the lane eight away; else the others' are read too (cache hits).  A thread has
+// neighbouring heads of a token, all queries, keys or values, which share what is
+// read of the tables and weights.
 #include "cbq_q4.h"
 
 namespace {
@@ -19,6 +23,7 @@ namespace {
 using namespace cbq_q4;
 
 constexpr int kThreads = 256;
+constexpr int64_t kFourThreads = 4 * 256 * 4 * 64;       // four waves a SIMD of 256 CUs
 constexpr int kLanes = 16, kRows = kThreads / kLanes;    // lanes a row, rows a block
 
 struct AppendArgs {
@@ -28,10 +33,10 @@ struct AppendArgs {
     const int64_t *positions, *slots;
     void *q_out;
     Pool pool;
-    int64_t n_pos, n_slots, rows[3];
+    int64_t N, n_pos, n_slots, units[3];    // units: of heads that a thread has, of each kind
     uint32_t first[3];                      // first block of each
-    CbqDiv heads[3];
-    int rot, norm;
+    CbqDiv heads[3];                        // units a token
+    int n_q, n_kv, rot, norm;
     float eps;
 };
 
@@ -53,15 +58,59 @@ __device__ __forceinline__ void load4(const T *p, A (&x)[4])
     }
 }
 
-// A lane's values of a row, [group][4] from d0 on, normed and turned.  VEC: aligned
-// fours, and rot / 2 in whole fours, so that all of one turn alike.
-template <typename T, typename A, int HD, bool VEC>
+// x of the lane `by` further on (cyclically) in its sixteen
+template <int BY> __device__ __forceinline__ float rotated(float x)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 | BY, 0xf, 0xf, true));
+}
+template <int BY> __device__ __forceinline__ double rotated(double x)
+{
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(x), 0x120 | BY, 0xf, 0xf, true),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(x), 0x120 | BY, 0xf, 0xf, true));
+}
+// f over the sixteen lanes of a row, in all of them
+template <typename A, typename F> __device__ __forceinline__ A over_row(A x, F f)
+{
+    x = f(x, rotated<8>(x));
+    x = f(x, rotated<4>(x));
+    x = f(x, rotated<2>(x));
+    return f(x, rotated<1>(x));
+}
+
+// How a lane's values meet those that they turn with
+enum { kWhole1 = 1, kWhole2 = 2, kHalf = 0, kRead = -1, kSingle = -2 };
+// kWholeN: half the rotated part is N groups, kHalf: half a group; kRead: whole fours,
+// read; kSingle: one value at a time (any address, any even rot)
+
+template <int HD, int MODE> struct Angles {
+    static constexpr int kN = MODE > 0 ? MODE : MODE == kHalf ? 1 : HD / kGroup;   // tables' fours a lane
+    float c[kN][4], s[kN][4];
+
+    __device__ __forceinline__ void load(const AppendArgs &a, int64_t pos, int d0)
+    {
+        if constexpr (MODE == kSingle) return;
+        const float *ct = a.cos_t + pos * a.rot, *st = a.sin_t + pos * a.rot;
+        const int half = a.rot / 2;
+#pragma unroll
+        for (int g = 0; g < kN; g++) {
+            int d = g * kGroup + d0;
+            if (MODE == kHalf) d &= 31;
+            if (MODE == kRead) d = d >= a.rot ? 0 : d < half ? d : d - half;
+            load4<float, float, true>(ct + d, c[g]);
+            load4<float, float, true>(st + d, s[g]);
+        }
+    }
+};
+
+// A lane's values of a row, [group][4] from d0 on, normed and turned
+template <typename T, typename A, int HD, int MODE>
 __device__ __forceinline__ void turned(const AppendArgs &a, const T *x, const float *w, int64_t pos,
-                                       int d0, A (&y)[HD / kGroup][4])
+                                       int d0, const Angles<HD, MODE> &t, A (&y)[HD / kGroup][4])
 {
     constexpr int G = HD / kGroup;
+    constexpr bool kVec = MODE != kSingle;
 #pragma unroll
-    for (int g = 0; g < G; g++) load4<T, A, VEC>(x + g * kGroup + d0, y[g]);
+    for (int g = 0; g < G; g++) load4<T, A, kVec>(x + g * kGroup + d0, y[g]);
     A r = (A)1;
     if (a.norm) {
         A s = (A)0;
@@ -69,159 +118,208 @@ __device__ __forceinline__ void turned(const AppendArgs &a, const T *x, const fl
         for (int g = 0; g < G; g++)
 #pragma unroll
             for (int i = 0; i < 4; i++) s += y[g][i] * y[g][i];
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, kLanes);
+        s = over_row(s, [](A p, A q) { return p + q; });
         r = (A)1 / sqrt(s / (A)HD + (A)a.eps);
     }
     const bool scaled = a.norm && w;
-    const int half = a.rot / 2;
-    const float *ct = a.cos_t + pos * a.rot, *st = a.sin_t + pos * a.rot;
 #pragma unroll
     for (int g = 0; g < G; g++) {
-        const int d = g * kGroup + d0;
-        A wt[4] = {r, r, r, r};
         if (scaled) {
-            load4<float, A, VEC>(w + d, wt);
+            A wt[4];
+            load4<float, A, kVec>(w + g * kGroup + d0, wt);
 #pragma unroll
-            for (int i = 0; i < 4; i++) wt[i] *= r;
+            for (int i = 0; i < 4; i++) y[g][i] *= wt[i];
         }
+        if (a.norm)
 #pragma unroll
-        for (int i = 0; i < 4; i++) y[g][i] *= wt[i];
-        if constexpr (VEC) {
-            if (d >= a.rot) continue;
-            const int at = d < half ? d : d - half, from = d < half ? d + half : d - half;
-            A c[4], s[4], other[4], ow[4] = {r, r, r, r};
-            load4<float, A, true>(ct + at, c);
-            load4<float, A, true>(st + at, s);
-            load4<T, A, true>(x + from, other);
-            if (scaled) {
-                load4<float, A, true>(w + from, ow);
+            for (int i = 0; i < 4; i++) y[g][i] *= r;
+    }
+    if constexpr (MODE > 0) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) ow[i] *= r;
-            }
+        for (int g = 0; g < MODE; g++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const A o = other[i] * ow[i];
-                y[g][i] = d < half ? y[g][i] * c[i] - o * s[i] : y[g][i] * c[i] + o * s[i];
+                const A lo = y[g][i], hi = y[g + MODE][i], c = (A)t.c[g][i], s = (A)t.s[g][i];
+                y[g][i] = lo * c - hi * s;
+                y[g + MODE][i] = hi * c + lo * s;
             }
-        } else {
+    } else if constexpr (MODE == kHalf) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int e = d + i;
-                if (e >= a.rot) continue;
-                const int at = e < half ? e : e - half, from = e < half ? e + half : e - half;
-                const A o = (A)(float)x[from] * (scaled ? r * (A)w[from] : r);
-                const A cs = (A)ct[at], sn = (A)st[at];
-                y[g][i] = e < half ? y[g][i] * cs - o * sn : y[g][i] * cs + o * sn;
+        for (int i = 0; i < 4; i++) {
+            const A mine = y[0][i], o = rotated<8>(mine), c = (A)t.c[0][i], s = (A)t.s[0][i];
+            y[0][i] = d0 < 32 ? mine * c - o * s : mine * c + o * s;
+        }
+    } else {
+        const int half = a.rot / 2;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const int d = g * kGroup + d0;
+            if constexpr (MODE == kRead) {
+                if (d >= a.rot) continue;
+                const int from = d < half ? d + half : d - half;
+                A other[4], ow[4] = {1, 1, 1, 1};
+                load4<T, A, true>(x + from, other);
+                if (scaled) load4<float, A, true>(w + from, ow);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const A o = other[i] * ow[i] * r, c = (A)t.c[g][i], s = (A)t.s[g][i];
+                    y[g][i] = d < half ? y[g][i] * c - o * s : y[g][i] * c + o * s;
+                }
+            } else {
+                const float *ct = a.cos_t + pos * a.rot, *st = a.sin_t + pos * a.rot;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int e = d + i;
+                    if (e >= a.rot) continue;
+                    const int at = e < half ? e : e - half, from = e < half ? e + half : e - half;
+                    const A o = (A)(float)x[from] * (scaled ? (A)w[from] : (A)1) * r;
+                    const A c = (A)ct[at], s = (A)st[at];
+                    y[g][i] = e < half ? y[g][i] * c - o * s : y[g][i] * c + o * s;
+                }
             }
         }
     }
 }
 
-// A group's pair and this lane's four codes of it
-__device__ __forceinline__ void quantise(const double (&y)[4], uint32_t &pair, uint32_t &codes)
+// A group's pair and this lane's four codes of it.  A: the type that holds y exactly.
+template <typename A> __device__ __forceinline__ void quantise(const A (&y)[4], uint32_t &pair, uint32_t &codes)
 {
-    double top = y[0], low = y[0], odd = 0;
+    A top = y[0], low = y[0], odd = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         top = fmax(top, y[i]);
         low = fmin(low, y[i]);
         odd += y[i] - y[i];                 // NaN once a value is not finite
     }
-#pragma unroll
-    for (int o = 1; o < kLanes; o <<= 1) {
-        top = fmax(top, __shfl_xor(top, o));
-        low = fmin(low, __shfl_xor(low, o));
-        odd += __shfl_xor(odd, o);
-    }
-    const __bf16 mb = (__bf16)(float)((top + low) / 2);
+    // the sixteen lanes' answers stand side by side in the wave's
+    const uint64_t bad = __ballot(!(odd == 0));
+    const bool sound = !(bad >> (threadIdx.x & 48) & 0xffff);
+    const double high = (double)over_row(top, [](A p, A q) { return fmax(p, q); }),
+                 deep = (double)over_row(low, [](A p, A q) { return fmin(p, q); });
+    const __bf16 mb = (__bf16)(float)((high + deep) / 2);
     const double m = (double)(float)mb;
-    const __bf16 sb = (__bf16)(float)(fmax(top - m, m - low) / 7.5);
-    const double s = (double)(float)sb;
+    // a 15th: its last place is 2^-29 of the number it is rounded to first
+    const float range = (float)(fmax(high - m, m - deep) * (1 / 7.5));
+    const __bf16 sb = (__bf16)range;
+    const float s = (float)sb;
     const uint32_t mid = __builtin_bit_cast(uint16_t, mb), scale = __builtin_bit_cast(uint16_t, sb);
     codes = 0x8888u;
-    if (!(odd == 0) || (mid & 0x7f80) == 0x7f80 || (scale & 0x7f80) == 0x7f80) {
-        pair = 0x7fc00000u;
-        return;
-    }
+    pair = 0x7fc00000u;
+    if (!sound || (mid & 0x7f80) == 0x7f80 || (scale & 0x7f80) == 0x7f80) return;
     pair = scale | mid << 16;
     if (!(s > 0)) return;
-    const double inv = 1 / s;
+    const double step = (double)s;
+    const double inv = ldexp((double)__builtin_amdgcn_rcpf(__builtin_amdgcn_frexp_mantf(s)), -__builtin_amdgcn_frexp_expf(s));
     codes = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const double d = y[i] - m;
-        double n = floor(d * inv);
-        const double left = fma(-n, s, d);  // exact: n has four bits, s eight
-        n += left < 0 ? -1 : left >= s ? 1 : 0;
-        const int c = (int)fmin(fmax(n, -8.0), 7.0) + 8;
-        codes |= (uint32_t)c << (4 * i);
+        const double d = (double)y[i] - m;
+        const float n = floorf((float)(d * inv));           // off by one at most
+        const double left = fma(-(double)n, step, d);       // exact: n has four bits, s eight
+        const int c = (int)n + 8 + (left < 0 ? -1 : left >= step ? 1 : 0);
+        codes |= (uint32_t)min(max(c, 0), 15) << (4 * i);
     }
 }
 
-template <typename T, int HD, bool VEC>
+template <typename T, int HD, int MODE, int R>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a)
 {
     constexpr int G = HD / kGroup;
+    constexpr bool kVec = MODE != kSingle;
     const uint32_t block = cbq_block(blockIdx.x, blockIdx.y);
     const int kind = block >= a.first[2] ? 2 : block >= a.first[1] ? 1 : 0;
-    const int64_t row = (int64_t)(block - a.first[kind]) * kRows + threadIdx.x / kLanes;
-    if (row >= a.rows[kind]) return;        // whole rows: no lane waits on a left one
-    const uint32_t t = cbq_div((uint32_t)row, a.heads[kind]), j = (uint32_t)row - t * a.heads[kind].d;
+    const int64_t unit = (int64_t)(block - a.first[kind]) * kRows + threadIdx.x / kLanes;
+    if (unit >= a.units[kind]) return;      // whole rows: no lane waits on a left one
+    const uint32_t t = cbq_div((uint32_t)unit, a.heads[kind]), j = ((uint32_t)unit - t * a.heads[kind].d) * R;
     const int lane = threadIdx.x % kLanes, d0 = 4 * lane;
-    const T *x = (const T *)a.x[kind] + t * a.st[kind][0] + j * a.st[kind][1];
+    const int64_t st = a.st[kind][1];
+    const T *x = (const T *)a.x[kind] + t * a.st[kind][0] + j * st;
     const int64_t p = a.positions[t];
     const bool placed = p >= 0 && p < a.n_pos;
+    Angles<HD, MODE> angles;
+    if (kind < 2) angles.load(a, placed ? p : 0, d0);
     if (kind == 0) {
-        float y[G][4];
-        turned<T, float, HD, VEC>(a, x, a.w[0], placed ? p : 0, d0, y);
-        T *out = (T *)a.q_out + row * HD + d0;
+        T *out = (T *)a.q_out + ((int64_t)t * a.n_q + j) * HD + d0;
 #pragma unroll
-        for (int g = 0; g < G; g++) {
-            Pack<T, 4> o;
+        for (int h = 0; h < R; h++) {
+            float y[G][4];
+            turned<T, float, HD, MODE>(a, x + h * st, a.w[0], placed ? p : 0, d0, angles, y);
 #pragma unroll
-            for (int e = 0; e < 4; e++) o.e[e] = (T)y[g][e];
-            *(Pack<T, 4> *)(out + g * kGroup) = o;
+            for (int g = 0; g < G; g++) {
+                Pack<T, 4> o;
+#pragma unroll
+                for (int e = 0; e < 4; e++) o.e[e] = (T)y[g][e];
+                *(Pack<T, 4> *)(out + h * HD + g * kGroup) = o;
+            }
         }
         return;
     }
     const int64_t slot = a.slots[t];
     if (!placed || slot < 0 || slot >= a.n_slots) return;       // uniform over the row's lanes
-    double y[G][4];
-    if (kind == 1) {
-        turned<T, double, HD, VEC>(a, x, a.w[1], p, d0, y);
-    } else {
-#pragma unroll
-        for (int g = 0; g < G; g++) load4<T, double, VEC>(x + g * kGroup + d0, y[g]);
-    }
-    Pack<uint16_t, G> codes;
-    uint32_t pair[G];
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        uint32_t c;
-        quantise(y[g], pair[g], c);
-        codes.e[g] = (uint16_t)c;
-    }
     const uint32_t id = cbq_div((uint32_t)slot, a.pool.page), r = (uint32_t)slot - id * a.pool.page.d;
-    const uint32_t at = code_at(a.pool, id, r) + j * a.pool.code_st[1];
-    *(Pack<uint16_t, G> *)(a.pool.codes[kind - 1] + (uint64_t)at * kCodeUnit + lane * 2 * G) = codes;
-    uint32_t *to = a.pool.pairs[kind - 1] + (uint64_t)(pair_at(a.pool, id, r) + j * a.pool.pair_st[1]);
 #pragma unroll
-    for (int g = 0; g < G; g++)
-        if (lane == g) to[g] = pair[g];
+    for (int h = 0; h < R; h++) {
+        Pack<uint16_t, G> codes;
+        uint32_t pair[G], c;
+        if (kind == 1) {
+            double y[G][4];
+            turned<T, double, HD, MODE>(a, x + h * st, a.w[1], p, d0, angles, y);
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                quantise(y[g], pair[g], c);
+                codes.e[g] = (uint16_t)c;
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                float y[4];
+                load4<T, float, kVec>(x + h * st + g * kGroup + d0, y);
+                quantise(y, pair[g], c);
+                codes.e[g] = (uint16_t)c;
+            }
+        }
+        const uint32_t at = code_at(a.pool, id, r) + (j + h) * a.pool.code_st[1];
+        *(Pack<uint16_t, G> *)(a.pool.codes[kind - 1] + (uint64_t)at * kCodeUnit + lane * 2 * G) = codes;
+        uint32_t *to = a.pool.pairs[kind - 1] + (uint64_t)(pair_at(a.pool, id, r) + (j + h) * a.pool.pair_st[1]);
+#pragma unroll
+        for (int g = 0; g < G; g++)
+            if (lane == g) to[g] = pair[g];
+    }
+}
+
+template <typename T, int HD, int MODE, int R> int launch_units(AppendArgs &a, hipStream_t stream)
+{
+    int64_t blocks = 0;
+    for (int i = 0; i < 3; i++) {
+        const int n = (i == 0 ? a.n_q : a.n_kv) / R;
+        a.heads[i] = cbq_div_make((uint32_t)n);
+        a.units[i] = a.N * n;
+        a.first[i] = (uint32_t)blocks;
+        blocks += cbq_ceil(a.units[i], kRows);
+    }
+    const CbqGrid grid = cbq_grid(blocks);
+    append_kernel<T, HD, MODE, R><<<dim3(grid.x, grid.y), kThreads, 0, stream>>>(a);
+    return cbq_launch_status("cbq_paged_append_q4");
+}
+
+template <typename T, int HD, int MODE> int launch_mode(AppendArgs &a, hipStream_t stream)
+{
+    if constexpr (MODE != kSingle) {
+        const bool four = a.n_q % 4 == 0 && a.n_kv % 4 == 0 && a.N * (a.n_q + 2ll * a.n_kv) * kLanes / 4 >= kFourThreads;
+        if (four) return launch_units<T, HD, MODE, 4>(a, stream);
+    }
+    return launch_units<T, HD, MODE, 1>(a, stream);
 }
 
 template <typename T, int HD> int launch_append(AppendArgs &a, bool vec, hipStream_t stream)
 {
-    int64_t blocks = 0;
-    for (int i = 0; i < 3; i++) {
-        a.first[i] = (uint32_t)blocks;
-        blocks += cbq_ceil(a.rows[i], kRows);
-    }
-    const CbqGrid grid = cbq_grid(blocks);
-    if (vec) append_kernel<T, HD, true><<<dim3(grid.x, grid.y), kThreads, 0, stream>>>(a);
-    else append_kernel<T, HD, false><<<dim3(grid.x, grid.y), kThreads, 0, stream>>>(a);
-    return cbq_launch_status("cbq_paged_append_q4");
+    if (!vec) return launch_mode<T, HD, kSingle>(a, stream);
+    if (a.rot == 64) return launch_mode<T, HD, kHalf>(a, stream);
+    if constexpr (HD >= 128)
+        if (a.rot == 128) return launch_mode<T, HD, kWhole1>(a, stream);
+    if constexpr (HD == 256)
+        if (a.rot == 256) return launch_mode<T, HD, kWhole2>(a, stream);
+    return launch_mode<T, HD, kRead>(a, stream);
 }
 
 template <typename T> int launch_append_hd(AppendArgs &a, int hd, bool vec, hipStream_t stream)
@@ -314,15 +412,13 @@ extern "C" int cbq_paged_append_q4(const void *q, const void *k, const void *v, 
         a.st[i][0] = st[i][0];
         a.st[i][1] = st[i][1];
         vec = vec && (uintptr_t)x[i] % (4 * e) == 0 && st[i][0] % 4 == 0 && st[i][1] % 4 == 0;
-        const int n = i == 0 ? n_q : cache->n_kv;
-        a.heads[i] = cbq_div_make((uint32_t)n);
-        a.rows[i] = N * n;
     }
     a.cos_t = cos_table; a.sin_t = sin_table; a.w[0] = q_weight; a.w[1] = k_weight;
     a.positions = positions; a.slots = slots; a.q_out = q_out;
     a.pool = make_pool(*cache);
     a.n_pos = n_pos;
     a.n_slots = cache->n_pages * cache->page;
+    a.N = N; a.n_q = n_q; a.n_kv = cache->n_kv;
     a.rot = rot; a.norm = norm; a.eps = eps;
     if (x_dtype == CBQ_F32) return launch_append_hd<float>(a, cache->hd, vec, stream);
     if (x_dtype == CBQ_BF16) return launch_append_hd<__bf16>(a, cache->hd, vec, stream);

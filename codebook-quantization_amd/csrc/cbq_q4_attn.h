@@ -4,13 +4,20 @@
 //
 // out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - max), in one pass over the
 // keys with a running maximum.  With k_jd = m + s (c - 7.5) in a group g of 64 values,
-//   q.k_j = sum_g s_jg A_jg + (m_jg - 23.5 s_jg) Q_g,   A_jg = sum_d q_d (c_jd + 16),
-//   sum_j p_j v_jd = B_d - 23.5 C_g + sum_j p_j m_jg,   B_d = sum_j (p_j s_jg) (c_jd + 16),
-// Q_g the group's sum of q and C_g that of p_j s_jg: the codes go to the matrix cores
-// as they are.  c + 16 is one bf16 number, the code in its mantissa's upper bits under
-// a constant exponent: a shift and a masked or make two of them.  No value is
-// rounded on the way; q and p_j s_jg are cut into as many bf16 parts as their type
-// has bits for (bf16: one, fp16: two, fp32: three), and C_g sums the same parts.
+//   q.k_j = sum_g s_jg A_jg + (m_jg - 7.5 s_jg) Q_g,        A_jg = sum_d q_d c_jd,
+//   sum_j p_j v_jd = B_d - 7.5 C_g + sum_j p_j m_jg,         B_d = sum_j (p_j s_jg) c_jd,
+// Q_g the group's sum of q and C_g that of p_j s_jg: the codes go to the matrix cores as
+// they are, and no dequantised value is rounded.  A code needs no conversion: the bits
+// 0..15 of an fp16 number are the subnormals c 2^-24, and 16 c 2^-24 where the code
+// lies in a byte's upper half, which the products take exactly.  So two codes cost a mask
+// (and half a shift or a byte permute); as bf16 numbers c + 16 under a constant
+// exponent they cost three operations, and 24 sequences of 4000 to 32000 keys 155 us.
+//
+// The other operands have to fit fp16.  A query row is scaled to a largest value in
+// [2^14, 2^15), fp32 cut into two parts.  p_j s_jg is taken against 2^E, E the largest
+// exponent of the scales of the values that the wave has met: its 11 bits (two parts
+// of fp32: 22) hold down to 2^-26 of the largest scale, below that it loses them one by
+// one.
 //
 // Rows are the query heads of a kv head beside the tokens, 16 a tile: row r of a
 // sequence is token r / rep, head r % rep.  Of a prefix the rows are the whole
@@ -18,12 +25,16 @@
 //
 // Products, with the keys in the left operand: S^T = K Q^T (16 keys x 16 rows) leaves
 // a lane with one row and four keys; two such tiles are the right operand of O^T =
-// V^T P^T, so weights never leave their lane.  A lane's eight keys there are eight
-// neighbouring ones, and the codes' order in a row (four of each group side by side)
-// gives it of each key one word, whose nibble n belongs to output tile n: no
-// transpose, no LDS for the codes.
+// V^T P^T, so weights never leave their lane.  The codes' order in a row (four of each
+// group side by side) gives a lane there of each of its eight keys one word, whose
+// nibble n belongs to output tile n: no transpose.
+//
+// A wave walks tiles of 32 keys of its own.  Codes, pairs and page ids go from memory
+// straight to LDS, kDepth - 1 tiles ahead, without registers on the way and without a
+// wait but for the tile that is due.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "cbq_q4.h"
@@ -34,14 +45,23 @@ namespace cbq_q4 {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
+#ifndef Q4D
+#define Q4D 2
+#endif
+#ifndef Q4W
+#define Q4W 3
+#endif
 constexpr int kBlock = kAttnWaves * CBQ_WAVE;
 
 // The running maximum stands this far (in exp2's domain) above the scores of its last
-// move, so that it moves seldom and no weight passes 1: a weight keeps all its bits.
-constexpr float kSlack = 8.0f;
+// move, so that it moves seldom and no weight passes 1.
+constexpr float kSlack = 2.0f;
+
+// p s 2^(kUp - E) < 2^14: fp16 has room for it, and 2^-14 is its smallest whole number
+constexpr int kUp = 14, kNone = -1000;      // kNone: no scale yet
 
 struct AttnArgs {
     const void *q;
@@ -52,14 +72,16 @@ struct AttnArgs {
     void *out;
     float *part_o;                          // [part][token][n_q][hd]
     float2 *part_ml;                        // [part][token][n_q]: running maximum, sum
-    CbqDiv rep;
+    CbqDiv rep, tiles_a_page;               // of pages of whole tiles
+    uint32_t code_row, pair_row;            // bytes from row to row, of such pages
+    int32_t whole;                          // every tile lies in one page
     int32_t prefix, batch, tokens, n_q, n_kv;
     float c, q_mul;                         // exp2(c * (q_mul q) . k); q_mul folds scale's sign
     float c_low;                            // what c's rounding left, for fp32
     Plan plan;
 };
 
-template <typename T> constexpr int kParts = sizeof(T) == 4 ? 3 : std::is_same_v<T, __bf16> ? 1 : 2;
+template <typename T> constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
 
 // max / sum over the four lanes that hold one row (lane, lane ^ 16, ^ 32, ^ 48)
 __device__ __forceinline__ float groups_max(float x)
@@ -77,113 +99,288 @@ __device__ __forceinline__ float groups_sum(float x)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Nothing is moved over this: operands unpacked or read ahead of their turn cost
+// registers, and with them waves
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
+
+// x, computed in this branch and not before it
+__device__ __forceinline__ uint32_t here(uint32_t x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c)
 {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ uint32_t pack2(float a, float b)
-{
-    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
-}
-
-// x = the sum of N bf16 parts (up to x's own bits); part n is taken off x
+// a and b as N fp16 parts each
 template <int N> __device__ __forceinline__ void cut(float a, float b, uint32_t (&part)[N])
 {
 #pragma unroll
     for (int n = 0; n < N; n++) {
-        part[n] = pack2(a, b);
-        if (n + 1 < N) {
-            a -= __uint_as_float(part[n] << 16);
-            b -= __uint_as_float(part[n] & 0xffff0000u);
-        }
+        const f16x2 x = {(_Float16)a, (_Float16)b};
+        part[n] = __builtin_bit_cast(uint32_t, x);
+        a -= (float)x[0];
+        b -= (float)x[1];
     }
 }
 
-// Two codes, at bits 3..6 of either half, as the bf16 numbers c + 16
-__device__ __forceinline__ uint32_t code_pair(uint32_t x) { return (x & 0x00780078u) | 0x41804180u; }
+// Two codes of a word: c 2^-24, or 16 c 2^-24 (upper halves of bytes), as fp16 numbers
+constexpr uint32_t kLower = 0x000f000fu, kUpper = 0x00f000f0u;
 
-// Eight codes (low nibble first) as c + 16, in the order 0 4 1 5 2 6 3 7
+// Eight codes (low nibble first) in the order 0 4 1 5 2 6 3 7, odd ones 16 times as large
 __device__ __forceinline__ u32x4 eight_codes(uint32_t w)
 {
-    return u32x4{code_pair(w << 3), code_pair(w >> 1), code_pair(w >> 5), code_pair(w >> 9)};
+    return u32x4{w & kLower, w & kUpper, w >> 8 & kLower, w >> 8 & kUpper};
 }
 
 template <int HD> struct Geo {
     static constexpr int kG = HD / kGroup;              // groups of a row
-    static constexpr int kKw = HD / 32;                 // words of codes of a key a lane holds
-    static constexpr int kPairs = (kG + 1) / 2;         // pairs a lane loads, of keys and of values
-    static constexpr int kScales = 4 * kG * kTile;      // floats of a wave's tile in LDS
+    static constexpr int kRow = HD / 2, kPieces = HD / 32;      // bytes of a row's codes, 16 of them a piece
+    static constexpr int kRows = CBQ_WAVE / kPieces;    // rows that a copy takes
+    static constexpr int kCopies = kTile / kRows;       // copies of a tile's keys (and values)
+    static constexpr int kPairCopies = (kG + 1) / 2;    // of their pairs: 64 a copy
+    static constexpr int kOps = 2 * kCopies + 2 * kPairCopies + 1;      // of a tile, its ids among them
+    // a wave's LDS: a ring of tiles, one of page ids, scales and mids of the tile at hand
+    static constexpr int kDepth = HD == 256 ? 3 : Q4D;
+    static constexpr int kCodes = kTile * kRow, kPairs = kPairCopies * 256;
+    static constexpr int kSlot = 2 * kCodes + 2 * kPairs;
+    static constexpr int kIds = kDepth * kSlot, kScales = kIds + kDepth * 256;
+    static constexpr int kWave = kScales + 4 * kG * kTile * 4;
     static constexpr int kWide = HD < 128 ? HD : 128;   // values of a row joined at once
+    // Piece p of row r lies at p ^ mix(r): the pieces that sixteen rows are read at
+    // together fall on 64 different banks.
+    static __device__ __forceinline__ int mix(int row) { return row / (512 / HD) & (kPieces - 1); }
 };
 
-// The codes of one tile, in registers: of two keys for S^T and eight values for O^T
-template <int HD> struct Codes {
-    using G = Geo<HD>;
-    uint32_t k[2][G::kKw];                  // HD / 8 bytes of a key: a quarter of its row
-    uint32_t v[8][HD == 256 ? 2 : 1];       // HD / 32 bytes of a value: four codes a group
-    uint32_t kp[G::kPairs], vp[G::kPairs];  // pairs: of key lane % 32, group lane / 32 (+ 2)
-    uint32_t there;                         // keys of the tile that are there
+// ---- tiles on their way to LDS ------------------------------------------------------------------
+// Written as asm, so that the compiler neither waits for a copy before an LDS read nor
+// counts it: arrived() does.  A copy takes 16 (4) bytes a lane to its place in the
+// wave's next 1024 (256) bytes at `lds`; M0 holds that address, with a wait state between
+// its write and the load.  The LDS reads before it are done.
+__device__ __forceinline__ void copy16(uint32_t lds, const char *base, uint32_t offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(lds), "v"(offset), "s"(base) : "m0", "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t lds, const char *from)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :: "s"(lds), "v"(from) : "m0", "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t lds, const char *base, uint32_t offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                 :: "s"(lds), "v"(offset), "s"(base) : "m0", "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t lds, const char *from)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_waitcnt lgkmcnt(0)\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                 :: "s"(lds), "v"(from) : "m0", "memory");
+}
+// All but the last N of this wave's copies have arrived
+template <int N> __device__ __forceinline__ void arrived()
+{
+    static_assert(N >= 0 && N < 64, "a six-bit counter");
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
 
-    __device__ __forceinline__ void load(const AttnArgs &a, int h, int32_t id, uint32_t row)
+// A wave's tiles `first`, `first` + kAttnWaves, .. below `end`, numbered 0, 1, ..
+template <int HD> struct Tiles {
+    using G = Geo<HD>;
+    const AttnArgs &a;
+    const int32_t *own;
+    int32_t pre_tiles, length, first, end, h;
+    char *lds;                              // this wave's
+    uint32_t at;                            // its address
+    uint32_t there[G::kDepth - 1];          // of the tiles on their way, in turn: keys that are there
+
+    __device__ __forceinline__ int32_t tile(int n) const { return first + n * kAttnWaves; }
+    // Place of the tile's key `key` in its table's order; the last one's past their end
+    __device__ __forceinline__ int32_t place(int32_t tile, int key, bool &in) const
     {
-        const int lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
-        // an id outside the pool (or no key) reads page 0, row 0 and is hidden
-        const bool in = id >= 0 && id < a.pool.n_pages;
-        there = (uint32_t)__ballot(in);
-        const uint32_t p = in ? id : 0, at = in ? row : 0;
-        const uint32_t co = code_at(a.pool, p, at) + h * a.pool.code_st[1];
-        const uint64_t po = pair_at(a.pool, p, at) + h * a.pool.pair_st[1];
-#pragma unroll
-        for (int i = 0; i < G::kPairs; i++) {
-            const int g = G::kG == 1 ? 0 : (lane >> 5) + 2 * i;
-            kp[i] = a.pool.pairs[0][po + g];
-            vp[i] = a.pool.pairs[1][po + g];
-        }
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const uint64_t o = (uint64_t)__shfl(co, 8 * (r >> 2) + (r & 3) + 4 * t) * kCodeUnit;
-            const char *from = a.pool.codes[0] + o + g4 * (HD / 8);
-            if constexpr (HD == 64) *(u32x2 *)k[t] = *(const u32x2 *)from;
-            else
-#pragma unroll
-                for (int i = 0; i < G::kKw / 4; i++)
-                    *(u32x4 *)(k[t] + 4 * i) = *(const u32x4 *)(from + 16 * i);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint64_t o = (uint64_t)__shfl(co, 8 * g4 + i) * kCodeUnit;
-            const char *from = a.pool.codes[1] + o + r * (HD / 32);
-            if constexpr (HD == 64) v[i][0] = *(const uint16_t *)from;
-            else if constexpr (HD == 128) v[i][0] = *(const uint32_t *)from;
-            else *(u32x2 *)v[i] = *(const u32x2 *)from;
-        }
+        const bool shared = tile < pre_tiles;
+        const int32_t j = (shared ? tile : tile - pre_tiles) * kTile + key, n = shared ? a.prefix : length;
+        in = j < n;
+        return in ? j : n - 1;
     }
-    // The tile's pairs as floats: scales and mids - 23.5 scales of the keys, scales and
-    // mids of the values, each [group][key]; 0 for a key that is not there.
-    __device__ __forceinline__ void spread(float *lds) const
+    // Page ids of tile n's keys (of one that is there, where n is past the end)
+    __device__ __forceinline__ void ask_ids(int n) const
+    {
+        bool in;
+        const int32_t t = tile(n) < end ? tile(n) : tile(0);
+        const int32_t j = place(t, threadIdx.x & 31, in);
+        const char *table = (const char *)(t < pre_tiles ? a.prefix_table : own);
+        copy4(at + G::kIds + n % G::kDepth * 256, table, 4 * cbq_div((uint32_t)j, a.pool.page));
+    }
+    // Tile n into slot n % kDepth, its ids there; and the ids of tile n + kDepth - 1.
+    // What is not there is read from page 0, row 0.  Returns the keys that are.
+    __device__ __forceinline__ uint32_t ask(int n) const
+    {
+        uint32_t in_pool;
+        const int lane = threadIdx.x & 63;
+        const int32_t t = tile(n);
+        const int32_t *ids = (const int32_t *)(lds + G::kIds + n % G::kDepth * 256);
+        const uint32_t to = at + n % G::kDepth * G::kSlot;
+        const char *kc = a.pool.codes[0], *vc = a.pool.codes[1];
+        const char *kp = (const char *)a.pool.pairs[0], *vp = (const char *)a.pool.pairs[1];
+        const int sub = lane / G::kPieces, piece = lane % G::kPieces;
+        if (a.whole) {                      // the tile lies in one page
+            bool in;
+            const uint32_t j = (t < pre_tiles ? t : t - pre_tiles), left = (t < pre_tiles ? a.prefix : length) - j * kTile;
+            const int32_t id = __builtin_amdgcn_readfirstlane(ids[0]);
+            in = id >= 0 && id < a.pool.n_pages;
+            const uint32_t page = in ? id : 0, row = (j - cbq_div(j, a.tiles_a_page) * a.tiles_a_page.d) * kTile;
+            const uint64_t co = (uint64_t)(code_at(a.pool, page, row) + h * a.pool.code_st[1]) * kCodeUnit,
+                           po = (uint64_t)(pair_at(a.pool, page, row) + h * a.pool.pair_st[1]) * kPairUnit;
+            in_pool = !in ? 0 : left >= kTile ? ~0u : (1u << left) - 1;
+#pragma unroll
+            for (int i = 0; i < G::kPairCopies; i++) {
+                const uint32_t o = (lane & 31) * a.pair_row + (G::kG == 1 ? 0 : (lane >> 5) + 2 * i) * kPairUnit;
+                copy4(to + 2 * G::kCodes + i * 256, kp + po, o);
+                copy4(to + 2 * G::kCodes + G::kPairs + i * 256, vp + po, o);
+            }
+#pragma unroll
+            for (int i = 0; i < G::kCopies; i++) {
+                const int r = i * G::kRows + sub;
+                const uint32_t o = r * a.code_row + (piece ^ G::mix(r)) * 16;
+                copy16(to + i * 1024, kc + co, o);
+                copy16(to + G::kCodes + i * 1024, vc + co, o);
+            }
+        } else {
+            auto row_of = [&](int key, uint32_t &page, uint32_t &row) {
+                bool in;
+                const uint32_t j = (uint32_t)place(t, key, in);
+                const int32_t id = ids[key];
+                in = in && id >= 0 && id < a.pool.n_pages;
+                page = in ? id : 0;
+                row = in ? j - cbq_div(j, a.pool.page) * a.pool.page.d : 0;
+                return in;
+            };
+            uint32_t page, row;
+            in_pool = (uint32_t)__ballot(row_of(lane & 31, page, row));
+            const uint64_t po = (uint64_t)(pair_at(a.pool, page, row) + h * a.pool.pair_st[1]) * kPairUnit;
+#pragma unroll
+            for (int i = 0; i < G::kPairCopies; i++) {
+                const uint64_t o = po + (G::kG == 1 ? 0 : (lane >> 5) + 2 * i) * kPairUnit;
+                copy4(to + 2 * G::kCodes + i * 256, kp + o);
+                copy4(to + 2 * G::kCodes + G::kPairs + i * 256, vp + o);
+            }
+#pragma unroll
+            for (int i = 0; i < G::kCopies; i++) {
+                const int r = i * G::kRows + sub;
+                row_of(r, page, row);
+                const uint64_t o = (uint64_t)(code_at(a.pool, page, row) + h * a.pool.code_st[1]) * kCodeUnit +
+                                   (piece ^ G::mix(r)) * 16;
+                copy16(to + i * 1024, kc + o);
+                copy16(to + G::kCodes + i * 1024, vc + o);
+            }
+        }
+        ask_ids(n + G::kDepth - 1);
+        return in_pool;
+    }
+    __device__ __forceinline__ void begin()
+    {
+        at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+        at = __builtin_amdgcn_readfirstlane(at);
+        if (tile(0) >= end) return;
+#pragma unroll
+        for (int n = 0; n < G::kDepth - 1; n++) ask_ids(n);
+        arrived<0>();
+#pragma unroll
+        for (int n = 0; n < G::kDepth - 1; n++)
+            there[n] = tile(n) < end ? ask(n) : 0;
+    }
+    // Tile n has arrived, and the tile behind those under way is asked for: the keys of n
+    // that are there.
+    __device__ __forceinline__ uint32_t next(int n)
+    {
+        const uint32_t now = there[0];
+#pragma unroll
+        for (int i = 0; i + 2 < G::kDepth; i++) there[i] = there[i + 1];
+        if (tile(n + G::kDepth - 2) < end) arrived<(G::kDepth - 2) * G::kOps>();
+        else arrived<0>();
+        if (tile(n + G::kDepth - 1) < end) there[G::kDepth - 2] = ask(n + G::kDepth - 1);
+        return now;
+    }
+};
+
+// A tile in LDS.  Key 16 t + 4 i + g of it is number 4 t + i of lane group g (lane / 16):
+// four neighbouring rows a read.
+template <int HD> struct Slot {
+    using G = Geo<HD>;
+    const char *lds;
+
+    // The pairs of key lane % 32, group lane / 32 + 2 i, of keys (0) and values (1)
+    __device__ __forceinline__ uint32_t pair(int which, int i) const
+    {
+        return *(const uint32_t *)(lds + 2 * G::kCodes + which * G::kPairs + i * 256 + (threadIdx.x & 63) * 4);
+    }
+    // The largest exponent of the lane's value scales; kNone where none counts
+    __device__ __forceinline__ int exponent(uint32_t there) const
+    {
+        const bool in = there >> (threadIdx.x & 31) & 1;
+        int e = kNone;
+#pragma unroll
+        for (int i = 0; i < G::kPairCopies; i++) {
+            const float s = pair_scale(pair(1, i));
+            if (in && s > 0.f && s < INFINITY) e = max(e, __builtin_amdgcn_frexp_expf(s));
+        }
+        return e;
+    }
+    // The tile's pairs as floats: scales and mids - 7.5 scales of the keys, scales (times
+    // 2^(kUp - E)) and mids of the values, each [group][lane group][eight keys]; 0 for a
+    // key that is not there.
+    __device__ __forceinline__ void spread(float *to, uint32_t there, int E) const
     {
         const int lane = threadIdx.x & 63, key = lane & 31;
         const bool in = there >> key & 1;
         if (G::kG == 1 && lane >= 32) return;
+        to += (lane >> 5) * kTile + (key & 3) * 8 + (key >> 2);
 #pragma unroll
-        for (int i = 0; i < G::kPairs; i++) {
-            float *to = lds + ((lane >> 5) + 2 * i) * kTile + key;
-            const float s = pair_scale(kp[i]), m = pair_mid(kp[i]);
-            to[0] = in ? s : 0.f;
-            to[G::kG * kTile] = in ? fmaf(-23.5f, s, m) : 0.f;
-            to[2 * G::kG * kTile] = in ? pair_scale(vp[i]) : 0.f;
-            to[3 * G::kG * kTile] = in ? pair_mid(vp[i]) : 0.f;
+        for (int i = 0; i < G::kPairCopies; i++) {
+            const uint32_t k = pair(0, i), v = pair(1, i);
+            const float s = pair_scale(k), m = pair_mid(k);
+            float vs = pair_scale(v), vm = pair_mid(v);
+            // a scale that is not finite makes the mid so: p = 0 keeps it out by the mid alone
+            if (!(vs >= 0.f && vs < INFINITY)) vs = 0.f, vm = __builtin_nanf("");
+            to[2 * i * kTile] = in ? s : 0.f;
+            to[(G::kG + 2 * i) * kTile] = in ? fmaf(-7.5f, s, m) : 0.f;
+            to[(2 * G::kG + 2 * i) * kTile] = in ? __builtin_amdgcn_ldexpf(vs, kUp - E) : 0.f;
+            to[(3 * G::kG + 2 * i) * kTile] = in ? vm : 0.f;
         }
     }
-    // Eight codes of group g, the lane's half hf, of key tile t
-    __device__ __forceinline__ uint32_t key_codes(int t, int g, int hf) const
+    // This lane's quarter of a key's codes: row lane % 16 of S^T's tile t
+    __device__ __forceinline__ void keys(int t, uint32_t (&k)[HD / 32]) const
     {
-        if constexpr (HD == 64) return k[t][hf];
+        const int x = threadIdx.x & 15, g4 = threadIdx.x >> 4 & 3, row = 16 * t + 4 * (x & 3) + (x >> 2);
+        const char *from = lds + row * G::kRow;
+        if constexpr (HD == 64) *(u32x2 *)k = *(const u32x2 *)(from + ((g4 >> 1) ^ G::mix(row)) * 16 + (g4 & 1) * 8);
+        else
+#pragma unroll
+            for (int i = 0; i < HD / 128; i++)
+                *(u32x4 *)(k + 4 * i) = *(const u32x4 *)(from + ((g4 * (HD / 128) + i) ^ G::mix(row)) * 16);
+    }
+    // Eight codes of group g, the quarter's half hf
+    static __device__ __forceinline__ uint32_t key_codes(const uint32_t (&k)[HD / 32], int g, int hf)
+    {
+        if constexpr (HD == 64) return k[hf];
         const int stride = HD / 128;        // words of four values of every group
-        return __builtin_amdgcn_perm(k[t][(2 * hf + 1) * stride + g / 2], k[t][2 * hf * stride + g / 2],
+        return __builtin_amdgcn_perm(k[(2 * hf + 1) * stride + g / 2], k[2 * hf * stride + g / 2],
                                      g & 1 ? 0x07060302u : 0x05040100u);
+    }
+    // Four codes of each group, 4 (lane % 16) .., of this lane's value number n
+    __device__ __forceinline__ void value(int n, uint32_t (&v)[HD == 256 ? 2 : 1]) const
+    {
+        const int x = threadIdx.x & 15, g4 = threadIdx.x >> 4 & 3, row = 4 * n + g4;
+        constexpr int kEach = HD / 32, kIn = 16 / kEach;        // bytes a lane, lanes a piece
+        const char *from = lds + G::kCodes + row * G::kRow + ((x / kIn) ^ G::mix(row)) * 16 + x % kIn * kEach;
+        if constexpr (HD == 64) v[0] = *(const uint16_t *)from;
+        else if constexpr (HD == 128) v[0] = *(const uint32_t *)from;
+        else *(u32x2 *)v = *(const u32x2 *)from;
     }
 };
 
@@ -191,45 +388,68 @@ template <int HD> struct Codes {
 template <typename T, int HD, int RT> struct Rows {
     using G = Geo<HD>;
     static constexpr int N = kParts<T>;
+    // fp32 takes C off B tile by tile, so that B stays as small as the output: its sums'
+    // roundings count there.
+    static constexpr bool kCentred = N > 1;
     u32x4 q[RT][N][HD / 32];
     float qsum[RT][G::kG];
-    f32x4 o[RT][HD / 16], ps[RT][G::kG];    // B, and C in every element
+    f32x4 o[RT][HD / 16], ps[RT][G::kG];    // B 2^-24 (16 B 2^-24 where odd), and C in every element
     float mids[RT][G::kG];                  // this lane's keys' part of sum p m
     float m[RT], l[RT];                     // running maximum (exp2's domain); this lane's part of sum p
+    float c[RT], c_low[RT];                 // exp2's factors, the row's scaling taken back
+    int E;                                  // p s is times 2^(kUp - E)
 
     // Row `row` of 16 from row0 on (zeros from n on): of query token token0 + row / rep,
     // head h * rep + row % rep.
     __device__ __forceinline__ void start(const AttnArgs &a, int h, int64_t token0, int row0, int n)
     {
         const int lane = threadIdx.x & 63, g4 = lane >> 4;
+        E = kNone;
 #pragma unroll
         for (int t = 0; t < RT; t++) {
             const int row = row0 + 16 * t + (lane & 15);
             const bool in = row < n;
             const uint32_t token = cbq_div(in ? row : 0, a.rep), head = (in ? row : 0) - token * a.rep.d;
             const T *x = (const T *)a.q + (token0 + token) * a.q_st[0] + ((int64_t)h * a.rep.d + head) * a.q_st[1];
+            float f[G::kG][2][8], top = 0.f;
+#pragma unroll
+            for (int g = 0; g < G::kG; g++)
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                    struct alignas(16) Eight { T e[8]; };
+                    const Eight e = *(const Eight *)(x + 64 * g + 16 * g4 + 8 * hf);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        f[g][hf][i] = in ? (float)e.e[i] * a.q_mul : 0.f;
+                        top = fmaxf(top, fabsf(f[g][hf][i]));
+                    }
+                }
+            top = groups_max(top);
+            const int up = 15 - __builtin_amdgcn_frexp_expf(top);       // top 2^up in [2^14, 2^15)
+            // factors that are not 0 (a hidden key's -inf times 0 is none) and finite
+            c[t] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c, 24 - up), 0x1p-149f), 3.0e38f);
+            c_low[t] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c_low, 24 - up), 0x1p-149f), 3.0e38f);
 #pragma unroll
             for (int g = 0; g < G::kG; g++) {
                 float sum = 0.f;
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
-                    struct alignas(16) Eight { T e[8]; };
-                    const Eight e = *(const Eight *)(x + 64 * g + 16 * g4 + 8 * hf);
-                    float f[8];
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        f[i] = in ? (float)e.e[i] * a.q_mul : 0.f;
-                        sum += f[i];
+                        f[g][hf][i] = __builtin_amdgcn_ldexpf(f[g][hf][i], up);
+                        sum += f[g][hf][i];
                     }
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
+                        // the odd codes come 16 times as large
+                        const float less = i & 1 ? 0.0625f : 1.0f;
                         uint32_t part[N];
-                        cut<N>(f[i], f[i + 4], part);
+                        cut<N>(f[g][hf][i] * less, f[g][hf][i + 4] * less, part);
 #pragma unroll
                         for (int p = 0; p < N; p++) q[t][p][2 * g + hf][i] = part[p];
                     }
                 }
-                qsum[t][g] = groups_sum(sum);
+                qsum[t][g] = groups_sum(sum) * 0x1p-24f;
                 ps[t][g] = f32x4{0, 0, 0, 0};
                 mids[t][g] = 0.f;
             }
@@ -240,10 +460,32 @@ template <typename T, int HD, int RT> struct Rows {
         }
     }
 
-    // One tile.  MASKED: bits[t] holds the keys that the lane's row of tile t sees.
-    template <bool MASKED>
-    __device__ __forceinline__ void tile(const AttnArgs &a, const Codes<HD> &c, const float *lds,
-                                         const uint32_t (&bits)[RT])
+    // A tile whose scales' largest exponent is e, over the wave
+    __device__ __forceinline__ void follow(int e)
+    {
+        if (!__ballot(e > E)) return;
+        for (int i = 32; i > 0; i >>= 1) e = max(e, __shfl_xor(e, i));
+        e = __builtin_amdgcn_readfirstlane(e) + 1;          // one bit of room
+        const int down = E == kNone ? 0 : E - e;
+        E = e;
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+#pragma unroll
+            for (int d = 0; d < HD / 16; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[r][d][i] = __builtin_amdgcn_ldexpf(o[r][d][i], down);
+            if (!kCentred)
+#pragma unroll
+                for (int g = 0; g < G::kG; g++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) ps[r][g][i] = __builtin_amdgcn_ldexpf(ps[r][g][i], down);
+        }
+    }
+
+    // One tile.  bits[t] holds the keys that the lane's row of tile t sees; hidden: some row
+    // does not see all.
+    __device__ __forceinline__ void tile(const Slot<HD> &slot, const float *lds, const uint32_t (&bits)[RT],
+                                         bool hidden)
     {
         const int lane = threadIdx.x & 63, g4 = lane >> 4;
         const float *mine = lds + 8 * g4;               // this lane's eight keys
@@ -253,6 +495,9 @@ template <typename T, int HD, int RT> struct Rows {
         f32x4 s[RT][2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
+            phase();
+            uint32_t codes[HD / 32];
+            slot.keys(t, codes);
 #pragma unroll
             for (int g = 0; g < G::kG; g++) {
                 const f32x4 off = four(1, g, t);
@@ -269,7 +514,7 @@ template <typename T, int HD, int RT> struct Rows {
                 for (int r = 0; r < RT; r++) acc[r] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
-                    const u32x4 k = eight_codes(c.key_codes(t, g, hf));
+                    const u32x4 k = eight_codes(slot.key_codes(codes, g, hf));
 #pragma unroll
                     for (int r = 0; r < RT; r++)
 #pragma unroll
@@ -282,18 +527,22 @@ template <typename T, int HD, int RT> struct Rows {
                     for (int i = 0; i < 4; i++) s[r][t][i] = fmaf(scale[i], acc[r][i], s[r][t][i]);
             }
         }
+        phase();
         float p[RT][8];
 #pragma unroll
         for (int r = 0; r < RT; r++) {
-            const uint32_t seen = MASKED ? bits[r] >> (8 * g4) : ~0u;
+            if (hidden) {
+                const uint32_t seen = here(bits[r] >> g4);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    s[r][i / 4][i % 4] = seen >> (4 * i) & 1 ? s[r][i / 4][i % 4] : -INFINITY;
+            }
             float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if (MASKED) s[r][i / 4][i % 4] = seen >> i & 1 ? s[r][i / 4][i % 4] : -INFINITY;
-                top = fmaxf(top, s[r][i / 4][i % 4]);
-            }
-            top = groups_max(top) * a.c;
-            if (__ballot(top > m[r])) {
+            for (int i = 0; i < 8; i++) top = fmaxf(top, s[r][i / 4][i % 4]);
+            // the row's maximum is found where one of its lanes passes it
+            if (__ballot(top * c[r] > m[r])) {
+                top = groups_max(top) * c[r];
                 const float to = top > m[r] ? top + kSlack : m[r];
                 const float f = top > m[r] ? __builtin_amdgcn_exp2f(m[r] - to) : 1.0f;
                 m[r] = to;
@@ -301,7 +550,7 @@ template <typename T, int HD, int RT> struct Rows {
 #pragma unroll
                 for (int g = 0; g < G::kG; g++) {
                     mids[r][g] *= f;
-                    ps[r][g] *= f;
+                    if (!kCentred) ps[r][g] *= f;
                 }
 #pragma unroll
                 for (int d = 0; d < HD / 16; d++) o[r][d] *= f;
@@ -309,25 +558,30 @@ template <typename T, int HD, int RT> struct Rows {
             const float base = m[r] == -INFINITY ? 0.f : -m[r];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                float e = fmaf(a.c, s[r][i / 4][i % 4], base);
-                if (sizeof(T) == 4) e = fmaf(a.c_low, s[r][i / 4][i % 4], e);
+                float e = fmaf(c[r], s[r][i / 4][i % 4], base);
+                if (sizeof(T) == 4) e = fmaf(c_low[r], s[r][i / 4][i % 4], e);
                 p[r][i] = __builtin_amdgcn_exp2f(e);
                 l[r] += p[r][i];
             }
         }
+        uint32_t codes[8][HD == 256 ? 2 : 1];
+#pragma unroll
+        for (int i = 0; i < 8; i++) slot.value(i, codes[i]);
 #pragma unroll
         for (int g = 0; g < G::kG; g++) {
+            phase();
             u32x4 w[RT][N];                 // p s, in parts
 #pragma unroll
             for (int r = 0; r < RT; r++) {
-                const uint32_t seen = MASKED ? bits[r] >> (8 * g4) : ~0u;
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    f32x4 scale = four(2, g, t), mid = four(3, g, t);
-                    if (MASKED)             // what a hidden key holds may be NaN
+                    const f32x4 scale = four(2, g, t);
+                    f32x4 mid = four(3, g, t);
+                    if (hidden) {           // what a hidden key holds may be NaN
+                        const uint32_t seen = here(bits[r] >> (16 * t + g4));
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (!(seen >> (4 * t + i) & 1)) scale[i] = mid[i] = 0.f;
+                        for (int i = 0; i < 4; i++) mid[i] = seen >> (4 * i) & 1 ? mid[i] : 0.f;
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; i++) mids[r][g] = fmaf(p[r][4 * t + i], mid[i], mids[r][g]);
 #pragma unroll
@@ -338,26 +592,36 @@ template <typename T, int HD, int RT> struct Rows {
                         for (int n = 0; n < N; n++) w[r][n][2 * t + i] = part[n];
                     }
                 }
+                const u32x4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+                f32x4 sum = kCentred ? f32x4{0, 0, 0, 0} : ps[r][g];
 #pragma unroll
-                for (int n = 0; n < N; n++)
-                    ps[r][g] = mma(u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}, w[r][n], ps[r][g]);
+                for (int n = 0; n < N; n++) sum = mma(ones, w[r][n], sum);
+                if (!kCentred) ps[r][g] = sum;
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            o[r][4 * g + j][i] = fmaf(j & 1 ? -120 * 0x1p-24f : -7.5f * 0x1p-24f, sum[i],
+                                                      o[r][4 * g + j][i]);
             }
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                // nibble 4 g + j of a value's words: byte (4 g + j) / 2, its upper half if odd
+            for (int j = 0; j < 4; j += 2) {
+                // nibbles 4 g + j, 4 g + j + 1 of the values' words: one byte
                 const int nib = 4 * g + j, word = nib / 8, byte = nib % 8 / 2;
-                const uint32_t sel = (uint32_t)(byte + 4) << 16 | (uint32_t)byte;
                 u32x4 x;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t e = c.v[2 * i][word], f = c.v[2 * i + 1][word];
-                    x[i] = code_pair(j & 1 ? __builtin_amdgcn_perm(f >> 1, e >> 1, sel)
-                                           : __builtin_amdgcn_perm(f << 3, e << 3, sel));
-                }
+                for (int i = 0; i < 4; i++)
+                    x[i] = __builtin_amdgcn_perm(codes[2 * i + 1][word], codes[2 * i][word],
+                                                 0x0c000c00u | (uint32_t)(byte + 4) << 16 | (uint32_t)byte);
+                const u32x4 low = x & kLower, high = x & kUpper;
 #pragma unroll
                 for (int r = 0; r < RT; r++)
 #pragma unroll
-                    for (int n = 0; n < N; n++) o[r][nib] = mma(x, w[r][n], o[r][nib]);
+                    for (int n = 0; n < N; n++) {
+                        o[r][nib] = mma(low, w[r][n], o[r][nib]);
+                        o[r][nib + 1] = mma(high, w[r][n], o[r][nib + 1]);
+                    }
             }
         }
     }
@@ -365,6 +629,7 @@ template <typename T, int HD, int RT> struct Rows {
     // Sums over the lanes of a row, and the values that B, C and the mids make
     __device__ __forceinline__ void finish()
     {
+        const int up = E == kNone ? 0 : E - kUp;
 #pragma unroll
         for (int r = 0; r < RT; r++) {
             l[r] = groups_sum(l[r]);
@@ -372,10 +637,12 @@ template <typename T, int HD, int RT> struct Rows {
             for (int g = 0; g < G::kG; g++) {
                 const float add = groups_sum(mids[r][g]);
 #pragma unroll
-                for (int j = 0; j < 4; j++)
+                for (int i = 0; i < 4; i++) {
+                    const float off = kCentred ? add : add - 7.5f * __builtin_amdgcn_ldexpf(ps[r][g][i], up);
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        o[r][4 * g + j][i] = fmaf(-23.5f, ps[r][g][i], o[r][4 * g + j][i]) + add;
+                    for (int j = 0; j < 4; j++)
+                        o[r][4 * g + j][i] = off + __builtin_amdgcn_ldexpf(o[r][4 * g + j][i], up + (j & 1 ? 20 : 24));
+                }
             }
         }
     }
@@ -459,7 +726,7 @@ __device__ __forceinline__ void join_waves(const AttnArgs &a, Rows<T, HD, RT> &w
 
 template <int HD> constexpr int attn_lds()
 {
-    constexpr int tiles = kAttnWaves * Geo<HD>::kScales * 4;
+    constexpr int tiles = kAttnWaves * Geo<HD>::kWave;
     constexpr int join = kAttnWaves * 16 * Geo<HD>::kWide * 4 + kAttnWaves * 16 * 8 + 16 * 4;
     return tiles > join ? tiles : join;
 }
@@ -481,7 +748,10 @@ __device__ __forceinline__ void walk(const AttnArgs &a, char *lds, const Work &w
         if (w.first >= end && a.plan.parts > 1) return;     // the merge counts own parts by the length
     }
     const int64_t token0 = w.seq >= 0 ? (int64_t)w.seq * a.tokens : 0;
-    float *scales = (float *)lds + wave * G::kScales;
+    char *mine = lds + wave * G::kWave;
+    float *scales = (float *)(mine + G::kScales);
+    Tiles<HD> tiles = {a, own, pre_tiles, length, w.first + wave, end, w.h, mine};
+    tiles.begin();
     Rows<T, HD, RT> rows;
     rows.start(a, w.h, token0, row0, n);
     // own keys that the lane's row of each tile sees
@@ -489,44 +759,28 @@ __device__ __forceinline__ void walk(const AttnArgs &a, char *lds, const Work &w
 #pragma unroll
     for (int t = 0; t < RT; t++)
         sees[t] = length - a.tokens + 1 + (int32_t)cbq_div(row0 + 16 * t + (lane & 15), a.rep);
-    int32_t id = -1;
-    uint32_t row = 0;
-    auto look = [&](int32_t tile) {                     // this lane's key's page
-        id = -1;
-        if (tile >= end) return;
-        const int32_t j = tile_key(tile, pre_tiles, a.prefix, length, lane & 31);
-        if (j < 0) return;
-        const uint32_t entry = cbq_div((uint32_t)j, a.pool.page);
-        row = (uint32_t)j - entry * a.pool.page.d;
-        id = (tile < pre_tiles ? a.prefix_table : own)[entry];
-    };
-    int32_t tile = w.first + wave;
-    Codes<HD> next;
-    look(tile);
-    if (tile < end) next.load(a, w.h, id, row);
-    look(tile + kAttnWaves);
-    for (; tile < end; tile += kAttnWaves) {
-        const Codes<HD> now = next;
-        if (tile + kAttnWaves < end) next.load(a, w.h, id, row);
-        look(tile + 2 * kAttnWaves);
-        now.spread(scales);
+    for (int i = 0; tiles.tile(i) < end; i++) {
+        const uint32_t there = tiles.next(i);
+        const int32_t tile = tiles.tile(i);
+        const Slot<HD> slot = {mine + i % G::kDepth * G::kSlot};
+        rows.follow(slot.exponent(there));
+        slot.spread(scales, there, rows.E);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         const int32_t key0 = (tile - pre_tiles) * kTile;
         uint32_t bits[RT];
-        bool whole = now.there == ~0u;
+        bool whole = there == ~0u;
 #pragma unroll
         for (int t = 0; t < RT; t++) {
-            bits[t] = now.there;
+            bits[t] = there;
             if (tile >= pre_tiles) {
                 const int32_t left = sees[t] - key0;
                 if (left < kTile) bits[t] &= left <= 0 ? 0u : (1u << left) - 1;
             }
             whole = whole && bits[t] == ~0u;
         }
-        if (__all(whole)) rows.template tile<false>(a, now, scales, bits);
-        else rows.template tile<true>(a, now, scales, bits);
+        rows.tile(slot, scales, bits, !__all(whole));
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -535,17 +789,21 @@ __device__ __forceinline__ void walk(const AttnArgs &a, char *lds, const Work &w
     join_waves<T, HD, RT>(a, rows, lds, w.h, token0, row0, n, to);
 }
 
-template <typename T, int HD, int RT> __global__ __launch_bounds__(kBlock, 2) void q4_kernel(AttnArgs a)
+template <typename T, int HD, int RT> __global__ __launch_bounds__(kBlock, HD == 256 ? 1 : RT == 1 ? Q4W : RT == 2 ? 2 : 1) void q4_kernel(AttnArgs a)
 {
-    __shared__ __attribute__((aligned(16))) char lds[attn_lds<HD>()];
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     const int32_t pre_tiles = (a.prefix + kTile - 1) / kTile,
                   cap_tiles = (int32_t)((a.capacity + kTile - 1) / kTile);
     const uint32_t block = cbq_block(blockIdx.x, blockIdx.y);
     if (block >= a.plan.blocks) return;
     const Work w = work_of(a.plan, block, a.n_kv, a.batch, pre_tiles, cap_tiles);
     const int to = a.plan.parts > 1 ? w.part : -1, rows = a.tokens * (int)a.rep.d;
-    if (w.seq < 0) walk<T, HD, RT>(a, lds, w, w.tile * 16 * RT, a.batch * rows, to);
-    else walk<T, HD, 1>(a, lds, w, w.tile * 16, rows, to);
+    if constexpr (RT == 1) {
+        walk<T, HD, 1>(a, lds, w, w.tile * 16, w.seq < 0 ? a.batch * rows : rows, to);
+    } else {
+        if (w.seq < 0) walk<T, HD, RT>(a, lds, w, w.tile * 16 * RT, a.batch * rows, to);
+        else walk<T, HD, 1>(a, lds, w, w.tile * 16, rows, to);
+    }
 }
 
 // ---- merge of the parts: a block a (token, head) -------------------------------------------------
@@ -587,13 +845,40 @@ template <typename T, int HD> __global__ __launch_bounds__(kBlock) void q4_merge
 }
 
 // ---- launches of one type -------------------------------------------------------------------------
+// More than 64 KiB of LDS is asked for once a kernel and device.
+template <auto K> bool lds_allowed(int lds)
+{
+    static std::atomic<uint64_t> asked{0};
+    if (lds <= 65536) return true;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return false;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev <= 63 && asked.load(std::memory_order_relaxed) & bit) return true;
+    if (hipFuncSetAttribute((const void *)K, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+        return false;
+    asked.fetch_or(bit, std::memory_order_relaxed);
+    return true;
+}
+
+template <typename T, int HD, int RT> int launch_rows(const AttnArgs &a, hipStream_t stream)
+{
+    const char *what = "cbq_prefix_attn_decode_q4";
+    const CbqGrid grid = cbq_grid(a.plan.blocks);
+    constexpr int lds = attn_lds<HD>();
+    if (!lds_allowed<q4_kernel<T, HD, RT>>(lds)) return cbq_launch_status(what);
+    q4_kernel<T, HD, RT><<<dim3(grid.x, grid.y), kBlock, lds, stream>>>(a);
+    return cbq_launch_status(what);
+}
+
 template <typename T, int HD> int launch(const AttnArgs &a, hipStream_t stream)
 {
-    CbqGrid grid = cbq_grid(a.plan.blocks);
-    q4_kernel<T, HD, 1><<<dim3(grid.x, grid.y), kBlock, 0, stream>>>(a);
-    int rc = cbq_launch_status("cbq_prefix_attn_decode_q4");
+    constexpr int wide = widest(HD, sizeof(T));
+    int rc;
+    if (a.plan.rt == 1) rc = launch_rows<T, HD, 1>(a, stream);
+    else if (a.plan.rt == 2) rc = launch_rows<T, HD, wide < 2 ? wide : 2>(a, stream);
+    else rc = launch_rows<T, HD, wide>(a, stream);
     if (rc != CK_SUCCESS || a.plan.parts == 1) return rc;
-    grid = cbq_grid((int64_t)a.batch * a.tokens * a.n_q);
+    const CbqGrid grid = cbq_grid((int64_t)a.batch * a.tokens * a.n_q);
     q4_merge_kernel<T, HD><<<dim3(grid.x, grid.y), kBlock, 0, stream>>>(a);
     return cbq_launch_status("cbq_prefix_attn_decode_q4 merge");
 }

@@ -21,21 +21,22 @@ bool sizes_ok(const cbq_paged_q4 *c, int64_t prefix, int64_t width, int64_t batc
            batch * tokens <= kMaxKeys && batch * tokens * n_q <= kMaxKeys;
 }
 
-bool make_plan(const cbq_paged_q4 *c, int64_t prefix, int64_t width, int64_t batch, int64_t tokens,
-               int64_t n_q, Plan &p)
+bool make_plan(const cbq_paged_q4 *c, int type_bytes, int64_t prefix, int64_t width, int64_t batch,
+               int64_t tokens, int64_t n_q, Plan &p)
 {
-    p = plan(c->hd, c->n_kv, tokens * (n_q / c->n_kv), prefix, width * c->page, batch);
+    p = plan(c->hd, type_bytes, c->n_kv, tokens * (n_q / c->n_kv), prefix, width * c->page, batch);
     return plan_fits(p);
 }
 
 }  // namespace
 
 extern "C" size_t cbq_prefix_attn_decode_q4_workspace(const cbq_paged_q4 *cache, int64_t prefix,
-                                                      int width, int batch, int tokens, int n_q)
+                                                      int width, int batch, int tokens, int n_q,
+                                                      int dtype)
 {
     Plan p;
     if (!sizes_ok(cache, prefix, width, batch, tokens, n_q) || batch < 1 ||
-        !make_plan(cache, prefix, width, batch, tokens, n_q, p))
+        !make_plan(cache, dtype == CBQ_F32 ? 4 : 2, prefix, width, batch, tokens, n_q, p))
         return 0;
     return (size_t)p.bytes;
 }
@@ -59,7 +60,7 @@ extern "C" int cbq_prefix_attn_decode_q4(const void *q, const int64_t *q_stride,
     if ((((uintptr_t)q | (uintptr_t)out) & 15) || q_stride[0] * e % 16 || q_stride[1] * e % 16)
         return CK_ERR_ARG;
     AttnArgs a = {};
-    if (!make_plan(cache, prefix, width, batch, tokens, n_q, a.plan)) return CK_ERR_ARG;
+    if (!make_plan(cache, (int)e, prefix, width, batch, tokens, n_q, a.plan)) return CK_ERR_ARG;
     if (a.plan.bytes && (!workspace || workspace_bytes < (size_t)a.plan.bytes ||
                          ((uintptr_t)workspace & 15) != 0))
         return CK_ERR_ARG;
@@ -75,6 +76,11 @@ extern "C" int cbq_prefix_attn_decode_q4(const void *q, const int64_t *q_stride,
     a.part_o = (float *)workspace;
     a.part_ml = (float2 *)((float *)workspace + (a.plan.parts > 1 ? a.plan.parts * rows * cache->hd : 0));
     a.rep = cbq_div_make((uint32_t)(n_q / cache->n_kv));
+    // pages of whole tiles, whose rows a 32-bit offset from the tile's first reaches
+    a.whole = cache->page % kTile == 0 && cache->code_stride[2] < (1 << 24) && cache->scale_stride[2] < (1 << 24);
+    a.tiles_a_page = cbq_div_make(a.whole ? (uint32_t)cache->page / kTile : 1);
+    a.code_row = a.whole ? (uint32_t)cache->code_stride[2] : 0;
+    a.pair_row = a.whole ? (uint32_t)cache->scale_stride[2] * 2 : 0;
     a.prefix = (int32_t)prefix; a.batch = batch; a.tokens = tokens; a.n_q = n_q;
     a.n_kv = cache->n_kv;
     // The running maximum needs a factor above 0: the queries take scale's sign,

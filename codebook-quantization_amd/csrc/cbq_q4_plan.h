@@ -21,21 +21,29 @@ struct Plan {
     int64_t blocks, bytes;
 };
 
+// 16 widest rows of the prefix a block: as many as a wave's registers hold
+#ifndef Q4RT
+#define Q4RT 1
+#endif
+constexpr int widest(int hd, int type_bytes) { return hd == 256 ? 1 : Q4RT; }
+
 inline int64_t part_bytes(int64_t parts, int64_t rows, int hd)
 {
     return parts > 1 ? parts * rows * (hd + 2) * 4 : 0;
 }
 
 // rows: query rows of a sequence and kv head (tokens times query heads a kv head)
-inline Plan plan(int hd, int n_kv, int64_t rows, int64_t prefix, int64_t capacity, int64_t batch)
+inline Plan plan(int hd, int type_bytes, int n_kv, int64_t rows, int64_t prefix, int64_t capacity, int64_t batch)
 {
     Plan p = {};
     const int64_t pre_tiles = cbq_ceil(prefix, kTile), cap_tiles = cbq_ceil(capacity, kTile);
     const int64_t own_tiles = cbq_ceil(rows, 16);
-    p.rt = 1;
+    const int64_t all = cbq_ceil(batch * rows, 16);
+    p.rt = prefix ? (int32_t)cbq_min(all > 2 ? 4 : all, widest(hd, type_bytes)) : 1;
     p.own_tiles = (int32_t)own_tiles;
     if (pre_tiles + cap_tiles <= 4 * kAttnWaves) {
         p.joint = 1;
+        p.rt = 1;
         p.own_parts = p.parts = 1;
         p.own_chunk = (int32_t)cbq_max(pre_tiles + cap_tiles, 1);
         p.blocks = n_kv * batch * own_tiles;

@@ -254,7 +254,7 @@ at::Tensor prefix_attention_decode_q4(const at::Tensor &q, const at::Tensor &k_c
     const int64_t xs[2] = {x.stride(0), x.stride(1)};
     const int tokens = (int)(N / batch);
     const size_t nws = cbq_prefix_attn_decode_q4_workspace(&c, prefix, (int)width, (int)batch, tokens,
-                                                           (int)n_q);
+                                                           (int)n_q, type);
     at::Tensor ws;
     if (nws) ws = at::empty({(int64_t)nws}, q.options().dtype(at::kByte));
     check_done(cbq_prefix_attn_decode_q4(x.data_ptr(), xs, type, &c, prefix_table.data_ptr<int32_t>(),

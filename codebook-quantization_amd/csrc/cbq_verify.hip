@@ -2,10 +2,11 @@
 //
 // Draft i is kept while u_i q_i(d_i) < p_i(d_i) and all before it are; one token more
 // is drawn from w = max(p - q, 0) of the row behind them, or from p, by the inverse of
-// its sums.  Two numbers a draft decide which row that is, so every block finds it for
+// its sums.  Two numbers a draft decide which row that is, so every wave finds it for
 // itself, and only that row of p (and of q) is read: HBM bounds a large batch, two
-// launches a small one.  The first launch adds the row up in chunks, the second finds
-// the chunk in which the sums pass u times the total and reads that chunk again.
+// launches and their chains of dependent loads a small one.  The first launch adds the
+// row up, 512 tokens a sum, the second finds the sum in which they pass u times the
+// total and reads its tokens again.
 //
 // All of it in 64 bits: a vocabulary of 10^5 has borders every 10^-5 of the sum, and
 // fp32 sums would move one in a hundred draws to another token.
@@ -15,8 +16,10 @@
 
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / CBQ_WAVE, kPer = 8;
-constexpr int kChunk = kThreads * kPer;     // tokens of a chunk
+constexpr int kThreads = 256, kWaves = kThreads / CBQ_WAVE;
+constexpr int kPer = 8, kUnit = CBQ_WAVE * kPer;        // tokens of a sum
+
+constexpr int64_t kFull = 8 * 4 * 256;     // eight waves a SIMD of 256 CUs
 
 struct VerifyArgs {
     const void *p, *q;
@@ -26,38 +29,50 @@ struct VerifyArgs {
     const float *uniforms;
     int64_t *tokens;
     int32_t *counts;
-    double2 *sums;                          // [batch][chunk]: of w, of p
-    int32_t n_max, chunks;
+    double2 *sums;                          // [batch][unit]: of w, of p
+    int32_t *kept;                          // [batch]
+    int32_t n_max, units, each;             // each: units a wave adds up
     int64_t vocab;
+};
+
+template <typename T> struct alignas(sizeof(T)) Four {  // rows begin anywhere
+    T e[4];
 };
 
 // The row that a sequence's last token is drawn from
 template <typename T> struct Row {
     const T *p, *q;
-    int kept, n;
     int64_t without;                        // token whose w is 0 (a certain draft's), or -1
 
-    __device__ __forceinline__ double target(int64_t v) const
+    // p and w of n tokens from v on (n < 4: the row's last ones)
+    __device__ __forceinline__ void four(int64_t v, int64_t n, double (&x)[4], double (&w)[4]) const
     {
-        const double x = (double)(float)p[v];
-        return x > 0 ? x : 0;
-    }
-    // w(v), given p(v)
-    __device__ __forceinline__ double rest(int64_t v, double x) const
-    {
-        if (v == without) return 0;
-        if (!q) return x;
-        const double w = (double)(float)p[v] - (double)(float)q[v];
-        return w > 0 ? w : 0;
+        Four<T> a = {}, b = {};
+        if (n >= 4) {
+            a = *(const Four<T> *)(p + v);
+            if (q) b = *(const Four<T> *)(q + v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; i++)
+                if (i < n) {
+                    a.e[i] = p[v + i];
+                    if (q) b.e[i] = q[v + i];
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const double y = (double)(float)a.e[i], z = y - (double)(float)b.e[i];
+            x[i] = y > 0 ? y : 0;
+            w[i] = z > 0 && v + i != without ? z : 0;
+        }
     }
 };
 
-template <typename T> __device__ __forceinline__ Row<T> find_row(const VerifyArgs &a, int b)
+// The first of a sequence's drafts that is refused, or their count
+template <typename T> __device__ __forceinline__ int find_kept(const VerifyArgs &a, int b)
 {
     const int lane = threadIdx.x & 63;
-    Row<T> r;
     const int n = a.n_drafts ? (int)cbq_clamp_length(a.n_drafts[b], a.n_max) : a.n_max;
-    int kept = n;
     for (int i0 = 0; i0 < n; i0 += CBQ_WAVE) {
         const int i = i0 + lane;
         bool keep = true;
@@ -72,13 +87,15 @@ template <typename T> __device__ __forceinline__ Row<T> find_row(const VerifyArg
             keep = (double)a.uniforms[(int64_t)b * (a.n_max + 1) + i] * q < p;
         }
         const uint64_t refused = __ballot(!keep);
-        if (refused) {
-            kept = i0 + __builtin_ctzll(refused);
-            break;
-        }
+        if (refused) return i0 + __builtin_ctzll(refused);
     }
-    r.kept = kept;
-    r.n = n;
+    return n;
+}
+
+template <typename T> __device__ __forceinline__ Row<T> row_of(const VerifyArgs &a, int b, int kept)
+{
+    const int n = a.n_drafts ? (int)cbq_clamp_length(a.n_drafts[b], a.n_max) : a.n_max;
+    Row<T> r;
     r.p = (const T *)a.p + b * a.p_st[0] + kept * a.p_st[1];
     r.q = kept < n && a.q ? (const T *)a.q + b * a.q_st[0] + kept * a.q_st[1] : nullptr;
     r.without = kept < n && !a.q ? a.drafts[(int64_t)b * a.n_max + kept] : -1;
@@ -93,34 +110,33 @@ __device__ __forceinline__ double wave_sum(double x)
 
 template <typename T> __global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a)
 {
-    __shared__ double2 part[kWaves];
-    const int b = blockIdx.y, chunk = blockIdx.x;
-    const Row<T> r = find_row<T>(a, b);
-    const int64_t v0 = (int64_t)chunk * kChunk + threadIdx.x;
-    double w = 0, p = 0;
+    const int b = blockIdx.y, lane = threadIdx.x & 63;
+    const int64_t first = ((int64_t)blockIdx.x * kWaves + threadIdx.x / CBQ_WAVE) * a.each;
+    if (first >= a.units) return;
+    const int kept = find_kept<T>(a, b);
+    if (first == 0 && lane == 0) a.kept[b] = kept;
+    const Row<T> r = row_of<T>(a, b, kept);
+    const int64_t end = first + a.each < a.units ? first + a.each : a.units;
+    for (int64_t u = first; u < end; u++) {
+        double w = 0, p = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-        const int64_t v = v0 + i * kThreads;
-        if (v < a.vocab) {
-            const double x = r.target(v);
-            p += x;
-            w += r.rest(v, x);
+        for (int i = 0; i < kPer / 4; i++) {
+            const int64_t v = u * kUnit + i * 4 * CBQ_WAVE + lane * 4;
+            double x[4], y[4];
+            r.four(v, a.vocab - v, x, y);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                p += x[k];
+                w += y[k];
+            }
         }
-    }
-    w = wave_sum(w);
-    p = wave_sum(p);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x / CBQ_WAVE] = make_double2(w, p);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < kWaves; i++) {
-            w += part[i].x;
-            p += part[i].y;
-        }
-        a.sums[(int64_t)b * a.chunks + chunk] = make_double2(w, p);
+        w = wave_sum(w);
+        p = wave_sum(p);
+        if (lane == 0) a.sums[(int64_t)b * a.units + u] = make_double2(w, p);
     }
 }
 
-// One wave a sequence.  Sums of lanes before this one, and of all.
+// The sum of the lanes before this one, and of all
 __device__ __forceinline__ double lanes_before(double x, double &all)
 {
     const int lane = threadIdx.x & 63;
@@ -134,77 +150,99 @@ __device__ __forceinline__ double lanes_before(double x, double &all)
     return lane ? before : 0;
 }
 
-template <typename T> __global__ __launch_bounds__(CBQ_WAVE) void pick_kernel(VerifyArgs a)
+// A block a sequence: its waves add up the sums, the first one finds the token
+template <typename T> __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a)
 {
-    const int b = blockIdx.x, lane = threadIdx.x;
-    const Row<T> r = find_row<T>(a, b);
-    const double2 *sums = a.sums + (int64_t)b * a.chunks;
+    __shared__ double2 part[kWaves];
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const double2 *sums = a.sums + (int64_t)b * a.units;
+    const int kept = a.kept[b];
     double w = 0, p = 0;
-    for (int c = lane; c < a.chunks; c += CBQ_WAVE) {
-        w += sums[c].x;
-        p += sums[c].y;
+    for (int u = tid; u < a.units; u += kThreads) {
+        w += sums[u].x;
+        p += sums[u].y;
     }
     w = wave_sum(w);
     p = wave_sum(p);
+    if (lane == 0) part[tid / CBQ_WAVE] = make_double2(w, p);
+    __syncthreads();
+    if (tid >= CBQ_WAVE) return;
+    const Row<T> r = row_of<T>(a, b, kept);
+    w = p = 0;
+    for (int i = 0; i < kWaves; i++) {
+        w += part[i].x;
+        p += part[i].y;
+    }
     const bool all = !(w > 0);              // nothing left: p itself
     const double goal = (double)a.uniforms[(int64_t)b * (a.n_max + 1) + a.n_max] * (all ? p : w);
-    // the first chunk whose sum passes the goal, or the last that adds to it
+    // the first unit whose sum passes the goal, or the last that adds to it; eight a lane
     double before = 0, start = 0;
-    int at = -1;
+    int64_t at = -1;
     bool passed = false;
-    for (int c0 = 0; c0 < a.chunks && !passed; c0 += CBQ_WAVE) {
-        const int c = c0 + lane;
-        const double x = c < a.chunks ? (all ? sums[c].y : sums[c].x) : 0;
-        double total;
-        const double mine = before + lanes_before(x, total);
-        const uint64_t over = __ballot(x > 0 && mine + x > goal), some = __ballot(x > 0);
+    for (int64_t u0 = 0; u0 < a.units && !passed; u0 += kUnit) {
+        double x[kPer], sum = 0, total;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int64_t u = u0 + lane * kPer + i;
+            const double2 s = u < a.units ? sums[u] : make_double2(0, 0);
+            x[i] = all ? s.y : s.x;
+            sum += x[i];
+        }
+        double run = before + lanes_before(sum, total);
+        double here = 0;
+        int mine = -1, last = -1;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            if (x[i] > 0 && mine < 0) {
+                last = i;
+                here = run;
+                if (run + x[i] > goal) mine = i;
+            }
+            run += x[i];
+        }
+        const uint64_t over = __ballot(mine >= 0), some = __ballot(last >= 0);
         passed = over != 0;
         const int from = passed ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
         if (from >= 0) {
-            at = c0 + from;
-            start = __shfl(mine, from);
+            at = u0 + from * kPer + __shfl(last, from);     // mine, where it is one
+            start = __shfl(here, from);
         }
         before += total;
     }
     int64_t token = -1;
     if (at >= 0) {
-        // the same inside the chunk, 64 lanes by 8 tokens in order
-        const int64_t base = (int64_t)at * kChunk;
-        bool found = false;
-        for (int i0 = 0; i0 < kChunk && !found; i0 += CBQ_WAVE * kPer) {
-            const int64_t v0 = base + i0 + lane * kPer;
-            double x[kPer], sum = 0;
+        // the same inside the unit, eight tokens a lane in order
+        double x[kPer], sum = 0, total;
+        const int64_t v0 = at * kUnit + lane * kPer;
 #pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                x[i] = 0;
-                if (v0 + i < a.vocab) {
-                    x[i] = r.target(v0 + i);
-                    if (!all) x[i] = r.rest(v0 + i, x[i]);
-                }
-                sum += x[i];
-            }
-            double total;
-            double run = start + lanes_before(sum, total);
-            int64_t mine = -1, last = -1;
+        for (int i = 0; i < kPer / 4; i++) {
+            double y[4], z[4];
+            r.four(v0 + 4 * i, a.vocab - v0 - 4 * i, y, z);
 #pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                run += x[i];
-                if (x[i] > 0) {
-                    last = v0 + i;
-                    if (mine < 0 && run > goal) mine = v0 + i;
-                }
+            for (int k = 0; k < 4; k++) {
+                x[4 * i + k] = all ? y[k] : z[k];
+                sum += x[4 * i + k];
             }
-            const uint64_t over = __ballot(mine >= 0), some = __ballot(last >= 0);
-            found = over != 0;
-            if (found) token = __shfl(mine, __builtin_ctzll(over));
-            else if (some) token = __shfl(last, 63 - __builtin_clzll(some));
-            start += total;
         }
+        double run = start + lanes_before(sum, total);
+        int mine = -1, last = -1;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            run += x[i];
+            if (x[i] > 0) {
+                last = i;
+                if (mine < 0 && run > goal) mine = i;
+            }
+        }
+        const uint64_t over = __ballot(mine >= 0), some = __ballot(last >= 0);
+        const int from = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some | 1);
+        const int in = __shfl(over ? mine : last, from);
+        if (in >= 0) token = at * kUnit + from * kPer + in;
     }
     for (int i = lane; i <= a.n_max; i += CBQ_WAVE)
         a.tokens[(int64_t)b * (a.n_max + 1) + i] =
-            i < r.kept ? a.drafts[(int64_t)b * a.n_max + i] : i == r.kept ? token : -1;
-    if (lane == 0) a.counts[b] = r.kept + 1;
+            i < kept ? a.drafts[(int64_t)b * a.n_max + i] : i == kept ? token : -1;
+    if (lane == 0) a.counts[b] = kept + 1;
 }
 
 template <typename T> int launch(const VerifyArgs &a, int batch, hipStream_t stream)
@@ -219,9 +257,10 @@ template <typename T> int launch(const VerifyArgs &a, int batch, hipStream_t str
         x.uniforms += (int64_t)b * (a.n_max + 1);
         x.tokens += (int64_t)b * (a.n_max + 1);
         x.counts += b;
-        x.sums += (int64_t)b * a.chunks;
-        sums_kernel<T><<<dim3(a.chunks, n), kThreads, 0, stream>>>(x);
-        pick_kernel<T><<<n, CBQ_WAVE, 0, stream>>>(x);
+        x.sums += (int64_t)b * a.units;
+        x.kept += b;
+        sums_kernel<T><<<dim3((uint32_t)cbq_ceil(a.units, kWaves * a.each), n), kThreads, 0, stream>>>(x);
+        pick_kernel<T><<<n, kThreads, 0, stream>>>(x);
         const int rc = cbq_launch_status("cbq_verify_drafts");
         if (rc != CK_SUCCESS) return rc;
     }
@@ -233,13 +272,15 @@ bool sizes_ok(int64_t batch, int64_t vocab)
     return batch >= 0 && batch < (1 << 24) && vocab >= 1 && vocab < (1ll << 31);
 }
 
-int64_t chunks_of(int64_t vocab) { return cbq_ceil(vocab, kChunk); }
+int64_t units_of(int64_t vocab) { return cbq_ceil(vocab, kUnit); }
+
+size_t sums_bytes(int64_t batch, int64_t vocab) { return (size_t)batch * units_of(vocab) * sizeof(double2); }
 
 }  // namespace
 
 extern "C" size_t cbq_verify_drafts_workspace(int batch, int64_t vocab)
 {
-    return sizes_ok(batch, vocab) ? (size_t)batch * chunks_of(vocab) * sizeof(double2) : 0;
+    return sizes_ok(batch, vocab) ? sums_bytes(batch, vocab) + (size_t)batch * sizeof(int32_t) : 0;
 }
 
 extern "C" int cbq_verify_drafts(const void *probs, const int64_t *p_stride, const int64_t *drafts,
@@ -270,8 +311,12 @@ extern "C" int cbq_verify_drafts(const void *probs, const int64_t *p_stride, con
     a.counts = counts;
     a.sums = (double2 *)workspace;
     a.n_max = n_max;
-    a.chunks = (int32_t)chunks_of(vocab);
+    a.kept = (int32_t *)((char *)workspace + sums_bytes(batch, vocab));
+    a.units = (int32_t)units_of(vocab);
     a.vocab = vocab;
+    // every wave finds the row first, three loads one after the other: few waves take a
+    // unit each, many as many as leave eight waves a SIMD
+    a.each = (int32_t)cbq_min(cbq_max(batch * (int64_t)a.units / kFull, 1), 16);
     if (dtype == CBQ_F32) return launch<float>(a, batch, stream);
     if (dtype == CBQ_BF16) return launch<__bf16>(a, batch, stream);
     return launch<_Float16>(a, batch, stream);

@@ -80,7 +80,7 @@ int cbq_paged_read_q4(const cbq_paged_q4 *cache, const int64_t *slots, int64_t N
  * workspace: cbq_prefix_attn_decode_q4_workspace bytes (which may be 0), 16-byte
  * aligned, overwritten by every call. */
 size_t cbq_prefix_attn_decode_q4_workspace(const cbq_paged_q4 *cache, int64_t prefix, int width,
-                                           int batch, int tokens, int n_q);
+                                           int batch, int tokens, int n_q, int dtype);
 int cbq_prefix_attn_decode_q4(const void *q, const int64_t *q_stride, int dtype,
                               const cbq_paged_q4 *cache, const int32_t *prefix_table,
                               int64_t prefix, const int32_t *tables, int64_t table_stride,
