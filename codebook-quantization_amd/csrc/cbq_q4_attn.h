@@ -4,14 +4,17 @@
 //
 // out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - max), in one pass over the
 // keys with a running maximum.  With k_jd = m + s (c - 7.5) in a group g of 64 values,
-//   q.k_j = sum_g s_jg A_jg + (m_jg - 7.5 s_jg) Q_g,        A_jg = sum_d q_d c_jd,
-//   sum_j p_j v_jd = B_d - 7.5 C_g + sum_j p_j m_jg,         B_d = sum_j (p_j s_jg) c_jd,
-// Q_g the group's sum of q and C_g that of p_j s_jg: the codes go to the matrix cores as
-// they are, and no dequantised value is rounded.  A code needs no conversion: the bits
-// 0..15 of an fp16 number are the subnormals c 2^-24, and 16 c 2^-24 where the code
-// lies in a byte's upper half, which the products take exactly.  So two codes cost a mask
-// (and half a shift or a byte permute); as bf16 numbers c + 16 under a constant
-// exponent they cost three operations, and 24 sequences of 4000 to 32000 keys 155 us.
+//   q.k_j = sum_g s_jg A_jg + m_jg Q_g,              A_jg = sum_d q_d (c_jd + z) - R_g,
+//   sum_j p_j v_jd = B_d - (z + 7.5) C_g + sum_j p_j m_jg,   B_d = sum_j (p_j s_jg) (c_jd + z),
+// Q_g the group's sum of q, R_g that of (z + 7.5) q, with which the products begin, and C_g
+// that of p_j s_jg: the codes go to the matrix cores as they are, and no dequantised value
+// is rounded.  c + z is one fp16 number, the code in its mantissa under a constant
+// exponent: z is 16, 64 or 256 where the code's lowest bit is bit 6, 4 or 2, so a
+// masked or makes two of them, and a shift serves four.  A large z costs the sums bits:
+// 256 for half the keys' codes of 16-bit queries (2^-18 of a score), 64 for half the
+// values' of bf16 ones, else 16; fp32 queries pay a packed addition for c - 7.5, z none.
+// (The code's bits alone, a subnormal number, need no or; but the products add those
+// without their leading zeros: ten bits of every sum.)
 //
 // The other operands have to fit fp16.  A query row is scaled to a largest value in
 // [2^14, 2^15), fp32 cut into two parts.  p_j s_jg is taken against 2^E, E the largest
@@ -48,12 +51,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-#ifndef Q4D
-#define Q4D 2
-#endif
-#ifndef Q4W
-#define Q4W 3
-#endif
 constexpr int kBlock = kAttnWaves * CBQ_WAVE;
 
 // The running maximum stands this far (in exp2's domain) above the scores of its last
@@ -116,26 +113,89 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c)
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// a and b as N fp16 parts each
+// a and b as N fp16 parts each.  What is taken off them is the part that was made, its bits:
+// a product under way to a and to fp16 would round to either of two neighbours.
 template <int N> __device__ __forceinline__ void cut(float a, float b, uint32_t (&part)[N])
 {
 #pragma unroll
     for (int n = 0; n < N; n++) {
-        const f16x2 x = {(_Float16)a, (_Float16)b};
-        part[n] = __builtin_bit_cast(uint32_t, x);
-        a -= (float)x[0];
-        b -= (float)x[1];
+        part[n] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+        if (n + 1 < N) {
+            asm("" : "+v"(part[n]));
+            const f16x2 x = __builtin_bit_cast(f16x2, part[n]);
+            a -= (float)x[0];
+            b -= (float)x[1];
+        }
     }
 }
 
-// Two codes of a word: c 2^-24, or 16 c 2^-24 (upper halves of bytes), as fp16 numbers
-constexpr uint32_t kLower = 0x000f000fu, kUpper = 0x00f000f0u;
-
-// Eight codes (low nibble first) in the order 0 4 1 5 2 6 3 7, odd ones 16 times as large
-__device__ __forceinline__ u32x4 eight_codes(uint32_t w)
+// a x and b y as N fp16 parts each: products rounded once, by one operation each where
+// one part is asked for
+template <int N> __device__ __forceinline__ void cut_products(float a, float x, float b, float y, uint32_t (&part)[N])
 {
-    return u32x4{w & kLower, w & kUpper, w >> 8 & kLower, w >> 8 & kUpper};
+    if constexpr (N == 1) {                 // (a sum with 0 keeps the product and its rounding in one)
+        const f16x2 z = {(_Float16)fmaf(a, x, 0.f), (_Float16)fmaf(b, y, 0.f)};
+        part[0] = __builtin_bit_cast(uint32_t, z);
+    } else {
+        cut<N>(a * x, b * y, part);
+    }
 }
+
+// Two codes of a word, at bits FROM .. FROM + 3 of either half, as the fp16 numbers c + z.
+// The constants stay in registers, a scalar and a vector one: an operation of three
+// operands takes no literal.
+template <int FROM> struct Pair {
+    uint32_t mask, magic;
+    __device__ __forceinline__ Pair()
+    {
+        constexpr uint32_t bits = 0x000f000fu << FROM, exponent = (uint32_t)(25 - FROM) << 10;
+        asm("s_mov_b32 %0, %1" : "=s"(mask) : "i"(bits));
+        asm("v_mov_b32 %0, %1" : "=v"(magic) : "i"(exponent << 16 | exponent));
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (x & mask) | magic; }
+};
+
+// z + 7.5 of a key's codes (even and odd ones) and of a value's (lower and upper ones)
+template <typename T> struct Zeros {
+    static constexpr bool kNone = sizeof(T) == 4;
+    static constexpr float kEven = kNone ? 0 : 263.5f, kOdd = kNone ? 0 : 23.5f;
+    static constexpr float kLow = kNone ? 0 : 23.5f, kHigh = kNone ? 0 : std::is_same_v<T, __bf16> ? 71.5f : 23.5f;
+};
+
+template <typename T> struct Unpack {
+    Pair<6> six;
+    Pair<4> four;
+    Pair<2> two;
+
+    // Eight codes of a key (low nibble first) in the order 0 4 1 5 2 6 3 7
+    __device__ __forceinline__ u32x4 key(uint32_t w) const
+    {
+        if constexpr (Zeros<T>::kNone) {
+            return u32x4{bare(w << 6), bare(w << 2), bare(w >> 2), bare(w >> 6)};
+        } else {
+            const uint32_t x = w << 2, y = w >> 6;
+            return u32x4{two(x), six(x), two(y), six(y)};
+        }
+    }
+    // The lower and upper codes of two values' bytes (bits 0..7 of either half)
+    __device__ __forceinline__ uint32_t low(uint32_t x) const
+    {
+        if constexpr (Zeros<T>::kNone) return bare(x << 6);
+        else return six(x << 6);
+    }
+    __device__ __forceinline__ uint32_t high(uint32_t x) const
+    {
+        if constexpr (Zeros<T>::kNone) return bare(x << 2);
+        else if constexpr (Zeros<T>::kHigh == 71.5f) return four(x);
+        else return six(x << 2);
+    }
+    // c - 7.5, exactly
+    __device__ __forceinline__ uint32_t bare(uint32_t x) const
+    {
+        const f16x2 off = {(_Float16)-23.5f, (_Float16)-23.5f};
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, six(x)) + off);
+    }
+};
 
 template <int HD> struct Geo {
     static constexpr int kG = HD / kGroup;              // groups of a row
@@ -145,7 +205,7 @@ template <int HD> struct Geo {
     static constexpr int kPairCopies = (kG + 1) / 2;    // of their pairs: 64 a copy
     static constexpr int kOps = 2 * kCopies + 2 * kPairCopies + 1;      // of a tile, its ids among them
     // a wave's LDS: a ring of tiles, one of page ids, scales and mids of the tile at hand
-    static constexpr int kDepth = HD == 256 ? 3 : Q4D;
+    static constexpr int kDepth = HD == 256 ? 3 : 2;
     static constexpr int kCodes = kTile * kRow, kPairs = kPairCopies * 256;
     static constexpr int kSlot = 2 * kCodes + 2 * kPairs;
     static constexpr int kIds = kDepth * kSlot, kScales = kIds + kDepth * 256;
@@ -331,9 +391,9 @@ template <int HD> struct Slot {
         }
         return e;
     }
-    // The tile's pairs as floats: scales and mids - 7.5 scales of the keys, scales (times
-    // 2^(kUp - E)) and mids of the values, each [group][lane group][eight keys]; 0 for a
-    // key that is not there.
+    // The tile's pairs as floats: scales and mids of the keys, scales (times 2^(kUp - E)) and
+    // mids of the values, each [group][lane group][eight keys]; 0 for a key that is not
+    // there.
     __device__ __forceinline__ void spread(float *to, uint32_t there, int E) const
     {
         const int lane = threadIdx.x & 63, key = lane & 31;
@@ -348,7 +408,7 @@ template <int HD> struct Slot {
             // a scale that is not finite makes the mid so: p = 0 keeps it out by the mid alone
             if (!(vs >= 0.f && vs < INFINITY)) vs = 0.f, vm = __builtin_nanf("");
             to[2 * i * kTile] = in ? s : 0.f;
-            to[(G::kG + 2 * i) * kTile] = in ? fmaf(-7.5f, s, m) : 0.f;
+            to[(G::kG + 2 * i) * kTile] = in ? m : 0.f;
             to[(2 * G::kG + 2 * i) * kTile] = in ? __builtin_amdgcn_ldexpf(vs, kUp - E) : 0.f;
             to[(3 * G::kG + 2 * i) * kTile] = in ? vm : 0.f;
         }
@@ -388,12 +448,12 @@ template <int HD> struct Slot {
 template <typename T, int HD, int RT> struct Rows {
     using G = Geo<HD>;
     static constexpr int N = kParts<T>;
-    // fp32 takes C off B tile by tile, so that B stays as small as the output: its sums'
-    // roundings count there.
-    static constexpr bool kCentred = N > 1;
+    static constexpr bool kCentred = Zeros<T>::kNone;       // nothing to take off the sums
     u32x4 q[RT][N][HD / 32];
     float qsum[RT][G::kG];
-    f32x4 o[RT][HD / 16], ps[RT][G::kG];    // B 2^-24 (16 B 2^-24 where odd), and C in every element
+    f32x4 less[RT][G::kG];                  // -R in every element, which the products begin with
+    Unpack<T> unpack;
+    f32x4 o[RT][HD / 16], ps[RT][G::kG];    // B, and C in every element
     float mids[RT][G::kG];                  // this lane's keys' part of sum p m
     float m[RT], l[RT];                     // running maximum (exp2's domain); this lane's part of sum p
     float c[RT], c_low[RT];                 // exp2's factors, the row's scaling taken back
@@ -427,29 +487,31 @@ template <typename T, int HD, int RT> struct Rows {
             top = groups_max(top);
             const int up = 15 - __builtin_amdgcn_frexp_expf(top);       // top 2^up in [2^14, 2^15)
             // factors that are not 0 (a hidden key's -inf times 0 is none) and finite
-            c[t] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c, 24 - up), 0x1p-149f), 3.0e38f);
-            c_low[t] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c_low, 24 - up), 0x1p-149f), 3.0e38f);
+            c[t] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c, -up), 0x1p-149f), 3.0e38f);
+            c_low[t] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c_low, -up), 0x1p-149f), 3.0e38f);
 #pragma unroll
             for (int g = 0; g < G::kG; g++) {
-                float sum = 0.f;
+                float even = 0.f, odd = 0.f;
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         f[g][hf][i] = __builtin_amdgcn_ldexpf(f[g][hf][i], up);
-                        sum += f[g][hf][i];
+                        (i & 1 ? odd : even) += f[g][hf][i];
                     }
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        // the odd codes come 16 times as large
-                        const float less = i & 1 ? 0.0625f : 1.0f;
                         uint32_t part[N];
-                        cut<N>(f[g][hf][i] * less, f[g][hf][i + 4] * less, part);
+                        cut<N>(f[g][hf][i], f[g][hf][i + 4], part);
 #pragma unroll
                         for (int p = 0; p < N; p++) q[t][p][2 * g + hf][i] = part[p];
                     }
                 }
-                qsum[t][g] = groups_sum(sum) * 0x1p-24f;
+                even = groups_sum(even);
+                odd = groups_sum(odd);
+                qsum[t][g] = even + odd;
+                const float r = kCentred ? 0.f : -Zeros<T>::kEven * even - Zeros<T>::kOdd * odd;
+                less[t][g] = f32x4{r, r, r, r};
                 ps[t][g] = f32x4{0, 0, 0, 0};
                 mids[t][g] = 0.f;
             }
@@ -511,15 +573,14 @@ template <typename T, int HD, int RT> struct Rows {
             for (int g = 0; g < G::kG; g++) {
                 f32x4 acc[RT];
 #pragma unroll
-                for (int r = 0; r < RT; r++) acc[r] = f32x4{0, 0, 0, 0};
+                for (int r = 0; r < RT; r++) acc[r] = kCentred ? f32x4{0, 0, 0, 0} : less[r][g];
+                const u32x4 k[2] = {unpack.key(slot.key_codes(codes, g, 0)), unpack.key(slot.key_codes(codes, g, 1))};
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++) {
-                    const u32x4 k = eight_codes(slot.key_codes(codes, g, hf));
+                for (int p = 0; p < N; p++)
 #pragma unroll
-                    for (int r = 0; r < RT; r++)
+                    for (int hf = 0; hf < 2; hf++)
 #pragma unroll
-                        for (int p = 0; p < N; p++) acc[r] = mma(k, q[r][p][2 * g + hf], acc[r]);
-                }
+                        for (int r = 0; r < RT; r++) acc[r] = mma(k[hf], q[r][p][2 * g + hf], acc[r]);
                 const f32x4 scale = four(0, g, t);
 #pragma unroll
                 for (int r = 0; r < RT; r++)
@@ -587,23 +648,15 @@ template <typename T, int HD, int RT> struct Rows {
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         uint32_t part[N];
-                        cut<N>(p[r][4 * t + 2 * i] * scale[2 * i], p[r][4 * t + 2 * i + 1] * scale[2 * i + 1], part);
+                        cut_products<N>(p[r][4 * t + 2 * i], scale[2 * i], p[r][4 * t + 2 * i + 1], scale[2 * i + 1], part);
 #pragma unroll
                         for (int n = 0; n < N; n++) w[r][n][2 * t + i] = part[n];
                     }
                 }
                 const u32x4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-                f32x4 sum = kCentred ? f32x4{0, 0, 0, 0} : ps[r][g];
+                if (!kCentred)
 #pragma unroll
-                for (int n = 0; n < N; n++) sum = mma(ones, w[r][n], sum);
-                if (!kCentred) ps[r][g] = sum;
-                else
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            o[r][4 * g + j][i] = fmaf(j & 1 ? -120 * 0x1p-24f : -7.5f * 0x1p-24f, sum[i],
-                                                      o[r][4 * g + j][i]);
+                    for (int n = 0; n < N; n++) ps[r][g] = mma(ones, w[r][n], ps[r][g]);
             }
 #pragma unroll
             for (int j = 0; j < 4; j += 2) {
@@ -614,7 +667,12 @@ template <typename T, int HD, int RT> struct Rows {
                 for (int i = 0; i < 4; i++)
                     x[i] = __builtin_amdgcn_perm(codes[2 * i + 1][word], codes[2 * i][word],
                                                  0x0c000c00u | (uint32_t)(byte + 4) << 16 | (uint32_t)byte);
-                const u32x4 low = x & kLower, high = x & kUpper;
+                u32x4 low, high;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    low[i] = unpack.low(x[i]);
+                    high[i] = unpack.high(x[i]);
+                }
 #pragma unroll
                 for (int r = 0; r < RT; r++)
 #pragma unroll
@@ -638,10 +696,12 @@ template <typename T, int HD, int RT> struct Rows {
                 const float add = groups_sum(mids[r][g]);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float off = kCentred ? add : add - 7.5f * __builtin_amdgcn_ldexpf(ps[r][g][i], up);
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        o[r][4 * g + j][i] = off + __builtin_amdgcn_ldexpf(o[r][4 * g + j][i], up + (j & 1 ? 20 : 24));
+                    for (int j = 0; j < 4; j++) {
+                        const float b = o[r][4 * g + j][i];
+                        const float z = j & 1 ? Zeros<T>::kHigh : Zeros<T>::kLow;
+                        o[r][4 * g + j][i] = add + __builtin_amdgcn_ldexpf(kCentred ? b : fmaf(-z, ps[r][g][i], b), up);
+                    }
                 }
             }
         }
@@ -724,11 +784,350 @@ __device__ __forceinline__ void join_waves(const AttnArgs &a, Rows<T, HD, RT> &w
     }
 }
 
-template <int HD> constexpr int attn_lds()
+// ---- a shared prefix against many rows ------------------------------------------------------------
+// 64 RT rows a block of one kv head, 16 RT a wave, for bf16 queries: with that many rows
+// a tile's values are worth making once, as fp16 numbers in LDS for all four waves, and
+// the scales' products with every row fall away.  Keys and values are taken against
+// the largest exponents of the block's keys, found in a first pass over their pairs:
+// (c - 8) s + (m + s / 2) in two packed operations, rounded once to fp16 (11 bits down to
+// 2^-28 of the largest value), an eighth of a bf16 query's and output's own rounding.
+//
+// A slot of 16 bytes holds eight values in the order 0 4 1 5 2 6 3 7 that the codes'
+// masks give them; queries are read in that order, and outputs put back.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+template <int HD> struct Made {
+    static constexpr int kKeys = HD == 256 ? 32 : 64;               // of a tile
+    static constexpr int kSlots = HD / 8, kRow = HD * 2;            // slots and bytes of a row
+    static constexpr int kLanes = kBlock / 2 / kKeys;               // threads a row of keys, or of values
+    static constexpr int kPiece = HD / 2 / kLanes;                  // bytes of codes a thread takes
+    static constexpr int kSide = kKeys * kRow;                      // bytes of the keys, or the values
+    static constexpr int kThere = 4 * kSide;                        // two buffers, then flags and sums
+    static constexpr int kLds = kThere + 2 * kKeys * 4 + kAttnWaves * 8;
+    static_assert(kPiece == 16 || kPiece == 32, "whole loads");
+    // Slot s of a row lies at s ^ mix(row): 16 rows' equal slots on different banks, and four
+    // rows' equal quads of slots for the transpose reads of the values
+    static __device__ __forceinline__ constexpr int mix(int row)
+    {
+        if (kSlots == 8) return (row >> 1 & 1) << 2 | (row >> 3 & 1) << 1 | (row >> 2 & 1);
+        return (row & 3) << 2 | (row >> 2 & 3);
+    }
+};
+
+// The largest exponent of a group's values: of max(8 s, |m|), which half of none exceeds
+__device__ __forceinline__ int pair_exponent(uint32_t p)
 {
+    const float x = fmaxf(8.f * pair_scale(p), fabsf(pair_mid(p)));
+    return x > 0.f && x < INFINITY ? __builtin_amdgcn_frexp_expf(x) : kNone;
+}
+
+// One thread's codes and pairs of a tile: a piece of one row, of the keys (the block's
+// first half) or the values
+template <int HD> struct Raw {
+    using M = Made<HD>;
+    static constexpr int kG = HD / kGroup, kWords = M::kPiece / 4;
+    uint32_t w[kWords], pair[kG];
+    int32_t id;                             // page of the next tile's row
+    uint32_t at;
+    bool in;
+
+    static __device__ __forceinline__ int side() { return threadIdx.x / (kBlock / 2); }
+    static __device__ __forceinline__ int row() { return threadIdx.x % (kBlock / 2) / M::kLanes; }
+    static __device__ __forceinline__ int piece() { return threadIdx.x % M::kLanes; }
+
+    __device__ __forceinline__ void look(const AttnArgs &a, int32_t key0, int32_t end)
+    {
+        const int32_t j = key0 + row();
+        id = -1;
+        if (j >= end) return;
+        const uint32_t entry = cbq_div((uint32_t)j, a.pool.page);
+        at = (uint32_t)j - entry * a.pool.page.d;
+        id = a.prefix_table[entry];
+    }
+    // The tile that look() has found the pages of; no key, or an id outside the pool: zeros
+    __device__ __forceinline__ void load(const AttnArgs &a, int h)
+    {
+        in = id >= 0 && id < a.pool.n_pages;
+        const uint32_t p = in ? id : 0, r = in ? at : 0;
+        const char *codes = (side() ? a.pool.codes[1] : a.pool.codes[0]) +
+                            (uint64_t)(code_at(a.pool, p, r) + h * a.pool.code_st[1]) * kCodeUnit + piece() * M::kPiece;
+        const uint32_t *pairs = (side() ? a.pool.pairs[1] : a.pool.pairs[0]) +
+                                (uint64_t)(pair_at(a.pool, p, r) + h * a.pool.pair_st[1]);
+#pragma unroll
+        for (int i = 0; i < kWords / 4; i++) *(u32x4 *)(w + 4 * i) = *(const u32x4 *)(codes + 16 * i);
+#pragma unroll
+        for (int g = 0; g < kG; g++) pair[g] = pairs[g];
+    }
+    // The values of the piece, times 2^up, slot by slot into a tile whose keys begin at `tile`
+    static constexpr int kMine = kWords;    // slots a thread
+    f16x2 off[kG], low[kG], high[kG];       // m + s / 2, s and s / 16, twice
+
+    __device__ __forceinline__ void begin(float *there, int up)
+    {
+#pragma unroll
+        for (int g = 0; g < kG; g++) {
+            float s = __builtin_amdgcn_ldexpf(pair_scale(pair[g]), up), m = __builtin_amdgcn_ldexpf(pair_mid(pair[g]), up);
+            if (!(s >= 0.f && s < INFINITY)) s = 0.f, m = __builtin_nanf("");
+            if (!in) s = m = 0.f;
+            const _Float16 b = (_Float16)fmaf(0.5f, s, m), one = (_Float16)s, part = (_Float16)(s * 0.0625f);
+            off[g] = f16x2{b, b};
+            low[g] = f16x2{one, one};
+            high[g] = f16x2{part, part};
+        }
+        if (threadIdx.x < kBlock / 2 && piece() == 0) there[row()] = in ? 0.f : -INFINITY;
+    }
+    __device__ __forceinline__ void slot(char *tile, int i) const
+    {
+        const int g = i % kG, n = i / kG;
+        // the words of four values of every group, twice: eight of group g
+        uint32_t x;
+        if constexpr (HD == 64) x = w[n];
+        else x = __builtin_amdgcn_perm(w[(2 * n + 1) * (kG / 2) + g / 2], w[2 * n * (kG / 2) + g / 2],
+                                       g & 1 ? 0x07060302u : 0x05040100u);
+        const f16x2 eight = {(_Float16)-1032.f, (_Float16)-1032.f}, more = {(_Float16)-1152.f, (_Float16)-1152.f};
+        constexpr uint32_t kLower = 0x000f000fu, kUpper = 0x00f000f0u;      // 1024 + c, 1024 + 16 c
+        auto half = [](uint32_t y, uint32_t mask) { return __builtin_bit_cast(f16x2, (y & mask) | 0x64006400u); };
+        const f16x2 x0 = (half(x, kLower) + eight) * low[g] + off[g], x1 = (half(x, kUpper) + more) * high[g] + off[g],
+                    x2 = (half(x >> 8, kLower) + eight) * low[g] + off[g],
+                    x3 = (half(x >> 8, kUpper) + more) * high[g] + off[g];
+        const int at = 8 * g + piece() * (8 / M::kLanes) + n;
+        *(u32x4 *)(tile + side() * M::kSide + row() * M::kRow + (at ^ M::mix(row())) * 16) =
+            u32x4{__builtin_bit_cast(uint32_t, x0), __builtin_bit_cast(uint32_t, x1),
+                  __builtin_bit_cast(uint32_t, x2), __builtin_bit_cast(uint32_t, x3)};
+    }
+};
+
+template <typename T, int HD, int RT>
+__device__ __forceinline__ void shared_rows(const AttnArgs &a, char *lds, const Work &w, int row0, int n, int part)
+{
+    using M = Made<HD>;
+    constexpr int kC = HD / 32, kD = HD / 16;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15,
+              g4 = lane >> 4;
+    const int32_t first = w.first * kTile, end = (int32_t)cbq_min((int64_t)w.end * kTile, a.prefix);
+    float *there = (float *)(lds + M::kThere);
+    int2 *tops = (int2 *)(lds + M::kThere + 2 * M::kKeys * 4);
+    Raw<HD> raw;
+    raw.look(a, first, end);
+    // the queries: rows row0 + 16 (RT wave + t) + lane % 16
+    u32x4 q[RT][kC];
+    f32x4 o[RT][kD];
+    float m[RT], l[RT], c[RT];
+    const int mine = row0 + 16 * RT * wave;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int row = mine + 16 * t + r;
+        const bool in = row < n;
+        const uint32_t token = cbq_div(in ? row : 0, a.rep), head = (in ? row : 0) - token * a.rep.d;
+        const T *x = (const T *)a.q + token * a.q_st[0] + ((int64_t)w.h * a.rep.d + head) * a.q_st[1];
+        float f[kC][8], top = 0.f;
+#pragma unroll
+        for (int d = 0; d < kC; d++) {
+            struct alignas(16) Eight { T e[8]; };
+            const Eight e = *(const Eight *)(x + 32 * d + 8 * g4);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                f[d][i] = in ? (float)e.e[i] * a.q_mul : 0.f;
+                top = fmaxf(top, fabsf(f[d][i]));
+            }
+        }
+        const int up = 15 - __builtin_amdgcn_frexp_expf(groups_max(top));
+        c[t] = __builtin_amdgcn_ldexpf(a.c, -up);
+#pragma unroll
+        for (int d = 0; d < kC; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t one[1];
+                cut<1>(__builtin_amdgcn_ldexpf(f[d][i], up), __builtin_amdgcn_ldexpf(f[d][i + 4], up), one);
+                q[t][d][i] = one[0];
+            }
+#pragma unroll
+        for (int d = 0; d < kD; d++) o[t][d] = f32x4{0, 0, 0, 0};
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+    }
+    // largest exponents of the part's keys and values, eight keys' pairs under way at once
+    int2 top = {kNone, kNone};
+    constexpr int kAhead = 8;
+    for (int32_t j0 = first + tid; j0 < end; j0 += kAhead * kBlock) {
+        uint64_t po[kAhead];
+        bool in[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const int32_t j = j0 + i * kBlock;
+            const uint32_t entry = cbq_div((uint32_t)(j < end ? j : j0), a.pool.page);
+            const uint32_t row = (uint32_t)(j < end ? j : j0) - entry * a.pool.page.d;
+            const int32_t id = a.prefix_table[entry];
+            in[i] = j < end && id >= 0 && id < a.pool.n_pages;
+            po[i] = pair_at(a.pool, in[i] ? id : 0, in[i] ? row : 0) + w.h * a.pool.pair_st[1];
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; i++)
+#pragma unroll
+            for (int g = 0; g < HD / kGroup; g++) {
+                const int x = pair_exponent(a.pool.pairs[0][po[i] + g]), y = pair_exponent(a.pool.pairs[1][po[i] + g]);
+                top.x = max(top.x, in[i] ? x : kNone);
+                top.y = max(top.y, in[i] ? y : kNone);
+            }
+    }
+    for (int i = 32; i > 0; i >>= 1) {
+        top.x = max(top.x, __shfl_xor(top.x, i));
+        top.y = max(top.y, __shfl_xor(top.y, i));
+    }
+    if (lane == 0) tops[wave] = top;
+    raw.load(a, w.h);
+    raw.look(a, first + M::kKeys, end);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kAttnWaves; i++) {
+        top.x = max(top.x, tops[i].x);
+        top.y = max(top.y, tops[i].y);
+    }
+    // a value is below 2^(top + 1): 2^14 of it is left
+    const int k_up = top.x == kNone ? 0 : 13 - __builtin_amdgcn_readfirstlane(top.x),
+              v_up = top.y == kNone ? 0 : 13 - __builtin_amdgcn_readfirstlane(top.y);
+#pragma unroll
+    for (int t = 0; t < RT; t++) c[t] = fminf(fmaxf(__builtin_amdgcn_ldexpf(c[t], -k_up), 0x1p-149f), 3.0e38f);
+    int buffer = 0;
+    const int up = Raw<HD>::side() ? v_up : k_up;
+    raw.begin(there, up);
+#pragma unroll
+    for (int i = 0; i < Raw<HD>::kMine; i++) raw.slot(lds, i);
+    for (int32_t key = first; key < end; key += M::kKeys) {
+        __syncthreads();                                // the tile is there
+        raw.load(a, w.h);                               // the next one (past the end: zeros)
+        raw.look(a, key + 2 * M::kKeys, end);
+        const char *K = lds + buffer * 2 * M::kSide, *V = K + M::kSide;
+        const float *bias = there + buffer * M::kKeys;
+        const bool hidden = __ballot(lane < M::kKeys && bias[lane < M::kKeys ? lane : 0] != 0.f);
+        constexpr int kT = M::kKeys / 16;
+        f32x4 s[RT][kT];
+#pragma unroll
+        for (int t = 0; t < kT; t++) {
+#pragma unroll
+            for (int x = 0; x < RT; x++) s[x][t] = f32x4{0, 0, 0, 0};
+            const int row = 16 * t + r;
+#pragma unroll
+            for (int d = 0; d < kC; d++) {
+                const u32x4 e = *(const u32x4 *)(K + row * M::kRow + ((4 * d + g4) ^ M::mix(row)) * 16);
+#pragma unroll
+                for (int x = 0; x < RT; x++) s[x][t] = mma(e, q[x][d], s[x][t]);
+            }
+        }
+        if (hidden)
+#pragma unroll
+            for (int t = 0; t < kT; t++) {
+                const f32x4 b = *(const f32x4 *)(bias + 16 * t + 4 * g4);
+#pragma unroll
+                for (int x = 0; x < RT; x++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[x][t][i] = b[i] == 0.f ? s[x][t][i] : -INFINITY;
+            }
+        u32x4 p[RT][kT / 2];
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            float high = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < kT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) high = fmaxf(high, s[x][t][i]);
+            if (__ballot(high * c[x] > m[x])) {
+                high = groups_max(high) * c[x];
+                const float to = high > m[x] ? high + kSlack : m[x];
+                const float f = high > m[x] ? __builtin_amdgcn_exp2f(m[x] - to) : 1.0f;
+                m[x] = to;
+                l[x] *= f;
+#pragma unroll
+                for (int d = 0; d < kD; d++) o[x][d] *= f;
+            }
+            const float base = m[x] == -INFINITY ? 0.f : -m[x];
+#pragma unroll
+            for (int t = 0; t < kT; t++) {
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    e[i] = __builtin_amdgcn_exp2f(fmaf(c[x], s[x][t][i], base));
+                    l[x] += e[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    uint32_t one[1];
+                    cut<1>(e[2 * i], e[2 * i + 1], one);
+                    p[x][t / 2][t % 2 * 2 + i] = one[0];
+                }
+            }
+        }
+        // The values' products, a slot of the next tile made beside every second: lane (g4, r)
+        // points the transpose read at key 4 g4 + r / 4, values 4 (r % 4) .. of sixteen, and
+        // gets keys 4 g4 .. + 3 of value r.
+        buffer ^= 1;
+        char *next = lds + buffer * 2 * M::kSide;
+        raw.begin(there + buffer * M::kKeys, up);
+        constexpr int kSteps = kT / 2 * kD, kEvery = kSteps / Raw<HD>::kMine;
+#pragma unroll
+        for (int step = 0; step < kSteps; step++) {
+            const int d = step % kD, k0 = step / kD * 32;
+            u32x4 e;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int row = k0 + 16 * t + 4 * g4 + (r >> 2);
+                const char *from = V + row * M::kRow + ((2 * d + (r >> 1 & 1)) ^ M::mix(row)) * 16 + (r & 1) * 8;
+                const u32x2 four = __builtin_bit_cast(
+                    u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s16x4 *)from));
+                e[2 * t] = four[0];
+                e[2 * t + 1] = four[1];
+            }
+#pragma unroll
+            for (int x = 0; x < RT; x++) o[x][d] = mma(e, p[x][k0 / 32], o[x][d]);
+            if (step % kEvery == 0) raw.slot(next, step / kEvery);
+        }
+    }
+    // a wave's rows through its part of LDS, in the values' order
+    __syncthreads();
+    float *out = (float *)(lds + wave * 16 * HD * 4);
+    constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int from = mine + 16 * t;
+        if (from >= n) break;
+        const float total = groups_sum(l[t]);
+#pragma unroll
+        for (int d = 0; d < kD; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int at = d * 16 + 8 * (g4 >> 1) + (g4 & 1 ? kOrder[4 + i] : kOrder[i]);
+                out[r * HD + (at ^ (r & 7) << 2)] = __builtin_amdgcn_ldexpf(o[t][d][i], -v_up);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const int rows = n - from < 16 ? n - from : 16;
+        for (int e = lane; e < 16 * (HD / 4); e += CBQ_WAVE) {
+            const int rr = e / (HD / 4), piece = e % (HD / 4);
+            const float sum = __shfl(total, rr);
+            const f32x4 x = *(const f32x4 *)(out + rr * HD + (piece ^ (rr & 7)) * 4);
+            const uint32_t row = from + rr, token = cbq_div(row, a.rep);
+            if (rr < rows) put_values<T, HD>(a, part, token, w.h * a.rep.d + row - token * a.rep.d, piece * 4, x, sum);
+        }
+        if (part >= 0 && lane < rows) {
+            const uint32_t row = from + r, token = cbq_div(row, a.rep);
+            a.part_ml[((int64_t)part * a.batch * a.tokens + token) * a.n_q + (int64_t)w.h * a.rep.d + row -
+                      token * a.rep.d] = make_float2(m[t], total);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+
+template <int HD, int RT> constexpr int attn_lds()
+{
+    constexpr int made = RT ? Made<HD>::kLds : 0;
     constexpr int tiles = kAttnWaves * Geo<HD>::kWave;
     constexpr int join = kAttnWaves * 16 * Geo<HD>::kWide * 4 + kAttnWaves * 16 * 8 + 16 * 4;
-    return tiles > join ? tiles : join;
+    constexpr int both = tiles > join ? tiles : join;
+    return both > made ? both : made;
 }
 
 // Rows row0 .. (of n) against the key tiles [first, end); seq -1: prefix rows of the
@@ -768,19 +1167,17 @@ __device__ __forceinline__ void walk(const AttnArgs &a, char *lds, const Work &w
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        // the first token sees the fewest own keys
         const int32_t key0 = (tile - pre_tiles) * kTile;
+        const bool own_end = tile >= pre_tiles && key0 + kTile > length - a.tokens + 1;
         uint32_t bits[RT];
-        bool whole = there == ~0u;
+        if (there != ~0u || own_end)
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            bits[t] = there;
-            if (tile >= pre_tiles) {
-                const int32_t left = sees[t] - key0;
-                if (left < kTile) bits[t] &= left <= 0 ? 0u : (1u << left) - 1;
+            for (int t = 0; t < RT; t++) {
+                const int32_t left = own_end ? sees[t] - key0 : kTile;
+                bits[t] = there & (left >= kTile ? ~0u : left <= 0 ? 0u : (1u << left) - 1);
             }
-            whole = whole && bits[t] == ~0u;
-        }
-        rows.tile(slot, scales, bits, !__all(whole));
+        rows.tile(slot, scales, bits, there != ~0u || own_end);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -789,7 +1186,14 @@ __device__ __forceinline__ void walk(const AttnArgs &a, char *lds, const Work &w
     join_waves<T, HD, RT>(a, rows, lds, w.h, token0, row0, n, to);
 }
 
-template <typename T, int HD, int RT> __global__ __launch_bounds__(kBlock, HD == 256 ? 1 : RT == 1 ? Q4W : RT == 2 ? 2 : 1) void q4_kernel(AttnArgs a)
+// Waves a SIMD: their registers, and tiles two (or, of one wave, three) deep in LDS, leave
+// room for so many.  24 sequences of 4000 to 32000 keys, bf16, hd 128: three waves two
+// tiles deep 114 us, two waves three deep 143, four waves (which spill) two deep 133.
+constexpr int simd_waves(int hd, int rt) { return hd == 256 ? 1 : rt ? 2 : 3; }
+
+// RT: 64 RT rows a block of the prefix; 0: 16, as the own keys'.
+template <typename T, int HD, int RT>
+__global__ __launch_bounds__(kBlock, simd_waves(HD, RT)) void q4_kernel(AttnArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int32_t pre_tiles = (a.prefix + kTile - 1) / kTile,
@@ -798,12 +1202,13 @@ template <typename T, int HD, int RT> __global__ __launch_bounds__(kBlock, HD ==
     if (block >= a.plan.blocks) return;
     const Work w = work_of(a.plan, block, a.n_kv, a.batch, pre_tiles, cap_tiles);
     const int to = a.plan.parts > 1 ? w.part : -1, rows = a.tokens * (int)a.rep.d;
-    if constexpr (RT == 1) {
-        walk<T, HD, 1>(a, lds, w, w.tile * 16, w.seq < 0 ? a.batch * rows : rows, to);
-    } else {
-        if (w.seq < 0) walk<T, HD, RT>(a, lds, w, w.tile * 16 * RT, a.batch * rows, to);
-        else walk<T, HD, 1>(a, lds, w, w.tile * 16, rows, to);
+    if constexpr (RT > 0) {
+        if (w.seq < 0) {
+            shared_rows<T, HD, RT>(a, lds, w, w.tile * 64 * RT, a.batch * rows, to);
+            return;
+        }
     }
+    walk<T, HD, 1>(a, lds, w, w.tile * 16, w.seq < 0 ? a.batch * rows : rows, to);
 }
 
 // ---- merge of the parts: a block a (token, head) -------------------------------------------------
@@ -864,7 +1269,7 @@ template <typename T, int HD, int RT> int launch_rows(const AttnArgs &a, hipStre
 {
     const char *what = "cbq_prefix_attn_decode_q4";
     const CbqGrid grid = cbq_grid(a.plan.blocks);
-    constexpr int lds = attn_lds<HD>();
+    constexpr int lds = attn_lds<HD, RT>();
     if (!lds_allowed<q4_kernel<T, HD, RT>>(lds)) return cbq_launch_status(what);
     q4_kernel<T, HD, RT><<<dim3(grid.x, grid.y), kBlock, lds, stream>>>(a);
     return cbq_launch_status(what);
@@ -872,10 +1277,10 @@ template <typename T, int HD, int RT> int launch_rows(const AttnArgs &a, hipStre
 
 template <typename T, int HD> int launch(const AttnArgs &a, hipStream_t stream)
 {
-    constexpr int wide = widest(HD, sizeof(T));
+    constexpr int wide = std::is_same_v<T, __bf16> ? widest(HD) : 0;
     int rc;
-    if (a.plan.rt == 1) rc = launch_rows<T, HD, 1>(a, stream);
-    else if (a.plan.rt == 2) rc = launch_rows<T, HD, wide < 2 ? wide : 2>(a, stream);
+    if (a.plan.rt == 0) rc = launch_rows<T, HD, 0>(a, stream);
+    else if (a.plan.rt == 1) rc = launch_rows<T, HD, wide ? 1 : 0>(a, stream);
     else rc = launch_rows<T, HD, wide>(a, stream);
     if (rc != CK_SUCCESS || a.plan.parts == 1) return rc;
     const CbqGrid grid = cbq_grid((int64_t)a.batch * a.tokens * a.n_q);

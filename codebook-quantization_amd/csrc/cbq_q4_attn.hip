@@ -21,10 +21,10 @@ bool sizes_ok(const cbq_paged_q4 *c, int64_t prefix, int64_t width, int64_t batc
            batch * tokens <= kMaxKeys && batch * tokens * n_q <= kMaxKeys;
 }
 
-bool make_plan(const cbq_paged_q4 *c, int type_bytes, int64_t prefix, int64_t width, int64_t batch,
+bool make_plan(const cbq_paged_q4 *c, int dtype, int64_t prefix, int64_t width, int64_t batch,
                int64_t tokens, int64_t n_q, Plan &p)
 {
-    p = plan(c->hd, type_bytes, c->n_kv, tokens * (n_q / c->n_kv), prefix, width * c->page, batch);
+    p = plan(c->hd, dtype == CBQ_BF16, c->n_kv, tokens * (n_q / c->n_kv), prefix, width * c->page, batch);
     return plan_fits(p);
 }
 
@@ -36,7 +36,7 @@ extern "C" size_t cbq_prefix_attn_decode_q4_workspace(const cbq_paged_q4 *cache,
 {
     Plan p;
     if (!sizes_ok(cache, prefix, width, batch, tokens, n_q) || batch < 1 ||
-        !make_plan(cache, dtype == CBQ_F32 ? 4 : 2, prefix, width, batch, tokens, n_q, p))
+        !make_plan(cache, dtype, prefix, width, batch, tokens, n_q, p))
         return 0;
     return (size_t)p.bytes;
 }
@@ -60,7 +60,7 @@ extern "C" int cbq_prefix_attn_decode_q4(const void *q, const int64_t *q_stride,
     if ((((uintptr_t)q | (uintptr_t)out) & 15) || q_stride[0] * e % 16 || q_stride[1] * e % 16)
         return CK_ERR_ARG;
     AttnArgs a = {};
-    if (!make_plan(cache, (int)e, prefix, width, batch, tokens, n_q, a.plan)) return CK_ERR_ARG;
+    if (!make_plan(cache, dtype, prefix, width, batch, tokens, n_q, a.plan)) return CK_ERR_ARG;
     if (a.plan.bytes && (!workspace || workspace_bytes < (size_t)a.plan.bytes ||
                          ((uintptr_t)workspace & 15) != 0))
         return CK_ERR_ARG;

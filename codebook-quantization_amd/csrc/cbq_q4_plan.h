@@ -9,10 +9,11 @@ namespace cbq_q4 {
 
 constexpr int kTile = 32;                   // keys of a wave's tile
 constexpr int kAttnWaves = 4;               // waves a block, whose tiles take turns
+constexpr int64_t kManyTiles = 16 * 1024;
 constexpr int64_t kMaxBlocks = (1ll << 31) - 1, kMaxParts = 1 << 20, kAttnCus = 256;
 
 struct Plan {
-    int32_t rt;                             // 16 rt rows a block of the prefix
+    int32_t rt;                             // 64 rt rows a block of the prefix, or 0: 16
     int32_t tiles;                          // row tiles of the prefix, of all sequences
     int32_t pre_parts, pre_chunk;           // parts of the prefix and their key tiles
     int32_t own_parts, own_chunk, own_tiles;    // parts of the own keys; 16-row tiles of a sequence
@@ -21,11 +22,8 @@ struct Plan {
     int64_t blocks, bytes;
 };
 
-// 16 widest rows of the prefix a block: as many as a wave's registers hold
-#ifndef Q4RT
-#define Q4RT 1
-#endif
-constexpr int widest(int hd, int type_bytes) { return hd == 256 ? 1 : Q4RT; }
+// 64 widest rows of the prefix a block, as many as a wave's registers hold
+constexpr int widest(int hd) { return hd == 256 ? 1 : 2; }
 
 inline int64_t part_bytes(int64_t parts, int64_t rows, int hd)
 {
@@ -33,26 +31,27 @@ inline int64_t part_bytes(int64_t parts, int64_t rows, int hd)
 }
 
 // rows: query rows of a sequence and kv head (tokens times query heads a kv head)
-inline Plan plan(int hd, int type_bytes, int n_kv, int64_t rows, int64_t prefix, int64_t capacity, int64_t batch)
+inline Plan plan(int hd, bool bf16, int n_kv, int64_t rows, int64_t prefix, int64_t capacity, int64_t batch)
 {
     Plan p = {};
     const int64_t pre_tiles = cbq_ceil(prefix, kTile), cap_tiles = cbq_ceil(capacity, kTile);
     const int64_t own_tiles = cbq_ceil(rows, 16);
-    const int64_t all = cbq_ceil(batch * rows, 16);
-    p.rt = prefix ? (int32_t)cbq_min(all > 2 ? 4 : all, widest(hd, type_bytes)) : 1;
+    const int64_t all = batch * rows;
+    const bool many = bf16 && all > 16 && cbq_ceil(all, 16) * pre_tiles * n_kv >= kManyTiles;
+    p.rt = many ? (int32_t)cbq_min(all > 64 ? 2 : 1, widest(hd)) : 0;
     p.own_tiles = (int32_t)own_tiles;
-    if (pre_tiles + cap_tiles <= 4 * kAttnWaves) {
+    if (pre_tiles + cap_tiles <= 8 * kAttnWaves) {
         p.joint = 1;
-        p.rt = 1;
+        p.rt = 0;
         p.own_parts = p.parts = 1;
         p.own_chunk = (int32_t)cbq_max(pre_tiles + cap_tiles, 1);
         p.blocks = n_kv * batch * own_tiles;
         return p;
     }
-    int64_t tiles = cbq_ceil(batch * rows, 16 * p.rt), pre_parts = 0, pre_chunk = 1;
+    int64_t tiles = cbq_ceil(all, p.rt ? 64 * p.rt : 16), pre_parts = 0, pre_chunk = 1;
     if (pre_tiles) {
-        const int64_t want = cbq_max(1, 2 * kAttnCus / (tiles * n_kv));
-        pre_chunk = cbq_max(2 * kAttnWaves, cbq_ceil(cbq_ceil(pre_tiles, want), kAttnWaves) * kAttnWaves);
+        const int64_t want = cbq_max(1, (p.rt ? kAttnCus : 2 * kAttnCus) / (tiles * n_kv)), unit = p.rt ? 2 : kAttnWaves;
+        pre_chunk = cbq_max(p.rt ? 4 : 2 * kAttnWaves, cbq_ceil(cbq_ceil(pre_tiles, want), unit) * unit);
         pre_parts = cbq_ceil(pre_tiles, pre_chunk);
     } else {
         tiles = 0;

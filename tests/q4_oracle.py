@@ -3,15 +3,21 @@ verification of drafts (torch, CPU), and the batches that the tests run them on.
 
 Tolerances of the attention.  With HALF half a step of fp32, a row's weights p_j,
 and of each key's group g scale s, mid m:
-  - a score is summed from q (c + 16) s and (m - 23.5 s) q: hd products and sums and
-    eight roundings more (the offset, the factors, the maximum, exp2's argument), each
-    off by HALF of S = |scale| max_j sum_d |q_d| (54.5 s + |m|).  That is a relative
-    error of its weight, and twice that of the quotient, of sum p |v| / sum p;
-  - the weighted sums add p s (c + 16), 23.5 p s and p m: n terms, 32 at a time and
-    joined over waves and parts: fewer than n / 16 + 64 half steps of sum p (54.5 s +
-    |m|) / sum p;
-  - p s is cut to the bits of the queries' type: bf16 one part, half a step 2^-8 of it,
-    fp16 two (2^-16), fp32 three (2^-24), times |c - 7.5| <= 7.5;
+  - a score is summed from q (c + z) s, (z + 7.5) q s and q m, z at most 16 (of 16-bit
+    queries 256 for half the codes): hd products and sums and eight roundings more (the
+    factors, the maximum, exp2's argument), each off by HALF of S = |scale| max_j sum_d
+    |q_d| (54.5 s + |m|), 280 s more for 16 bits.  That is a relative error of its weight,
+    and twice that of the quotient, of sum p |v| / sum p;
+  - the weighted sums add p s (c + z), (z + 7.5) p s and p m, z at most 16 (bf16: 64 for
+    half of them): n terms, 32 at a time and joined over waves and parts: fewer than n /
+    16 + 64 half steps of sum p (54.5 s + |m|) / sum p, bf16 151 s;
+  - p s is cut to fp16 numbers, one for 16-bit queries (half a step, 2^-11 of it), two for
+    fp32 (2^-22), times |c - 7.5| <= 7.5, and below 2^-14 of their range to a whole
+    step of 2^-25: n 2^-25 max s / sum p times 7.5;
+  - a prefix that more than 16 rows of bf16 queries share may be made into fp16 numbers
+    first: 2^-11 of each key and value, |m| + 7.5 s of it at most, and 2^-11 of p: a
+    score is off by 2^-11 |scale| max_j sum_d |q_d| (7.5 s + |m|), and the sums by 2^-10
+    of sum p (7.5 s + |m|) / sum p;
   - the output is rounded once, half a step of its type (fp16: 2^-25 at least).
 """
 import random
@@ -21,7 +27,7 @@ import torch
 from serve_oracle import HALF, TYPES, half_step
 
 GROUP = 64
-CUT = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -16}
+CUT = {torch.float32: 2.0 ** -22, torch.bfloat16: 2.0 ** -11, torch.float16: 2.0 ** -11}
 
 
 def order(hd):
@@ -136,7 +142,9 @@ def attend(batch, q, tokens, scale):
         length = len(there) - batch.prefix
         for h in range(batch.n_kv):
             (kc, ks, km), (vc, vs, vm) = (parts(codes[:, i, h], pairs[:, i, h]) for i in range(2))
-            k, v, k_big, v_big = km + ks * kc, vm + vs * vc, 54.5 * ks + km.abs(), 54.5 * vs + vm.abs()
+            k, v = km + ks * kc, vm + vs * vc
+            k_big = (54.5 if batch.dtype == torch.float32 else 334.5) * ks + km.abs()
+            v_big = (151 if batch.dtype == torch.bfloat16 else 54.5) * vs + vm.abs()
             for t in range(tokens):
                 see = there.clone()
                 see[batch.prefix + max(length - (tokens - 1 - t), 0):] = False
@@ -152,7 +160,13 @@ def attend(batch, q, tokens, scale):
                     out[at] = p @ v[see]
                     big = abs(scale) * float((k_big[see] @ x.abs()).max())
                     tol[at] = (half * out[at].abs() + 2 * (batch.hd + 8) * big * HALF * (p @ v[see].abs())
-                               + (n / 16 + 64) * HALF * (p @ v_big[see]) + cut * 7.5 * (p @ vs[see]))
+                               + (n / 16 + 64) * HALF * (p @ v_big[see]) + cut * 7.5 * (p @ vs[see])
+                               + 7.5 * n * 2.0 ** -25 * vs[see].amax(0) * p.max())
+                    if (batch.prefix and tokens * batch.rep * len(batch.lens) > 16
+                            and batch.dtype == torch.bfloat16):
+                        made = vm[see].abs() + 7.5 * vs[see]
+                        big = abs(scale) * float(((km[see].abs() + 7.5 * ks[see]) @ x.abs()).max())
+                        tol[at] += 2.0 ** -10 * ((p @ made) + big * (p @ v[see].abs()))
                     if batch.dtype == torch.float16:
                         tol[at] += 2.0 ** -25
     return out, tol
