@@ -114,13 +114,4 @@ CBQ_PAGED_FN Work work_of(const Plan &p, uint32_t block, int n_kv, int batch, in
     return w;
 }
 
-// Key `lane` of key tile `tile`: its place in its table's order and the keys of that
-// table, `prefix` shared or `length` own ones; place -1 past their end.
-CBQ_PAGED_FN int32_t tile_key(int32_t tile, int32_t pre_tiles, int32_t prefix, int32_t length, int lane)
-{
-    const bool shared = tile < pre_tiles;
-    const int32_t j = (shared ? tile : tile - pre_tiles) * kTile + lane;
-    return j < (shared ? prefix : length) ? j : -1;
-}
-
 }  // namespace cbq_q4
