@@ -5,9 +5,8 @@
 // or value's y, 64 values a group, a scale, a mid and codes.  The codes are steps:
 // a sum in another order, or a rounding on the way, would move a value next to a
 // border to the next code.  So keys are normed, turned and cut in 64 bits, whose
-// rate here is fp32's, and the quotient (y - m) / s, which only a true division
-// places right at a border, is estimated by a reciprocal and settled by its exact
-// remainder.  Queries go in fp32.
+// rate here is fp32's, and a code is the nearest border by a fast quotient and one exact
+// comparison with it.  Queries go in fp32, values stay in theirs.
 //
 // Sixteen lanes hold a row, four neighbouring values of each group a lane, which are
 // neighbours in the row's codes too; a row's sum and a group's range take four
@@ -15,7 +14,12 @@
 // groups, or half a group, the values that turn together are the lane's own, or those of
 // the lane eight away; else the others' are read too (cache hits).  A thread has
 // neighbouring heads of a token, all queries, keys or values, which share what is
-// read of the tables and weights.
+// read of the tables and weights, and asks for all of them before it uses one.
+//
+// Bound by bytes where prompts are long: 12416 tokens of 32 + 8 + 8 heads of 128 in bf16,
+// 268 MB, in 64 us, 4.2 TB/s where a copy of 1 GiB reaches 5.3.  (Heads asked for one by
+// one and every code settled by the remainder of a 64-bit quotient: 98 us.)  By latency
+// where few: one token takes 4 us.
 #include "cbq_q4.h"
 
 namespace {
@@ -57,6 +61,23 @@ __device__ __forceinline__ void load4(const T *p, A (&x)[4])
         for (int i = 0; i < 4; i++) x[i] = (A)(float)p[i];
     }
 }
+
+// A lane's values of a row as they lie in memory, [group][4] from d0 on
+template <typename T, int HD, bool VEC> struct Row {
+    Pack<T, 4> e[HD / kGroup];
+
+    __device__ __forceinline__ void load(const T *x, int d0)
+    {
+#pragma unroll
+        for (int g = 0; g < HD / kGroup; g++) {
+            const T *from = x + g * kGroup + d0;
+            if constexpr (VEC) e[g] = *(const Pack<T, 4> *)from;
+            else
+#pragma unroll
+                for (int i = 0; i < 4; i++) e[g].e[i] = from[i];
+        }
+    }
+};
 
 // x of the lane `by` further on (cyclically) in its sixteen
 template <int BY> __device__ __forceinline__ float rotated(float x)
@@ -102,15 +123,40 @@ template <int HD, int MODE> struct Angles {
     }
 };
 
-// A lane's values of a row, [group][4] from d0 on, normed and turned
+// Its weights of a norm
+template <int HD, bool VEC> struct Weights {
+    float e[HD / kGroup][4];
+
+    __device__ __forceinline__ void load(const float *w, int d0)
+    {
+#pragma unroll
+        for (int g = 0; g < HD / kGroup; g++) load4<float, float, VEC>(w + g * kGroup + d0, e[g]);
+    }
+};
+
+// 1 / sqrt(x): for a double two Newton steps behind an estimate of 20 bits at least
+__device__ __forceinline__ float inv_root(float x) { return 1.f / sqrtf(x); }
+__device__ __forceinline__ double inv_root(double x)
+{
+    double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+    for (int i = 0; i < 2; i++) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
+    return y;
+}
+
+// A lane's values of a row, normed and turned.  x, w: the row and the weights, for values
+// that turn with those of neither this lane nor its neighbour.
 template <typename T, typename A, int HD, int MODE>
-__device__ __forceinline__ void turned(const AppendArgs &a, const T *x, const float *w, int64_t pos,
-                                       int d0, const Angles<HD, MODE> &t, A (&y)[HD / kGroup][4])
+__device__ __forceinline__ void turned(const AppendArgs &a, const Row<T, HD, (MODE != kSingle)> &row,
+                                       const Weights<HD, (MODE != kSingle)> &weights, const T *x,
+                                       const float *w, int64_t pos, int d0, const Angles<HD, MODE> &t,
+                                       A (&y)[HD / kGroup][4])
 {
     constexpr int G = HD / kGroup;
-    constexpr bool kVec = MODE != kSingle;
 #pragma unroll
-    for (int g = 0; g < G; g++) load4<T, A, kVec>(x + g * kGroup + d0, y[g]);
+    for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[g][i] = (A)(float)row.e[g].e[i];
     A r = (A)1;
     if (a.norm) {
         A s = (A)0;
@@ -119,17 +165,14 @@ __device__ __forceinline__ void turned(const AppendArgs &a, const T *x, const fl
 #pragma unroll
             for (int i = 0; i < 4; i++) s += y[g][i] * y[g][i];
         s = over_row(s, [](A p, A q) { return p + q; });
-        r = (A)1 / sqrt(s / (A)HD + (A)a.eps);
+        r = inv_root(s / (A)HD + (A)a.eps);
     }
     const bool scaled = a.norm && w;
 #pragma unroll
     for (int g = 0; g < G; g++) {
-        if (scaled) {
-            A wt[4];
-            load4<float, A, kVec>(w + g * kGroup + d0, wt);
+        if (scaled)
 #pragma unroll
-            for (int i = 0; i < 4; i++) y[g][i] *= wt[i];
-        }
+            for (int i = 0; i < 4; i++) y[g][i] *= (A)weights.e[g][i];
         if (a.norm)
 #pragma unroll
             for (int i = 0; i < 4; i++) y[g][i] *= r;
@@ -181,7 +224,26 @@ __device__ __forceinline__ void turned(const AppendArgs &a, const T *x, const fl
     }
 }
 
-// A group's pair and this lane's four codes of it.  A: the type that holds y exactly.
+// fp32 first, then bf16: the compiler makes one rounding of the two otherwise, which
+// differs where the first ends halfway between two numbers of the second
+__device__ __forceinline__ __bf16 twice_rounded(double x)
+{
+    float y = (float)x;
+    asm("" : "+v"(y));
+    return (__bf16)y;
+}
+
+// A group's scale and mid from its largest and smallest value
+__device__ __forceinline__ void group_pair(double high, double deep, __bf16 &scale, __bf16 &mid)
+{
+    mid = twice_rounded((high + deep) / 2);
+    const double m = (double)(float)mid;
+    // 1 / 7.5: its last place is 2^-29 of the number it is rounded to first
+    scale = twice_rounded(fmax(high - m, m - deep) * (1 / 7.5));
+}
+
+// A group's pair and this lane's four codes of it, for any values.  A: the type that
+// holds y exactly.
 template <typename A> __device__ __forceinline__ void quantise(const A (&y)[4], uint32_t &pair, uint32_t &codes)
 {
     A top = y[0], low = y[0], odd = 0;
@@ -194,13 +256,10 @@ template <typename A> __device__ __forceinline__ void quantise(const A (&y)[4], 
     // the sixteen lanes' answers stand side by side in the wave's
     const uint64_t bad = __ballot(!(odd == 0));
     const bool sound = !(bad >> (threadIdx.x & 48) & 0xffff);
-    const double high = (double)over_row(top, [](A p, A q) { return fmax(p, q); }),
-                 deep = (double)over_row(low, [](A p, A q) { return fmin(p, q); });
-    const __bf16 mb = (__bf16)(float)((high + deep) / 2);
+    __bf16 mb, sb;
+    group_pair((double)over_row(top, [](A p, A q) { return fmax(p, q); }),
+               (double)over_row(low, [](A p, A q) { return fmin(p, q); }), sb, mb);
     const double m = (double)(float)mb;
-    // a 15th: its last place is 2^-29 of the number it is rounded to first
-    const float range = (float)(fmax(high - m, m - deep) * (1 / 7.5));
-    const __bf16 sb = (__bf16)range;
     const float s = (float)sb;
     const uint32_t mid = __builtin_bit_cast(uint16_t, mb), scale = __builtin_bit_cast(uint16_t, sb);
     codes = 0x8888u;
@@ -221,6 +280,59 @@ template <typename A> __device__ __forceinline__ void quantise(const A (&y)[4], 
     }
 }
 
+// The same for ordinary groups, or false (for all lanes of the row): values finite and a
+// scale that is an ordinary number, and then |y - m| < 7.6 s.  So k = rint((y - m) / s) is
+// the nearest border whatever the estimate's roundings, and the code is k + 8, less one
+// where y lies below m + k s.  With y of 32 bits the border has to be a number of 24 bits:
+// m = 0 or exponents of s and m at most 12 apart (of values that scatter about one group
+// in a thousand is not, and of 16-bit ones hardly any).  With y of 64 bits y - m - k s is exact.
+__device__ __forceinline__ bool quick(const float (&y)[4], uint32_t &pair, uint32_t &codes)
+{
+    // the maximum that a NaN passes through
+    auto most = [](float p, float q) { return __builtin_elementwise_maximum(p, q); };
+    auto least = [](float p, float q) { return __builtin_elementwise_minimum(p, q); };
+    const float top = most(most(most(y[0], y[1]), y[2]), y[3]), low = least(least(least(y[0], y[1]), y[2]), y[3]);
+    __bf16 mb, sb;
+    group_pair((double)over_row(top, most), (double)over_row(low, least), sb, mb);
+    const uint32_t mid = __builtin_bit_cast(uint16_t, mb), scale = __builtin_bit_cast(uint16_t, sb);
+    const int em = mid >> 7 & 255, es = scale >> 7 & 255;
+    const bool easy = es - 2u <= 248u && ((mid & 0x7fff) == 0 || (em > 0 && em - es + 12u <= 24u));
+    pair = scale | mid << 16;
+    const float m = (float)mb, s = (float)sb, inv = __builtin_amdgcn_rcpf(s);
+    constexpr float kWhole = 12582912.f + 8.f;      // the integer that is added to stands in the last bits
+    codes = 0;
+#pragma unroll
+    for (int i = 3; i >= 0; i--) {
+        const float u = fmaf(y[i] - m, inv, kWhole);
+        codes = (codes << 4) + (__float_as_uint(u) - (y[i] < fmaf(u - kWhole, s, m)));
+    }
+    return easy;
+}
+__device__ __forceinline__ bool quick(const double (&y)[4], uint32_t &pair, uint32_t &codes)
+{
+    auto most = [](double p, double q) { return fmax(p, q); };
+    auto least = [](double p, double q) { return fmin(p, q); };
+    const double top = most(most(y[0], y[1]), most(y[2], y[3])), low = least(least(y[0], y[1]), least(y[2], y[3]));
+    const double all = (y[0] + y[1]) + (y[2] + y[3]);
+    const uint64_t bad = __ballot(!(fabs(all) < HUGE_VAL));
+    __bf16 mb, sb;
+    group_pair(over_row(top, most), over_row(low, least), sb, mb);
+    const uint32_t mid = __builtin_bit_cast(uint16_t, mb), scale = __builtin_bit_cast(uint16_t, sb);
+    const bool easy = (scale >> 7 & 255) - 2u <= 248u && (mid >> 7 & 255) < 255 && !(bad >> (threadIdx.x & 48) & 0xffff);
+    pair = scale | mid << 16;
+    const float s = (float)sb, inv = __builtin_amdgcn_rcpf(s);
+    const double m = (double)(float)mb, step = (double)s;
+    constexpr float kWhole = 12582912.f + 8.f;
+    codes = 0;
+#pragma unroll
+    for (int i = 3; i >= 0; i--) {
+        const double d = y[i] - m;
+        const float u = fmaf((float)d, inv, kWhole);
+        codes = (codes << 4) + (__float_as_uint(u) - (fma((double)(kWhole - u), step, d) < 0));
+    }
+    return easy;
+}
+
 template <typename T, int HD, int MODE, int R>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a)
 {
@@ -234,16 +346,23 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a)
     const int lane = threadIdx.x % kLanes, d0 = 4 * lane;
     const int64_t st = a.st[kind][1];
     const T *x = (const T *)a.x[kind] + t * a.st[kind][0] + j * st;
-    const int64_t p = a.positions[t];
+    // everything is asked for before the first use
+    Row<T, HD, kVec> rows[R];
+#pragma unroll
+    for (int h = 0; h < R; h++) rows[h].load(x + h * st, d0);
+    const int64_t p = a.positions[t], slot = kind ? a.slots[t] : 0;
     const bool placed = p >= 0 && p < a.n_pos;
     Angles<HD, MODE> angles;
+    Weights<HD, kVec> weights;
+    const float *w = kind < 2 ? a.w[kind] : nullptr;
+    if (a.norm && w) weights.load(w, d0);
     if (kind < 2) angles.load(a, placed ? p : 0, d0);
     if (kind == 0) {
         T *out = (T *)a.q_out + ((int64_t)t * a.n_q + j) * HD + d0;
 #pragma unroll
         for (int h = 0; h < R; h++) {
             float y[G][4];
-            turned<T, float, HD, MODE>(a, x + h * st, a.w[0], placed ? p : 0, d0, angles, y);
+            turned<T, float, HD, MODE>(a, rows[h], weights, x + h * st, w, placed ? p : 0, d0, angles, y);
 #pragma unroll
             for (int g = 0; g < G; g++) {
                 Pack<T, 4> o;
@@ -254,36 +373,66 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a)
         }
         return;
     }
-    const int64_t slot = a.slots[t];
     if (!placed || slot < 0 || slot >= a.n_slots) return;       // uniform over the row's lanes
     const uint32_t id = cbq_div((uint32_t)slot, a.pool.page), r = (uint32_t)slot - id * a.pool.page.d;
-#pragma unroll
-    for (int h = 0; h < R; h++) {
+    const uint32_t code0 = code_at(a.pool, id, r) + j * a.pool.code_st[1],
+                   pair0 = pair_at(a.pool, id, r) + j * a.pool.pair_st[1];
+    auto store = [&](int h, const uint32_t (&pair)[G], const uint32_t (&c)[G]) {
         Pack<uint16_t, G> codes;
-        uint32_t pair[G], c;
-        if (kind == 1) {
-            double y[G][4];
-            turned<T, double, HD, MODE>(a, x + h * st, a.w[1], p, d0, angles, y);
 #pragma unroll
-            for (int g = 0; g < G; g++) {
-                quantise(y[g], pair[g], c);
-                codes.e[g] = (uint16_t)c;
-            }
-        } else {
-#pragma unroll
-            for (int g = 0; g < G; g++) {
-                float y[4];
-                load4<T, float, kVec>(x + h * st + g * kGroup + d0, y);
-                quantise(y, pair[g], c);
-                codes.e[g] = (uint16_t)c;
-            }
-        }
-        const uint32_t at = code_at(a.pool, id, r) + (j + h) * a.pool.code_st[1];
-        *(Pack<uint16_t, G> *)(a.pool.codes[kind - 1] + (uint64_t)at * kCodeUnit + lane * 2 * G) = codes;
-        uint32_t *to = a.pool.pairs[kind - 1] + (uint64_t)(pair_at(a.pool, id, r) + (j + h) * a.pool.pair_st[1]);
+        for (int g = 0; g < G; g++) codes.e[g] = (uint16_t)c[g];
+        *(Pack<uint16_t, G> *)(a.pool.codes[kind - 1] + (uint64_t)(code0 + h * a.pool.code_st[1]) * kCodeUnit +
+                               lane * 2 * G) = codes;
+        uint32_t *to = a.pool.pairs[kind - 1] + (uint64_t)(pair0 + h * a.pool.pair_st[1]);
 #pragma unroll
         for (int g = 0; g < G; g++)
             if (lane == g) to[g] = pair[g];
+    };
+    uint32_t pair[G], c[G], odd = 0;        // odd: heads with a group that is no ordinary one
+    if (kind == 1) {
+#pragma unroll
+        for (int h = 0; h < R; h++) {
+            double y[G][4];
+            turned<T, double, HD, MODE>(a, rows[h], weights, x + h * st, w, p, d0, angles, y);
+            bool easy = true;
+#pragma unroll
+            for (int g = 0; g < G; g++) easy = quick(y[g], pair[g], c[g]) && easy;
+            if (easy) store(h, pair, c);
+            else odd |= 1u << h;
+        }
+        for (; odd; odd &= odd - 1) {
+            const int h = __builtin_ctz(odd);
+            double y[G][4];
+            rows[0].load(x + h * st, d0);
+            turned<T, double, HD, MODE>(a, rows[0], weights, x + h * st, w, p, d0, angles, y);
+#pragma unroll
+            for (int g = 0; g < G; g++) quantise(y[g], pair[g], c[g]);
+            store(h, pair, c);
+        }
+        return;
+    }
+#pragma unroll
+    for (int h = 0; h < R; h++) {
+        bool easy = true;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const float y[4] = {(float)rows[h].e[g].e[0], (float)rows[h].e[g].e[1], (float)rows[h].e[g].e[2],
+                                (float)rows[h].e[g].e[3]};
+            easy = quick(y, pair[g], c[g]) && easy;
+        }
+        if (easy) store(h, pair, c);
+        else odd |= 1u << h;
+    }
+    for (; odd; odd &= odd - 1) {
+        const int h = __builtin_ctz(odd);
+        rows[0].load(x + h * st, d0);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const float y[4] = {(float)rows[0].e[g].e[0], (float)rows[0].e[g].e[1], (float)rows[0].e[g].e[2],
+                                (float)rows[0].e[g].e[3]};
+            quantise(y, pair[g], c[g]);
+        }
+        store(h, pair, c);
     }
 }
 
@@ -338,9 +487,14 @@ struct ReadArgs {
     uint32_t n_kv;
 };
 
+// Bound by its bytes: 30011 rows of 8 heads of 128, 35 MB to 123 MB of bf16, in 32 us, 4.9
+// TB/s where a copy of 1 GiB reaches 5.3.  The values are stored past the caches: with
+// lines kept there for them the same rows take 47 us when the calls before have filled
+// them; 384 rows take 7 us either way.
 template <typename T, int HD> __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a)
 {
     constexpr int G = HD / kGroup;
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T))));     // of four values
     const int64_t at = (int64_t)cbq_block(blockIdx.x, blockIdx.y) * kRows + threadIdx.x / kLanes;
     if (at >= 2 * a.rows) return;
     const int kind = at >= a.rows, lane = threadIdx.x % kLanes;
@@ -364,7 +518,7 @@ template <typename T, int HD> __global__ __launch_bounds__(kThreads) void read_k
 #pragma unroll
         for (int i = 0; i < 4; i++)         // s (c - 7.5) is exact: one rounding in fp32
             o.e[i] = (T)fmaf(pair_scale(pair[g]), (float)(codes.e[g] >> (4 * i) & 15) - 7.5f, pair_mid(pair[g]));
-        *(Pack<T, 4> *)(out + g * kGroup) = o;
+        __builtin_nontemporal_store(__builtin_bit_cast(Words, o), (Words *)(out + g * kGroup));
     }
 }
 

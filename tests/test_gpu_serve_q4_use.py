@@ -16,6 +16,49 @@ def ops(cuda):
     return cbq_ops.load()
 
 
+# ---- many tokens: several heads a thread ----------------------------------------------
+
+@pytest.mark.parametrize("dtype,hd,rot,norm", [("bf16", 128, 128, True), ("f32", 64, 64, True),
+                                               ("f16", 256, 256, False), ("bf16", 64, 16, True)])
+def test_append_many(cuda, ops, dtype, hd, rot, norm):
+    """70000 head rows, among them some whose groups are no ordinary ones: constants, zeros,
+    one value far from the others, numbers too large or small, NaN.  Queries within
+    rounding; every code, scale and mid as the 64-bit form's."""
+    N, H, page, eps = 5900, 4, 16, 1e-6
+    g = torch.Generator().manual_seed(hd)
+    x = torch.randn(N, 3 * H, hd, generator=g)
+    x[7::50, 5] = 2.5
+    x[9::50, 9] = 0.0
+    x[11::50, 10] = 40.0 + 0.001 * x[11::50, 10]
+    x[13::50, 11, 3] = 3e4
+    x[15::50, 8] *= 6e-8 if dtype == "f16" else 1e-36
+    x[17::50, 9] *= 1.5e4 if dtype == "f16" else 1e36
+    x[19::50, 10, 1] = float("nan")
+    x[21::50, 4, hd - 1] = float("inf")
+    x = x.to(so.TYPES[dtype])
+    n_pages = -(-N // page) + 1
+    codes = torch.zeros(n_pages, 2, H, page, hd // 2, dtype=torch.uint8)
+    pairs = torch.zeros(n_pages, 2, H, page, hd // 64, 2, dtype=torch.bfloat16)
+    dev = codes.cuda(), pairs.cuda()
+    angles = torch.rand(90, rot // 2, generator=g, dtype=torch.float64) * 100
+    cos, sin = (torch.cat([t, t], 1).float() for t in (angles.cos(), angles.sin()))
+    positions = torch.randint(0, 90, (N,), generator=g)
+    slots = torch.randperm(n_pages * page, generator=g)[:N]
+    w = [1 + 0.1 * torch.randn(hd, generator=g) if norm else None for _ in range(2)]
+    y = x.cuda()
+    out = ops.paged_append_q4(y[:, :H], y[:, H:2 * H], y[:, 2 * H:], cos.cuda(), sin.cuda(), positions.cuda(),
+                              slots.cuda(), dev[0][:, 0], dev[1][:, 0], dev[0][:, 1], dev[1][:, 1], norm,
+                              *[t if t is None else t.cuda() for t in w], eps)
+    want, mag = so.append_rows(x[:, :H], w[0], cos, sin, positions, norm, eps)
+    small = 2.0 ** -25 if dtype == "f16" else 0.0
+    so.near(out, want, so.half_step(out.dtype) * want.abs() + 32 * so.HALF * mag + small, "append q")
+    keys, _ = so.append_rows(x[:, H:2 * H], w[1], cos, sin, positions, norm, eps)
+    for i, v in enumerate((keys, x[:, 2 * H:])):
+        codes[slots // page, i, :, slots % page], pairs[slots // page, i, :, slots % page] = qo.quantise(v)
+    assert torch.equal(dev[0].cpu(), codes), "codes"
+    assert torch.equal(dev[1].cpu().nan_to_num(7e7), pairs.nan_to_num(7e7)), "pairs"
+
+
 # ---- a long prefix, many rows: tiles of it made into values once ----------------------
 
 @pytest.mark.parametrize("hd,lens,prefix,n_kv,rep,tokens,page,rows_first", [
