@@ -9,6 +9,9 @@ namespace cbq_q4 {
 
 constexpr int kTile = 32;                   // keys of a wave's tile
 constexpr int kAttnWaves = 4;               // waves a block, whose tiles take turns
+// (16 rows, tile, kv head) products of a prefix from which on its tiles are made into values
+// in LDS for all of a block's rows; with fewer the rounds of barriers cost more than they
+// save.  64 sequences of 32 heads behind 30011 keys: 80 us, and 110 with every wave's own.
 constexpr int64_t kManyTiles = 16 * 1024;
 constexpr int64_t kMaxBlocks = (1ll << 31) - 1, kMaxParts = 1 << 20, kAttnCus = 256;
 
@@ -40,22 +43,30 @@ inline Plan plan(int hd, bool bf16, int n_kv, int64_t rows, int64_t prefix, int6
     const bool many = bf16 && all > 16 && cbq_ceil(all, 16) * pre_tiles * n_kv >= kManyTiles;
     p.rt = many ? (int32_t)cbq_min(all > 64 ? 2 : 1, widest(hd)) : 0;
     p.own_tiles = (int32_t)own_tiles;
-    if (pre_tiles + cap_tiles <= 8 * kAttnWaves) {
+    // One block for all keys of a row tile, no parts to join: of few tiles a wave the join
+    // costs as much as it saves, and where every CU has two such blocks parts bring no more
+    // of them.  64 sequences of 32 heads, 900 to 1900 keys: 36 us against 43 in parts, but one
+    // of 1200 keys 18 against 10; 300 to 3800 keys 57 against 49: lengths this uneven.
+    const int64_t alone = n_kv * batch * own_tiles;
+    if (pre_tiles + cap_tiles <= (alone >= 2 * kAttnCus ? 24 : 4) * kAttnWaves) {
         p.joint = 1;
         p.rt = 0;
         p.own_parts = p.parts = 1;
         p.own_chunk = (int32_t)cbq_max(pre_tiles + cap_tiles, 1);
-        p.blocks = n_kv * batch * own_tiles;
+        p.blocks = alone;
         return p;
     }
     int64_t tiles = cbq_ceil(all, p.rt ? 64 * p.rt : 16), pre_parts = 0, pre_chunk = 1;
     if (pre_tiles) {
+        // two blocks a CU for the prefix (four: 33 sequences of 3 tokens behind 5000 keys take 37
+        // us instead of 34); one where they share tiles (two: 97 us instead of 80, above)
         const int64_t want = cbq_max(1, (p.rt ? kAttnCus : 2 * kAttnCus) / (tiles * n_kv)), unit = p.rt ? 2 : kAttnWaves;
         pre_chunk = cbq_max(p.rt ? 4 : 2 * kAttnWaves, cbq_ceil(cbq_ceil(pre_tiles, want), unit) * unit);
         pre_parts = cbq_ceil(pre_tiles, pre_chunk);
     } else {
         tiles = 0;
     }
+    // four blocks a CU for the own keys (two: 36 us instead of 34, there), 4 to 64 tiles each
     const int64_t share = cbq_ceil(cap_tiles * batch * n_kv * own_tiles, 4 * kAttnCus);
     int64_t own_chunk = cbq_min(cbq_max(cbq_ceil(share, kAttnWaves), 1), 16) * kAttnWaves;
     // more of a wider table than its parts and blocks are counted for

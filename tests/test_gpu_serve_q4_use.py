@@ -106,6 +106,16 @@ def test_shared_large_scores(cuda, ops):
         check(ops, batch, 1, f"scale {scale}", scale, batch.queries(1, 3.0))
 
 
+# ---- many sequences: a block for all of a sequence's keys --------------------------------
+
+@pytest.mark.parametrize("dtype,hd,prefix,page", [("bf16", 64, 500, 32), ("f16", 128, 0, 24), ("f32", 64, 77, 64),
+                                                  ("bf16", 256, 300, 16)])
+def test_many_sequences(cuda, ops, dtype, hd, prefix, page):
+    """520 blocks and more, prefix and own keys in one walk, lengths of 0 to 900."""
+    batch = qo.Batch([i * 61 % 900 for i in range(130)], prefix, 4, 2, hd, page, dtype, room=0, seed=hd + prefix)
+    check(ops, batch, 1, f"{dtype} hd={hd} 130 sequences behind {prefix}")
+
+
 # ---- far pages, streams, graphs ---------------------------------------------------------
 
 def test_far_pages(cuda, ops):
