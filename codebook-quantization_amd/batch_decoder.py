@@ -304,7 +304,8 @@ class BatchDecoder:
         """n_new tokens of each prompt behind the prefix, drawn from softmax(logits /
         temperature) (EOS ignored).  drafts: that many tokens a step at most, those that
         followed the sequence's two newest tokens where they stood last before, are run
-        beside the newest one.  generator: of the device's random numbers."""
+        beside the newest one; pages and positions have to suffice for them too, n_new +
+        drafts tokens behind each prompt.  generator: of the device's random numbers."""
         if not temperature > 0:
             raise ValueError(f"a temperature of {temperature}")
         if drafts < 0:

@@ -57,17 +57,20 @@ inline Plan plan(int hd, bool bf16, int n_kv, int64_t rows, int64_t prefix, int6
         return p;
     }
     int64_t tiles = cbq_ceil(all, p.rt ? 64 * p.rt : 16), pre_parts = 0, pre_chunk = 1;
+    // Blocks a CU: two for the prefix (four: 33 sequences of 3 tokens behind 5000 keys take 37
+    // us instead of 34), four for the own keys, 4 to 64 tiles each (two: 36 us, there).  One
+    // for each with hd 256, of which a CU holds one block (two and four: one sequence of 9000
+    // keys 31 us instead of 21, 50 of 2 tokens behind 2000 keys 52 instead of 44); one for
+    // a prefix whose tiles are shared (two: 97 us instead of 80, above).
+    const int64_t pre_blocks = (p.rt || hd == 256 ? 1 : 2) * kAttnCus, own_blocks = (hd == 256 ? 1 : 4) * kAttnCus;
     if (pre_tiles) {
-        // two blocks a CU for the prefix (four: 33 sequences of 3 tokens behind 5000 keys take 37
-        // us instead of 34); one where they share tiles (two: 97 us instead of 80, above)
-        const int64_t want = cbq_max(1, (p.rt ? kAttnCus : 2 * kAttnCus) / (tiles * n_kv)), unit = p.rt ? 2 : kAttnWaves;
+        const int64_t want = cbq_max(1, pre_blocks / (tiles * n_kv)), unit = p.rt ? 2 : kAttnWaves;
         pre_chunk = cbq_max(p.rt ? 4 : 2 * kAttnWaves, cbq_ceil(cbq_ceil(pre_tiles, want), unit) * unit);
         pre_parts = cbq_ceil(pre_tiles, pre_chunk);
     } else {
         tiles = 0;
     }
-    // four blocks a CU for the own keys (two: 36 us instead of 34, there), 4 to 64 tiles each
-    const int64_t share = cbq_ceil(cap_tiles * batch * n_kv * own_tiles, 4 * kAttnCus);
+    const int64_t share = cbq_ceil(cap_tiles * batch * n_kv * own_tiles, own_blocks);
     int64_t own_chunk = cbq_min(cbq_max(cbq_ceil(share, kAttnWaves), 1), 16) * kAttnWaves;
     // more of a wider table than its parts and blocks are counted for
     const int64_t most = cbq_min(kMaxParts / 2, (kMaxBlocks - n_kv * tiles * pre_parts) / (n_kv * batch * own_tiles));
