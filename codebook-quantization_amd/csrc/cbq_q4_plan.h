@@ -11,7 +11,7 @@ constexpr int kTile = 32;                   // keys of a wave's tile
 constexpr int kAttnWaves = 4;               // waves a block, whose tiles take turns
 // (16 rows, tile, kv head) products of a prefix from which on its tiles are made into values
 // in LDS for all of a block's rows; with fewer the rounds of barriers cost more than they
-// save.  64 sequences of 32 heads behind 30011 keys: 80 us, and 110 with every wave's own.
+// save.  64 sequences of 32 heads behind 30011 keys: 78 us, and 110 with every wave's own.
 constexpr int64_t kManyTiles = 16 * 1024;
 constexpr int64_t kMaxBlocks = (1ll << 31) - 1, kMaxParts = 1 << 20, kAttnCus = 256;
 
@@ -61,7 +61,7 @@ inline Plan plan(int hd, bool bf16, int n_kv, int64_t rows, int64_t prefix, int6
     // us instead of 34), four for the own keys, 4 to 64 tiles each (two: 36 us, there).  One
     // for each with hd 256, of which a CU holds one block (two and four: one sequence of 9000
     // keys 31 us instead of 21, 50 of 2 tokens behind 2000 keys 52 instead of 44); one for
-    // a prefix whose tiles are shared (two: 97 us instead of 80, above).
+    // a prefix whose tiles are shared (two: 97 us instead of 80, then).
     const int64_t pre_blocks = (p.rt || hd == 256 ? 1 : 2) * kAttnCus, own_blocks = (hd == 256 ? 1 : 4) * kAttnCus;
     if (pre_tiles) {
         const int64_t want = cbq_max(1, pre_blocks / (tiles * n_kv)), unit = p.rt ? 2 : kAttnWaves;
