@@ -194,7 +194,7 @@ class BatchDecoder:
             self.pool.give(pages)
             raise
         self._prefix_pages, self.prefix, self._prefix_table = pages, len(ids), table
-        self._prefix_ids = list(ids)
+        self._prefix_ids = [int(t) for t in ids]
 
     @torch.no_grad()
     def start(self, prompts: Sequence[Sequence[int]], room: int) -> torch.Tensor:
@@ -312,6 +312,12 @@ class BatchDecoder:
             raise ValueError(f"{drafts} drafts")
         if n_new < 1:
             return [[] for _ in prompts]
+        try:
+            return self._sample(prompts, n_new, temperature, drafts, generator)
+        finally:
+            self.release()
+
+    def _sample(self, prompts, n_new, temperature, drafts, generator) -> List[List[int]]:
         # a sequence that is done waits for the others, whose drafts need rows of it too
         logits = self.start(prompts, n_new - 1 + (drafts + 1 if drafts else 0))
         batch = len(prompts)
@@ -342,7 +348,6 @@ class BatchDecoder:
                     texts[b].add(row[:kept[b]])
                 else:                                   # done: its token was run for the others' sake
                     self._lens[b] -= kept[b]
-        self.release()
         return said
 
 
@@ -356,7 +361,7 @@ class _Text:
             self.add(p)
 
     def add(self, tokens: Sequence[int]) -> None:
-        for t in tokens:
+        for t in map(int, tokens):
             n = len(self.tokens)
             if n > 1:                                   # the newest pair is not looked up as itself
                 self.after[self.tokens[-2], self.tokens[-1]] = n

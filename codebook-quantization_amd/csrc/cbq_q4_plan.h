@@ -14,6 +14,7 @@ constexpr int kAttnWaves = 4;               // waves a block, whose tiles take t
 // save.  64 sequences of 32 heads behind 30011 keys: 78 us, and 110 with every wave's own.
 constexpr int64_t kManyTiles = 16 * 1024;
 constexpr int64_t kMaxBlocks = (1ll << 31) - 1, kMaxParts = 1 << 20, kAttnCus = 256;
+constexpr int64_t kMaxBytes = 1ll << 30;      // of the own parts' sums, where there are several
 
 struct Plan {
     int32_t rt;                             // 64 rt rows a block of the prefix, or 0: 16
@@ -72,8 +73,10 @@ inline Plan plan(int hd, bool bf16, int n_kv, int64_t rows, int64_t prefix, int6
     }
     const int64_t share = cbq_ceil(cap_tiles * batch * n_kv * own_tiles, own_blocks);
     int64_t own_chunk = cbq_min(cbq_max(cbq_ceil(share, kAttnWaves), 1), 16) * kAttnWaves;
-    // more of a wider table than its parts and blocks are counted for
-    const int64_t most = cbq_min(kMaxParts / 2, (kMaxBlocks - n_kv * tiles * pre_parts) / (n_kv * batch * own_tiles));
+    // more of a wider table than its parts and blocks are counted for, or than a workspace of
+    // 1 GiB holds (of rows so many that their blocks are plenty)
+    const int64_t most = cbq_min(cbq_min(kMaxParts / 2, cbq_max(1, kMaxBytes / part_bytes(2, batch * rows * n_kv, hd) * 2)),
+                                 (kMaxBlocks - n_kv * tiles * pre_parts) / (n_kv * batch * own_tiles));
     if (most > 0) own_chunk = cbq_max(own_chunk, cbq_ceil(cbq_ceil(cap_tiles, most), kAttnWaves) * kAttnWaves);
     const int64_t own_parts = cbq_max(cbq_ceil(cap_tiles, own_chunk), pre_parts ? 0 : 1);
     p.tiles = (int32_t)tiles;

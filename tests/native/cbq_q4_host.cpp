@@ -87,6 +87,12 @@ int main()
     one(256, true, 8, 40, 12000, 128, 20);
     one(128, true, 8, 3, 30000, 128, 20);
     for (int i = 0; i < 4; i++) CHECK(kinds[i] > 0);
+    // many rows against wide tables: the own parts' sums stay below 1 GiB
+    for (int64_t rows : {1ll, 4ll, 300ll, 100000ll})
+        for (int64_t batch : {1ll, 60ll, 3000ll}) {
+            const Plan p = plan(128, false, 8, rows, 0, 1 << 24, batch);
+            CHECK(plan_fits(p) && (p.own_parts <= 2 || p.bytes <= kMaxBytes));
+        }
     // the largest tables and batches that the entry points allow
     for (int64_t batch : {1ll, 1ll << 20, (1ll << 30) - 1})
         for (int64_t capacity : {0ll, 1000ll, (1ll << 31) - 65536})

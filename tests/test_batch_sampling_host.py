@@ -139,6 +139,7 @@ def test_sample_without_numbers(batch):
     batch.model.linears["lm_head"] = lambda x: torch.full((len(x), VOCAB), float("nan"))
     with pytest.raises(RuntimeError, match="no numbers"):
         batch.sample([[1, 2]], 4)
+    assert len(batch.pool._free) == 40 and not batch._own
     assert batch.generate([[1]], 0) == [[]]
 
 

@@ -116,6 +116,13 @@ def test_many_sequences(cuda, ops, dtype, hd, prefix, page):
     check(ops, batch, 1, f"{dtype} hd={hd} 130 sequences behind {prefix}")
 
 
+@pytest.mark.parametrize("dtype,hd,page", [("bf16", 128, 96), ("f32", 64, 160), ("f16", 256, 33), ("bf16", 64, 1000)])
+def test_odd_pages(cuda, ops, dtype, hd, page):
+    """Pages of whole tiles whose count is no power of two, pages that end inside one."""
+    batch = qo.Batch([5, 700, 161, 96, 1500], 490, 2, 3, hd, page, dtype, room=1, seed=page)
+    check(ops, batch, 2, f"{dtype} hd={hd} pages of {page}")
+
+
 # ---- far pages, streams, graphs ---------------------------------------------------------
 
 def test_far_pages(cuda, ops):
