@@ -347,14 +347,26 @@ template <int HD> struct Tiles {
         ask_ids(n + G::kDepth - 1);
         return in_pool;
     }
-    __device__ __forceinline__ void begin()
+    // The first tiles' page ids, asked for before the length is known: of the tiles below
+    // `upto`, where the tables end.
+    __device__ __forceinline__ void look(int32_t upto)
     {
         at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
         at = __builtin_amdgcn_readfirstlane(at);
-        if (tile(0) >= end) return;
+        if (tile(0) >= upto) return;
 #pragma unroll
-        for (int n = 0; n < G::kDepth - 1; n++) ask_ids(n);
-        arrived<0>();
+        for (int n = 0; n < G::kDepth - 1; n++) {
+            const int32_t t = tile(n) < upto ? tile(n) : tile(0);
+            const bool shared = t < pre_tiles;
+            const uint32_t j = (uint32_t)(shared ? t : t - pre_tiles) * kTile + (threadIdx.x & 31),
+                           last = (shared ? (uint32_t)a.prefix : (uint32_t)a.capacity) - 1;
+            copy4(at + G::kIds + n * 256, (const char *)(shared ? a.prefix_table : own),
+                  4 * cbq_div(j < last ? j : last, a.pool.page));
+        }
+    }
+    // The first tiles, whose ids are there
+    __device__ __forceinline__ void begin()
+    {
 #pragma unroll
         for (int n = 0; n < G::kDepth - 1; n++)
             there[n] = tile(n) < end ? ask(n) : 0;
@@ -464,25 +476,59 @@ template <typename T, int HD, int RT> struct Rows {
     float c[RT], c_low[RT];                 // exp2's factors, the row's scaling taken back
     int E;                                  // p s is times 2^(kUp - E)
 
-    // Row `row` of 16 from row0 on (zeros from n on): of query token token0 + row / rep,
-    // head h * rep + row % rep.
-    __device__ __forceinline__ void start(const AttnArgs &a, int h, int64_t token0, int row0, int n)
+    // This lane's quarter of a row's values, eight at a time
+    struct Queries {
+        u32x4 e[RT][G::kG][2][sizeof(T) / 2];
+    };
+    // Row `row` of 16 from row0 on (the first for those from n on): of query token token0 +
+    // row / rep, head h * rep + row % rep.
+    static __device__ __forceinline__ void load(const AttnArgs &a, int h, int64_t token0, int row0, int n, Queries &x)
     {
         const int lane = threadIdx.x & 63, g4 = lane >> 4;
-        E = kNone;
 #pragma unroll
         for (int t = 0; t < RT; t++) {
             const int row = row0 + 16 * t + (lane & 15);
-            const bool in = row < n;
-            const uint32_t token = cbq_div(in ? row : 0, a.rep), head = (in ? row : 0) - token * a.rep.d;
-            const T *x = (const T *)a.q + (token0 + token) * a.q_st[0] + ((int64_t)h * a.rep.d + head) * a.q_st[1];
+            const uint32_t token = cbq_div(row < n ? row : 0, a.rep), head = (row < n ? row : 0) - token * a.rep.d;
+            const T *from = (const T *)a.q + (token0 + token) * a.q_st[0] + ((int64_t)h * a.rep.d + head) * a.q_st[1];
+#pragma unroll
+            for (int g = 0; g < G::kG; g++)
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                    for (int i = 0; i < (int)sizeof(T) / 2; i++)
+                        x.e[t][g][hf][i] = *(const u32x4 *)((const char *)(from + 64 * g + 16 * g4 + 8 * hf) + 16 * i);
+        }
+    }
+    // They are there: the compiler waits for them here, and not behind what is asked for next
+    static __device__ __forceinline__ void loaded(Queries &x)
+    {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int g = 0; g < G::kG; g++)
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                    for (int i = 0; i < (int)sizeof(T) / 2; i++) asm volatile("" : "+v"(x.e[t][g][hf][i]));
+    }
+    // Zeros for rows from n on
+    __device__ __forceinline__ void start(const AttnArgs &a, int row0, int n, const Queries &x)
+    {
+        const int lane = threadIdx.x & 63;
+        E = kNone;
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const bool in = row0 + 16 * t + (lane & 15) < n;
             float f[G::kG][2][8], top = 0.f;
 #pragma unroll
             for (int g = 0; g < G::kG; g++)
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
-                    struct alignas(16) Eight { T e[8]; };
-                    const Eight e = *(const Eight *)(x + 64 * g + 16 * g4 + 8 * hf);
+                    struct Eight { T e[8]; };
+                    struct Words { u32x4 e[sizeof(T) / 2]; } words;
+#pragma unroll
+                    for (int i = 0; i < (int)sizeof(T) / 2; i++) words.e[i] = x.e[t][g][hf][i];
+                    const Eight e = __builtin_bit_cast(Eight, words);
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         f[g][hf][i] = in ? (float)e.e[i] * a.q_mul : 0.f;
@@ -1150,21 +1196,28 @@ __device__ __forceinline__ void walk(const AttnArgs &a, char *lds, const Work &w
     using G = Geo<HD>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int32_t pre_tiles = (a.prefix + kTile - 1) / kTile;
-    int32_t length = 0, end = w.end;
-    const int32_t *own = nullptr;
-    if (w.seq >= 0) {
-        length = cbq_clamp_length(a.lengths[w.seq], a.capacity);
-        own = a.tables + w.seq * a.table_st;
-        end = (int32_t)cbq_min(end, (int64_t)pre_tiles + cbq_ceil(length, kTile));
-        if (w.first >= end && a.plan.parts > 1) return;     // the merge counts own parts by the length
-    }
     const int64_t token0 = w.seq >= 0 ? (int64_t)w.seq * a.tokens : 0;
     char *mine = lds + wave * G::kWave;
     float *scales = (float *)(mine + G::kScales);
-    Tiles<HD> tiles = {a, own, pre_tiles, length, w.first + wave, end, w.h, mine};
+    // page ids, queries and the length under way at once, then the tiles
+    Tiles<HD> tiles = {a, w.seq >= 0 ? a.tables + w.seq * a.table_st : nullptr, pre_tiles, 0, w.first + wave, w.end, w.h,
+                       mine};
+    tiles.look(w.end);
+    typename Rows<T, HD, RT>::Queries queries;
+    Rows<T, HD, RT>::load(a, w.h, token0, row0, n, queries);
+    int32_t length = 0, end = w.end;
+    if (w.seq >= 0) {
+        length = cbq_clamp_length(a.lengths[w.seq], a.capacity);
+        end = (int32_t)cbq_min(end, (int64_t)pre_tiles + cbq_ceil(length, kTile));
+    }
+    arrived<0>();
+    Rows<T, HD, RT>::loaded(queries);
+    if (w.first >= end && a.plan.parts > 1) return;         // the merge counts own parts by the length
+    tiles.length = length;
+    tiles.end = end;
     tiles.begin();
     Rows<T, HD, RT> rows;
-    rows.start(a, w.h, token0, row0, n);
+    rows.start(a, row0, n, queries);
     // own keys that the lane's row of each tile sees
     int32_t sees[RT];
 #pragma unroll
