@@ -268,7 +268,8 @@ template <typename A> __device__ __forceinline__ void quantise(const A (&y)[4], 
     pair = scale | mid << 16;
     if (!(s > 0)) return;
     const double step = (double)s;
-    const double inv = ldexp((double)__builtin_amdgcn_rcpf(__builtin_amdgcn_frexp_mantf(s)), -__builtin_amdgcn_frexp_expf(s));
+    const double inv = ldexp((double)__builtin_amdgcn_rcpf(__builtin_amdgcn_frexp_mantf(s)),
+                             -__builtin_amdgcn_frexp_expf(s));
     codes = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {

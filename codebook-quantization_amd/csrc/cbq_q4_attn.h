@@ -1255,7 +1255,7 @@ __device__ __forceinline__ void walk(const AttnArgs &a, char *lds, const Work &w
 
 // Waves a SIMD: their registers, and tiles two (or, of one wave, three) deep in LDS, leave
 // room for so many.  24 sequences of 4000 to 32000 keys, bf16, hd 128: three waves two
-// tiles deep 114 us, two waves three deep 143, four waves (which spill) two deep 133.
+// tiles deep took 114 us, two waves three deep 143, four waves (which spill) two deep 133.
 constexpr int simd_waves(int hd, int rt) { return hd == 256 ? 1 : rt ? 2 : 3; }
 
 // RT: 64 RT rows a block of the prefix; 0: 16, as the own keys'.

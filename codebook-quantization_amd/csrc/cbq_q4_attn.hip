@@ -10,6 +10,8 @@ namespace {
 
 // Largest joint axis and count of rows: a tile's indexes past either stay below 2^31.
 constexpr int64_t kMaxKeys = (1ll << 31) - 65536;
+// Entries of a table: their bytes are a 32-bit offset.
+constexpr int64_t kMaxEntries = 1ll << 30;
 
 bool sizes_ok(const cbq_paged_q4 *c, int64_t prefix, int64_t width, int64_t batch, int64_t tokens,
               int64_t n_q)
@@ -17,6 +19,7 @@ bool sizes_ok(const cbq_paged_q4 *c, int64_t prefix, int64_t width, int64_t batc
     return c && (c->hd == 64 || c->hd == 128 || c->hd == 256) && c->n_kv >= 1 && n_q >= 1 &&
            n_q < (1 << 20) && n_q % c->n_kv == 0 && c->page >= 1 && c->page <= 65536 &&
            prefix >= 0 && prefix <= kMaxKeys && width >= 0 && width * c->page <= kMaxKeys &&
+           width < kMaxEntries && cbq_ceil(prefix, c->page) < kMaxEntries &&
            prefix + width * c->page <= kMaxKeys && batch >= 0 && batch < (1 << 30) && tokens >= 1 &&
            batch * tokens <= kMaxKeys && batch * tokens * n_q <= kMaxKeys;
 }

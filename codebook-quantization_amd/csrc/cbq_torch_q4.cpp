@@ -238,8 +238,9 @@ at::Tensor prefix_attention_decode_q4(const at::Tensor &q, const at::Tensor &k_c
                     prefix <= prefix_table.size(0) * c.page,
                 op, ": prefix_table names ", prefix_table.size(0), " pages of ", c.page,
                 " rows for ", prefix, " keys");
-    TORCH_CHECK(width < (1ll << 31) && prefix + width * c.page <= (1ll << 31) - 65536, op,
-                ": too many keys");
+    TORCH_CHECK(width < (1ll << 30) && prefix + width * c.page <= (1ll << 31) - 65536 &&
+                    (prefix + c.page - 1) / c.page < (1ll << 30),
+                op, ": too many keys");
     TORCH_CHECK(N < (1ll << 31) && batch < (1ll << 30) && n_q < (1ll << 20) &&
                     N * n_q <= (1ll << 31) - 65536,
                 op, ": too many rows");

@@ -78,7 +78,7 @@ int cbq_paged_read_q4(const cbq_paged_q4 *cache, const int64_t *slots, int64_t N
  * made into fp16 numbers, and its weights are.  A query that is not finite gives
  * NaN where it sees a key; keys whose scale passes 2^96 may, whatever the query.
  * n_q % n_kv == 0; n_q < 2^20, batch < 2^30, batch * tokens * n_q <= 2^31 - 65536;
- * prefix + width * page <= 2^31 - 65536.
+ * prefix + width * page <= 2^31 - 65536, fewer than 2^30 entries of a table.
  * workspace: cbq_prefix_attn_decode_q4_workspace bytes (which may be 0), 16-byte
  * aligned, overwritten by every call. */
 size_t cbq_prefix_attn_decode_q4_workspace(const cbq_paged_q4 *cache, int64_t prefix, int width,

@@ -76,6 +76,8 @@ def test_attention_refusals(lib):
         assert call(_cache(p), **kw) == 2, kw
     for kw in POOLS + _pointers(p):
         assert call(_cache(p, **kw)) == 2, kw
+    one = _cache(p, page=1)                                     # tables of 2^30 entries
+    assert call(one, width=1 << 30) == 2 and call(one, prefix=1 << 30) == 2
     assert call(_cache(p), batch=0) == 0                        # nothing to do
     assert lib.cbq_prefix_attn_decode_q4_workspace(ctypes.byref(_cache(p, hd=65)), 10, 3, 2, 1, 4, 1) == 0
 
