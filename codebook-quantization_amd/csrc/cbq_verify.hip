@@ -5,7 +5,7 @@
 // its sums.  Two numbers a draft decide which row that is, so every wave finds it for
 // itself, and only that row of p (and of q) is read: HBM bounds a large batch, two
 // launches and their chains of dependent loads a small one.  The first launch adds the
-// row up, 512 tokens a sum, the second finds the sum in which they pass u times the
+// row up, a wave 512 tokens, the second finds the sum in which they pass u times the
 // total and reads its tokens again.
 //
 // 64 sequences of seven drafts, 151936 tokens, fp32: 21 us, of which the sums take 16 (78
@@ -23,8 +23,6 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / CBQ_WAVE;
 constexpr int kPer = 8, kUnit = CBQ_WAVE * kPer;        // tokens of a sum
 
-constexpr int64_t kFull = 8 * 4 * 256;     // eight waves a SIMD of 256 CUs
-
 struct VerifyArgs {
     const void *p, *q;
     int64_t p_st[2], q_st[2];
@@ -35,7 +33,7 @@ struct VerifyArgs {
     int32_t *counts;
     double2 *sums;                          // [batch][unit]: of w, of p
     int32_t *kept;                          // [batch]
-    int32_t n_max, units, each;             // each: units a wave adds up
+    int32_t n_max, units;
     int64_t vocab;
 };
 
@@ -115,29 +113,26 @@ __device__ __forceinline__ double wave_sum(double x)
 template <typename T> __global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a)
 {
     const int b = blockIdx.y, lane = threadIdx.x & 63;
-    const int64_t first = ((int64_t)blockIdx.x * kWaves + threadIdx.x / CBQ_WAVE) * a.each;
-    if (first >= a.units) return;
+    const int64_t u = (int64_t)blockIdx.x * kWaves + threadIdx.x / CBQ_WAVE;
+    if (u >= a.units) return;
     const int kept = find_kept<T>(a, b);
-    if (first == 0 && lane == 0) a.kept[b] = kept;
+    if (u == 0 && lane == 0) a.kept[b] = kept;
     const Row<T> r = row_of<T>(a, b, kept);
-    const int64_t end = first + a.each < a.units ? first + a.each : a.units;
-    for (int64_t u = first; u < end; u++) {
-        double w = 0, p = 0;
+    double w = 0, p = 0;
 #pragma unroll
-        for (int i = 0; i < kPer / 4; i++) {
-            const int64_t v = u * kUnit + i * 4 * CBQ_WAVE + lane * 4;
-            double x[4], y[4];
-            r.four(v, a.vocab - v, x, y);
+    for (int i = 0; i < kPer / 4; i++) {
+        const int64_t v = u * kUnit + i * 4 * CBQ_WAVE + lane * 4;
+        double x[4], y[4];
+        r.four(v, a.vocab - v, x, y);
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                p += x[k];
-                w += y[k];
-            }
+        for (int k = 0; k < 4; k++) {
+            p += x[k];
+            w += y[k];
         }
-        w = wave_sum(w);
-        p = wave_sum(p);
-        if (lane == 0) a.sums[(int64_t)b * a.units + u] = make_double2(w, p);
     }
+    w = wave_sum(w);
+    p = wave_sum(p);
+    if (lane == 0) a.sums[(int64_t)b * a.units + u] = make_double2(w, p);
 }
 
 // The sum of the lanes before this one, and of all
@@ -263,7 +258,7 @@ template <typename T> int launch(const VerifyArgs &a, int batch, hipStream_t str
         x.counts += b;
         x.sums += (int64_t)b * a.units;
         x.kept += b;
-        sums_kernel<T><<<dim3((uint32_t)cbq_ceil(a.units, kWaves * a.each), n), kThreads, 0, stream>>>(x);
+        sums_kernel<T><<<dim3((uint32_t)cbq_ceil(a.units, kWaves), n), kThreads, 0, stream>>>(x);
         pick_kernel<T><<<n, kThreads, 0, stream>>>(x);
         const int rc = cbq_launch_status("cbq_verify_drafts");
         if (rc != CK_SUCCESS) return rc;
@@ -318,9 +313,6 @@ extern "C" int cbq_verify_drafts(const void *probs, const int64_t *p_stride, con
     a.kept = (int32_t *)((char *)workspace + sums_bytes(batch, vocab));
     a.units = (int32_t)units_of(vocab);
     a.vocab = vocab;
-    // every wave finds the row first, three loads one after the other: few waves take a
-    // unit each, many as many as leave eight waves a SIMD
-    a.each = (int32_t)cbq_min(cbq_max(batch * (int64_t)a.units / kFull, 1), 16);
     if (dtype == CBQ_F32) return launch<float>(a, batch, stream);
     if (dtype == CBQ_BF16) return launch<__bf16>(a, batch, stream);
     return launch<_Float16>(a, batch, stream);
