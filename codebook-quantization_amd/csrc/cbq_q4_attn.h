@@ -64,7 +64,8 @@ constexpr int kBlock = kAttnWaves * CBQ_WAVE;
 // move, so that it moves seldom and no weight passes 1.
 constexpr float kSlack = 2.0f;
 
-// p s 2^(kUp - E) < 2^14: fp16 has room for it, and 2^-14 is its smallest whole number
+// p s 2^(kUp - E) < 2^14, and p 2^kUp <= 2^14: fp16 has room for them, and 2^-14 is its
+// smallest whole number
 constexpr int kUp = 14, kNone = -1000;      // kNone: no scale yet
 
 struct AttnArgs {
@@ -1101,7 +1102,9 @@ __device__ __forceinline__ void shared_rows(const AttnArgs &a, char *lds, const 
 #pragma unroll
                 for (int d = 0; d < kD; d++) o[x][d] *= f;
             }
-            const float base = m[x] == -INFINITY ? 0.f : -m[x];
+            // weights times 2^kUp, in sums and products alike: the largest is below 2^14, and
+            // fp16's 11 bits hold down to 2^-28 of it
+            const float base = m[x] == -INFINITY ? 0.f : (float)kUp - m[x];
 #pragma unroll
             for (int t = 0; t < kT; t++) {
                 float e[4];
@@ -1151,13 +1154,13 @@ __device__ __forceinline__ void shared_rows(const AttnArgs &a, char *lds, const 
     for (int t = 0; t < RT; t++) {
         const int from = mine + 16 * t;
         if (from >= n) break;
-        const float total = groups_sum(l[t]);
+        const float total = __builtin_amdgcn_ldexpf(groups_sum(l[t]), -kUp);
 #pragma unroll
         for (int d = 0; d < kD; d++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int at = d * 16 + 8 * (g4 >> 1) + (g4 & 1 ? kOrder[4 + i] : kOrder[i]);
-                out[r * HD + (at ^ (r & 7) << 2)] = __builtin_amdgcn_ldexpf(o[t][d][i], -v_up);
+                out[r * HD + (at ^ (r & 7) << 2)] = __builtin_amdgcn_ldexpf(o[t][d][i], -v_up - kUp);
             }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();

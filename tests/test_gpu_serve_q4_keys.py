@@ -1,0 +1,49 @@
+"""prefix_attention_decode_q4 by rows (q4_checks.py): small weights beside a large one."""
+import math
+
+import pytest
+import torch
+
+import q4_checks as qc
+import q4_oracle as qo
+import serve_oracle as so
+from test_gpu_serve_q4 import decode
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(cuda):
+    import cbq_ops
+    return cbq_ops.load()
+
+
+@pytest.mark.parametrize("dtype,hd,n_kv,rep,prefix", [
+    ("bf16", 64, 8, 64, 8300), ("bf16", 128, 8, 64, 8300), ("bf16", 256, 8, 64, 8300),      # tiles shared
+    ("bf16", 128, 2, 4, 2000), ("f16", 64, 2, 4, 2000)])
+@pytest.mark.parametrize("gap", [12.0, 21.7, 23.4])
+def test_weak_keys(cuda, ops, dtype, hd, n_kv, rep, prefix, gap):
+    """One key in sixteen has the weight 1 and the value 0, the others 2^-gap and values
+    around 4096: the output is theirs alone.  A weight holds fp16's 11 bits down to 2^-25
+    of the largest one, where the maximum stands 4 times above it: half a step of the
+    output, of each weight and (twice) of each value, below four."""
+    batch = qo.Batch([0, 3], prefix, n_kv, rep, hd, 16, dtype, seed=hd)
+    batch.pairs[:, 0] = 0.0                             # keys: scale 0, mid 0
+    for page in batch.prefix_table.tolist():
+        batch.codes[page, 1], batch.pairs[page, 1] = qo.quantise(
+            4096 * (1 + torch.randn(n_kv, 16, hd, generator=batch.g)))
+        batch.pairs[page, 0, :, 5, 0, 1] = 1.0          # the strong key: 64 ones
+        batch.pairs[page, 1, :, 5] = 0.0
+    page = int(batch.tables[1, 0])
+    batch.codes[page, 1], batch.pairs[page, 1] = qo.quantise(4096 + torch.zeros(n_kv, 16, hd))
+    q = torch.zeros(2, n_kv * rep, hd, dtype=batch.dtype)
+    q[..., :64] = 1.0
+    out = decode(ops, batch, q, gap * math.log(2) / 64)
+    j = torch.arange(prefix)
+    at = batch.prefix_table[j // 16].long(), j % 16
+    v = qo.values(batch.codes[at[0], 1, :, at[1]], batch.pairs[at[0], 1, :, at[1]])     # [keys, n_kv, hd]
+    strong = int((j % 16 == 5).sum())
+    w = 2.0 ** -gap
+    for b, own in enumerate((0, 3)):
+        want = w * (v.sum(0) + own * 4096.0) / (strong + w * (prefix - strong + own))
+        qc.near_rows(out[b], want.repeat_interleave(rep, 0), 4 * so.half_step(batch.dtype), f"sequence {b}")
