@@ -843,8 +843,10 @@ __device__ __forceinline__ void join_waves(const AttnArgs &a, Rows<T, HD, RT> &w
 // a tile's values are worth making once, as fp16 numbers in LDS for all four waves, and
 // the scales' products with every row fall away.  Keys and values are taken against
 // the largest exponents of the block's keys, found in a first pass over their pairs:
-// (c - 8) s + (m + s / 2) in two packed operations, rounded once to fp16 (11 bits down to
-// 2^-28 of the largest value), an eighth of a bf16 query's and output's own rounding.
+// (c - 8) s + (m + s / 2) in two packed operations.  The second addend is rounded to fp16
+// and the sum again: each an eighth of a bf16 query's and output's own rounding, and s, of
+// eight bits, not at all: so for 8 s down to 2^-27 of the largest 8 s or |m|, below that the
+// roundings are to fp16's smallest number.
 //
 // A slot of 16 bytes holds eight values in the order 0 4 1 5 2 6 3 7 that the codes'
 // masks give them; queries are read in that order, and outputs put back.
@@ -922,7 +924,7 @@ template <int HD> struct Raw {
     }
     // The values of the piece, times 2^up, slot by slot into a tile whose keys begin at `tile`
     static constexpr int kMine = kWords;    // slots a thread
-    f16x2 off[kG], low[kG], high[kG];       // m + s / 2, s and s / 16, twice
+    f16x2 off[kG], step[kG];                // m + s / 2 and s, twice
 
     __device__ __forceinline__ void begin(float *there, int up)
     {
@@ -931,10 +933,9 @@ template <int HD> struct Raw {
             float s = __builtin_amdgcn_ldexpf(pair_scale(pair[g]), up), m = __builtin_amdgcn_ldexpf(pair_mid(pair[g]), up);
             if (!(s >= 0.f && s < INFINITY)) s = 0.f, m = __builtin_nanf("");
             if (!in) s = m = 0.f;
-            const _Float16 b = (_Float16)fmaf(0.5f, s, m), one = (_Float16)s, part = (_Float16)(s * 0.0625f);
+            const _Float16 b = (_Float16)fmaf(0.5f, s, m), one = (_Float16)s;
             off[g] = f16x2{b, b};
-            low[g] = f16x2{one, one};
-            high[g] = f16x2{part, part};
+            step[g] = f16x2{one, one};
         }
         if (threadIdx.x < kBlock / 2 && piece() == 0) there[row()] = in ? 0.f : -INFINITY;
     }
@@ -946,12 +947,14 @@ template <int HD> struct Raw {
         if constexpr (HD == 64) x = w[n];
         else x = __builtin_amdgcn_perm(w[(2 * n + 1) * (kG / 2) + g / 2], w[2 * n * (kG / 2) + g / 2],
                                        g & 1 ? 0x07060302u : 0x05040100u);
-        const f16x2 eight = {(_Float16)-1032.f, (_Float16)-1032.f}, more = {(_Float16)-1152.f, (_Float16)-1152.f};
+        // c - 8, exactly: the upper codes' 16 (c - 8) a sixteenth
+        const f16x2 eight = {(_Float16)-1032.f, (_Float16)-1032.f}, more = {(_Float16)-72.f, (_Float16)-72.f},
+                    part = {(_Float16)0.0625f, (_Float16)0.0625f};
         constexpr uint32_t kLower = 0x000f000fu, kUpper = 0x00f000f0u;      // 1024 + c, 1024 + 16 c
         auto half = [](uint32_t y, uint32_t mask) { return __builtin_bit_cast(f16x2, (y & mask) | 0x64006400u); };
-        const f16x2 x0 = (half(x, kLower) + eight) * low[g] + off[g], x1 = (half(x, kUpper) + more) * high[g] + off[g],
-                    x2 = (half(x >> 8, kLower) + eight) * low[g] + off[g],
-                    x3 = (half(x >> 8, kUpper) + more) * high[g] + off[g];
+        const f16x2 x0 = (half(x, kLower) + eight) * step[g] + off[g], x1 = (half(x, kUpper) * part + more) * step[g] + off[g],
+                    x2 = (half(x >> 8, kLower) + eight) * step[g] + off[g],
+                    x3 = (half(x >> 8, kUpper) * part + more) * step[g] + off[g];
         const int at = 8 * g + piece() * (8 / M::kLanes) + n;
         *(u32x4 *)(tile + side() * M::kSide + row() * M::kRow + (at ^ M::mix(row())) * 16) =
             u32x4{__builtin_bit_cast(uint32_t, x0), __builtin_bit_cast(uint32_t, x1),
@@ -1045,9 +1048,9 @@ __device__ __forceinline__ void shared_rows(const AttnArgs &a, char *lds, const 
         top.x = max(top.x, tops[i].x);
         top.y = max(top.y, tops[i].y);
     }
-    // a value is below 2^(top + 1): 2^14 of it is left
-    const int k_up = top.x == kNone ? 0 : 13 - __builtin_amdgcn_readfirstlane(top.x),
-              v_up = top.y == kNone ? 0 : 13 - __builtin_amdgcn_readfirstlane(top.y);
+    // a value is below 2^(top + 1): 2^15 of it is left
+    const int k_up = top.x == kNone ? 0 : 14 - __builtin_amdgcn_readfirstlane(top.x),
+              v_up = top.y == kNone ? 0 : 14 - __builtin_amdgcn_readfirstlane(top.y);
 #pragma unroll
     for (int t = 0; t < RT; t++) c[t] = fminf(fmaxf(__builtin_amdgcn_ldexpf(c[t], -k_up), 0x1p-149f), 3.0e38f);
     int buffer = 0;

@@ -13,6 +13,37 @@ half steps: 64 + n / 64 half steps.
 """
 import torch
 
+import q4_oracle as qo
+
+
+def joint(batch, b):
+    """Keys and values [2][n_kv, keys, hd] of sequence b in 64 bits (0 where a page is not
+    there) and which are there."""
+    codes, pairs, there = batch.rows(b)
+    x = qo.values(codes, pairs)
+    return [torch.where(there[None, :, None], x[:, i].transpose(0, 1), 0.0) for i in range(2)], there
+
+
+def exact(batch, q, tokens, scale, count=None):
+    """Outputs [N, n_q, hd] in 64 bits; count: how often key j of a joint axis counts (a
+    mistake, planted)."""
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    for b in range(len(batch.lens)):
+        (k, v), there = joint(batch, b)
+        n = len(there)
+        times = there.double() if count is None else there * count[:n].double()
+        ends = batch.prefix + (n - batch.prefix - tokens + 1 + torch.arange(tokens)).clamp(min=0)
+        w = times * (torch.arange(n)[None] < ends[:, None])             # [tokens, keys]
+        for h in range(batch.n_kv):
+            at = slice(b * tokens, (b + 1) * tokens), slice(h * batch.rep, (h + 1) * batch.rep)
+            s = q[at].double() @ k[h].T * scale                         # [tokens, rep, keys]
+            s = s.masked_fill((w == 0)[:, None], -float("inf"))
+            if n and bool((w > 0).any()):
+                p = (s - s.amax(-1, keepdim=True).clamp(min=-1e300)).exp() * w[:, None]
+                total = p.sum(-1, keepdim=True)
+                out[at] = p @ v[h] / torch.where(total > 0, total, 1.0)
+    return out
+
 
 def near_rows(got, want, bar, what):
     got = got.double().cpu()

@@ -1,4 +1,5 @@
-"""prefix_attention_decode_q4 by rows (q4_checks.py): small weights beside a large one."""
+"""prefix_attention_decode_q4 by rows (q4_checks.py): small weights beside a large one,
+small values beside large ones."""
 import math
 
 import pytest
@@ -47,3 +48,20 @@ def test_weak_keys(cuda, ops, dtype, hd, n_kv, rep, prefix, gap):
     for b, own in enumerate((0, 3)):
         want = w * (v.sum(0) + own * 4096.0) / (strong + w * (prefix - strong + own))
         qc.near_rows(out[b], want.repeat_interleave(rep, 0), 4 * so.half_step(batch.dtype), f"sequence {b}")
+
+
+def test_small_values(cuda, ops):
+    """Values of one group 2^-27 of the other's, in tiles that are made into fp16 numbers
+    against the largest.  The largest scale becomes 2^10 or more, so the group's s are 2^-18.8
+    or more, rounded to fp16's smallest number: off by 2^-25, 2^-6.2 of them, 3.5 half steps of
+    bf16; their middles and sums by 2^-25 each, of values of 4 s and more 0.9; the output by
+    one.  Seven half steps of a row in all; the other group's, whose scales are exact, two."""
+    batch = qo.Batch([0, 3], 8300, 8, 64, 128, 16, "bf16", seed=5)
+    scales = batch.pairs[batch.prefix_table.long(), 1, :, :12, :, 0].float()
+    assert float(scales[..., 1].min() / scales.amax()) >= 2.0 ** -1.8
+    batch.pairs[:, 1, :, :, 1] *= 2.0 ** -27
+    q = batch.queries(1, 1.5)
+    out = decode(ops, batch, q, 128 ** -0.5)
+    want = qc.exact(batch, q, 1, 128 ** -0.5)
+    for half, steps in ((slice(0, 64), 2), (slice(64, 128), 7)):
+        qc.near_rows(out[..., half], want[..., half], steps * so.half_step(batch.dtype), f"values {half}")
