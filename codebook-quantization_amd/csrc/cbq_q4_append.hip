@@ -137,14 +137,15 @@ template <int HD, bool VEC> struct Weights {
     }
 };
 
-// 1 / sqrt(x): for a double two Newton steps behind an estimate of 20 bits at least
+// 1 / sqrt(x): for a double two Newton steps behind an estimate of 20 bits at least; the
+// steps make NaN of infinity's 0
 __device__ __forceinline__ float inv_root(float x) { return 1.f / sqrtf(x); }
 __device__ __forceinline__ double inv_root(double x)
 {
     double y = __builtin_amdgcn_rsq(x);
 #pragma unroll
     for (int i = 0; i < 2; i++) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
-    return y;
+    return x == HUGE_VAL ? 0 : y;
 }
 
 // A lane's values of a row, normed and turned.  x, w: the row and the weights, for values
