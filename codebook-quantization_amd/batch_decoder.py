@@ -249,9 +249,8 @@ class BatchDecoder:
             if several:
                 return self.ops.prefix_attention_prompt(q, starts, *own)
             return self.ops.prefix_attention_decode(q, *own)
-        x = self._layers(tokens.reshape(-1), positions, slots, attend)
-        self._lens = lens
-        logits = self.model.linears["lm_head"](x)
+        logits = self.model.linears["lm_head"](self._layers(tokens.reshape(-1), positions, slots, attend))
+        self._lens = lens                       # nothing failed
         return logits.unflatten(0, (batch, T)) if several else logits
 
     @torch.no_grad()
