@@ -311,14 +311,14 @@ class BatchDecoder:
             raise ValueError(f"{drafts} drafts")
         if n_new < 1:
             return [[] for _ in prompts]
+        # a sequence that is done waits for the others, whose drafts need rows of it too
+        logits = self.start(prompts, n_new - 1 + (drafts + 1 if drafts else 0))
         try:
-            return self._sample(prompts, n_new, temperature, drafts, generator)
+            return self._sample(prompts, logits, n_new, temperature, drafts, generator)
         finally:
             self.release()
 
-    def _sample(self, prompts, n_new, temperature, drafts, generator) -> List[List[int]]:
-        # a sequence that is done waits for the others, whose drafts need rows of it too
-        logits = self.start(prompts, n_new - 1 + (drafts + 1 if drafts else 0))
+    def _sample(self, prompts, logits, n_new, temperature, drafts, generator) -> List[List[int]]:
         batch = len(prompts)
 
         def uniforms(n):

@@ -30,3 +30,24 @@ def test_head_fails(batch):
     out, kept = batch.verify(t, d, u)
     assert out.tolist() == [[7, 8, 9, 10], [5, 6, -1, -1]] and kept == [4, 2]
     assert batch._lens == [5, 4] and batch.runs[-1] == batch.runs[1]
+
+
+def test_refused_sample(batch):
+    """A sample() that is refused leaves the sequences that were started, as generate()
+    does; one that fails later gives its pages back."""
+    batch.start([[5], [2, 3]], 8)
+    own, free = [list(r) for r in batch._own], len(batch.pool._free)
+    for call in (lambda: batch.generate([[1]], 61), lambda: batch.sample([[1]], 61),
+                 lambda: batch.sample([[1]], 50, drafts=40), lambda: batch.sample([], 3),
+                 lambda: batch.sample([[1], []], 3), lambda: batch.sample([[1]], 3, temperature=0.0)):
+        with pytest.raises(ValueError):
+            call()
+        assert batch._own == own and batch._lens == [1, 2] and len(batch.pool._free) == free
+    assert batch.step(torch.tensor([6, 4])).argmax(-1).tolist() == [7, 5]
+
+    def broken(*args):
+        raise RuntimeError("not verified")
+    batch.ops.verify_drafts = broken
+    with pytest.raises(RuntimeError, match="not verified"):
+        batch.sample([[1]], 3)
+    assert len(batch.pool._free) == 40 and not batch._own
