@@ -1,5 +1,5 @@
-"""prefix_attention_decode_q4 by rows (q4_checks.py): small weights beside a large one,
-small values beside large ones."""
+"""prefix_attention_decode_q4 by rows and by single keys (q4_checks.py): small weights beside
+a large one, small values beside large ones, keys at every kind of border."""
 import math
 
 import pytest
@@ -65,3 +65,34 @@ def test_small_values(cuda, ops):
     want = qc.exact(batch, q, 1, 128 ** -0.5)
     for half, steps in ((slice(0, 64), 2), (slice(64, 128), 7)):
         qc.near_rows(out[..., half], want[..., half], steps * so.half_step(batch.dtype), f"values {half}")
+
+
+SHAPES = [  # lens, prefix, n_kv, rep, hd, page, tokens, rows_first, room, types
+    ([5, 0], 5500, 12, 64, 64, 64, 1, False, 1, ["bf16", "f16"]),       # shared tiles, 128 rows a block
+    ([40, 3, 17], 5601, 16, 11, 128, 16, 3, False, 1, ["bf16", "f32"]),
+    ([1, 70], 5500, 16, 50, 256, 32, 1, True, 1, ["bf16"]),             # 64 rows a block
+    ([9], 8300, 32, 18, 128, 48, 1, False, 1, ["bf16"]),
+    ([130, 600, 31, 5], 900, 1, 4, 64, 32, 2, False, 3, ["f32", "bf16", "f16"]),
+    ([130, 600, 31, 5], 900, 2, 4, 256, 24, 2, False, 3, ["f32", "bf16", "f16"]),
+    ([90, 7, 1200], 33, 2, 7, 128, 17, 4, False, 1, ["f32", "bf16", "f16"]),        # 28 rows a sequence
+    ([9000, 31, 4000], 0, 2, 4, 128, 64, 1, False, 9, ["f32", "bf16", "f16"]),
+    ([2500, 8100], 3000, 4, 12, 64, 256, 5, False, 0, ["bf16", "f16"]),
+    ([i * 61 % 900 for i in range(130)], 300, 4, 2, 64, 32, 1, False, 0, ["bf16", "f32"]),  # a block a sequence
+    ([i * 37 % 300 for i in range(130)], 700, 4, 2, 128, 24, 1, False, 0, ["f16"]),
+]
+
+
+@pytest.mark.parametrize("dtype,shape", [(t, s[:-1]) for s in SHAPES for t in s[-1]],
+                         ids=[f"{t}-{i}" for i, s in enumerate(SHAPES) for t in s[-1]])
+def test_rows_and_borders(cuda, ops, dtype, shape):
+    """Every row within its roundings; rows of two keys, one at a border of tiles or at
+    either end, of prefix and own keys alike: each counts, and once."""
+    lens, prefix, n_kv, rep, hd, page, tokens, rows_first, room = shape
+    batch = qo.Batch(lens, prefix, n_kv, rep, hd, page, dtype, rows_first, room, seed=hd + prefix)
+    scale = hd ** -0.5
+    q = batch.queries(tokens, 1.5)
+    worst = qc.near_rows(decode(ops, batch, q, scale), qc.exact(batch, q, tokens, scale), qc.bound(batch), dtype)
+    print(f"{dtype} hd={hd} prefix={prefix}: rows within {worst / qc.bound(batch):.2f} of the bound", flush=True)
+    q, two = qc.planted(batch, tokens, scale)
+    worst = qc.near_planted(decode(ops, batch, q, scale), qc.exact(batch, q, tokens, scale), two, batch, dtype)
+    print(f"  two keys: {16 * worst:.2f} of the bound", flush=True)
