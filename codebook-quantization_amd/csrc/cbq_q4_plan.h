@@ -48,8 +48,17 @@ inline Plan plan(int hd, bool bf16, int n_kv, int64_t rows, int64_t prefix, int6
     // costs as much as it saves, and where every CU has two such blocks parts bring no more
     // of them.  64 sequences of 32 heads, 900 to 1900 keys: 36 us against 43 in parts, but one
     // of 1200 keys 18 against 10; 300 to 3800 keys 57 against 49: lengths this uneven.
+    // But every such block walks the prefix for itself, which parts read for 16 rows of all
+    // sequences: 1 ns more a tile of 128 values, against 4 us and 10 ns a 1000 values of the
+    // parts' sums, written, read and joined.  100 own keys and 32 heads on 8 of 128, bf16, in one
+    // block and in parts: 64 sequences behind 100 keys 11 and 16 us, behind 460 17 both, behind
+    // 2900 50 and 28; 1024 behind 100 93 and 123, behind 2900 549 and 183.  Over 4340 sizes of 1
+    // to 1500 sequences the choice takes 1.1 % more than the shorter of both (3.6 % and five
+    // times at worst without the prefix's part of it; one block everywhere 18 %, parts 15 %).
     const int64_t alone = n_kv * batch * own_tiles;
-    if (pre_tiles + cap_tiles <= (alone >= 2 * kAttnCus ? 24 : 4) * kAttnWaves) {
+    const double again = 1e-3 * hd / 128 * (double)(alone - n_kv * cbq_ceil(all, 16)) * (double)pre_tiles,
+                 sums = 4 + 1e-5 * hd * (double)(all * n_kv);
+    if (pre_tiles + cap_tiles <= (alone >= 2 * kAttnCus ? 24 : 4) * kAttnWaves && again <= sums) {
         p.joint = 1;
         p.rt = 0;
         p.own_parts = p.parts = 1;

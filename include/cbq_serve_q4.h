@@ -69,9 +69,10 @@ int cbq_paged_read_q4(const cbq_paged_q4 *cache, const int64_t *slots, int64_t N
  * own keys up to the (tokens - 1 - t)-th from the end, and
  *   out[b * tokens + t, i] = softmax(q[b * tokens + t, i] . k_j * scale) . v_j
  * over the keys it sees, query head i reading kv head i / (n_q / n_kv); a token that
- * sees no key gets zeros.  The prefix's keys are read for many sequences at a time.  q
- * [batch * tokens, n_q, hd] of type dtype, strides {token, head} in elements, 16-byte
- * aligned; out contiguous, of q's type.  Keys and values count as the values they
+ * sees no key gets zeros.  The prefix's keys are read for many sequences at a time (a
+ * short prefix's by each sequence, where that is less work).  q [batch * tokens, n_q, hd]
+ * of type dtype, strides {token, head} in elements, 16-byte aligned; out contiguous, of q's
+ * type.  Keys and values count as the values they
  * stand for; scores, maxima, sums and the weighted values are fp32.  A weight times
  * a value's scale is rounded to an fp16 number (of fp32 queries to two: 22 bits); a
  * long prefix that more than 16 query rows a kv head share is, for bf16 queries,

@@ -79,6 +79,8 @@ SHAPES = [  # lens, prefix, n_kv, rep, hd, page, tokens, rows_first, room, types
     ([2500, 8100], 3000, 4, 12, 64, 256, 5, False, 0, ["bf16", "f16"]),
     ([i * 61 % 900 for i in range(130)], 300, 4, 2, 64, 32, 1, False, 0, ["bf16", "f32"]),  # a block a sequence
     ([i * 37 % 300 for i in range(130)], 700, 4, 2, 128, 24, 1, False, 0, ["f16"]),
+    ([i * 37 % 300 for i in range(130)], 0, 4, 2, 256, 32, 1, False, 0, ["bf16"]),
+    ([i * 7 % 90 for i in range(130)], 2900, 8, 2, 64, 16, 1, False, 0, ["bf16", "f16", "f32"]),  # few own keys
 ]
 
 
