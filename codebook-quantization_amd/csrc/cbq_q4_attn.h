@@ -464,116 +464,107 @@ template <int HD> struct Slot {
     }
 };
 
-// ---- a wave's state over 16 RT rows -----------------------------------------------------------
-template <typename T, int HD, int RT> struct Rows {
+// ---- a wave's state over 16 rows --------------------------------------------------------------
+template <typename T, int HD> struct Rows {
     using G = Geo<HD>;
     static constexpr int N = kParts<T>;
     static constexpr bool kCentred = Zeros<T>::kNone;       // nothing to take off the sums
-    u32x4 q[RT][N][HD / 32];
-    float qsum[RT][G::kG];
-    f32x4 less[RT][G::kG];                  // -R in every element, which the products begin with
+    u32x4 q[N][HD / 32];
+    float qsum[G::kG];
+    f32x4 less[G::kG];                      // -R in every element, which the products begin with
     Unpack<T> unpack;
-    f32x4 o[RT][HD / 16], ps[RT][G::kG];    // B, and C in every element
-    float mids[RT][G::kG];                  // this lane's keys' part of sum p m
-    float m[RT], l[RT];                     // running maximum (exp2's domain); this lane's part of sum p
-    float c[RT], c_low[RT];                 // exp2's factors, the row's scaling taken back
+    f32x4 o[HD / 16], ps[G::kG];            // B, and C in every element
+    float mids[G::kG];                      // this lane's keys' part of sum p m
+    float m, l;                             // running maximum (exp2's domain); this lane's part of sum p
+    float c, c_low;                         // exp2's factors, the row's scaling taken back
     int E;                                  // p s is times 2^(kUp - E)
 
     // This lane's quarter of a row's values, eight at a time
     struct Queries {
-        u32x4 e[RT][G::kG][2][sizeof(T) / 2];
+        u32x4 e[G::kG][2][sizeof(T) / 2];
     };
     // Row `row` of 16 from row0 on (the first for those from n on): of query token token0 +
     // row / rep, head h * rep + row % rep.
     static __device__ __forceinline__ void load(const AttnArgs &a, int h, int64_t token0, int row0, int n, Queries &x)
     {
-        const int lane = threadIdx.x & 63, g4 = lane >> 4;
+        const int lane = threadIdx.x & 63, g4 = lane >> 4, row = row0 + (lane & 15);
+        const uint32_t token = cbq_div(row < n ? row : 0, a.rep), head = (row < n ? row : 0) - token * a.rep.d;
+        const T *from = (const T *)a.q + (token0 + token) * a.q_st[0] + ((int64_t)h * a.rep.d + head) * a.q_st[1];
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            const int row = row0 + 16 * t + (lane & 15);
-            const uint32_t token = cbq_div(row < n ? row : 0, a.rep), head = (row < n ? row : 0) - token * a.rep.d;
-            const T *from = (const T *)a.q + (token0 + token) * a.q_st[0] + ((int64_t)h * a.rep.d + head) * a.q_st[1];
+        for (int g = 0; g < G::kG; g++)
 #pragma unroll
-            for (int g = 0; g < G::kG; g++)
+            for (int hf = 0; hf < 2; hf++)
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-                    for (int i = 0; i < (int)sizeof(T) / 2; i++)
-                        x.e[t][g][hf][i] = *(const u32x4 *)((const char *)(from + 64 * g + 16 * g4 + 8 * hf) + 16 * i);
-        }
+                for (int i = 0; i < (int)sizeof(T) / 2; i++)
+                    x.e[g][hf][i] = *(const u32x4 *)((const char *)(from + 64 * g + 16 * g4 + 8 * hf) + 16 * i);
     }
     // They are there: the compiler waits for them here, and not behind what is asked for next
     static __device__ __forceinline__ void loaded(Queries &x)
     {
 #pragma unroll
-        for (int t = 0; t < RT; t++)
+        for (int g = 0; g < G::kG; g++)
 #pragma unroll
-            for (int g = 0; g < G::kG; g++)
+            for (int hf = 0; hf < 2; hf++)
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-                    for (int i = 0; i < (int)sizeof(T) / 2; i++) asm volatile("" : "+v"(x.e[t][g][hf][i]));
+                for (int i = 0; i < (int)sizeof(T) / 2; i++) asm volatile("" : "+v"(x.e[g][hf][i]));
     }
     // Zeros for rows from n on
     __device__ __forceinline__ void start(const AttnArgs &a, int row0, int n, const Queries &x)
     {
         const int lane = threadIdx.x & 63;
         E = kNone;
+        const bool in = row0 + (lane & 15) < n;
+        float f[G::kG][2][8], top = 0.f;
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            const bool in = row0 + 16 * t + (lane & 15) < n;
-            float f[G::kG][2][8], top = 0.f;
+        for (int g = 0; g < G::kG; g++)
 #pragma unroll
-            for (int g = 0; g < G::kG; g++)
+            for (int hf = 0; hf < 2; hf++) {
+                struct Eight { T e[8]; };
+                struct Words { u32x4 e[sizeof(T) / 2]; } words;
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++) {
-                    struct Eight { T e[8]; };
-                    struct Words { u32x4 e[sizeof(T) / 2]; } words;
+                for (int i = 0; i < (int)sizeof(T) / 2; i++) words.e[i] = x.e[g][hf][i];
+                const Eight e = __builtin_bit_cast(Eight, words);
 #pragma unroll
-                    for (int i = 0; i < (int)sizeof(T) / 2; i++) words.e[i] = x.e[t][g][hf][i];
-                    const Eight e = __builtin_bit_cast(Eight, words);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        f[g][hf][i] = in ? (float)e.e[i] * a.q_mul : 0.f;
-                        top = fmaxf(top, fabsf(f[g][hf][i]));
-                    }
+                for (int i = 0; i < 8; i++) {
+                    f[g][hf][i] = in ? (float)e.e[i] * a.q_mul : 0.f;
+                    top = fmaxf(top, fabsf(f[g][hf][i]));
                 }
-            top = groups_max(top);
-            const int up = 15 - __builtin_amdgcn_frexp_expf(top);       // top 2^up in [2^14, 2^15)
-            // factors that are not 0 (a hidden key's -inf times 0 is none) and finite
-            c[t] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c, -up), 0x1p-149f), 3.0e38f);
-            c_low[t] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c_low, -up), 0x1p-149f), 3.0e38f);
-#pragma unroll
-            for (int g = 0; g < G::kG; g++) {
-                float even = 0.f, odd = 0.f;
-#pragma unroll
-                for (int hf = 0; hf < 2; hf++) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        f[g][hf][i] = __builtin_amdgcn_ldexpf(f[g][hf][i], up);
-                        (i & 1 ? odd : even) += f[g][hf][i];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint32_t part[N];
-                        cut<N>(f[g][hf][i], f[g][hf][i + 4], part);
-#pragma unroll
-                        for (int p = 0; p < N; p++) q[t][p][2 * g + hf][i] = part[p];
-                    }
-                }
-                even = groups_sum(even);
-                odd = groups_sum(odd);
-                qsum[t][g] = even + odd;
-                const float r = kCentred ? 0.f : -Zeros<T>::kEven * even - Zeros<T>::kOdd * odd;
-                less[t][g] = f32x4{r, r, r, r};
-                ps[t][g] = f32x4{0, 0, 0, 0};
-                mids[t][g] = 0.f;
             }
+        top = groups_max(top);
+        const int up = 15 - __builtin_amdgcn_frexp_expf(top);       // top 2^up in [2^14, 2^15)
+        // factors that are not 0 (a hidden key's -inf times 0 is none) and finite
+        c = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c, -up), 0x1p-149f), 3.0e38f);
+        c_low = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c_low, -up), 0x1p-149f), 3.0e38f);
 #pragma unroll
-            for (int d = 0; d < HD / 16; d++) o[t][d] = f32x4{0, 0, 0, 0};
-            m[t] = -INFINITY;
-            l[t] = 0.f;
+        for (int g = 0; g < G::kG; g++) {
+            float even = 0.f, odd = 0.f;
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    f[g][hf][i] = __builtin_amdgcn_ldexpf(f[g][hf][i], up);
+                    (i & 1 ? odd : even) += f[g][hf][i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t part[N];
+                    cut<N>(f[g][hf][i], f[g][hf][i + 4], part);
+#pragma unroll
+                    for (int p = 0; p < N; p++) q[p][2 * g + hf][i] = part[p];
+                }
+            }
+            even = groups_sum(even);
+            odd = groups_sum(odd);
+            qsum[g] = even + odd;
+            const float r = kCentred ? 0.f : -Zeros<T>::kEven * even - Zeros<T>::kOdd * odd;
+            less[g] = f32x4{r, r, r, r};
+            ps[g] = f32x4{0, 0, 0, 0};
+            mids[g] = 0.f;
         }
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) o[d] = f32x4{0, 0, 0, 0};
+        m = -INFINITY;
+        l = 0.f;
     }
 
     // A tile whose scales' largest exponent is e, over the wave
@@ -585,30 +576,25 @@ template <typename T, int HD, int RT> struct Rows {
         const int down = E == kNone ? 0 : E - e;
         E = e;
 #pragma unroll
-        for (int r = 0; r < RT; r++) {
+        for (int d = 0; d < HD / 16; d++)
 #pragma unroll
-            for (int d = 0; d < HD / 16; d++)
+            for (int i = 0; i < 4; i++) o[d][i] = __builtin_amdgcn_ldexpf(o[d][i], down);
+        if (!kCentred)
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[r][d][i] = __builtin_amdgcn_ldexpf(o[r][d][i], down);
-            if (!kCentred)
+            for (int g = 0; g < G::kG; g++)
 #pragma unroll
-                for (int g = 0; g < G::kG; g++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) ps[r][g][i] = __builtin_amdgcn_ldexpf(ps[r][g][i], down);
-        }
+                for (int i = 0; i < 4; i++) ps[g][i] = __builtin_amdgcn_ldexpf(ps[g][i], down);
     }
 
-    // One tile.  bits[t] holds the keys that the lane's row of tile t sees; hidden: some row
-    // does not see all.
-    __device__ __forceinline__ void tile(const Slot<HD> &slot, const float *lds, const uint32_t (&bits)[RT],
-                                         bool hidden)
+    // One tile.  bits holds the keys that the lane's row sees; hidden: some row does not see all.
+    __device__ __forceinline__ void tile(const Slot<HD> &slot, const float *lds, uint32_t bits, bool hidden)
     {
         const int lane = threadIdx.x & 63, g4 = lane >> 4;
         const float *mine = lds + 8 * g4;               // this lane's eight keys
         auto four = [&](int which, int g, int t) {
             return *(const f32x4 *)(mine + (which * G::kG + g) * kTile + 4 * t);
         };
-        f32x4 s[RT][2];
+        f32x4 s[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             phase();
@@ -618,66 +604,52 @@ template <typename T, int HD, int RT> struct Rows {
             for (int g = 0; g < G::kG; g++) {
                 const f32x4 off = four(1, g, t);
 #pragma unroll
-                for (int r = 0; r < RT; r++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        s[r][t][i] = g == 0 ? off[i] * qsum[r][g] : fmaf(off[i], qsum[r][g], s[r][t][i]);
+                for (int i = 0; i < 4; i++) s[t][i] = g == 0 ? off[i] * qsum[g] : fmaf(off[i], qsum[g], s[t][i]);
             }
 #pragma unroll
             for (int g = 0; g < G::kG; g++) {
-                f32x4 acc[RT];
-#pragma unroll
-                for (int r = 0; r < RT; r++) acc[r] = kCentred ? f32x4{0, 0, 0, 0} : less[r][g];
+                f32x4 acc = kCentred ? f32x4{0, 0, 0, 0} : less[g];
                 const u32x4 k[2] = {unpack.key(slot.key_codes(codes, g, 0)), unpack.key(slot.key_codes(codes, g, 1))};
 #pragma unroll
                 for (int p = 0; p < N; p++)
 #pragma unroll
-                    for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-                        for (int r = 0; r < RT; r++) acc[r] = mma(k[hf], q[r][p][2 * g + hf], acc[r]);
+                    for (int hf = 0; hf < 2; hf++) acc = mma(k[hf], q[p][2 * g + hf], acc);
                 const f32x4 scale = four(0, g, t);
 #pragma unroll
-                for (int r = 0; r < RT; r++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) s[r][t][i] = fmaf(scale[i], acc[r][i], s[r][t][i]);
+                for (int i = 0; i < 4; i++) s[t][i] = fmaf(scale[i], acc[i], s[t][i]);
             }
         }
         phase();
-        float p[RT][8];
+        if (hidden) {
+            const uint32_t seen = here(bits >> g4);
 #pragma unroll
-        for (int r = 0; r < RT; r++) {
-            if (hidden) {
-                const uint32_t seen = here(bits[r] >> g4);
+            for (int i = 0; i < 8; i++) s[i / 4][i % 4] = seen >> (4 * i) & 1 ? s[i / 4][i % 4] : -INFINITY;
+        }
+        float p[8], top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    s[r][i / 4][i % 4] = seen >> (4 * i) & 1 ? s[r][i / 4][i % 4] : -INFINITY;
+        for (int i = 0; i < 8; i++) top = fmaxf(top, s[i / 4][i % 4]);
+        // the row's maximum is found where one of its lanes passes it
+        if (__ballot(top * c > m)) {
+            top = groups_max(top) * c;
+            const float to = top > m ? top + kSlack : m;
+            const float f = top > m ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int g = 0; g < G::kG; g++) {
+                mids[g] *= f;
+                if (!kCentred) ps[g] *= f;
             }
-            float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 8; i++) top = fmaxf(top, s[r][i / 4][i % 4]);
-            // the row's maximum is found where one of its lanes passes it
-            if (__ballot(top * c[r] > m[r])) {
-                top = groups_max(top) * c[r];
-                const float to = top > m[r] ? top + kSlack : m[r];
-                const float f = top > m[r] ? __builtin_amdgcn_exp2f(m[r] - to) : 1.0f;
-                m[r] = to;
-                l[r] *= f;
+            for (int d = 0; d < HD / 16; d++) o[d] *= f;
+        }
+        const float base = m == -INFINITY ? 0.f : -m;
 #pragma unroll
-                for (int g = 0; g < G::kG; g++) {
-                    mids[r][g] *= f;
-                    if (!kCentred) ps[r][g] *= f;
-                }
-#pragma unroll
-                for (int d = 0; d < HD / 16; d++) o[r][d] *= f;
-            }
-            const float base = m[r] == -INFINITY ? 0.f : -m[r];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float e = fmaf(c[r], s[r][i / 4][i % 4], base);
-                if (sizeof(T) == 4) e = fmaf(c_low[r], s[r][i / 4][i % 4], e);
-                p[r][i] = __builtin_amdgcn_exp2f(e);
-                l[r] += p[r][i];
-            }
+        for (int i = 0; i < 8; i++) {
+            float e = fmaf(c, s[i / 4][i % 4], base);
+            if (sizeof(T) == 4) e = fmaf(c_low, s[i / 4][i % 4], e);
+            p[i] = __builtin_amdgcn_exp2f(e);
+            l += p[i];
         }
         uint32_t codes[8][HD == 256 ? 2 : 1];
 #pragma unroll
@@ -685,33 +657,30 @@ template <typename T, int HD, int RT> struct Rows {
 #pragma unroll
         for (int g = 0; g < G::kG; g++) {
             phase();
-            u32x4 w[RT][N];                 // p s, in parts
+            u32x4 w[N];                     // p s, in parts
 #pragma unroll
-            for (int r = 0; r < RT; r++) {
+            for (int t = 0; t < 2; t++) {
+                const f32x4 scale = four(2, g, t);
+                f32x4 mid = four(3, g, t);
+                if (hidden) {               // what a hidden key holds may be NaN
+                    const uint32_t seen = here(bits >> (16 * t + g4));
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const f32x4 scale = four(2, g, t);
-                    f32x4 mid = four(3, g, t);
-                    if (hidden) {           // what a hidden key holds may be NaN
-                        const uint32_t seen = here(bits[r] >> (16 * t + g4));
-#pragma unroll
-                        for (int i = 0; i < 4; i++) mid[i] = seen >> (4 * i) & 1 ? mid[i] : 0.f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) mids[r][g] = fmaf(p[r][4 * t + i], mid[i], mids[r][g]);
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        uint32_t part[N];
-                        cut_products<N>(p[r][4 * t + 2 * i], scale[2 * i], p[r][4 * t + 2 * i + 1], scale[2 * i + 1], part);
-#pragma unroll
-                        for (int n = 0; n < N; n++) w[r][n][2 * t + i] = part[n];
-                    }
+                    for (int i = 0; i < 4; i++) mid[i] = seen >> (4 * i) & 1 ? mid[i] : 0.f;
                 }
-                const u32x4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-                if (!kCentred)
 #pragma unroll
-                    for (int n = 0; n < N; n++) ps[r][g] = mma(ones, w[r][n], ps[r][g]);
+                for (int i = 0; i < 4; i++) mids[g] = fmaf(p[4 * t + i], mid[i], mids[g]);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    uint32_t part[N];
+                    cut_products<N>(p[4 * t + 2 * i], scale[2 * i], p[4 * t + 2 * i + 1], scale[2 * i + 1], part);
+#pragma unroll
+                    for (int n = 0; n < N; n++) w[n][2 * t + i] = part[n];
+                }
             }
+            const u32x4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+            if (!kCentred)
+#pragma unroll
+                for (int n = 0; n < N; n++) ps[g] = mma(ones, w[n], ps[g]);
 #pragma unroll
             for (int j = 0; j < 4; j += 2) {
                 // nibbles 4 g + j, 4 g + j + 1 of the values' words: one byte
@@ -728,12 +697,10 @@ template <typename T, int HD, int RT> struct Rows {
                     high[i] = unpack.high(x[i]);
                 }
 #pragma unroll
-                for (int r = 0; r < RT; r++)
-#pragma unroll
-                    for (int n = 0; n < N; n++) {
-                        o[r][nib] = mma(low, w[r][n], o[r][nib]);
-                        o[r][nib + 1] = mma(high, w[r][n], o[r][nib + 1]);
-                    }
+                for (int n = 0; n < N; n++) {
+                    o[nib] = mma(low, w[n], o[nib]);
+                    o[nib + 1] = mma(high, w[n], o[nib + 1]);
+                }
             }
         }
     }
@@ -742,20 +709,17 @@ template <typename T, int HD, int RT> struct Rows {
     __device__ __forceinline__ void finish()
     {
         const int up = E == kNone ? 0 : E - kUp;
+        l = groups_sum(l);
 #pragma unroll
-        for (int r = 0; r < RT; r++) {
-            l[r] = groups_sum(l[r]);
+        for (int g = 0; g < G::kG; g++) {
+            const float add = groups_sum(mids[g]);
 #pragma unroll
-            for (int g = 0; g < G::kG; g++) {
-                const float add = groups_sum(mids[r][g]);
+            for (int i = 0; i < 4; i++) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float b = o[r][4 * g + j][i];
-                        const float z = j & 1 ? Zeros<T>::kHigh : Zeros<T>::kLow;
-                        o[r][4 * g + j][i] = add + __builtin_amdgcn_ldexpf(kCentred ? b : fmaf(-z, ps[r][g][i], b), up);
-                    }
+                for (int j = 0; j < 4; j++) {
+                    const float b = o[4 * g + j][i];
+                    const float z = j & 1 ? Zeros<T>::kHigh : Zeros<T>::kLow;
+                    o[4 * g + j][i] = add + __builtin_amdgcn_ldexpf(kCentred ? b : fmaf(-z, ps[g][i], b), up);
                 }
             }
         }
@@ -780,8 +744,8 @@ __device__ __forceinline__ void put_values(const AttnArgs &a, int part, int64_t 
 }
 
 // The four waves' states of rows row0 .. (n rows in all) joined in LDS and written.
-template <typename T, int HD, int RT>
-__device__ __forceinline__ void join_waves(const AttnArgs &a, Rows<T, HD, RT> &w, char *lds, int h,
+template <typename T, int HD>
+__device__ __forceinline__ void join_waves(const AttnArgs &a, Rows<T, HD> &w, char *lds, int h,
                                            int64_t token0, int row0, int n, int part)
 {
     constexpr int kWide = Geo<HD>::kWide;
@@ -789,51 +753,47 @@ __device__ __forceinline__ void join_waves(const AttnArgs &a, Rows<T, HD, RT> &w
     float *O = (float *)lds;                            // [wave][16][kWide]
     float2 *ML = (float2 *)(O + kAttnWaves * 16 * kWide);   // [wave][16]
     float *total = (float *)(ML + kAttnWaves * 16);     // [16]
+    __syncthreads();                                // LDS is free
+    if (lane < 16) ML[wave * 16 + r] = make_float2(w.m, w.l);
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        if (row0 + 16 * t >= n) break;                  // uniform over the block
-        __syncthreads();                                // LDS is free
-        if (lane < 16) ML[wave * 16 + r] = make_float2(w.m[t], w.l[t]);
-        __syncthreads();
-        float top = -INFINITY, sum = 0.f;
+    for (int i = 0; i < kAttnWaves; i++) top = fmaxf(top, ML[i * 16 + r].x);
+    const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int i = 0; i < kAttnWaves; i++) top = fmaxf(top, ML[i * 16 + r].x);
-        const float base = top == -INFINITY ? 0.f : top;
+    for (int i = 0; i < kAttnWaves; i++)
+        sum += __builtin_amdgcn_exp2f(ML[i * 16 + r].x - base) * ML[i * 16 + r].y;
+    const float f = __builtin_amdgcn_exp2f(w.m - base);
+    if (wave == 0 && lane < 16) total[r] = sum;
+    const int rows = n - row0 < 16 ? n - row0 : 16;
+    if (part >= 0 && wave == 0 && lane < rows) {
+        const uint32_t row = row0 + r, token = cbq_div(row, a.rep);
+        a.part_ml[((int64_t)part * a.batch * a.tokens + token0 + token) * a.n_q +
+                  (int64_t)h * a.rep.d + row - token * a.rep.d] = make_float2(top, sum);
+    }
 #pragma unroll
-        for (int i = 0; i < kAttnWaves; i++)
-            sum += __builtin_amdgcn_exp2f(ML[i * 16 + r].x - base) * ML[i * 16 + r].y;
-        const float f = __builtin_amdgcn_exp2f(w.m[t] - base);
-        if (wave == 0 && lane < 16) total[r] = sum;
-        const int rows = n - row0 - 16 * t < 16 ? n - row0 - 16 * t : 16;
-        if (part >= 0 && wave == 0 && lane < rows) {
-            const uint32_t row = row0 + 16 * t + r, token = cbq_div(row, a.rep);
-            a.part_ml[((int64_t)part * a.batch * a.tokens + token0 + token) * a.n_q +
-                      (int64_t)h * a.rep.d + row - token * a.rep.d] = make_float2(top, sum);
-        }
+    for (int d0 = 0; d0 < HD; d0 += kWide) {
+        if (d0) __syncthreads();
+        // row r's pieces at (piece ^ r): 16 rows of one piece would share their banks
 #pragma unroll
-        for (int d0 = 0; d0 < HD; d0 += kWide) {
-            if (d0) __syncthreads();
-            // row r's pieces at (piece ^ r): 16 rows of one piece would share their banks
+        for (int g = d0 / kGroup; g < (d0 + kWide) / kGroup; g++)
 #pragma unroll
-            for (int g = d0 / kGroup; g < (d0 + kWide) / kGroup; g++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const f32x4 x = {w.o[t][4 * g][i], w.o[t][4 * g + 1][i], w.o[t][4 * g + 2][i],
-                                     w.o[t][4 * g + 3][i]};
-                    const int piece = (g - d0 / kGroup) * 16 + 4 * g4 + i;
-                    *(f32x4 *)(O + (wave * 16 + r) * kWide + (piece ^ r) * 4) = x * f;
-                }
-            __syncthreads();
-            for (int e = tid; e < rows * (kWide / 4); e += kBlock) {
-                const int rr = e / (kWide / 4), piece = e % (kWide / 4);
-                f32x4 x = {0, 0, 0, 0};
-#pragma unroll
-                for (int i = 0; i < kAttnWaves; i++)
-                    x += *(const f32x4 *)(O + (i * 16 + rr) * kWide + (piece ^ rr) * 4);
-                const uint32_t row = row0 + 16 * t + rr, token = cbq_div(row, a.rep);
-                put_values<T, HD>(a, part, token0 + token, h * a.rep.d + row - token * a.rep.d,
-                                  d0 + piece * 4, x, total[rr]);
+            for (int i = 0; i < 4; i++) {
+                const f32x4 x = {w.o[4 * g][i], w.o[4 * g + 1][i], w.o[4 * g + 2][i],
+                                 w.o[4 * g + 3][i]};
+                const int piece = (g - d0 / kGroup) * 16 + 4 * g4 + i;
+                *(f32x4 *)(O + (wave * 16 + r) * kWide + (piece ^ r) * 4) = x * f;
             }
+        __syncthreads();
+        for (int e = tid; e < rows * (kWide / 4); e += kBlock) {
+            const int rr = e / (kWide / 4), piece = e % (kWide / 4);
+            f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < kAttnWaves; i++)
+                x += *(const f32x4 *)(O + (i * 16 + rr) * kWide + (piece ^ rr) * 4);
+            const uint32_t row = row0 + rr, token = cbq_div(row, a.rep);
+            put_values<T, HD>(a, part, token0 + token, h * a.rep.d + row - token * a.rep.d,
+                              d0 + piece * 4, x, total[rr]);
         }
     }
 }
@@ -1198,7 +1158,7 @@ template <int HD, int RT> constexpr int attn_lds()
 
 // Rows row0 .. (of n) against the key tiles [first, end); seq -1: prefix rows of the
 // whole batch.
-template <typename T, int HD, int RT>
+template <typename T, int HD>
 __device__ __forceinline__ void walk(const AttnArgs &a, char *lds, const Work &w, int row0, int n, int to)
 {
     using G = Geo<HD>;
@@ -1211,26 +1171,23 @@ __device__ __forceinline__ void walk(const AttnArgs &a, char *lds, const Work &w
     Tiles<HD> tiles = {a, w.seq >= 0 ? a.tables + w.seq * a.table_st : nullptr, pre_tiles, 0, w.first + wave, w.end, w.h,
                        mine};
     tiles.look(w.end);
-    typename Rows<T, HD, RT>::Queries queries;
-    Rows<T, HD, RT>::load(a, w.h, token0, row0, n, queries);
+    typename Rows<T, HD>::Queries queries;
+    Rows<T, HD>::load(a, w.h, token0, row0, n, queries);
     int32_t length = 0, end = w.end;
     if (w.seq >= 0) {
         length = cbq_clamp_length(a.lengths[w.seq], a.capacity);
         end = (int32_t)cbq_min(end, (int64_t)pre_tiles + cbq_ceil(length, kTile));
     }
     arrived<0>();
-    Rows<T, HD, RT>::loaded(queries);
+    Rows<T, HD>::loaded(queries);
     if (w.first >= end && a.plan.parts > 1) return;         // the merge counts own parts by the length
     tiles.length = length;
     tiles.end = end;
     tiles.begin();
-    Rows<T, HD, RT> rows;
+    Rows<T, HD> rows;
     rows.start(a, row0, n, queries);
-    // own keys that the lane's row of each tile sees
-    int32_t sees[RT];
-#pragma unroll
-    for (int t = 0; t < RT; t++)
-        sees[t] = length - a.tokens + 1 + (int32_t)cbq_div(row0 + 16 * t + (lane & 15), a.rep);
+    // own keys that the lane's row sees
+    const int32_t sees = length - a.tokens + 1 + (int32_t)cbq_div(row0 + (lane & 15), a.rep);
     for (int i = 0; tiles.tile(i) < end; i++) {
         const uint32_t there = tiles.next(i);
         const int32_t tile = tiles.tile(i);
@@ -1243,20 +1200,16 @@ __device__ __forceinline__ void walk(const AttnArgs &a, char *lds, const Work &w
         // the first token sees the fewest own keys
         const int32_t key0 = (tile - pre_tiles) * kTile;
         const bool own_end = tile >= pre_tiles && key0 + kTile > length - a.tokens + 1;
-        uint32_t bits[RT];
-        if (there != ~0u || own_end)
-#pragma unroll
-            for (int t = 0; t < RT; t++) {
-                const int32_t left = own_end ? sees[t] - key0 : kTile;
-                bits[t] = there & (left >= kTile ? ~0u : left <= 0 ? 0u : (1u << left) - 1);
-            }
+        const int32_t left = own_end ? sees - key0 : kTile;
+        uint32_t bits = ~0u;
+        if (there != ~0u || own_end) bits = there & (left >= kTile ? ~0u : left <= 0 ? 0u : (1u << left) - 1);
         rows.tile(slot, scales, bits, there != ~0u || own_end);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
     rows.finish();
-    join_waves<T, HD, RT>(a, rows, lds, w.h, token0, row0, n, to);
+    join_waves<T, HD>(a, rows, lds, w.h, token0, row0, n, to);
 }
 
 // Waves a SIMD: their registers, and tiles two (or, of one wave, three) deep in LDS, leave
@@ -1281,7 +1234,7 @@ __global__ __launch_bounds__(kBlock, simd_waves(HD, RT)) void q4_kernel(AttnArgs
             return;
         }
     }
-    walk<T, HD, 1>(a, lds, w, w.tile * 16, w.seq < 0 ? a.batch * rows : rows, to);
+    walk<T, HD>(a, lds, w, w.tile * 16, w.seq < 0 ? a.batch * rows : rows, to);
 }
 
 // ---- merge of the parts: a block a (token, head) -------------------------------------------------
