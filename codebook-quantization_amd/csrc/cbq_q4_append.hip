@@ -17,7 +17,7 @@
 // read of the tables and weights, and asks for all of them before it uses one.
 //
 // Bound by bytes where prompts are long: 12416 tokens of 32 + 8 + 8 heads of 128 in bf16,
-// 268 MB, in 64 us, 4.2 TB/s where a copy of 1 GiB reaches 5.3.  (Heads asked for one by
+// 268 MB, in 60 us, 4.5 TB/s where a copy of 1 GiB reaches 5.3.  (Heads asked for one by
 // one and every code settled by the remainder of a 64-bit quotient: 98 us.)  By latency
 // where few: one token takes 4 us.
 #include "cbq_q4.h"
@@ -29,7 +29,9 @@ using namespace cbq_q4;
 constexpr int kThreads = 256;
 // Four heads a thread where that leaves four waves a SIMD of 256 CUs, else one.  32 + 8 + 8
 // heads of 128 in bf16, with their read, one and four: 100 tokens 6.2 and 8.4 us, 700 10.9 and
-// 11.3, 3000 26.1 and 25.3, 12000 104 and 73.
+// 11.3, 3000 26.1 and 25.3, 12000 104 and 73.  Head counts that four does not divide have one:
+// of 12000 tokens 14 + 2 + 2 heads go at 3.5 TB/s, 6 + 6 + 6 at 2.7 (12 + 4 + 4 and 8 + 8 + 8 by
+// four at 3.6 and 3.2).
 constexpr int64_t kFourThreads = 4 * 256 * 4 * 64;
 constexpr int kLanes = 16, kRows = kThreads / kLanes;    // lanes a row, rows a block
 

@@ -18,9 +18,9 @@
 //
 // The other operands have to fit fp16.  A query row is scaled to a largest value in
 // [2^14, 2^15), fp32 cut into two parts.  p_j s_jg is taken against 2^E, E the largest
-// exponent of the scales of the values that the wave has met: its 11 bits (two parts
-// of fp32: 22) hold down to 2^-26 of the largest scale, below that it loses them one by
-// one.
+// exponent of the scales of the values that the wave has met: its 11 bits hold down to
+// 2^-26 of the largest scale, the 22 of fp32's two parts to 2^-15; below that it is off by
+// 2^-37 of that scale.
 //
 // Rows are the query heads of a kv head beside the tokens, 16 a tile: row r of a
 // sequence is token r / rep, head r % rep.  Of a prefix the rows are the whole
@@ -40,8 +40,9 @@
 // cache, where a copy of 1 GiB moves 5.3; the vector units bound it, 1300 cycles a tile
 // and wave, three waves a SIMD.  One sequence of 384 keys: 10 us, two launches and the
 // chain of their loads (ids, pages, parts).  Ids, queries and the length are asked for at
-// once: one after the other, 16 sequences of 4 tokens behind 1000 keys take 18.5 us
-// instead of 14.6, and the long ones 114.
+// once: one after the other, 16 sequences of 4 tokens behind 1000 keys took 18.5 us
+// instead of 14.6, and the long ones 114.  fp32 queries take twice the products and
+// an addition a pair of codes: the long ones 148 us in a captured graph, bf16 there 120.
 #pragma once
 
 #include <atomic>
@@ -811,11 +812,13 @@ __device__ __forceinline__ void join_waves(const AttnArgs &a, Rows<T, HD> &w, ch
 // A slot of 16 bytes holds eight values in the order 0 4 1 5 2 6 3 7 that the codes'
 // masks give them; queries are read in that order, and outputs put back.
 //
-// 64 sequences of 32 heads of 128 behind 30011 keys, 200 to 1500 own ones: 78 us, of which
+// 64 sequences of 32 heads of 128 behind 30011 keys, 200 to 1500 own ones: 77 us, of which
 // the products would take 26.  A wave's chain from tile to tile bounds it (products,
 // softmax, products: 2.3 us a tile of 64 keys, one such wave a SIMD beside those of own
-// keys): 64 rows a block, two or three blocks a CU, take 101 to 108, 256 rows 123, and a
-// launch for the prefix alone 104, without the own keys' blocks beside it.
+// keys).  In a captured graph, where it takes 78 to 83: 64 rows a block, one to three blocks
+// a CU, 95 to 101, 128 rows and two blocks 92, every wave's own tiles 110.  When it took 80,
+// 256 rows a block took 123, and a launch for the prefix alone, without the own keys' blocks
+// beside it, 104.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -1213,8 +1216,9 @@ __device__ __forceinline__ void walk(const AttnArgs &a, char *lds, const Work &w
 }
 
 // Waves a SIMD: their registers, and tiles two (or, of one wave, three) deep in LDS, leave
-// room for so many.  24 sequences of 4000 to 32000 keys, bf16, hd 128: three waves two
-// tiles deep took 114 us, two waves three deep 143, four waves (which spill) two deep 133.
+// room for so many.  24 sequences of 4000 to 32000 keys, bf16, hd 128, in a captured graph:
+// three waves two tiles deep 120 us, two waves three deep 143, four waves (which spill) two
+// deep 275.
 constexpr int simd_waves(int hd, int rt) { return hd == 256 ? 1 : rt ? 2 : 3; }
 
 // RT: 64 RT rows a block of the prefix; 0: 16, as the own keys'.

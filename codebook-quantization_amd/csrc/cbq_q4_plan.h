@@ -11,7 +11,8 @@ constexpr int kTile = 32;                   // keys of a wave's tile
 constexpr int kAttnWaves = 4;               // waves a block, whose tiles take turns
 // (16 rows, tile, kv head) products of a prefix from which on its tiles are made into values
 // in LDS for all of a block's rows; with fewer the rounds of barriers cost more than they
-// save.  64 sequences of 32 heads behind 30011 keys: 78 us, and 110 with every wave's own.
+// save.  64 sequences of 32 heads behind 30011 keys, in a captured graph as below: 83 us, and
+// 110 with every wave's own.
 constexpr int64_t kManyTiles = 16 * 1024;
 constexpr int64_t kMaxBlocks = (1ll << 31) - 1, kMaxParts = 1 << 20, kAttnCus = 256;
 constexpr int64_t kMaxBytes = 1ll << 30;      // of the own parts' sums, where there are several
@@ -46,8 +47,8 @@ inline Plan plan(int hd, bool bf16, int n_kv, int64_t rows, int64_t prefix, int6
     p.own_tiles = (int32_t)own_tiles;
     // One block for all keys of a row tile, no parts to join: of few tiles a wave the join
     // costs as much as it saves, and where every CU has two such blocks parts bring no more
-    // of them.  64 sequences of 32 heads, 900 to 1900 keys: 36 us against 43 in parts, but one
-    // of 1200 keys 18 against 10; 300 to 3800 keys 57 against 49: lengths this uneven.
+    // of them.  64 sequences of 32 heads, 900 to 1900 keys: 32 us against 38 in parts, but one
+    // of 1200 keys 18 against 10; 300 to 3800 keys 54 against 47: lengths this uneven.
     // But every such block walks the prefix for itself, which parts read for 16 rows of all
     // sequences: 1 ns more a tile of 128 values, against 4 us and 10 ns a 1000 values of the
     // parts' sums, written, read and joined.  100 own keys and 32 heads on 8 of 128, bf16, in one
@@ -67,11 +68,11 @@ inline Plan plan(int hd, bool bf16, int n_kv, int64_t rows, int64_t prefix, int6
         return p;
     }
     int64_t tiles = cbq_ceil(all, p.rt ? 64 * p.rt : 16), pre_parts = 0, pre_chunk = 1;
-    // Blocks a CU: two for the prefix (four: 33 sequences of 3 tokens behind 5000 keys take 37
-    // us instead of 34), four for the own keys, 4 to 64 tiles each (two: 36 us, there).  One
+    // Blocks a CU: two for the prefix (four: 33 sequences of 3 tokens behind 5000 keys take 36
+    // us instead of 34), four for the own keys, 4 to 64 tiles each (two: 35.5 us, there).  One
     // for each with hd 256, of which a CU holds one block (two and four: one sequence of 9000
-    // keys 31 us instead of 21, 50 of 2 tokens behind 2000 keys 52 instead of 44); one for
-    // a prefix whose tiles are shared (two: 97 us instead of 80, then).
+    // keys 26 us instead of 18, 50 of 2 tokens behind 2000 keys 52 instead of 49); one for
+    // a prefix whose tiles are shared (two: 92 us instead of 83, then).
     const int64_t pre_blocks = (p.rt || hd == 256 ? 1 : 2) * kAttnCus, own_blocks = (hd == 256 ? 1 : 4) * kAttnCus;
     if (pre_tiles) {
         const int64_t want = cbq_max(1, pre_blocks / (tiles * n_kv)), unit = p.rt ? 2 : kAttnWaves;

@@ -72,10 +72,10 @@ int cbq_paged_read_q4(const cbq_paged_q4 *cache, const int64_t *slots, int64_t N
  * sees no key gets zeros.  The prefix's keys are read for many sequences at a time (a
  * short prefix's by each sequence, where that is less work).  q [batch * tokens, n_q, hd]
  * of type dtype, strides {token, head} in elements, 16-byte aligned; out contiguous, of q's
- * type.  Keys and values count as the values they
- * stand for; scores, maxima, sums and the weighted values are fp32.  A weight times
- * a value's scale is rounded to an fp16 number (of fp32 queries to two: 22 bits); a
- * long prefix that more than 16 query rows a kv head share is, for bf16 queries,
+ * type.  Keys and values count as the values they stand for; scores, maxima, sums and the
+ * weighted values are fp32.  A weight times a value's scale is rounded to an fp16 number
+ * (of fp32 queries to two: 22 bits, down to 2^-15 of the largest scale, below that 2^-37 of
+ * it); a long prefix that more than 16 query rows a kv head share is, for bf16 queries,
  * made into fp16 numbers, and its weights are.  A query that is not finite gives
  * NaN where it sees a key; keys whose scale passes 2^96 may, whatever the query.
  * n_q % n_kv == 0; n_q < 2^20, batch < 2^30, batch * tokens * n_q <= 2^31 - 65536;
